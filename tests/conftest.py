@@ -20,6 +20,12 @@ def built_libs():
 
 
 @pytest.fixture(scope="session")
+def attention_lib():
+    from unimonomoe_b200 import build
+    return build.build_attention()
+
+
+@pytest.fixture(scope="session")
 def oracle():
     from oracle import cpu_oracle
     cpu_oracle.build()

@@ -6,6 +6,7 @@ binary); here the variants share one source and differ by -D macros.
 
     python -m unimonomoe_b200.build            # every variant
     python -m unimonomoe_b200.build qwen_w1    # one
+    python -m unimonomoe_b200.build attention  # the attention half (also built with every variant)
 """
 from __future__ import annotations
 
@@ -99,6 +100,46 @@ def build_variant(variant: str, force: bool = False, verbose: bool = False) -> s
     return out
 
 
+ATTENTION = os.path.join(CSRC, "attention")
+ATTENTION_SOURCES = ["batch_plan.cu", "qk_norm_rope.cu", "kv4_store.cu", "kv4_decode.cu"]
+
+
+def attention_lib_path() -> str:
+    return os.path.join(LIBDIR, "libmono_attention.so")
+
+
+def build_attention(force: bool = False, verbose: bool = False) -> str:
+    """The attention half of the layer (include/mono_attention.h): one library for every geometry."""
+    out, header = attention_lib_path(), os.path.join(HERE, "..", "include", "mono_attention.h")
+    used = [os.path.join(ATTENTION, f) for f in os.listdir(ATTENTION)] + [os.path.join(CSRC, "ptx_sm100.cuh"), header, __file__]
+    if not force and os.path.exists(out) and all(os.path.getmtime(f) <= os.path.getmtime(out) for f in used):
+        return out
+    os.makedirs(LIBDIR, exist_ok=True)
+    nvcc = [os.environ.get("NVCC", "nvcc"), "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
+            "--expt-relaxed-constexpr", "-Xptxas", "-v", "-Xcompiler", "-fPIC"]
+
+    def compile_one(src):
+        obj = os.path.join(LIBDIR, os.path.splitext(src)[0] + ".o")
+        r = subprocess.run([*nvcc, "-c", os.path.join(ATTENTION, src), "-o", obj], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}{r.stderr}")
+        return obj, r.stdout + r.stderr
+
+    with ThreadPoolExecutor(max_workers=len(ATTENTION_SOURCES)) as ex:
+        built = list(ex.map(compile_one, ATTENTION_SOURCES))
+    r = subprocess.run([*nvcc, "-shared", *(obj for obj, _ in built), "-o", out], capture_output=True, text=True)
+    log = "".join(text for _, text in built) + r.stdout + r.stderr
+    with open(out + ".log", "w") as f:
+        f.write(log)
+    if r.returncode != 0:
+        raise RuntimeError(f"linking {out} failed:\n{r.stdout}{r.stderr}")
+    if verbose:
+        for line in log.splitlines():
+            if "registers" in line or "spill" in line:
+                print(f"[attention] {line.strip()}")
+    return out
+
+
 def build_microbench() -> str:
     """The hardware micro-benchmarks of csrc/sm100_microbench.cu as an executable (development tool)."""
     os.makedirs(LIBDIR, exist_ok=True)
@@ -125,6 +166,11 @@ if __name__ == "__main__":
         sel.remove("microbench")
         if not sel:
             sys.exit(0)
+    if "attention" in sel or not sel:
+        print("attention ->", build_attention(force="--force" in sys.argv, verbose=True))
+        if sel == ["attention"]:
+            sys.exit(0)
+        sel = [s for s in sel if s != "attention"]
     res = build_all(sel or None, force="--force" in sys.argv, verbose=True)
     for k, v in res.items():
         print(k, "->", v)

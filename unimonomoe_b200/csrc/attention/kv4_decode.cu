@@ -1,0 +1,617 @@
+// Attention over the 4-bit cache for requests of few query rows: one token, or a few guessed ahead. The rows of all query heads
+// that share a KV head are taken together, in blocks of 8 or 16.
+//
+// What bounds it is the cache, read once: 17/16 bytes for each key and value dim of a token. A CTA-wide product of 64 or more
+// rows on tcgen05 would be nearly all padding here, so the products go through mma.sync with the keys (and the dims of the
+// values) as its 16 rows and the query rows as its 8 columns, and what is made cheap is the way of a code into an operand:
+//  * A key's code c + 8 is left where it is and masked out of its word: as the low bits of an fp16 it is the subnormal
+//    (c + 8) 2^-24, four bits higher 2^-20. Half an instruction for a value; no conversion, no subtraction. The 16 goes into the
+//    query, the 8 is taken off the sum over a group: its accumulator starts at -8 sum(q). The sum is of 64 products of one size,
+//    so little is lost by it.
+//  * A value's code gets the exponent of 128 in the same instruction that masks it, and a packed subtraction leaves c itself.
+//    Taking 8 sum(p) off at the end instead would be cheaper, but a dim in which the token with nearly all of the weight
+//    has the code 0 would then be left with that token's rounding.
+//  * Scales meet the sums, not the values: a group's part of q.k is multiplied by the key's scale as fp32, a row's weight by
+//    the value's scale before it is rounded. Weights are bf16, whose exponents hold any product of the two: fp16 would round
+//    them eight times finer and lose those below 2^-31 of the largest, which a dim of that kind shows too.
+//  * The maximum is only moved when a weight would pass 2^8: one vote per step instead of a reduction.
+//
+// The work, all (request, KV head, row block) items in steps of 128 tokens, is cut into equal runs, one to a CTA; an item that
+// lies in several runs is joined by whoever of its CTAs finishes last, in the order of the runs, so the result does not depend on
+// which one that is. Each warp has every fourth pair of blocks, its own ring of copies in flight, and its own softmax state.
+#include "kv4_attention.cuh"
+
+namespace mono {
+namespace {
+
+using namespace kv4;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStep = 32 * kWarps;          // tokens of one step of a CTA
+constexpr float kLow = -1e38f;              // below every score
+constexpr float kRoom = 8.0f;               // log2 of what a weight may grow to before the maximum is moved
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// c + 8 in the low four bits of both halves, to c as bf16.
+__device__ __forceinline__ uint32_t signed_code(uint32_t x) {
+  const uint32_t y = (x & 0x000F000Fu) | 0x43004300u, off = 0x43084308u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float half_lo(uint32_t x) { return __half2float(__ushort_as_half(static_cast<unsigned short>(x & 0xFFFFu))); }
+__device__ __forceinline__ float half_hi(uint32_t x) { return __half2float(__ushort_as_half(static_cast<unsigned short>(x >> 16))); }
+
+template <int D, int NT>
+struct Shape {
+  static constexpr int NG = D / kGroup;
+  static constexpr int Rows = 8 * NT;                   // query rows of an item
+  static constexpr int Block = block_bytes(D);
+  static constexpr int Stage = 2 * Block;               // a pair of blocks
+  static constexpr int Stages = D == 256 ? 2 : 3;
+  static constexpr int Ring = Stages * Stage;           // of a warp
+  static constexpr int Part = Rows * (D + 2);           // floats of a warp's or a CTA's state: output, maximum, sum
+  static constexpr int Smem = kWarps * (Ring > Part * 4 ? Ring : (Part * 4 + 15) / 16 * 16);
+  static constexpr int PerSm = D == 256 ? 3 : NT == 2 && D == 128 ? 3 : 4;
+};
+
+// Steps of one item of a request; 0 if the request is not this kernel's.
+template <int Rows>
+__device__ __forceinline__ void cost_of(const AttnArgs& a, const Request& r, int& items, int& steps, int& lo) {
+  const int rows = r.n * a.group;
+  items = rows == 0 || rows > a.split_rows ? 0 : a.hk * ((rows + Rows - 1) / Rows);
+  lo = a.window > 0 ? max(r.len - r.n + 1 - a.window, 0) & ~(kTokens - 1) : 0;
+  steps = max(1, (r.len - lo + kStep - 1) / kStep);
+}
+
+template <int D, int NT>
+__global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(const AttnArgs a) {
+  using S = Shape<D, NT>;
+  constexpr int NG = S::NG;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_sum[kWarps];
+  __shared__ int s_found[2];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * (S::Smem / kWarps);
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+
+  // this CTA's run [u0, u1) of all steps, and the request that it begins in
+  const int chunk = (a.batch + kThreads - 1) / kThreads;
+  int mine = 0;
+  for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
+    int items, steps, lo;
+    cost_of<S::Rows>(a, request_of(a, b, blockIdx.x == 0), items, steps, lo);
+    mine += items * steps;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) s_sum[warp] = upto;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += s_sum[w];
+    total += s_sum[w];
+  }
+  const int per = (total + gridDim.x - 1) / static_cast<int>(gridDim.x);
+  const int u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  if (u0 >= u1) return;
+  if (upto - mine <= u0 && u0 < upto) {
+    int at = upto - mine, b = tid * chunk;
+    for (;; ++b) {
+      int items, steps, lo;
+      cost_of<S::Rows>(a, request_of(a, b, false), items, steps, lo);
+      if (at + items * steps > u0) break;
+      at += items * steps;
+    }
+    s_found[0] = b;
+    s_found[1] = at;
+  }
+  __syncthreads();
+  int b = s_found[0], at = s_found[1];       // request, and the step that its items begin at
+
+  for (int u = u0; u < u1;) {
+    Request r = request_of(a, b, false);
+    int items, steps, lo;
+    cost_of<S::Rows>(a, r, items, steps, lo);
+    while (u >= at + items * steps) {
+      at += items * steps;
+      r = request_of(a, ++b, false);
+      cost_of<S::Rows>(a, r, items, steps, lo);
+    }
+    const int item = (u - at) / steps, i0 = at + item * steps, i1 = i0 + steps;
+    const int e = min(i1, u1);
+    const int row_blocks = items / a.hk, head = item / row_blocks, rb = item - head * row_blocks;
+    const int rows = min(S::Rows, r.n * a.group - rb * S::Rows);
+
+    // tokens of this run, and the last one (exclusive) that any row of the block sees
+    const int place0 = r.len - r.n;
+    const int tok_first = rb * S::Rows / a.group, tok_last = (rb * S::Rows + rows - 1) / a.group;
+    const int seen = min(r.len, max(place0 + tok_last + 1, 0));
+    const int k0 = lo + (u - i0) * kStep, k1 = min(lo + (e - i0) * kStep, seen);
+    // every row sees all of [clear_lo, clear_hi)
+    const int clear_hi = max(place0 + tok_first + 1, 0), clear_lo = a.window > 0 ? max(place0 + tok_last + 1 - a.window, 0) : 0;
+
+    // query: B operand, row n = g of each tile; scaled by a power of two to an fp16 with its largest value near 2^14
+    uint32_t qf[NT][4 * NG][2];
+    float fac[NT][2], qs[NT][NG][2];
+    int hi_r[NT][2], lo_r[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = rb * S::Rows + nt * 8 + g;
+      const bool real = nt * 8 + g < rows;
+      float x[NG][2][8];
+      uint32_t top = 0;
+      if (real) {
+        const __nv_bfloat16* p = a.q + (r.first + row / a.group) * a.q_ts + (head * a.group + row % a.group) * a.q_hs;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p + 64 * gi + 16 * t + 8 * w)), x[gi][w]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[gi][w][j]) & 0x7FFFFFFFu);
+          }
+      } else {
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[gi][j >> 3][j & 7] = 0.0f;
+      }
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      const int ex = min(max(static_cast<int>(top >> 23) - 127, -100), 100);
+      const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
+      const float f = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(24 - 14 + ex + 127) << 23);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint32_t b0 = pack_f16(x[gi][w][2 * st] * up, x[gi][w][4 + 2 * st] * up);
+            const uint32_t b1 = pack_f16(x[gi][w][1 + 2 * st] * (up * 0.0625f), x[gi][w][5 + 2 * st] * (up * 0.0625f));
+            qf[nt][gi * 4 + w * 2 + st][0] = b0;
+            qf[nt][gi * 4 + w * 2 + st][1] = b1;
+            sum += half_lo(b0) + half_hi(b0) + 16.0f * (half_lo(b1) + half_hi(b1));
+          }
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+        sum *= -8.0f * 0x1p-24f;
+        qs[nt][gi][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
+        qs[nt][gi][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+      }
+      fac[nt][0] = __shfl_sync(0xFFFFFFFFu, f, 8 * t);
+      fac[nt][1] = __shfl_sync(0xFFFFFFFFu, f, 8 * t + 4);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {          // what row 2t + c of the tile sees: [lo_r, hi_r)
+        const int rr = nt * 8 + 2 * t + c, place = place0 + (rb * S::Rows + rr) / a.group;
+        hi_r[nt][c] = rr < rows ? min(place + 1, r.len) : 0;
+        lo_r[nt][c] = a.window > 0 ? place + 1 - a.window : 0;
+      }
+    }
+
+    float o[NT][4 * NG][4], l[NT][2], m[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4 * NG; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.0f;
+      l[nt][0] = l[nt][1] = 0.0f;
+      m[nt][0] = m[nt][1] = kLow;
+    }
+
+    // this warp's pairs of blocks: the warp-th, the (warp + 4)-th, ... of [k0, k1)
+    const int pairs = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;
+    const int count = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
+    const int per_page = 1 << (a.shift - 4);
+    auto fetch = [&](int i, int (&pg)[2]) {  // pages of the i-th pair
+      const int blk = (k0 >> 4) + 2 * (warp + kWarps * i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) pg[h] = i < count && (blk + h) * 16 < k1 ? page_of(a, b, (blk + h) >> (a.shift - 4)) : -1;
+    };
+    auto issue = [&](int i, const int (&pg)[2]) {
+      const int blk = (k0 >> 4) + 2 * (warp + kWarps * i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (pg[h] >= 0) {
+          const uint8_t* src = a.cache + ((static_cast<int64_t>(pg[h]) * a.hk + head) * per_page + ((blk + h) & (per_page - 1))) * S::Block;
+          const uint32_t dst = ring_at + (i % S::Stages) * S::Stage + h * S::Block;
+#pragma unroll
+          for (int j = 0; j < (S::Block + 511) / 512; ++j) {
+            const int off = j * 512 + lane * 16;
+            if (off < S::Block) cp16(dst + off, src + off);
+          }
+        }
+      cp_commit();
+    };
+    int pg[2];
+    fetch(0, pg);
+#pragma unroll
+    for (int i = 0; i < S::Stages - 1; ++i) {
+      int nx[2];
+      fetch(i + 1, nx);
+      issue(i, pg);
+      pg[0] = nx[0];
+      pg[1] = nx[1];
+    }
+
+    for (int i = 0; i < count; ++i) {
+      {
+        int nx[2];
+        fetch(i + S::Stages, nx);
+        __syncwarp();                        // all lanes are done with the stage that is written now
+        issue(i + S::Stages - 1, pg);
+        pg[0] = nx[0];
+        pg[1] = nx[1];
+      }
+      cp_wait<S::Stages - 1>();
+      __syncwarp();
+      const uint8_t* stage = ring + (i % S::Stages) * S::Stage;
+      const int key0 = k0 + 32 * (warp + kWarps * i);
+      const bool mask = key0 < clear_lo || key0 + 32 > clear_hi || key0 + 32 > k1;
+
+      float s[2][NT][4];
+      uint32_t vs[2][2][(NG + 1) / 2];       // value scales of tokens g and g + 8
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* blk = stage + h * S::Block;
+        uint32_t kw[2][2 * NG], ks[2][(NG + 1) / 2];
+        if constexpr (D == 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(blk + lane * 16);
+          kw[0][0] = x.x; kw[0][1] = x.y; kw[1][0] = x.z; kw[1][1] = x.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2 * NG / 4; ++j)
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              const uint4 x = *reinterpret_cast<const uint4*>(blk + (rr * (2 * NG / 4) + j) * 512 + lane * 16);
+              kw[rr][4 * j] = x.x; kw[rr][4 * j + 1] = x.y; kw[rr][4 * j + 2] = x.z; kw[rr][4 * j + 3] = x.w;
+            }
+        }
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+          const uint8_t* sc = blk + 16 * D + (g + 8 * rr) * 4 * NG;
+          if constexpr (NG == 1) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(sc);
+            ks[rr][0] = x & 0xFFFFu;
+            vs[h][rr][0] = x >> 16;
+          } else if constexpr (NG == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(sc);
+            ks[rr][0] = x.x;
+            vs[h][rr][0] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(sc);
+            ks[rr][0] = x.x; ks[rr][1] = x.y;
+            vs[h][rr][0] = x.z; vs[h][rr][1] = x.w;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[h][nt][c] = 0.0f;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            acc[nt][0] = acc[nt][2] = qs[nt][gi][0];
+            acc[nt][1] = acc[nt][3] = qs[nt][gi][1];
+          }
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              const uint32_t x0 = kw[0][2 * gi + w] >> (8 * st), x1 = kw[1][2 * gi + w] >> (8 * st);
+              const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u, a3 = x1 & 0x00F000F0u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(acc[nt], a0, a1, a2, a3, qf[nt][gi * 4 + w * 2 + st][0], qf[nt][gi * 4 + w * 2 + st][1]);
+            }
+          float f[2];
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr) f[rr] = __uint_as_float(gi & 1 ? ks[rr][gi >> 1] & 0xFFFF0000u : ks[rr][gi >> 1] << 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[h][nt][c] = fmaf(acc[nt][c], f[c >> 1], s[h][nt][c]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[h][nt][c] *= fac[nt][c & 1];
+      }
+      if (mask) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = key0 + 16 * h + g + 8 * (c >> 1);
+              if (key < lo_r[nt][c & 1] || key >= min(hi_r[nt][c & 1], k1)) s[h][nt][c] = -INFINITY;
+            }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          grow |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + kRoom;
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+            x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+            const float to = fmaxf(m[nt][c], x), by = ex2(m[nt][c] - to);
+            m[nt][c] = to;
+            l[nt][c] *= by;
+#pragma unroll
+            for (int j = 0; j < 4 * NG; ++j) {
+              o[nt][j][c] *= by;
+              o[nt][j][c + 2] *= by;
+            }
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* blk = stage + h * S::Block + 8 * D;
+        float p[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            p[nt][c] = ex2(s[h][nt][c] - m[nt][c & 1]);
+            l[nt][c & 1] += p[nt][c];
+          }
+        uint32_t vw[4][NG];
+        if constexpr (D == 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(blk + lane * 16);
+          vw[0][0] = x.x; vw[1][0] = x.y; vw[2][0] = x.z; vw[3][0] = x.w;
+        } else if constexpr (D == 128) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 x = *reinterpret_cast<const uint4*>(blk + j * 512 + lane * 16);
+            vw[2 * j][0] = x.x; vw[2 * j][1] = x.y; vw[2 * j + 1][0] = x.z; vw[2 * j + 1][1] = x.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 x = *reinterpret_cast<const uint4*>(blk + j * 512 + lane * 16);
+            vw[j][0] = x.x; vw[j][1] = x.y; vw[j][2] = x.z; vw[j][3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          float f[2];
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr)
+            f[rr] = __uint_as_float(gi & 1 ? vs[h][rr][gi >> 1] & 0xFFFF0000u : vs[h][rr][gi >> 1] << 16);
+          uint32_t pb[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float w[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = p[nt][c] * f[c >> 1];
+            if (mask) {                      // what lies behind the sequence, or is hidden from a row, may hold anything
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (s[h][nt][c] == -INFINITY) w[c] = 0.0f;
+            }
+            pb[nt][0] = transpose8(pack_bf16x2(w[0], w[1]));
+            pb[nt][1] = transpose8(pack_bf16x2(w[2], w[3]));
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(vw[0][gi], vw[1][gi], half ? 0x7632 : 0x5410);
+            const uint32_t y = __byte_perm(vw[2][gi], vw[3][gi], half ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              const uint32_t a0 = signed_code(x >> (8 * st)), a1 = signed_code(x >> (8 * st + 4));
+              const uint32_t a2 = signed_code(y >> (8 * st)), a3 = signed_code(y >> (8 * st + 4));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816_bf16(o[nt][gi * 4 + half * 2 + st], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();                         // the rings become the warps' states
+
+    float* part = reinterpret_cast<float*>(ring);
+    float* ml = part + S::Rows * D;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = l[nt][c];
+        x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+        x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+        x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+        const int row = nt * 8 + 2 * t + c;
+        if (g == 0) {
+          ml[2 * row] = m[nt][c];
+          ml[2 * row + 1] = x;
+        }
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(part + row * D + 64 * gi + 8 * g + 2 * j) = make_float2(o[nt][gi * 4 + j][c], o[nt][gi * 4 + j][c + 2]);
+      }
+    __syncthreads();
+
+    const bool whole = u == i0 && e == i1;
+    const int c0 = i0 / per, c1 = (i1 - 1) / per;        // the CTAs that share the item
+    float* mine_at = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
+    auto finish = [&](int row, int d, float4 x, float mx, float sum) {
+      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;   // a sum that is not a number stays one
+      const int rr = rb * S::Rows + row, tok = r.first + rr / a.group, hd = head * a.group + rr % a.group;
+      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(tok) * a.hq + hd) * D + d) =
+          make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+      if (d == 0 && a.lse) a.lse[static_cast<int64_t>(tok) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+    };
+    constexpr int Wf = S::Smem / kWarps / 4;             // floats from one warp's state to the next
+    for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
+      const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+      const float* base = reinterpret_cast<const float*>(smem);
+      float mx = kLow, sum = 0.0f;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, base[w * Wf + S::Rows * D + 2 * row]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float by = ex2(base[w * Wf + S::Rows * D + 2 * row] - mx);
+        const float4 y = *reinterpret_cast<const float4*>(base + w * Wf + row * D + d);
+        sum = fmaf(base[w * Wf + S::Rows * D + 2 * row + 1], by, sum);
+        x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y); x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
+      }
+      if (whole) {
+        finish(row, d, x, mx, sum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(mine_at + row * D + d), x);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(mine_at + S::Rows * D + 2 * row), make_float2(mx, sum));
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const uint32_t before = atomicAdd(a.counters + c0, 1u);
+        s_last = before == static_cast<uint32_t>(c1 - c0);
+        if (s_last) a.counters[c0] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
+          const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+          float mx = kLow, sum = 0.0f;
+          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+          for (int c = c0; c <= c1; ++c) {
+            const float* from = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + S::Rows * D + 2 * row));
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(from + row * D + d));
+            const float to = fmaxf(mx, ms.x), old = ex2(mx - to), by = ex2(ms.x - to);
+            mx = to;
+            sum = fmaf(ms.y, by, sum * old);
+            x.x = fmaf(y.x, by, x.x * old); x.y = fmaf(y.y, by, x.y * old);
+            x.z = fmaf(y.z, by, x.z * old); x.w = fmaf(y.w, by, x.w * old);
+          }
+          finish(row, d, x, mx, sum);
+        }
+      }
+    }
+    __syncthreads();                         // the rings are free again
+    u = e;
+  }
+}
+
+template <int D, int NT>
+int launch(const AttnArgs& a, cudaStream_t stream) {
+  using S = Shape<D, NT>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev >= 64 || !ready[dev]) {
+    e = cudaFuncSetAttribute(decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (dev < 64) ready[dev] = true;
+  }
+  decode_kernel<D, NT><<<MONO_ATTN_SMS * S::PerSm, kThreads, S::Smem, stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+namespace kv4 {
+// Query rows of a request up to which this kernel takes it, where the other one is there too.
+int decode_rows() { return 1 << 30; }
+int decode(const AttnArgs& a, int head_dim, int rows, cudaStream_t stream) {
+  if (head_dim == 256) return launch<256, 1>(a, stream);
+  if (head_dim == 128) return rows <= 8 ? launch<128, 1>(a, stream) : launch<128, 2>(a, stream);
+  return rows <= 8 ? launch<64, 1>(a, stream) : launch<64, 2>(a, stream);
+}
+}  // namespace kv4
+}  // namespace mono
+
+extern "C" size_t mono_attn_workspace_bytes(void) {
+  // counters of all CTAs, and two partial states for each: at most 16 rows of 128 dims or 8 of 256, or of 64
+  return MONO_ATTN_COUNTERS * 4 + static_cast<size_t>(MONO_ATTN_COUNTERS) * 2 * 16 * (128 + 2) * 4;
+}
+
+extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const uint8_t* cache,
+                                       int64_t num_pages, int page_size, const int32_t* block_table, int table_width,
+                                       const int32_t* seq_lens, const int32_t* query_start, int batch, int tokens,
+                                       int max_query_len, int q_heads, int kv_heads, int head_dim, float scale, int window,
+                                       void* out, float* lse, void* workspace, size_t workspace_bytes, uint32_t* status,
+                                       mono_attn_stream_t stream) {
+  using namespace mono;
+  using namespace mono::kv4;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
+  if (batch < 0 || tokens < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || table_width < 1 || num_pages < 1 ||
+      window < 0 || max_query_len < 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+    return MONO_ATTN_BAD_SIZE;
+  if (batch == 0 || tokens == 0) return 0;
+  if (!q || !cache || !block_table || !seq_lens || !query_start || !out || !workspace || !status) return MONO_ATTN_NULL;
+  if (workspace_bytes < mono_attn_workspace_bytes()) return MONO_ATTN_WORKSPACE;
+  AttnArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.cache = cache;
+  a.table = block_table; a.seq_lens = seq_lens; a.query_start = query_start;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.counters = static_cast<uint32_t*>(workspace);
+  a.partial = reinterpret_cast<float*>(a.counters + MONO_ATTN_COUNTERS);
+  a.status = status;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.num_pages = num_pages;
+  a.tokens = tokens; a.batch = batch; a.width = table_width; a.hq = q_heads; a.hk = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.shift = __builtin_ctz(page_size);
+  a.window = window;
+  a.split_rows = INT32_MAX;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const int64_t rows = static_cast<int64_t>(max_query_len) * a.group;
+  return decode(a, head_dim, rows > 1 << 20 ? 1 << 20 : static_cast<int>(rows), stream);
+}

@@ -1,0 +1,129 @@
+// The 4-bit key/value cache: where a code and a scale lie, how a row is quantised and read back.
+//
+// A page of one KV head is a run of blocks of 16 tokens, 17*D bytes each (D = head size, NG = D/64 groups of 64 dims):
+//   [0, 8D)      key codes      [8D, 16D)   value codes      [16D, 17D)  scales, per token NG of the key then NG of the value
+// A group x of 64 values is stored as a scale s and codes c in [-7, 7], kept as c + 8 in half a byte:
+//   s = round to five significant bits of max|x| / 7, within [2^-60, 2^60];   c = clamp(rint(x / s), -7, 7);   value s * c
+// Five bits of s and three of c make s * c exact in bfloat16: nothing is rounded when a key or value is read back, and
+// the matrix unit works on the values themselves. Rounding s costs at most 1/32 of a step of the largest code.
+// A group that holds an infinity or a NaN gets the scale NaN: what reads it sees that it was not finite.
+//
+// Codes lie in the order in which the lanes of a warp use them as the A operand of mma.m16n8k16 (lane = 4 g + t holds rows g
+// and g + 8, columns 2t, 2t+1, 2t+8, 2t+9), 16 bytes to a lane at a time, so that a block is loaded with full-width
+// shared-memory reads free of bank conflicts and no code is moved between lanes:
+//   keys:   token r = g or g + 8, dims 64 gi + 16 t + (0..15): two words for each of the two tokens and each group
+//   values: dims 64 gi + 8 g + (0..7) of tokens 2t, 2t+1, 2t+8, 2t+9: one word for each token and group
+// The order of the products inside a sum is free, so dims may stand in any column as long as the query's do too.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+
+namespace mono {
+namespace kv4 {
+
+constexpr int kGroup = 64;
+constexpr int kTokens = 16;               // tokens of a block
+constexpr float kScaleMin = 0x1p-60f, kScaleMax = 0x1p60f;
+
+__host__ __device__ constexpr int block_bytes(int d) { return 17 * d; }
+
+// Byte of the word that holds dims 8 l .. 8 l + 7 of token r, from the start of its block.
+template <int D>
+__device__ __forceinline__ int key_word(int r, int l) {
+  constexpr int NG = D / kGroup;
+  const int o = (r >> 3) * 8 * NG + (2 * (l >> 3) + (l & 1)) * 4;
+  return (o >> 4) * 512 + ((r & 7) * 4 + ((l & 7) >> 1)) * 16 + (o & 15);
+}
+template <int D>
+__device__ __forceinline__ int value_word(int r, int l) {
+  constexpr int NG = D / kGroup;
+  const int o = ((r >> 3) * 2 + (r & 1)) * 4 * NG + (l >> 3) * 4;
+  return 8 * D + (o >> 4) * 512 + ((l & 7) * 4 + ((r >> 1) & 3)) * 16 + (o & 15);
+}
+template <int D>
+__device__ __forceinline__ int scale_at(int r, bool value, int gi) {
+  constexpr int NG = D / kGroup;
+  return 16 * D + r * 4 * NG + (value ? 2 * NG : 0) + gi * 2;
+}
+
+// First byte of the block of `slot` (page * page_size + offset) for one head; page_shift = log2(page_size).
+template <int D>
+__device__ __forceinline__ int64_t block_at(int64_t slot, int head, int heads, int page_shift) {
+  const int64_t page = slot >> page_shift;
+  const int sub = static_cast<int>(slot & ((1 << page_shift) - 1)) >> 4;
+  return (((page * heads + head) << (page_shift - 4)) + sub) * block_bytes(D);
+}
+
+// To five significant bits, ties to even. Finite, normal s.
+__device__ __forceinline__ float round5(float s) {
+  uint32_t b = __float_as_uint(s);
+  b += 0x3FFFFu + ((b >> 19) & 1u);
+  return __uint_as_float(b & ~0x7FFFFu);
+}
+
+// Eight values of a row, in the eight adjacent lanes that share a group: their codes as one word, and the group's scale.
+// The lanes of `mask` take part, whole groups of eight.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t mask, float& scale) {
+  uint32_t top = 0;                        // magnitudes as integers: a NaN is above infinity, infinity above the rest
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(mask, top, d));
+  if (top >= 0x7F800000u) {
+    scale = __uint_as_float(0x7FC00000u);
+    return 0x88888888u;
+  }
+  const float s = fminf(fmaxf(round5(__fdiv_rn(__uint_as_float(top), 7.0f)), kScaleMin), kScaleMax);
+  scale = s;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.0f), 7.0f);
+    w |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
+  }
+  return w;
+}
+
+// Stores dims 8 l .. 8 l + 7 of one row: `blk` is its block, r its token there.
+template <int D>
+__device__ __forceinline__ void store8(uint8_t* blk, int r, bool value, int l, uint32_t word, float scale) {
+  *reinterpret_cast<uint32_t*>(blk + (value ? value_word<D>(r, l) : key_word<D>(r, l))) = word;
+  if ((l & 7) == 0)
+    *reinterpret_cast<uint16_t*>(blk + scale_at<D>(r, value, l >> 3)) = static_cast<uint16_t>(__float_as_uint(scale) >> 16);
+}
+
+// Device-side errors of the operators: the first one stays in the status word.
+enum Status : uint32_t {
+  kStatusOk = 0,
+  kBadPosition = 1,      // a position outside the rotation table
+  kBadSlot = 2,          // a slot outside the cache
+  kBadPage = 3,          // a block-table entry outside the cache
+  kTooLong = 4,          // a sequence longer than its row of the block table
+  kNoPages = 5,          // more pages needed than are free
+  kTooManyTokens = 6,    // more tokens than the outputs have rows
+  kBadLength = 7,        // a negative length, or query offsets that fall or pass the query's rows
+  kWaitTimeout = 8,      // a wait inside a kernel ran out
+};
+__device__ __forceinline__ void report(uint32_t* status, uint32_t code, uint32_t where) {
+  if (atomicCAS(status, 0u, code) == 0u) status[1] = where;
+}
+
+__device__ __forceinline__ void unpack_bf16x8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint4 pack_bf16x8(const float (&x)[8]) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+
+}  // namespace kv4
+}  // namespace mono

@@ -1,0 +1,138 @@
+// Keys and values into the 4-bit cache, and what they stand for back out of it, by slot.
+// Bound by memory: 2 bytes a value on one side, 17/32 on the other; a lane has eight dims, one word of the cache.
+#include <cuda_runtime.h>
+#include "kv4_format.cuh"
+#include "../../../include/mono_attention.h"
+
+namespace mono {
+namespace {
+
+constexpr int kWarps = 8;
+
+struct StoreArgs {
+  const __nv_bfloat16 *k, *v;               // stored, or
+  __nv_bfloat16 *k_out, *v_out;             // read
+  uint8_t* cache;
+  const int64_t* slots;
+  uint32_t* status;
+  int64_t k_ts, k_hs, v_ts, v_hs, slot_count, rows;
+  int heads, shift;
+};
+
+// Rows are (token, head, key or value), D/8 lanes each; a warp does 32/(D/8) of them at a time, U times.
+template <int D, int U, bool READ>
+__global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
+  constexpr int L = D / 8, R = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * R * U + sub;
+  if (first - sub >= a.rows) return;        // the whole warp
+  const uint32_t per = 2 * a.heads;
+  int64_t slot[U], token[U];
+  int head[U];
+  bool value[U], fine[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int64_t row = first + i * R;
+    fine[i] = row < a.rows;
+    const int64_t r = fine[i] ? row : a.rows - 1;
+    token[i] = r / per;
+    const int h = static_cast<int>(r - token[i] * per);
+    value[i] = h >= a.heads;
+    head[i] = value[i] ? h - a.heads : h;
+    slot[i] = a.slots[token[i]];
+    if (slot[i] < -1 || slot[i] >= a.slot_count) {
+      if (l == 0) kv4::report(a.status, kv4::kBadSlot, static_cast<uint32_t>(token[i]));
+      slot[i] = -1;
+    }
+  }
+  if constexpr (READ) {
+    uint32_t word[U];
+    float scale[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      word[i] = 0x88888888u;
+      scale[i] = 0.0f;
+      if (slot[i] >= 0) {
+        const uint8_t* blk = a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift);
+        const int r = static_cast<int>(slot[i] & 15);
+        word[i] = *reinterpret_cast<const uint32_t*>(blk + (value[i] ? kv4::value_word<D>(r, l) : kv4::key_word<D>(r, l)));
+        scale[i] = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(blk + kv4::scale_at<D>(r, value[i], l >> 3))) << 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = scale[i] * static_cast<float>(static_cast<int>((word[i] >> (4 * j)) & 15u) - 8);
+      if (fine[i]) *reinterpret_cast<uint4*>((value[i] ? a.v_out : a.k_out) + (token[i] * a.heads + head[i]) * D + 8 * l) = kv4::pack_bf16x8(x);
+    }
+  } else {
+    uint4 raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      raw[i] = *reinterpret_cast<const uint4*>((value[i] ? a.v + token[i] * a.v_ts + head[i] * a.v_hs : a.k + token[i] * a.k_ts + head[i] * a.k_hs) + 8 * l);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float x[8], s;
+      kv4::unpack_bf16x8(raw[i], x);
+      const uint32_t word = kv4::quantise8(x, 0xFFFFFFFFu, s);
+      if (fine[i] && slot[i] >= 0)
+        kv4::store8<D>(a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift), static_cast<int>(slot[i] & 15), value[i], l, word, s);
+    }
+  }
+}
+
+template <int D, bool READ>
+int launch(const StoreArgs& a, cudaStream_t stream) {
+  constexpr int U = 2;
+  const int64_t rows = 32 / (D / 8) * U * kWarps;
+  store_kernel<D, U, READ><<<static_cast<unsigned>((a.rows + rows - 1) / rows), kWarps * 32, 0, stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int check(int tokens, int heads, int head_dim, int64_t num_pages, int page_size) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
+  if (tokens < 0 || heads < 1 || num_pages < 1 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return MONO_ATTN_BAD_SIZE;
+  return 0;
+}
+
+}  // namespace
+}  // namespace mono
+
+extern "C" int mono_attn_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                    int64_t v_token_stride, int64_t v_head_stride, int tokens, int kv_heads, int head_dim,
+                                    uint8_t* cache, int64_t num_pages, int page_size, const int64_t* slots, uint32_t* status,
+                                    mono_attn_stream_t stream) {
+  using namespace mono;
+  if (const int rc = check(tokens, kv_heads, head_dim, num_pages, page_size)) return rc;
+  if (!k || !v || !cache || !slots || !status) return MONO_ATTN_NULL;
+  if (tokens == 0) return 0;
+  StoreArgs a{};
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.v = static_cast<const __nv_bfloat16*>(v);
+  a.cache = cache; a.slots = slots; a.status = status;
+  a.k_ts = k_token_stride; a.k_hs = k_head_stride; a.v_ts = v_token_stride; a.v_hs = v_head_stride;
+  a.slot_count = num_pages * page_size;
+  a.rows = static_cast<int64_t>(tokens) * kv_heads * 2;
+  a.heads = kv_heads;
+  a.shift = __builtin_ctz(page_size);
+  return head_dim == 64 ? launch<64, false>(a, stream) : head_dim == 128 ? launch<128, false>(a, stream) : launch<256, false>(a, stream);
+}
+
+extern "C" int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, const int64_t* slots, int tokens,
+                                  int kv_heads, int head_dim, void* k_out, void* v_out, uint32_t* status,
+                                  mono_attn_stream_t stream) {
+  using namespace mono;
+  if (const int rc = check(tokens, kv_heads, head_dim, num_pages, page_size)) return rc;
+  if (!k_out || !v_out || !cache || !slots || !status) return MONO_ATTN_NULL;
+  if (tokens == 0) return 0;
+  StoreArgs a{};
+  a.k_out = static_cast<__nv_bfloat16*>(k_out);
+  a.v_out = static_cast<__nv_bfloat16*>(v_out);
+  a.cache = const_cast<uint8_t*>(cache); a.slots = slots; a.status = status;
+  a.slot_count = num_pages * page_size;
+  a.rows = static_cast<int64_t>(tokens) * kv_heads * 2;
+  a.heads = kv_heads;
+  a.shift = __builtin_ctz(page_size);
+  return head_dim == 64 ? launch<64, true>(a, stream) : head_dim == 128 ? launch<128, true>(a, stream) : launch<256, true>(a, stream);
+}
