@@ -37,18 +37,23 @@ def attention(q, keys, values, starts, window, scale):
     out, size = (torch.zeros(T, H, D, dtype=torch.float64, device=q.device) for _ in range(2))
     lse = torch.full((T, H), -math.inf, dtype=torch.float64, device=q.device)
     for b, (k, v) in enumerate(zip(keys, values)):
-        n = len(k)
-        for t in range(starts[b], starts[b + 1]):
-            place = n - starts[b + 1] + t
-            lo = max(0, place + 1 - window) if window else 0
-            if place < 0 or lo > place:
-                continue
-            kk, vv = (x[lo:place + 1].double().repeat_interleave(H // x.shape[1], 1) for x in (k, v))
-            s = torch.einsum("hd,nhd->hn", q[t].double(), kk) * scale
-            lse[t] = torch.logsumexp(s, -1)
-            p = torch.softmax(s, -1)
-            out[t] = torch.einsum("hn,nhd->hd", p, vv)
-            size[t] = torch.einsum("hn,nhd->hd", p, vv.abs())
+        n, rows = len(k), slice(starts[b], starts[b + 1])
+        place = n - starts[b + 1] + torch.arange(starts[b], starts[b + 1], device=q.device)
+        if not len(place) or not n:
+            continue
+        j = torch.arange(n, device=q.device)
+        seen = j <= place[:, None]
+        if window:
+            seen &= j > place[:, None] - window
+        for h in range(H):
+            kk, vv = (x[:, h * x.shape[1] // H].double() for x in (k, v))
+            s = (q[rows, h].double() @ kk.t() * scale).masked_fill(~seen, -math.inf)
+            lse[rows, h] = torch.logsumexp(s, -1)
+            p = torch.where(seen, torch.softmax(s, -1), 0.0)
+            # a value that is not a number reaches only the rows that see it
+            bad = torch.isnan(vv)
+            for o, x in ((out, vv), (size, vv.abs())):
+                o[rows, h] = p @ x.masked_fill(bad, 0.0) + torch.where(seen.double() @ bad.double() > 0, math.nan, 0.0)
     return out, lse, size
 
 

@@ -340,6 +340,48 @@ def test_not_finite_keys_and_values_stay_where_they_are_seen(news):
     assert torch.isfinite(out[:-1]).all()
 
 
+PROMPTS = [([1000], [1000]), ([2500], [70]), ([129, 1, 640, 0, 257], [129, 1, 500, 0, 128]), ([40], [100]), ([3, 900], [70, 300]),
+           ([130, 130, 130, 130], [127, 128, 129, 130]), ([5000], [33])]
+
+
+@pytest.mark.parametrize("H,K,D,page", [(8, 1, 64, 16), (16, 2, 128, 16), (4, 4, 128, 64), (10, 2, 256, 32), (7, 1, 256, 16), (128, 1, 128, 16),
+                                        (130, 1, 64, 16)])
+@pytest.mark.parametrize("lens,news", PROMPTS)
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompts(H, K, D, page, lens, news, window):
+    cache, table, ln, st, q, keys, values, starts = make(lens, news, H, K, D, page, seed=H + D)
+    out, lse = A.kv4_attention(q, cache, table, ln, st, max(news), window=window, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, window, D ** -0.5))
+
+
+@pytest.mark.parametrize("most", [1, 1000])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-3])
+def test_other_scales_and_a_bound_that_is_too_low_or_too_high(most, scale):
+    """The bound chooses kernels only; a negative scale prefers what is least alike, a zero scale weighs all the same."""
+    H, K, D = 8, 2, 128
+    cache, table, ln, st, q, keys, values, starts = make([300, 90], [120, 3], H, K, D, 16, seed=9)
+    out, lse = A.kv4_attention(q, cache, table, ln, st, most, scale=scale, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, 0, scale))
+
+
+@pytest.mark.parametrize("count", [1, 40, 200])
+def test_many_values_that_are_not_numbers_in_a_prompt(count):
+    """Groups that are not numbers at several places of a prompt: the rows before each do not see it, with a window neither do
+    those far behind it."""
+    H, K, D, n = 2, 1, 128, 400
+    cache, table, ln, st, q, _, _, starts = make([n, n], [n, 300], H, K, D, 16, seed=4)
+    k, v = randn((n, K, D), 31), randn((n, K, D), 32)
+    v[torch.arange(count, device=DEV) + 150, 0, 70] = math.inf
+    i = torch.arange(n, device=DEV)
+    for b in range(2):
+        A.kv4_append(k, v if b == 0 else k, cache, table[b].long()[i // 16] * 16 + i % 16)
+    keys, values = [ref.quantised(k)] * 2, [ref.quantised(v), ref.quantised(k)]
+    close(A.kv4_attention(q, cache, table, ln, st, n), None, ref.attention(q, keys, values, starts, 0, D ** -0.5))
+    if count <= 40:
+        got = A.kv4_attention(q, cache, table, ln, st, n, window=90)
+        close(got, None, ref.attention(q, keys, values, starts, 90, D ** -0.5))
+
+
 def test_attention_out_strides_streams_and_graphs():
     H, K, D = 8, 2, 128
     cache, table, ln, st, q, keys, values, starts = make([300, 65, 900], [1, 1, 1], H, K, D, 16, seed=6)

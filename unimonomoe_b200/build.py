@@ -101,7 +101,7 @@ def build_variant(variant: str, force: bool = False, verbose: bool = False) -> s
 
 
 ATTENTION = os.path.join(CSRC, "attention")
-ATTENTION_SOURCES = ["batch_plan.cu", "qk_norm_rope.cu", "kv4_store.cu", "kv4_decode.cu"]
+ATTENTION_SOURCES = ["batch_plan.cu", "qk_norm_rope.cu", "kv4_store.cu", "kv4_attention.cu", "kv4_decode.cu", "kv4_prompt.cu"]
 
 
 def attention_lib_path() -> str:

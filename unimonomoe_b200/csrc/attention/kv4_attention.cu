@@ -1,0 +1,52 @@
+// Entry of the attention over the 4-bit cache: checks, and which kernels are launched.
+#include "kv4_attention.cuh"
+
+namespace mono {
+namespace kv4 {
+// Query rows for a KV head up to which a request goes to the kernel of few rows.
+constexpr int kSplitRows = 64;
+}  // namespace kv4
+}  // namespace mono
+
+extern "C" size_t mono_attn_workspace_bytes(void) {
+  const size_t a = mono::kv4::decode_partial_floats(), b = mono::kv4::prompt_partial_floats();
+  return MONO_ATTN_COUNTERS * sizeof(uint32_t) + (a > b ? a : b) * sizeof(float);
+}
+
+extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const uint8_t* cache,
+                                       int64_t num_pages, int page_size, const int32_t* block_table, int table_width,
+                                       const int32_t* seq_lens, const int32_t* query_start, int batch, int tokens,
+                                       int max_query_len, int q_heads, int kv_heads, int head_dim, float scale, int window,
+                                       void* out, float* lse, void* workspace, size_t workspace_bytes, uint32_t* status,
+                                       mono_attn_stream_t stream) {
+  using namespace mono::kv4;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
+  if (batch < 0 || tokens < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || table_width < 1 || num_pages < 1 ||
+      window < 0 || max_query_len < 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+    return MONO_ATTN_BAD_SIZE;
+  if (batch == 0 || tokens == 0) return 0;
+  if (!q || !cache || !block_table || !seq_lens || !query_start || !out || !workspace || !status) return MONO_ATTN_NULL;
+  if (workspace_bytes < mono_attn_workspace_bytes()) return MONO_ATTN_WORKSPACE;
+  AttnArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.cache = cache;
+  a.table = block_table; a.seq_lens = seq_lens; a.query_start = query_start;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.counters = static_cast<uint32_t*>(workspace);
+  a.partial = reinterpret_cast<float*>(a.counters + MONO_ATTN_COUNTERS);
+  a.status = status;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.num_pages = num_pages;
+  a.tokens = tokens; a.batch = batch; a.width = table_width; a.hq = q_heads; a.hk = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.shift = __builtin_ctz(page_size);
+  a.window = window;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  // max_query_len is only a bound: without the kernel of many rows the other one takes every request
+  const int64_t most = static_cast<int64_t>(max_query_len < tokens ? max_query_len : tokens) * a.group;
+  const bool many = most > kSplitRows && a.group <= 128;
+  a.split_rows = many ? kSplitRows : INT32_MAX;
+  if (const int rc = decode(a, head_dim, most > kSplitRows ? kSplitRows : static_cast<int>(most), stream)) return rc;
+  return many ? prompt(a, head_dim, stream) : 0;
+}

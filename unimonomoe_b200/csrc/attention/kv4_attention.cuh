@@ -51,6 +51,12 @@ __device__ __forceinline__ int page_of(const AttnArgs& a, int b, int col) {
   return 0;
 }
 
+// The two kernels: requests of up to a.split_rows query rows for a KV head, and those of more.
+int decode(const AttnArgs& a, int head_dim, int rows, cudaStream_t stream);
+int prompt(const AttnArgs& a, int head_dim, cudaStream_t stream);
+size_t decode_partial_floats();
+size_t prompt_partial_floats();
+
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

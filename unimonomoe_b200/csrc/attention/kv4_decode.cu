@@ -565,8 +565,7 @@ int launch(const AttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 namespace kv4 {
-// Query rows of a request up to which this kernel takes it, where the other one is there too.
-int decode_rows() { return 1 << 30; }
+size_t decode_partial_floats() { return static_cast<size_t>(MONO_ATTN_COUNTERS) * 2 * 16 * (128 + 2); }   // 16 rows of 128 dims, or 8 of 256
 int decode(const AttnArgs& a, int head_dim, int rows, cudaStream_t stream) {
   if (head_dim == 256) return launch<256, 1>(a, stream);
   if (head_dim == 128) return rows <= 8 ? launch<128, 1>(a, stream) : launch<128, 2>(a, stream);
@@ -574,44 +573,3 @@ int decode(const AttnArgs& a, int head_dim, int rows, cudaStream_t stream) {
 }
 }  // namespace kv4
 }  // namespace mono
-
-extern "C" size_t mono_attn_workspace_bytes(void) {
-  // counters of all CTAs, and two partial states for each: at most 16 rows of 128 dims or 8 of 256, or of 64
-  return MONO_ATTN_COUNTERS * 4 + static_cast<size_t>(MONO_ATTN_COUNTERS) * 2 * 16 * (128 + 2) * 4;
-}
-
-extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const uint8_t* cache,
-                                       int64_t num_pages, int page_size, const int32_t* block_table, int table_width,
-                                       const int32_t* seq_lens, const int32_t* query_start, int batch, int tokens,
-                                       int max_query_len, int q_heads, int kv_heads, int head_dim, float scale, int window,
-                                       void* out, float* lse, void* workspace, size_t workspace_bytes, uint32_t* status,
-                                       mono_attn_stream_t stream) {
-  using namespace mono;
-  using namespace mono::kv4;
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
-  if (batch < 0 || tokens < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || table_width < 1 || num_pages < 1 ||
-      window < 0 || max_query_len < 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
-    return MONO_ATTN_BAD_SIZE;
-  if (batch == 0 || tokens == 0) return 0;
-  if (!q || !cache || !block_table || !seq_lens || !query_start || !out || !workspace || !status) return MONO_ATTN_NULL;
-  if (workspace_bytes < mono_attn_workspace_bytes()) return MONO_ATTN_WORKSPACE;
-  AttnArgs a{};
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.cache = cache;
-  a.table = block_table; a.seq_lens = seq_lens; a.query_start = query_start;
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.lse = lse;
-  a.counters = static_cast<uint32_t*>(workspace);
-  a.partial = reinterpret_cast<float*>(a.counters + MONO_ATTN_COUNTERS);
-  a.status = status;
-  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
-  a.num_pages = num_pages;
-  a.tokens = tokens; a.batch = batch; a.width = table_width; a.hq = q_heads; a.hk = kv_heads;
-  a.group = q_heads / kv_heads;
-  a.shift = __builtin_ctz(page_size);
-  a.window = window;
-  a.split_rows = INT32_MAX;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t rows = static_cast<int64_t>(max_query_len) * a.group;
-  return decode(a, head_dim, rows > 1 << 20 ? 1 << 20 : static_cast<int>(rows), stream);
-}

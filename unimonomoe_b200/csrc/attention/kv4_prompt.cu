@@ -1,0 +1,808 @@
+// Attention over the 4-bit cache for requests of many query rows: chunks and whole prompts.
+//
+// A CTA takes 128 query rows (all query heads of one KV head for 128 / group tokens) against tiles of 128 keys:
+//   S = Q K^T and O += P V on tcgen05 (bf16, fp32 sums in tensor memory), the softmax between them in registers.
+// Eighteen warps, one CTA on an SM:
+//   8 turn codes into operands: a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
+//     128-byte-swizzled layout, keys for S with dims along K, values as they are (dims along N). A block's words are what a lane
+//     stores as 16 bytes, eight dims in the order 0 4 1 5 2 6 3 7 in which masking leaves them; queries are stored in the same
+//     order, and the output is put back from it.
+//   1 lists the segments of the CTA's run, a few ahead of the others.
+//   1 issues the products: S of tile j + 1 before O of tile j, so that the tensor cores have work while tile j is in the softmax.
+//   8 do the softmax: two threads to a row, half of the keys each; the row's maximum goes through shared memory. P goes back to
+//     tensor memory over S. O is only rescaled when a row's maximum has grown by more than 2^8 (by the warps of that row
+//     themselves; sums are fp32, so nothing is lost by a maximum that is a little old).
+// Work is cut into equal runs of tiles, one to a CTA; items that lie in several runs are joined as in kv4_decode.cu.
+// All waits are bounded.
+#include <climits>
+#include "kv4_attention.cuh"
+#include "../ptx_sm100.cuh"
+
+namespace mono {
+namespace {
+
+using namespace kv4;
+
+constexpr int kSoftmaxWarps = 8, kFillWarps = 8, kMmaWarp = 16, kPlanWarp = 17;
+constexpr int kThreads = 20 * 32;          // two warps are only there to make up a warpgroup
+// registers of a thread: 96 at launch; softmax, filling, the rest: 256 * 136 + 256 * 72 + 128 * 56 <= 640 * 96
+constexpr int kSoftmaxRegs = 136, kFillRegs = 72, kRestRegs = 56;
+constexpr int kSegs = 4;                    // segments that the roles may be apart
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
+constexpr float kLow = -1e38f, kRoom = 8.0f;
+constexpr int kNanList = 64;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+template <int D>
+struct Shape {
+  static constexpr int NG = D / kGroup;
+  static constexpr int Panels = D == 64 ? 1 : 2;        // of a slot
+  static constexpr int Slot = Panels * kPanel;
+  static constexpr int PerTile = NG / Panels;           // slots of a tile's keys, or of its values
+  static constexpr int Slots = D == 256 ? 5 : 6;
+  static constexpr int Q = NG * kPanel;
+  static constexpr int Part = kRows * (D + 2);          // floats of a CTA's state: output, maximum and sum
+};
+
+// Tiles [first, first + count) of keys for a row block: all query heads of a KV head for some tokens of a request.
+struct Segment {
+  int request, head, q_row, rows;           // first query row; query rows of the block
+  int place, end;                           // place of the first token; keys that any row sees
+  int first, count;
+  int c0, c1;                               // the CTAs that share the item: more than one where count is not all of it
+  int whole, more;
+};
+
+struct Control {
+  uint64_t seg_full[kSegs], seg_empty[kSegs];
+  uint64_t full[6], empty[6];               // ring slots
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2];
+  uint64_t o_done, o_all, o_free;           // a tile's products, a segment's; the segment's output has been read
+  uint32_t tmem, abort, last;
+  uint32_t nan_count;                       // value groups that are not numbers: key and group of the first kNanList of a segment,
+  int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
+  int found[2];
+  int wsum[20];
+  Segment seg[kSegs];
+  int32_t nan_list[kNanList];               // key * 16 + groups
+  float top[2][2][kRows];                   // of the two halves of a row, two tiles deep
+};
+
+template <int D>
+constexpr int smem_bytes() { return Shape<D>::Q + Shape<D>::Slots * Shape<D>::Slot + static_cast<int>(sizeof(Control)); }
+
+// sum of floor((a i + b) / m), i < n; a, b >= 0 (by Euclid's algorithm on a and m)
+__device__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
+    a %= m;
+    b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+// The row blocks of a request: `tb` tokens each, all query heads of a KV head.
+struct Item {
+  int place0, n, len, tb, window;
+  __device__ __forceinline__ int blocks() const { return (n + tb - 1) / tb; }
+  __device__ __forceinline__ int first_tile(int rb) const { return window > 0 ? max(place0 + rb * tb + 1 - window, 0) / kKeys : 0; }
+  __device__ __forceinline__ int seen(int rb) const { return min(len, max(place0 + min((rb + 1) * tb, n), 0)); }
+  // tiles of row block rb, at least one
+  __device__ __forceinline__ int tiles(int rb) const { return max(1, (seen(rb) + kKeys - 1) / kKeys - first_tile(rb)); }
+};
+
+__device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r) {
+  return {r.len - r.n, r.n * a.group > a.split_rows ? r.n : 0, r.len, kRows / a.group, a.window};
+}
+
+// Tiles of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
+// one only where the first queries have no place in the sequence.
+__device__ __forceinline__ int64_t tiles_before(const Item& it, int rb) {
+  int64_t sum = 0;
+  if (it.place0 < 0) {
+    for (int i = 0; i < rb; ++i) sum += it.tiles(i);
+    return sum;
+  }
+  const int full = min(rb, it.n / it.tb);                // blocks of tb tokens; a shorter one is the last
+  sum = floor_sum(full, kKeys, it.tb, static_cast<int64_t>(it.place0) + it.tb + kKeys - 1);
+  if (it.window > 0) {
+    const int64_t begin = static_cast<int64_t>(it.place0) + 1 - it.window;      // of the first row; blocks with a negative one begin at 0
+    const int64_t skip = begin < 0 ? min((-begin + it.tb - 1) / it.tb, static_cast<int64_t>(full)) : 0;
+    sum -= floor_sum(full - skip, kKeys, it.tb, max(begin + skip * it.tb, static_cast<int64_t>(0)));
+  }
+  if (rb > full) sum += it.tiles(full);
+  return sum;
+}
+
+// The segments of a CTA's run, one after another: tiles [t0, t1) of an item.
+struct Walk {
+  int b, head, rb, blocks, tiles, at, u, u1, t0, t1, i0;
+  Request r;
+  Item it;
+  __device__ __forceinline__ void load(const AttnArgs& a) {
+    r = request_of(a, b, false);
+    it = item_of(a, r);
+    blocks = it.blocks();
+  }
+  // Positions u in the unit space where item (b, head, rb) begins at `at`.
+  __device__ __forceinline__ void open() {
+    tiles = it.tiles(rb);
+    i0 = at;
+    t0 = u - at;
+    t1 = min(tiles, u1 - at);
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a) {   // false behind the run's end
+    u = at + t1;
+    if (u >= u1) return false;
+    at += tiles;
+    if (++rb == blocks) {
+      rb = 0;
+      if (++head == a.hk) {
+        head = 0;
+        do { ++b; load(a); } while (blocks == 0 && b + 1 < a.batch);
+      }
+    }
+    open();
+    return true;
+  }
+};
+
+// ---- waits
+// Phase `parity` of a barrier. One that does not come is reported, and from then on no such wait waits: every role runs through its
+// loop, whatever is in memory, and the launch ends. The segment list alone is always waited for, so that all roles run
+// through the same loops; nobody who keeps it waiting waits for anything else then.
+template <bool Always = false>
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Control& C, const AttnArgs& a) {
+  if (!mbar_try_wait(bar, parity)) {
+    const uint64_t t0 = globaltimer_ns();
+    volatile uint32_t* stop = &C.abort;
+    while (!mbar_try_wait(bar, parity)) {
+      if (!Always && *stop) break;
+      if (globaltimer_ns() - t0 > (Always ? 8 : 1) * kWaitNs) {
+        report(a.status, kWaitTimeout, blockIdx.x);
+        *stop = 1u;
+        break;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// Reads the segments in order.
+struct Reader {
+  uint32_t n = 0;
+  __device__ __forceinline__ Segment& take(Control& C, const AttnArgs& a) {
+    wait<true>(&C.seg_full[n % kSegs], (n / kSegs) & 1, C, a);
+    return C.seg[n % kSegs];
+  }
+  __device__ __forceinline__ void done(Control& C) {    // this warp has no more use for it
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&C.seg_empty[n % kSegs]);
+    ++n;
+  }
+};
+
+__device__ __forceinline__ uint32_t times2(uint32_t x, uint32_t s) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&s));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Eight codes of a word times the scale (in both halves), dims 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ uint4 values8(uint32_t w, uint32_t scale2) {
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t y = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u, off = 0x43084308u;
+    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
+    v[i] = times2(*reinterpret_cast<const uint32_t*>(&c), scale2);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// B operand with N along the rows of 128 bytes: 64 dims, then the next panel; 8 keys to 1024 bytes along K.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t at) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((at & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(kPanel >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+      "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+      "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+constexpr uint32_t kSCol = 0, kOCol = 256;
+
+// ---- the eight warps that fill the ring
+template <int D>
+__device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Control& C, int warp, int lane) {
+  using S = Shape<D>;
+  constexpr int NG = S::NG, NV = D / 64;                // 16-byte pieces of a lane in a block's codes
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q;
+  const int per_page_shift = a.shift - 4;
+  uint32_t slot = 0, round = 0;                         // ring position
+  Reader reader;
+  struct Raw {
+    uint4 code[NV];
+    uint32_t scale[4][(NG + 1) / 2];                    // two tokens of a key block, four of a value block
+  };
+  for (;;) {
+    const Segment& w = reader.take(C, a);
+    const uint32_t seg = reader.n;
+    // queries
+    wait(&C.q_empty, (seg & 1) ^ 1, C, a);
+    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    const int head = w.head, request = w.request;
+    for (int i = 0; i < 16; ++i) {
+      const int row = warp * 16 + i;
+      if (lane < D / 8) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < w.rows) {
+          v = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + row / a.group) * a.q_ts + (head * a.group + row % a.group) * a.q_hs + 8 * lane));
+          v = make_uint4(__byte_perm(v.x, v.z, 0x5410) ^ flip, __byte_perm(v.x, v.z, 0x7632) ^ flip,
+                         __byte_perm(v.y, v.w, 0x5410) ^ flip, __byte_perm(v.y, v.w, 0x7632) ^ flip);
+        }
+        sts128(q_at + (lane >> 3) * kPanel + row * 128 + (((lane & 7) ^ (row & 7)) << 4), v);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&C.q_full);
+
+    const int first = w.first, count = w.count, end = w.end, more = w.more;
+    auto load = [&](int j, bool value, Raw& x) {        // block `warp` of tile first + j
+      const int key = (first + j) * kKeys + warp * 16;
+      if (key < end) {
+        const int blk = key >> 4;
+        const int pg = page_of(a, request, blk >> per_page_shift);
+        const uint8_t* p = a.cache + (((static_cast<int64_t>(pg) * a.hk + head) << per_page_shift) + (blk & ((1 << per_page_shift) - 1))) * block_bytes(D);
+        const uint8_t* c = p + (value ? 8 * D : 0) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x.code[i] = __ldg(reinterpret_cast<const uint4*>(c + i * 512));
+#pragma unroll
+        for (int i = 0; i < (value ? 4 : 2); ++i) {
+          const int tok = value ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i;
+          const uint8_t* sc = p + 16 * D + tok * 4 * NG + (value ? 2 * NG : 0);
+          if constexpr (NG == 1) {
+            x.scale[i][0] = __ldg(reinterpret_cast<const uint16_t*>(sc));
+          } else if constexpr (NG == 2) {
+            x.scale[i][0] = __ldg(reinterpret_cast<const uint32_t*>(sc));
+          } else {
+            const uint2 y = __ldg(reinterpret_cast<const uint2*>(sc));
+            x.scale[i][0] = y.x;
+            x.scale[i][1] = y.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x.code[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < (NG + 1) / 2; ++k) x.scale[i][k] = 0;
+      }
+    };
+    auto both = [](uint32_t x, int gi) { return gi & 1 ? __byte_perm(x, x, 0x3232) : __byte_perm(x, x, 0x1010); };
+    auto store = [&](int j, bool value, const Raw& x) {
+      const int key0 = (first + j) * kKeys + warp * 16;
+#pragma unroll
+      for (int s = 0; s < S::PerTile; ++s) {
+        const uint32_t base = ring + slot * S::Slot;
+        wait(&C.empty[slot], (round & 1) ^ 1, C, a);
+        if (!value) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = warp * 16 + g + 8 * h;
+            uint32_t wd[2 * S::Panels];
+            if constexpr (D == 64) {
+              wd[0] = h ? x.code[0].z : x.code[0].x;
+              wd[1] = h ? x.code[0].w : x.code[0].y;
+            } else {
+              const uint4& c = x.code[h * (NV / 2) + s];
+              wd[0] = c.x; wd[1] = c.y; wd[2] = c.z; wd[3] = c.w;
+            }
+#pragma unroll
+            for (int p = 0; p < S::Panels; ++p) {
+              const int gi = s * S::Panels + p;
+              const uint32_t sc = both(x.scale[h][gi >> 1], gi);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) sts128(base + p * kPanel + row * 128 + (((2 * t + k) ^ g) << 4), values8(wd[2 * p + k], sc));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int tok = 2 * t + (u & 1) + 8 * (u >> 1), row = warp * 16 + tok;
+            const bool inside = key0 + tok < end;
+#pragma unroll
+            for (int p = 0; p < S::Panels; ++p) {
+              const int gi = s * S::Panels + p;
+              uint32_t wd;
+              if constexpr (D == 64) {
+                wd = u == 0 ? x.code[0].x : u == 1 ? x.code[0].y : u == 2 ? x.code[0].z : x.code[0].w;
+              } else if constexpr (D == 128) {
+                const uint4& c = x.code[u >> 1];
+                wd = u & 1 ? (gi ? c.w : c.z) : (gi ? c.y : c.x);
+              } else {
+                const uint4& c = x.code[u];
+                wd = gi == 0 ? c.x : gi == 1 ? c.y : gi == 2 ? c.z : c.w;
+              }
+              uint32_t sc = both(x.scale[u][gi >> 1], gi);
+              // behind the sequence there may be anything; a group that is not a number must not reach the rows that do not see it
+              if (!inside) sc = 0;
+              const bool nan = (sc & 0x7FFFu) > 0x7F80u;
+              if (__any_sync(0xFFFFFFFFu, nan)) {
+                wait(&C.o_free, (seg & 1) ^ 1, C, a);     // the list of the segment before has been read
+                if (nan) sc = 0;
+                if (nan && g == 0) {
+                  atomicMin(&C.nan_first[gi], key0 + tok);
+                  atomicMax(&C.nan_last[gi], key0 + tok);
+                  const uint32_t at = atomicAdd(&C.nan_count, 1u);
+                  if (at < kNanList) C.nan_list[at] = ((first + j) * kKeys + row) * 4 + gi;
+                }
+              }
+              sts128(base + p * kPanel + row * 128 + ((g ^ (row & 7)) << 4), values8(wd, sc));
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&C.full[slot]);
+        if (++slot == S::Slots) { slot = 0; ++round; }
+      }
+    };
+    Raw k, v;
+    load(0, false, k);
+    load(0, true, v);
+    store(0, false, k);
+    if (count > 1) load(1, false, k);
+    for (int j = 0; j < count; ++j) {
+      if (j + 1 < count) {
+        store(j + 1, false, k);
+        if (j + 2 < count) load(j + 2, false, k);
+      }
+      store(j, true, v);
+      if (j + 1 < count) load(j + 1, true, v);
+    }
+    reader.done(C);
+    if (!more) break;
+  }
+}
+
+// ---- the warp that issues the products
+template <int D>
+__device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Control& C) {
+  using S = Shape<D>;
+  const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q, tmem = C.tmem;
+  constexpr uint32_t qk = umma_idesc_bf16_f32(kRows, kKeys), pv = umma_idesc_bf16_f32(kRows, S::Panels * 64) | (1u << 16);
+  uint32_t slot = 0, round = 0, n = 0;                  // ring position; tiles so far
+  Reader reader;
+  auto release = [&]() {
+    if (elect_one_sync()) umma_commit(&C.empty[slot]);
+    if (++slot == S::Slots) { slot = 0; ++round; }
+  };
+  auto scores = [&](uint32_t tile) {
+#pragma unroll
+    for (int s = 0; s < S::PerTile; ++s) {
+      wait(&C.full[slot], round & 1, C, a);
+      tc_fence_after();
+      const uint32_t base = ring + slot * S::Slot;
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int p = 0; p < S::Panels; ++p)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem + kSCol + (tile & 1) * kKeys, umma_desc_sw128(q_at + (s * S::Panels + p) * kPanel + k * 32),
+                      umma_desc_sw128(base + p * kPanel + k * 32), qk, (s | p | k) != 0);
+      }
+      __syncwarp();
+      release();
+    }
+    if (elect_one_sync()) umma_commit(&C.s_full[tile & 1]);
+    __syncwarp();
+  };
+  for (;;) {
+    const Segment& w = reader.take(C, a);
+    const uint32_t seg = reader.n;
+    const int count = w.count, more = w.more;
+    reader.done(C);
+    wait(&C.q_full, seg & 1, C, a);
+    scores(n);
+    for (int j = 0; j < count; ++j) {
+      if (j + 1 < count) scores(n + 1);
+      if (j + 2 >= count && (j + 1 < count || count == 1)) {  // the last scores of the segment are on their way
+        if (elect_one_sync()) umma_commit(&C.q_empty);
+        __syncwarp();
+      }
+      if (j == 0) wait(&C.o_free, (seg & 1) ^ 1, C, a);
+      wait(&C.p_full[n & 1], (n >> 1) & 1, C, a);
+      tc_fence_after();
+#pragma unroll
+      for (int s = 0; s < S::PerTile; ++s) {
+        wait(&C.full[slot], round & 1, C, a);
+        tc_fence_after();
+        const uint32_t base = ring + slot * S::Slot;
+        if (elect_one_sync()) {
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_bf16_ts(tmem + kOCol + s * S::Panels * 64, tmem + kSCol + (n & 1) * kKeys + k * 8, desc_mn_sw128(base + k * 2048), pv,
+                         (j | k) != 0);
+        }
+        __syncwarp();
+        release();
+      }
+      if (elect_one_sync()) {
+        umma_commit(&C.o_done);
+        if (j + 1 == count) umma_commit(&C.o_all);
+      }
+      __syncwarp();
+      ++n;
+    }
+    if (!more) {
+      wait(&C.o_all, seg & 1, C, a);        // nothing is in flight when tensor memory is given back
+      break;
+    }
+  }
+}
+
+// ---- the eight warps of the softmax
+template <int D>
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int warp, int lane) {
+  using S = Shape<D>;
+  constexpr int Half = D / 2;                           // output columns of a thread
+  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+  const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);     // the queries carry its sign; not 0, for -inf times it stays -inf
+  uint32_t n = 0;
+  Reader reader;
+  for (;;) {
+    const Segment& w = reader.take(C, a);
+    const int first = w.first, count = w.count, more = w.more;
+    const bool real = row < w.rows;
+    const int place = w.place + row / a.group, hi = real ? place + 1 : 0, lo = a.window > 0 ? place + 1 - a.window : 0;
+    // every row of the block sees all of [clear_lo, clear_hi)
+    const int clear_hi = w.place + 1, clear_lo = a.window > 0 ? w.place + (w.rows - 1) / a.group + 1 - a.window : 0;
+    float m = kLow, l = 0.0f;
+    for (int j = 0; j < count; ++j, ++n) {
+      const int key0 = (first + j) * kKeys;
+      wait(&C.s_full[n & 1], (n >> 1) & 1, C, a);
+      tc_fence_after();
+      uint32_t raw[2][32];
+      tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64, raw[0]);
+      tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64 + 32, raw[1]);
+      tmem_ld_wait();
+      float s[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
+      if (key0 < clear_lo || key0 + kKeys > clear_hi) {
+        const int from = lo - key0 - half * 64, to = hi - key0 - half * 64;
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i < from || i >= to) s[i] = -INFINITY;
+      }
+      float x = s[0], y = s[1];
+#pragma unroll
+      for (int i = 2; i < 64; i += 2) {
+        x = fmaxf(x, s[i]);
+        y = fmaxf(y, s[i + 1]);
+      }
+      x = fmaxf(x, y);
+      C.top[n & 1][half][row] = x;
+      tc_fence_before();
+      named_bar_sync(1 + quarter, 64);      // the other half's maximum; and both halves of S have been read before P goes over it
+      x = fmaxf(x, C.top[n & 1][half ^ 1][row]) * scale;
+      if (__any_sync(0xFFFFFFFFu, x > m + kRoom)) {
+        const float to = fmaxf(m, x), by = ex2(m - to);
+        m = to;
+        l *= by;
+        if (j > 0) {
+          wait(&C.o_done, (n - 1) & 1, C, a);   // at most one tile behind: the scores of this one came after the products of n - 2
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < Half; i += 32) {
+            uint32_t o[32];
+            tmem_ld32(lanes + kOCol + half * Half + i, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+            tmem_st32(lanes + kOCol + half * Half + i, o);
+          }
+        }
+      }
+      uint32_t p[32];
+      float sum = 0.0f, sum2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float e0 = ex2(fmaf(s[2 * i], scale, -m)), e1 = ex2(fmaf(s[2 * i + 1], scale, -m));
+        sum += e0;
+        sum2 += e1;
+        p[i] = pack_bf16x2(e0, e1);
+      }
+      l += sum + sum2;
+      tmem_st32(lanes + kSCol + (n & 1) * kKeys + half * 32, p);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&C.p_full[n & 1]);
+    }
+    // the two halves' sums
+    C.top[n & 1][half][row] = l;
+    named_bar_sync(1 + quarter, 64);
+    l += C.top[n & 1][half ^ 1][row];
+    named_bar_sync(1 + quarter, 64);        // read before the next segment's first maximum
+
+    wait(&C.o_all, reader.n & 1, C, a);
+    tc_fence_after();
+    // groups that are not numbers and that this row sees
+    uint32_t nans = 0;
+    const uint32_t listed = *static_cast<volatile uint32_t*>(&C.nan_count);
+    if (listed) {
+      for (uint32_t i = 0; i < min(listed, static_cast<uint32_t>(kNanList)); ++i) {
+        const int key = C.nan_list[i] >> 2;
+        if (key >= lo && key < hi) nans |= 1u << (C.nan_list[i] & 3);
+      }
+      // more than the list holds: all keys between the first and the last count (which only a window can tell apart)
+      if (listed > kNanList)
+        for (int gi = 0; gi < S::NG; ++gi)
+          if (*static_cast<volatile int*>(&C.nan_first[gi]) < hi && *static_cast<volatile int*>(&C.nan_last[gi]) >= lo) nans |= 1u << gi;
+    }
+    const bool whole = w.whole;
+    const int c0 = w.c0, c1 = w.c1;
+    float* mine = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
+    auto write_out = [&](int rw, int d, const float (&x)[8], float inv) {       // eight dims, in the order of the operands
+      const int tk = w.q_row + rw / a.group, hd = w.head * a.group + rw % a.group;
+      float y[8] = {x[0] * inv, x[2] * inv, x[4] * inv, x[6] * inv, x[1] * inv, x[3] * inv, x[5] * inv, x[7] * inv};
+      *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(tk) * a.hq + hd) * D + d) = pack_bf16x8(y);
+    };
+    auto inverse = [](float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; };
+    auto write_lse = [&](int rw, float mx, float sum) {
+      const int tk = w.q_row + rw / a.group, hd = w.head * a.group + rw % a.group;
+      a.lse[static_cast<int64_t>(tk) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+    };
+    const float inv = inverse(l);
+#pragma unroll
+    for (int i = 0; i < Half; i += 32) {
+      uint32_t o[32];
+      tmem_ld32(lanes + kOCol + half * Half + i, o);
+      tmem_ld_wait();
+      if (real) {
+        const bool nan = nans >> ((half * Half + i) >> 6) & 1u;
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          float x[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) x[c] = nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[k + c]);
+          if (whole) {
+            write_out(row, half * Half + i + k, x, inv);
+          } else {
+            __stcg(reinterpret_cast<float4*>(mine + row * D + half * Half + i + k), make_float4(x[0], x[1], x[2], x[3]));
+            __stcg(reinterpret_cast<float4*>(mine + row * D + half * Half + i + k + 4), make_float4(x[4], x[5], x[6], x[7]));
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    named_bar_sync(5, 256);                 // everyone has read the list of this segment
+    if (warp == 0 && lane < 4) { C.nan_count = 0; C.nan_first[lane] = INT_MAX; C.nan_last[lane] = -1; }
+    __syncwarp();
+    mbar_arrive(&C.o_free);
+    if (whole) {
+      if (real && half == 0 && a.lse) write_lse(row, m, l);
+    } else {
+      if (real && half == 0) __stcg(reinterpret_cast<float2*>(mine + kRows * D + 2 * row), make_float2(m, l));
+      __threadfence();
+      named_bar_sync(5, 256);
+      if (warp == 0 && lane == 0) {
+        const uint32_t before = atomicAdd(a.counters + c0, 1u);
+        C.last = before == static_cast<uint32_t>(c1 - c0);
+        if (C.last) a.counters[c0] = 0;
+        __threadfence();
+      }
+      named_bar_sync(5, 256);
+      if (C.last) {
+        for (int idx = warp * 32 + lane; idx < w.rows * (D / 8); idx += 256) {
+          const int rw = idx / (D / 8), d = idx % (D / 8) * 8;
+          float mx = kLow, sum = 0.0f, x[8] = {};
+          for (int c = c0; c <= c1; ++c) {
+            const float* from = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + kRows * D + 2 * rw));
+            const float4 p0 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d)), p1 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d + 4));
+            const float to = fmaxf(mx, ms.x), old = ex2(mx - to), by = ex2(ms.x - to);
+            mx = to;
+            sum = fmaf(ms.y, by, sum * old);
+            x[0] = fmaf(p0.x, by, x[0] * old); x[1] = fmaf(p0.y, by, x[1] * old);
+            x[2] = fmaf(p0.z, by, x[2] * old); x[3] = fmaf(p0.w, by, x[3] * old);
+            x[4] = fmaf(p1.x, by, x[4] * old); x[5] = fmaf(p1.y, by, x[5] * old);
+            x[6] = fmaf(p1.z, by, x[6] * old); x[7] = fmaf(p1.w, by, x[7] * old);
+          }
+          write_out(rw, d, x, inverse(sum));
+          if (d == 0 && a.lse) write_lse(rw, mx, sum);
+        }
+      }
+    }
+    reader.done(C);
+    if (!more) break;
+  }
+}
+
+// ---- the warp that lists the segments
+__device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per, int u0, int u1, int lane) {
+  Walk w;
+  w.b = C.found[0];
+  w.load(a);
+  w.u = u0;
+  w.u1 = u1;
+  {  // the head and row block that u0 lies in: the lanes bisect together, 32 places at a time
+    const int64_t each = tiles_before(w.it, w.blocks);
+    const int64_t off = u0 - C.found[1];
+    w.head = static_cast<int>(off / each);
+    const int64_t rest = off - w.head * each;
+    int low = 0, high = w.blocks;           // tiles_before(low) <= rest < tiles_before(high)
+    while (high - low > 1) {
+      const int step = (high - low + 31) / 32, at = min(low + lane * step, high);
+      const bool below = at < high && tiles_before(w.it, at) <= rest;
+      const int k = 31 - __clz(static_cast<int>(__ballot_sync(0xFFFFFFFFu, below)));    // lane 0's place is always below
+      high = min(low + (k + 1) * step, high);
+      low += k * step;
+    }
+    w.rb = low;
+    w.at = C.found[1] + static_cast<int>(w.head * each + tiles_before(w.it, low));
+  }
+  w.open();
+  for (uint32_t n = 0;; ++n) {
+    wait<true>(&C.seg_empty[n % kSegs], ((n / kSegs) & 1) ^ 1, C, a);
+    Walk v = w;
+    const bool more = w.next(a);
+    if (lane == 0) {
+      const int tok = v.rb * v.it.tb;
+      C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
+                          v.it.first_tile(v.rb) + v.t0, v.t1 - v.t0, v.i0 / per, (v.i0 + v.tiles - 1) / per,
+                          v.t1 - v.t0 == v.tiles, more};
+      mbar_arrive(&C.seg_full[n % kSegs]);
+    }
+    if (!more) break;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
+  using S = Shape<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Control& C = *reinterpret_cast<Control*>(smem + S::Q + S::Slots * S::Slot);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // this CTA's run of all tiles
+  const int chunk = (a.batch + kThreads - 1) / kThreads;
+  int mine = 0;
+  for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
+    const Item it = item_of(a, request_of(a, b, blockIdx.x == 0));
+    mine += static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) C.wsum[warp] = upto;
+  __syncthreads();
+  int total = 0;
+  for (int i = 0; i < kThreads / 32; ++i) {
+    if (i < warp) upto += C.wsum[i];
+    total += C.wsum[i];
+  }
+  const int per = (total + gridDim.x - 1) / static_cast<int>(gridDim.x);
+  const int u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  if (u0 >= u1) return;                     // the whole CTA, before anything is allocated
+  if (upto - mine <= u0 && u0 < upto) {
+    int at = upto - mine, b = tid * chunk;
+    for (;; ++b) {
+      const Item it = item_of(a, request_of(a, b, false));
+      const int cost = static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
+      if (at + cost > u0) break;
+      at += cost;
+    }
+    C.found[0] = b;
+    C.found[1] = at;
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&C.tmem, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S::Slots; ++i) { mbar_init(&C.full[i], kFillWarps); mbar_init(&C.empty[i], 1); }
+    for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + 1); }
+    mbar_init(&C.q_full, kFillWarps);
+    mbar_init(&C.q_empty, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 32); }
+    mbar_init(&C.o_done, 1);
+    mbar_init(&C.o_all, 1);
+    mbar_init(&C.o_free, kSoftmaxWarps * 32);
+    mbar_init_fence();
+    C.abort = 0;
+    C.nan_count = 0;
+    for (int i = 0; i < 4; ++i) { C.nan_first[i] = INT_MAX; C.nan_last[i] = -1; }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  if (warp < kSoftmaxWarps) {
+    reg_inc<kSoftmaxRegs>();
+    softmax_role<D>(a, C, warp, lane);
+  } else if (warp < kSoftmaxWarps + kFillWarps) {
+    reg_dec<kFillRegs>();
+    fill_role<D>(a, smem, C, warp - kSoftmaxWarps, lane);
+  } else {
+    reg_dec<kRestRegs>();
+    if (warp == kMmaWarp) mma_role<D>(a, smem, C);
+    else if (warp == kPlanWarp) plan_role(a, C, per, u0, u1, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (C.abort) {                            // products may be in flight that nobody has waited for; they take microseconds
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000) __nanosleep(10000);
+  }
+  if (warp == kMmaWarp) tmem_dealloc(C.tmem, 512);
+}
+
+template <int D>
+int launch(const AttnArgs& a, cudaStream_t stream) {
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev >= 64 || !ready[dev]) {
+    e = cudaFuncSetAttribute(prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (dev < 64) ready[dev] = true;
+  }
+  prompt_kernel<D><<<MONO_ATTN_SMS, kThreads, smem_bytes<D>(), stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+static_assert(smem_bytes<256>() <= 232448 && smem_bytes<128>() <= 232448, "shared memory of an SM");
+
+}  // namespace
+
+namespace kv4 {
+size_t prompt_partial_floats() { return static_cast<size_t>(MONO_ATTN_SMS) * 2 * Shape<256>::Part; }
+int prompt(const AttnArgs& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? launch<64>(a, stream) : head_dim == 128 ? launch<128>(a, stream) : launch<256>(a, stream);
+}
+}  // namespace kv4
+}  // namespace mono
