@@ -192,20 +192,42 @@ struct Reader {
   }
 };
 
-__device__ __forceinline__ uint32_t times2(uint32_t x, uint32_t s) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&s));
+__device__ __forceinline__ uint32_t fma2(uint32_t x, uint32_t y, uint32_t z) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&z));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Eight codes of a word times the scale (in both halves), dims 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ uint4 values8(uint32_t w, uint32_t scale2) {
+__device__ __forceinline__ uint32_t add2(uint32_t x, uint32_t y) {
+  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A scale in both halves, and -24 times it (exact: five bits by two).
+struct Scale {
+  uint32_t s, n;
+  __device__ __forceinline__ Scale(uint32_t word, int gi) {
+    s = gi & 1 ? __byte_perm(word, word, 0x3232) : __byte_perm(word, word, 0x1010);
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&s), __float2bfloat162_rn(-24.0f));
+    n = *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+// Eight codes of a word times their scale, dims 0 4 1 5 2 6 3 7: a code c + 8 as the top four bits of the mantissa under the
+// exponent of 16 is 24 + c, and (24 + c) s - 24 s is exact in one fused multiply-add.
+__device__ __forceinline__ uint4 values8(uint32_t w, const Scale& s) {
   uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t y = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u, off = 0x43084308u;
-    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
-    v[i] = times2(*reinterpret_cast<const uint32_t*>(&c), scale2);
-  }
+  for (int i = 0; i < 4; ++i) v[i] = fma2(((i ? w >> (4 * i - 3) : w << 3) & 0x00780078u) | 0x41804180u, s.s, s.n);
   return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
+      "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
 }
 __device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -246,158 +268,201 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 constexpr uint32_t kSCol = 0, kOCol = 256;
 
 // ---- the eight warps that fill the ring
+// A lane's words and scales of a block of 16 tokens: of its keys (tokens g, g + 8), or of its values (2t, 2t+1, 2t+8, 2t+9).
+template <int D, bool VALUE>
+struct Raw {
+  static constexpr int NG = D / kGroup, Tok = VALUE ? 4 : 2, SW = (NG + 1) / 2;
+  uint4 code[NG];
+  uint32_t scale[Tok][SW];
+
+  // The block at p; null: one behind all keys, read as zeros.
+  __device__ __forceinline__ void load(const uint8_t* p, int g, int t, int lane) {
+    if (p == nullptr) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) code[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+#pragma unroll
+      for (int i = 0; i < Tok; ++i)
+#pragma unroll
+        for (int k = 0; k < SW; ++k) scale[i][k] = 0;
+      return;
+    }
+    const uint8_t* c = p + (VALUE ? 8 * D : 0) + lane * 16;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) code[i] = __ldg(reinterpret_cast<const uint4*>(c + i * 512));
+#pragma unroll
+    for (int i = 0; i < Tok; ++i) {
+      const int tok = VALUE ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i;
+      const uint8_t* sc = p + 16 * D + tok * 4 * NG + (VALUE ? 2 * NG : 0);
+      if constexpr (NG == 1) {
+        scale[i][0] = __ldg(reinterpret_cast<const uint16_t*>(sc));
+      } else if constexpr (NG == 2) {
+        scale[i][0] = __ldg(reinterpret_cast<const uint32_t*>(sc));
+      } else {
+        const uint2 y = __ldg(reinterpret_cast<const uint2*>(sc));
+        scale[i][0] = y.x;
+        scale[i][1] = y.y;
+      }
+    }
+  }
+  // Keys: word k (0, 1) of group gi of token g + 8 h. Values: the word of group gi of the u-th token.
+  __device__ __forceinline__ uint32_t key_word(int h, int gi, int k) const {
+    const int w = h * 2 * NG + 2 * gi + k;
+    const uint4& c = code[w >> 2];
+    return (w & 3) == 0 ? c.x : (w & 3) == 1 ? c.y : (w & 3) == 2 ? c.z : c.w;
+  }
+  __device__ __forceinline__ uint32_t value_word(int u, int gi) const {
+    const int w = u * NG + gi;
+    const uint4& c = code[w >> 2];
+    return (w & 3) == 0 ? c.x : (w & 3) == 1 ? c.y : (w & 3) == 2 ? c.z : c.w;
+  }
+};
+
 template <int D>
 __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Control& C, int warp, int lane) {
   using S = Shape<D>;
-  constexpr int NG = S::NG, NV = D / 64;                // 16-byte pieces of a lane in a block's codes
+  constexpr int NG = S::NG;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q;
-  const int per_page_shift = a.shift - 4;
+  const int page_shift = a.shift - 4;                   // blocks of a page
+  // where a lane stores: the two pieces of a key's row (tokens 8 further on 1024 bytes further), values of tokens 2t and 2t + 1
+  const uint32_t k_off = (warp * 16 + g) * 128 + (((2 * t) ^ g) << 4), k_flip = 16;   // 2t and 2t + 1 differ in the lowest bit
+  const uint32_t v_off0 = (warp * 16 + 2 * t) * 128 + ((g ^ (2 * t)) << 4), v_off1 = (warp * 16 + 2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4);
   uint32_t slot = 0, round = 0;                         // ring position
   Reader reader;
-  struct Raw {
-    uint4 code[NV];
-    uint32_t scale[4][(NG + 1) / 2];                    // two tokens of a key block, four of a value block
+  auto filled = [&]() {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&C.full[slot]);
+    if (++slot == S::Slots) { slot = 0; ++round; }
   };
   for (;;) {
     const Segment& w = reader.take(C, a);
     const uint32_t seg = reader.n;
-    // queries
+    const int first = w.first, count = w.count, end = w.end, more = w.more, request = w.request;
+    const int64_t head_at = static_cast<int64_t>(w.head) << page_shift, page_blocks = static_cast<int64_t>(a.hk) << page_shift;
+
+    // page of this warp's block of tile `lane` of each 32 tiles
+    int pages = 0;
+    auto block = [&](int j) -> const uint8_t* {
+      if ((j & 31) == 0) {
+        const int blk = (first + j + lane) * (kKeys / 16) + warp;
+        pages = blk * 16 < end ? page_of(a, request, blk >> page_shift) : 0;
+      }
+      const int blk = (first + j) * (kKeys / 16) + warp, pg = __shfl_sync(0xFFFFFFFFu, pages, j & 31);
+      return blk * 16 < end ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
+    };
+    Raw<D, false> k;
+    Raw<D, true> v;
+    const uint8_t* at = block(0);           // of the newest keys loaded; values follow one tile behind
+    k.load(at, g, t, lane);
+
+    // queries, in the order of the operands
     wait(&C.q_empty, (seg & 1) ^ 1, C, a);
-    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    const int head = w.head, request = w.request;
-    for (int i = 0; i < 16; ++i) {
-      const int row = warp * 16 + i;
-      if (lane < D / 8) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < w.rows) {
-          v = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + row / a.group) * a.q_ts + (head * a.group + row % a.group) * a.q_hs + 8 * lane));
-          v = make_uint4(__byte_perm(v.x, v.z, 0x5410) ^ flip, __byte_perm(v.x, v.z, 0x7632) ^ flip,
-                         __byte_perm(v.y, v.w, 0x5410) ^ flip, __byte_perm(v.y, v.w, 0x7632) ^ flip);
+    {
+      constexpr int Lanes = D / 8, Step = 32 / Lanes, N = 16 / Step;
+      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+      const int col = lane % Lanes;
+#pragma unroll
+      for (int i0 = 0; i0 < N; i0 += 4) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = warp * 16 + (i0 + i) * Step + lane / Lanes;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (i0 + i < N && row < w.rows)
+            x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + row / a.group) * a.q_ts + (w.head * a.group + row % a.group) * a.q_hs + 8 * col));
         }
-        sts128(q_at + (lane >> 3) * kPanel + row * 128 + (((lane & 7) ^ (row & 7)) << 4), v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = warp * 16 + (i0 + i) * Step + lane / Lanes;
+          if (i0 + i < N)
+            sts128(q_at + (col >> 3) * kPanel + row * 128 + (((col & 7) ^ (row & 7)) << 4),
+                   make_uint4(__byte_perm(x[i].x, x[i].z, 0x5410) ^ flip, __byte_perm(x[i].x, x[i].z, 0x7632) ^ flip,
+                              __byte_perm(x[i].y, x[i].w, 0x5410) ^ flip, __byte_perm(x[i].y, x[i].w, 0x7632) ^ flip));
+        }
       }
     }
+    reader.done(C);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&C.q_full);
 
-    const int first = w.first, count = w.count, end = w.end, more = w.more;
-    auto load = [&](int j, bool value, Raw& x) {        // block `warp` of tile first + j
-      const int key = (first + j) * kKeys + warp * 16;
-      if (key < end) {
-        const int blk = key >> 4;
-        const int pg = page_of(a, request, blk >> per_page_shift);
-        const uint8_t* p = a.cache + (((static_cast<int64_t>(pg) * a.hk + head) << per_page_shift) + (blk & ((1 << per_page_shift) - 1))) * block_bytes(D);
-        const uint8_t* c = p + (value ? 8 * D : 0) + lane * 16;
+    auto store_keys = [&]() {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x.code[i] = __ldg(reinterpret_cast<const uint4*>(c + i * 512));
+      for (int s = 0; s < S::PerTile; ++s) {
+        const uint32_t base = ring + slot * S::Slot + k_off;
+        wait(&C.empty[slot], (round & 1) ^ 1, C, a);
 #pragma unroll
-        for (int i = 0; i < (value ? 4 : 2); ++i) {
-          const int tok = value ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i;
-          const uint8_t* sc = p + 16 * D + tok * 4 * NG + (value ? 2 * NG : 0);
-          if constexpr (NG == 1) {
-            x.scale[i][0] = __ldg(reinterpret_cast<const uint16_t*>(sc));
-          } else if constexpr (NG == 2) {
-            x.scale[i][0] = __ldg(reinterpret_cast<const uint32_t*>(sc));
-          } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2*>(sc));
-            x.scale[i][0] = y.x;
-            x.scale[i][1] = y.y;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int p = 0; p < S::Panels; ++p) {
+            const int gi = s * S::Panels + p;
+            const Scale sc(k.scale[h][gi >> 1], gi);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sts128((base ^ (i * k_flip)) + p * kPanel + h * 1024, values8(k.key_word(h, gi, i), sc));
           }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) x.code[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < (NG + 1) / 2; ++k) x.scale[i][k] = 0;
+        filled();
       }
     };
-    auto both = [](uint32_t x, int gi) { return gi & 1 ? __byte_perm(x, x, 0x3232) : __byte_perm(x, x, 0x1010); };
-    auto store = [&](int j, bool value, const Raw& x) {
+    auto store_values = [&](int j) {
+      // behind the sequence there may be anything; a group that is not a number must not reach the rows that do not see it
       const int key0 = (first + j) * kKeys + warp * 16;
+      if (key0 + 16 > end) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (key0 + 2 * t + (u & 1) + 8 * (u >> 1) >= end)
+#pragma unroll
+            for (int i = 0; i < Raw<D, true>::SW; ++i) v.scale[u][i] = 0;
+      }
+      uint32_t sum = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < Raw<D, true>::SW; ++i) sum = add2(sum, v.scale[u][i]);
+      if (__any_sync(0xFFFFFFFFu, (sum & 0x7FFFu) > 0x7F80u || (sum & 0x7FFF0000u) > 0x7F800000u)) {
+        wait(&C.o_free, (seg & 1) ^ 1, C, a);           // the list of the segment before has been read
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            uint32_t& x = v.scale[u][gi >> 1];
+            if ((x >> (gi & 1) * 16 & 0x7FFFu) > 0x7F80u) {
+              x &= gi & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+              if (g == 0) {
+                const int key = key0 + 2 * t + (u & 1) + 8 * (u >> 1);
+                atomicMin(&C.nan_first[gi], key);
+                atomicMax(&C.nan_last[gi], key);
+                const uint32_t to = atomicAdd(&C.nan_count, 1u);
+                if (to < kNanList) C.nan_list[to] = key * 4 + gi;
+              }
+            }
+          }
+        __syncwarp();
+      }
 #pragma unroll
       for (int s = 0; s < S::PerTile; ++s) {
         const uint32_t base = ring + slot * S::Slot;
         wait(&C.empty[slot], (round & 1) ^ 1, C, a);
-        if (!value) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = warp * 16 + g + 8 * h;
-            uint32_t wd[2 * S::Panels];
-            if constexpr (D == 64) {
-              wd[0] = h ? x.code[0].z : x.code[0].x;
-              wd[1] = h ? x.code[0].w : x.code[0].y;
-            } else {
-              const uint4& c = x.code[h * (NV / 2) + s];
-              wd[0] = c.x; wd[1] = c.y; wd[2] = c.z; wd[3] = c.w;
-            }
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int p = 0; p < S::Panels; ++p) {
-              const int gi = s * S::Panels + p;
-              const uint32_t sc = both(x.scale[h][gi >> 1], gi);
-#pragma unroll
-              for (int k = 0; k < 2; ++k) sts128(base + p * kPanel + row * 128 + (((2 * t + k) ^ g) << 4), values8(wd[2 * p + k], sc));
-            }
+          for (int p = 0; p < S::Panels; ++p) {
+            const int gi = s * S::Panels + p;
+            sts128(base + (u & 1 ? v_off1 : v_off0) + p * kPanel + (u >> 1) * 1024, values8(v.value_word(u, gi), Scale(v.scale[u][gi >> 1], gi)));
           }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int tok = 2 * t + (u & 1) + 8 * (u >> 1), row = warp * 16 + tok;
-            const bool inside = key0 + tok < end;
-#pragma unroll
-            for (int p = 0; p < S::Panels; ++p) {
-              const int gi = s * S::Panels + p;
-              uint32_t wd;
-              if constexpr (D == 64) {
-                wd = u == 0 ? x.code[0].x : u == 1 ? x.code[0].y : u == 2 ? x.code[0].z : x.code[0].w;
-              } else if constexpr (D == 128) {
-                const uint4& c = x.code[u >> 1];
-                wd = u & 1 ? (gi ? c.w : c.z) : (gi ? c.y : c.x);
-              } else {
-                const uint4& c = x.code[u];
-                wd = gi == 0 ? c.x : gi == 1 ? c.y : gi == 2 ? c.z : c.w;
-              }
-              uint32_t sc = both(x.scale[u][gi >> 1], gi);
-              // behind the sequence there may be anything; a group that is not a number must not reach the rows that do not see it
-              if (!inside) sc = 0;
-              const bool nan = (sc & 0x7FFFu) > 0x7F80u;
-              if (__any_sync(0xFFFFFFFFu, nan)) {
-                wait(&C.o_free, (seg & 1) ^ 1, C, a);     // the list of the segment before has been read
-                if (nan) sc = 0;
-                if (nan && g == 0) {
-                  atomicMin(&C.nan_first[gi], key0 + tok);
-                  atomicMax(&C.nan_last[gi], key0 + tok);
-                  const uint32_t at = atomicAdd(&C.nan_count, 1u);
-                  if (at < kNanList) C.nan_list[at] = ((first + j) * kKeys + row) * 4 + gi;
-                }
-              }
-              sts128(base + p * kPanel + row * 128 + ((g ^ (row & 7)) << 4), values8(wd, sc));
-            }
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&C.full[slot]);
-        if (++slot == S::Slots) { slot = 0; ++round; }
+        filled();
       }
     };
-    Raw k, v;
-    load(0, false, k);
-    load(0, true, v);
-    store(0, false, k);
-    if (count > 1) load(1, false, k);
+    store_keys();
     for (int j = 0; j < count; ++j) {
+      v.load(at, g, t, lane);
       if (j + 1 < count) {
-        store(j + 1, false, k);
-        if (j + 2 < count) load(j + 2, false, k);
+        at = block(j + 1);
+        k.load(at, g, t, lane);
+        store_keys();
       }
-      store(j, true, v);
-      if (j + 1 < count) load(j + 1, true, v);
+      store_values(j);
     }
-    reader.done(C);
     if (!more) break;
   }
 }
@@ -504,20 +569,18 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64, raw[0]);
       tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64 + 32, raw[1]);
       tmem_ld_wait();
-      float s[64];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
+      float* s = reinterpret_cast<float*>(raw);
       if (key0 < clear_lo || key0 + kKeys > clear_hi) {
         const int from = lo - key0 - half * 64, to = hi - key0 - half * 64;
 #pragma unroll
         for (int i = 0; i < 64; ++i)
           if (i < from || i >= to) s[i] = -INFINITY;
       }
-      float x = s[0], y = s[1];
+      float x = fmaxf(s[0], s[1]), y = fmaxf(s[2], s[3]);
 #pragma unroll
-      for (int i = 2; i < 64; i += 2) {
-        x = fmaxf(x, s[i]);
-        y = fmaxf(y, s[i + 1]);
+      for (int i = 4; i < 64; i += 4) {
+        x = fmaxf(x, fmaxf(s[i], s[i + 1]));
+        y = fmaxf(y, fmaxf(s[i + 2], s[i + 3]));
       }
       x = fmaxf(x, y);
       C.top[n & 1][half][row] = x;
@@ -543,15 +606,16 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         }
       }
       uint32_t p[32];
-      float sum = 0.0f, sum2 = 0.0f;
+      float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float e0 = ex2(fmaf(s[2 * i], scale, -m)), e1 = ex2(fmaf(s[2 * i + 1], scale, -m));
-        sum += e0;
-        sum2 += e1;
-        p[i] = pack_bf16x2(e0, e1);
+        float2 e = fma_f32x2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
+        e.x = ex2(e.x);
+        e.y = ex2(e.y);
+        sum = add_f32x2(sum, e);
+        p[i] = pack_bf16x2(e.x, e.y);
       }
-      l += sum + sum2;
+      l += sum.x + sum.y;
       tmem_st32(lanes + kSCol + (n & 1) * kKeys + half * 32, p);
       tmem_st_wait();
       tc_fence_before();
