@@ -1,17 +1,20 @@
 // Attention over the 4-bit cache for requests of many query rows: chunks and whole prompts.
 //
-// A CTA takes 128 query rows (all query heads of one KV head for 128 / group tokens) against tiles of 128 keys:
+// A CTA takes row blocks (all query heads of one KV head for some tokens) against tiles of 128 keys:
 //   S = Q K^T and O += P V on tcgen05 (bf16, fp32 sums in tensor memory), the softmax between them in registers.
+// Heads of 64 and 128: two Q tiles of 128 rows, which share the operands made of the codes; one has its softmax while the other has the
+// tensor cores. Heads of 256, whose O alone takes half of tensor memory: one Q tile, and two tiles of keys at a time.
 // Eighteen warps, one CTA on an SM:
 //   8 turn codes into operands: a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
 //     128-byte-swizzled layout, keys for S with dims along K, values as they are (dims along N). A block's words are what a lane
 //     stores as 16 bytes, eight dims in the order 0 4 1 5 2 6 3 7 in which masking leaves them; queries are stored in the same
 //     order, and the output is put back from it.
 //   1 lists the segments of the CTA's run, a few ahead of the others.
-//   1 issues the products: S of tile j + 1 before O of tile j, so that the tensor cores have work while tile j is in the softmax.
-//   8 do the softmax: two threads to a row, half of the keys each; the row's maximum goes through shared memory. P goes back to
-//     tensor memory over S. O is only rescaled when a row's maximum has grown by more than 2^8 (by the warps of that row
-//     themselves; sums are fp32, so nothing is lost by a maximum that is a little old).
+//   1 issues the products.
+//   8 do the softmax, a thread to a row: four warps have one Q tile each, or every other tile of keys (the running maximum
+//     then goes through shared memory). S is read twice, for the maximum and for the weights, instead of being kept in
+//     128 registers. P goes back to tensor memory over S. O is only rescaled when a row's maximum has grown by more than 2^8 (by
+//     the warps of that row themselves; sums are fp32, so nothing is lost by a maximum that is a little old).
 // Work is cut into equal runs of tiles, one to a CTA; items that lie in several runs are joined as in kv4_decode.cu.
 // All waits are bounded.
 #include <climits>
@@ -25,13 +28,16 @@ using namespace kv4;
 
 constexpr int kSoftmaxWarps = 8, kFillWarps = 8, kMmaWarp = 16, kPlanWarp = 17;
 constexpr int kThreads = 20 * 32;          // two warps are only there to make up a warpgroup
-// registers of a thread: 96 at launch; softmax, filling, the rest: 256 * 136 + 256 * 72 + 128 * 56 <= 640 * 96
-constexpr int kSoftmaxRegs = 136, kFillRegs = 72, kRestRegs = 56;
+// registers of a thread: 96 at launch; softmax, filling, the rest: 256 * 112 + 256 * 96 + 128 * 64 = 640 * 96
+constexpr int kSoftmaxRegs = 112, kFillRegs = 96, kRestRegs = 64;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
-constexpr int kRows = 128, kKeys = 128;
+constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
 constexpr float kLow = -1e38f, kRoom = 8.0f;
 constexpr int kNanList = 64;
+// What an item costs beside its tiles, in tiles: loading its queries, filling and draining the pipeline, writing its output.
+// It counts where work is divided, for the first blocks of a prompt are many and short.
+constexpr int kOwn = 2;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D>
@@ -40,9 +46,12 @@ struct Shape {
   static constexpr int Panels = D == 64 ? 1 : 2;        // of a slot
   static constexpr int Slot = Panels * kPanel;
   static constexpr int PerTile = NG / Panels;           // slots of a tile's keys, or of its values
-  static constexpr int Slots = D == 256 ? 5 : 6;
-  static constexpr int Q = NG * kPanel;
-  static constexpr int Part = kRows * (D + 2);          // floats of a CTA's state: output, maximum and sum
+  static constexpr bool Twin = D <= 128;                // two Q tiles; else one, and the softmax warps take turns at the keys
+  static constexpr int Rows = Twin ? 2 * kRows : kRows; // of a row block
+  static constexpr int Slots = D == 64 ? 8 : 5;
+  static constexpr int Q = (Twin ? 2 : 1) * NG * kPanel;
+  static constexpr int Cols = Twin ? D : D / 2;         // output columns of a thread
+  static constexpr int Part = Rows * (D + 2);           // floats of a CTA's state: output, maximum and sum
 };
 
 // Tiles [first, first + count) of keys for a row block: all query heads of a KV head for some tokens of a request.
@@ -56,7 +65,7 @@ struct Segment {
 
 struct Control {
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t full[6], empty[6];               // ring slots
+  uint64_t full[8], empty[8];               // ring slots
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_full[2];
   uint64_t o_done, o_all, o_free;           // a tile's products, a segment's; the segment's output has been read
@@ -67,7 +76,7 @@ struct Control {
   int wsum[20];
   Segment seg[kSegs];
   int32_t nan_list[kNanList];               // key * 16 + groups
-  float top[2][2][kRows];                   // of the two halves of a row, two tiles deep
+  float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
 };
 
 template <int D>
@@ -101,20 +110,20 @@ struct Item {
   __device__ __forceinline__ int tiles(int rb) const { return max(1, (seen(rb) + kKeys - 1) / kKeys - first_tile(rb)); }
 };
 
-__device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r) {
-  return {r.len - r.n, r.n * a.group > a.split_rows ? r.n : 0, r.len, kRows / a.group, a.window};
+__device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r, int rows) {
+  return {r.len - r.n, r.n * a.group > a.split_rows ? r.n : 0, r.len, rows / a.group, a.window};
 }
 
-// Tiles of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
+// Tiles, and kOwn for each block, of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
 // one only where the first queries have no place in the sequence.
 __device__ __forceinline__ int64_t tiles_before(const Item& it, int rb) {
-  int64_t sum = 0;
+  int64_t sum = static_cast<int64_t>(rb) * kOwn;
   if (it.place0 < 0) {
     for (int i = 0; i < rb; ++i) sum += it.tiles(i);
     return sum;
   }
   const int full = min(rb, it.n / it.tb);                // blocks of tb tokens; a shorter one is the last
-  sum = floor_sum(full, kKeys, it.tb, static_cast<int64_t>(it.place0) + it.tb + kKeys - 1);
+  sum += floor_sum(full, kKeys, it.tb, static_cast<int64_t>(it.place0) + it.tb + kKeys - 1);
   if (it.window > 0) {
     const int64_t begin = static_cast<int64_t>(it.place0) + 1 - it.window;      // of the first row; blocks with a negative one begin at 0
     const int64_t skip = begin < 0 ? min((-begin + it.tb - 1) / it.tb, static_cast<int64_t>(full)) : 0;
@@ -125,26 +134,27 @@ __device__ __forceinline__ int64_t tiles_before(const Item& it, int rb) {
 }
 
 // The segments of a CTA's run, one after another: tiles [t0, t1) of an item.
+template <int Rows>
 struct Walk {
   int b, head, rb, blocks, tiles, at, u, u1, t0, t1, i0;
   Request r;
   Item it;
   __device__ __forceinline__ void load(const AttnArgs& a) {
     r = request_of(a, b, false);
-    it = item_of(a, r);
+    it = item_of(a, r, Rows);
     blocks = it.blocks();
   }
-  // Positions u in the unit space where item (b, head, rb) begins at `at`.
+  // The part of item (b, head, rb), which begins at `at`, that lies behind u: its tiles come behind its own kOwn units.
   __device__ __forceinline__ void open() {
     tiles = it.tiles(rb);
-    i0 = at;
-    t0 = u - at;
-    t1 = min(tiles, u1 - at);
+    i0 = at + kOwn;
+    t0 = max(u - i0, 0);
+    t1 = min(tiles, u1 - i0);               // t1 <= t0: the run ends before its tiles
   }
   __device__ __forceinline__ bool next(const AttnArgs& a) {   // false behind the run's end
-    u = at + t1;
+    u = i0 + t1;
     if (u >= u1) return false;
-    at += tiles;
+    at = i0 + tiles;
     if (++rb == blocks) {
       rb = 0;
       if (++head == a.hk) {
@@ -153,7 +163,7 @@ struct Walk {
       }
     }
     open();
-    return true;
+    return t1 > t0;
   }
 };
 
@@ -161,22 +171,36 @@ struct Walk {
 // Phase `parity` of a barrier. One that does not come is reported, and from then on no such wait waits: every role runs through its
 // loop, whatever is in memory, and the launch ends. The segment list alone is always waited for, so that all roles run
 // through the same loops; nobody who keeps it waiting waits for anything else then.
+// The clock is only read once in 64 polls: reading it takes longer than most waits.
+template <bool Always = false>
+__device__ __forceinline__ bool gave_up(uint32_t polls, uint64_t& since, Control& C, const AttnArgs& a) {
+  if ((polls & 63u) != 0u) return false;
+  volatile uint32_t* stop = &C.abort;
+  if (!Always && *stop) return true;
+  const uint64_t now = globaltimer_ns();
+  if (since == 0) since = now;
+  if (now - since <= (Always ? 8 : 1) * kWaitNs) return false;
+  report(a.status, kWaitTimeout, blockIdx.x);
+  *stop = 1u;
+  return true;
+}
 template <bool Always = false>
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Control& C, const AttnArgs& a) {
-  if (!mbar_try_wait(bar, parity)) {
-    const uint64_t t0 = globaltimer_ns();
-    volatile uint32_t* stop = &C.abort;
-    while (!mbar_try_wait(bar, parity)) {
-      if (!Always && *stop) break;
-      if (globaltimer_ns() - t0 > (Always ? 8 : 1) * kWaitNs) {
-        report(a.status, kWaitTimeout, blockIdx.x);
-        *stop = 1u;
-        break;
-      }
-    }
-  }
+  uint64_t since = 0;
+  for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up<Always>(polls, since, C, a); ++polls) {}
   __syncwarp();
 }
+
+// The same with a result that is the same for the whole warp in a way that the compiler sees, so that the code after it stays in
+// uniform control flow: the warp that issues the products, whose descriptors and addresses then stay in uniform registers.
+// (Moved there for each instruction, they took longer to issue than the tensor cores to work: 135 cycles instead of 64.)
+template <bool Always = false>
+__device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity, Control& C, const AttnArgs& a) {
+  uint64_t since = 0;
+  for (uint32_t polls = 1; !__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity)); ++polls)
+    if (__any_sync(0xFFFFFFFFu, gave_up<Always>(polls, since, C, a))) break;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
 
 // Reads the segments in order.
 struct Reader {
@@ -263,6 +287,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
       "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int count) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 constexpr uint32_t kSCol = 0, kOCol = 256;
@@ -339,6 +371,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
     const Segment& w = reader.take(C, a);
     const uint32_t seg = reader.n;
     const int first = w.first, count = w.count, end = w.end, more = w.more, request = w.request;
+    if (count == 0) break;
     const int64_t head_at = static_cast<int64_t>(w.head) << page_shift, page_blocks = static_cast<int64_t>(a.hk) << page_shift;
 
     // page of this warp's block of tile `lane` of each 32 tiles
@@ -353,30 +386,32 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
     };
     Raw<D, false> k;
     Raw<D, true> v;
-    const uint8_t* at = block(0);           // of the newest keys loaded; values follow one tile behind
+    const uint8_t *at = block(0), *then = nullptr;      // blocks whose values, whose keys are loaded next
     k.load(at, g, t, lane);
+    v.load(at, g, t, lane);
 
     // queries, in the order of the operands
     wait(&C.q_empty, (seg & 1) ^ 1, C, a);
     {
-      constexpr int Lanes = D / 8, Step = 32 / Lanes, N = 16 / Step;
+      constexpr int Lanes = D / 8, Step = 32 / Lanes, Mine = S::Rows / kFillWarps, N = Mine / Step;
       const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-      const int col = lane % Lanes;
+      const int col = lane % Lanes, rows = w.rows;
+      const bool twin = rows > kRows;
 #pragma unroll
-      for (int i0 = 0; i0 < N; i0 += 4) {
-        uint4 x[4];
+      for (int i0 = 0; i0 < N; i0 += 8) {
+        uint4 x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = warp * 16 + (i0 + i) * Step + lane / Lanes;
+        for (int i = 0; i < 8; ++i) {
+          const int row = warp * 16 + (i0 + i) * Step / 16 * kRows + (i0 + i) * Step % 16 + lane / Lanes;   // 16 rows of each Q tile
           x[i] = make_uint4(0, 0, 0, 0);
-          if (i0 + i < N && row < w.rows)
+          if (row < rows)
             x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + row / a.group) * a.q_ts + (w.head * a.group + row % a.group) * a.q_hs + 8 * col));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = warp * 16 + (i0 + i) * Step + lane / Lanes;
-          if (i0 + i < N)
-            sts128(q_at + (col >> 3) * kPanel + row * 128 + (((col & 7) ^ (row & 7)) << 4),
+        for (int i = 0; i < 8; ++i) {
+          const int row = warp * 16 + (i0 + i) * Step % 16 + lane / Lanes, tile = (i0 + i) * Step / 16;
+          if (tile == 0 || twin)
+            sts128(q_at + (tile * NG + (col >> 3)) * kPanel + row * 128 + (((col & 7) ^ (row & 7)) << 4),
                    make_uint4(__byte_perm(x[i].x, x[i].z, 0x5410) ^ flip, __byte_perm(x[i].x, x[i].z, 0x7632) ^ flip,
                               __byte_perm(x[i].y, x[i].w, 0x5410) ^ flip, __byte_perm(x[i].y, x[i].w, 0x7632) ^ flip));
         }
@@ -453,15 +488,38 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         filled();
       }
     };
+    // in the order in which the products take them; what is stored is loaded again at once, for the tile after
     store_keys();
+    if (count > 1) {
+      then = block(1);
+      k.load(then, g, t, lane);
+    }
     for (int j = 0; j < count; ++j) {
-      v.load(at, g, t, lane);
-      if (j + 1 < count) {
-        at = block(j + 1);
-        k.load(at, g, t, lane);
-        store_keys();
+      const bool keys = j + 1 < count;
+      const uint8_t* after = nullptr;
+      auto values = [&]() {
+        store_values(j);
+        if (keys) {
+          at = then;
+          v.load(at, g, t, lane);
+        }
+      };
+      auto next_keys = [&]() {
+        if (keys) store_keys();
+        if (j + 2 < count) {
+          const uint8_t* p = block(j + 2);
+          k.load(p, g, t, lane);
+          after = p;
+        }
+      };
+      if constexpr (S::Twin) {
+        values();
+        next_keys();
+      } else {
+        next_keys();
+        values();
       }
-      store_values(j);
+      then = after;
     }
     if (!more) break;
   }
@@ -471,73 +529,126 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
 template <int D>
 __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Control& C) {
   using S = Shape<D>;
-  const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q, tmem = C.tmem;
+  const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q, tmem = uniform(C.tmem);
   constexpr uint32_t qk = umma_idesc_bf16_f32(kRows, kKeys), pv = umma_idesc_bf16_f32(kRows, S::Panels * 64) | (1u << 16);
-  uint32_t slot = 0, round = 0, n = 0;                  // ring position; tiles so far
+  uint32_t slot = 0, round = 0;                         // ring position
   Reader reader;
-  auto release = [&]() {
-    if (elect_one_sync()) umma_commit(&C.empty[slot]);
+  auto advance = [&]() {
     if (++slot == S::Slots) { slot = 0; ++round; }
   };
-  auto scores = [&](uint32_t tile) {
-#pragma unroll
-    for (int s = 0; s < S::PerTile; ++s) {
-      wait(&C.full[slot], round & 1, C, a);
-      tc_fence_after();
-      const uint32_t base = ring + slot * S::Slot;
-      if (elect_one_sync()) {
-#pragma unroll
-        for (int p = 0; p < S::Panels; ++p)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16(tmem + kSCol + (tile & 1) * kKeys, umma_desc_sw128(q_at + (s * S::Panels + p) * kPanel + k * 32),
-                      umma_desc_sw128(base + p * kPanel + k * 32), qk, (s | p | k) != 0);
-      }
-      __syncwarp();
-      release();
-    }
-    if (elect_one_sync()) umma_commit(&C.s_full[tile & 1]);
+  auto filled = [&]() {
+    wait_warp(&C.full[slot], round & 1, C, a);
+    tc_fence_after();
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (elect_one_sync()) umma_commit(bar);
     __syncwarp();
   };
-  for (;;) {
-    const Segment& w = reader.take(C, a);
-    const uint32_t seg = reader.n;
-    const int count = w.count, more = w.more;
-    reader.done(C);
-    wait(&C.q_full, seg & 1, C, a);
-    scores(n);
-    for (int j = 0; j < count; ++j) {
-      if (j + 1 < count) scores(n + 1);
-      if (j + 2 >= count && (j + 1 < count || count == 1)) {  // the last scores of the segment are on their way
-        if (elect_one_sync()) umma_commit(&C.q_empty);
-        __syncwarp();
-      }
-      if (j == 0) wait(&C.o_free, (seg & 1) ^ 1, C, a);
-      wait(&C.p_full[n & 1], (n >> 1) & 1, C, a);
-      tc_fence_after();
+  // panels of a slot (the s-th of a tile's keys) against Q tile `tile`, into score buffer `buf`
+  auto scores = [&](int tile, int buf, int s, uint32_t at) {
+    const uint64_t dq = umma_desc_sw128(q_at + (tile * S::NG + s * S::Panels) * kPanel), dk = umma_desc_sw128(ring + at * S::Slot);
+    const uint32_t d = tmem + kSCol + buf * kKeys;
+    if (elect_one_sync()) {
 #pragma unroll
-      for (int s = 0; s < S::PerTile; ++s) {
-        wait(&C.full[slot], round & 1, C, a);
-        tc_fence_after();
-        const uint32_t base = ring + slot * S::Slot;
-        if (elect_one_sync()) {
+      for (int p = 0; p < S::Panels; ++p)
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_bf16_ts(tmem + kOCol + s * S::Panels * 64, tmem + kSCol + (n & 1) * kKeys + k * 8, desc_mn_sw128(base + k * 2048), pv,
-                         (j | k) != 0);
-        }
-        __syncwarp();
-        release();
-      }
-      if (elect_one_sync()) {
-        umma_commit(&C.o_done);
-        if (j + 1 == count) umma_commit(&C.o_all);
-      }
-      __syncwarp();
-      ++n;
+        for (int k = 0; k < 4; ++k) umma_bf16(d, dq + (p * kPanel + k * 32) / 16, dk + (p * kPanel + k * 32) / 16, qk, (s | p | k) != 0);
     }
+    __syncwarp();
+  };
+  // weights of buffer `buf` times the values of a slot (the s-th of a tile's values), onto the output of Q tile `tile`
+  auto values = [&](int tile, int buf, int s, uint32_t at, bool add) {
+    const uint64_t dv = desc_mn_sw128(ring + at * S::Slot);
+    const uint32_t d = tmem + kOCol + tile * kRows + s * S::Panels * 64, p = tmem + kSCol + buf * kKeys;
+    if (elect_one_sync()) {
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k) umma_bf16_ts(d, p + k * 8, dv + k * 2048 / 16, pv, add || k != 0);
+    }
+    __syncwarp();
+  };
+  uint32_t n[2] = {0, 0};                               // tiles so far in each score buffer
+  for (;;) {
+    const uint32_t seg = reader.n;
+    wait_warp<true>(&C.seg_full[seg % kSegs], (seg / kSegs) & 1, C, a);
+    const Segment& w = C.seg[seg % kSegs];
+    const int count = uniform(w.count), more = uniform(w.more);
+    const bool twin = S::Twin && uniform(w.rows) > kRows;
+    if (count == 0) break;
+    reader.done(C);
+    wait_warp(&C.q_full, seg & 1, C, a);
+    if constexpr (S::Twin) {
+      filled();
+      scores(0, 0, 0, slot);
+      commit(&C.s_full[0]);
+      if (twin) {
+        scores(1, 1, 0, slot);
+        commit(&C.s_full[1]);
+      }
+      commit(&C.empty[slot]);
+      if (count == 1) commit(&C.q_empty);
+      advance();
+      for (int j = 0; j < count; ++j) {
+        const uint32_t v = slot;
+        filled();
+        advance();
+        if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
+        wait_warp(&C.p_full[0], n[0]++ & 1, C, a);
+        tc_fence_after();
+        values(0, 0, 0, v, j > 0);
+        const uint32_t k = slot;
+        if (j + 1 < count) {
+          filled();
+          scores(0, 0, 0, k);
+          commit(&C.s_full[0]);
+        }
+        if (twin) {
+          wait_warp(&C.p_full[1], n[1]++ & 1, C, a);
+          tc_fence_after();
+          values(1, 1, 0, v, j > 0);
+        }
+        commit(&C.empty[v]);
+        if (j + 1 < count) {
+          if (twin) {
+            scores(1, 1, 0, k);
+            commit(&C.s_full[1]);
+          }
+          commit(&C.empty[k]);
+          if (j + 2 == count) commit(&C.q_empty);
+          advance();
+        }
+      }
+    } else {
+      auto next_scores = [&](uint32_t tile) {
+#pragma unroll
+        for (int s = 0; s < S::PerTile; ++s) {
+          filled();
+          scores(0, tile & 1, s, slot);
+          commit(&C.empty[slot]);
+          advance();
+        }
+        commit(&C.s_full[tile & 1]);
+      };
+      next_scores(n[0]);
+      if (count == 1) commit(&C.q_empty);
+      for (int j = 0; j < count; ++j, ++n[0]) {
+        if (j + 1 < count) next_scores(n[0] + 1);
+        if (j + 2 == count) commit(&C.q_empty);
+        if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
+        wait_warp(&C.p_full[n[0] & 1], (n[0] >> 1) & 1, C, a);
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < S::PerTile; ++s) {
+          filled();
+          values(0, n[0] & 1, s, slot, j > 0);
+          commit(&C.empty[slot]);
+          advance();
+        }
+        commit(&C.o_done);
+      }
+    }
+    commit(&C.o_all);
     if (!more) {
-      wait(&C.o_all, seg & 1, C, a);        // nothing is in flight when tensor memory is given back
+      wait_warp(&C.o_all, seg & 1, C, a);        // nothing is in flight when tensor memory is given back
       break;
     }
   }
@@ -547,86 +658,115 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
 template <int D>
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int warp, int lane) {
   using S = Shape<D>;
-  constexpr int Half = D / 2;                           // output columns of a thread
-  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
-  const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const int quarter = warp & 3, set = warp >> 2;        // lanes of tensor memory; which four warps
+  const int row = (S::Twin ? set * kRows : 0) + quarter * 32 + lane, tile_row = quarter * 32 + lane;
+  const int col0 = S::Twin ? 0 : set * S::Cols;         // output columns of this thread, in the epilogue
+  const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16), scores = lanes + kSCol + set * kKeys;
+  const uint32_t output = lanes + kOCol + set * kRows;  // of its Q tile, or its half of the only one
   const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);     // the queries carry its sign; not 0, for -inf times it stays -inf
-  uint32_t n = 0;
+  uint32_t n = 0, mine = 0;                             // tiles of keys so far (all, where sets take turns); this set's score buffers
   Reader reader;
   for (;;) {
     const Segment& w = reader.take(C, a);
     const int first = w.first, count = w.count, more = w.more;
-    const bool real = row < w.rows;
+    if (count == 0) break;
+    const bool real = row < w.rows, idle = S::Twin && set == 1 && w.rows <= kRows;
     const int place = w.place + row / a.group, hi = real ? place + 1 : 0, lo = a.window > 0 ? place + 1 - a.window : 0;
     // every row of the block sees all of [clear_lo, clear_hi)
     const int clear_hi = w.place + 1, clear_lo = a.window > 0 ? w.place + (w.rows - 1) / a.group + 1 - a.window : 0;
     float m = kLow, l = 0.0f;
-    for (int j = 0; j < count; ++j, ++n) {
+    // where the sets take turns, this one's next tile is the first or the second of the segment
+    for (int j = idle ? count : S::Twin ? 0 : (n ^ set) & 1; j < count; j += S::Twin ? 1 : 2, ++mine) {
       const int key0 = (first + j) * kKeys;
-      wait(&C.s_full[n & 1], (n >> 1) & 1, C, a);
+      wait(&C.s_full[set], mine & 1, C, a);
       tc_fence_after();
+      const bool mask = key0 < clear_lo || key0 + kKeys > clear_hi;
+      const int from = lo - key0, to = hi - key0;
+      auto hide = [&](float* s, int base) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (base + i < from || base + i >= to) s[i] = -INFINITY;
+      };
       uint32_t raw[2][32];
-      tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64, raw[0]);
-      tmem_ld32(lanes + kSCol + (n & 1) * kKeys + half * 64 + 32, raw[1]);
-      tmem_ld_wait();
-      float* s = reinterpret_cast<float*>(raw);
-      if (key0 < clear_lo || key0 + kKeys > clear_hi) {
-        const int from = lo - key0 - half * 64, to = hi - key0 - half * 64;
+      tmem_ld32(scores, raw[0]);
+      float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < from || i >= to) s[i] = -INFINITY;
-      }
-      float x = fmaxf(s[0], s[1]), y = fmaxf(s[2], s[3]);
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        tmem_ld32(scores + ((c + 1) & 3) * 32, raw[(c + 1) & 1]);     // after the last the first again
+        float* s = reinterpret_cast<float*>(raw[c & 1]);
+        if (mask) hide(s, c * 32);
 #pragma unroll
-      for (int i = 4; i < 64; i += 4) {
-        x = fmaxf(x, fmaxf(s[i], s[i + 1]));
-        y = fmaxf(y, fmaxf(s[i + 2], s[i + 3]));
-      }
-      x = fmaxf(x, y);
-      C.top[n & 1][half][row] = x;
-      tc_fence_before();
-      named_bar_sync(1 + quarter, 64);      // the other half's maximum; and both halves of S have been read before P goes over it
-      x = fmaxf(x, C.top[n & 1][half ^ 1][row]) * scale;
-      if (__any_sync(0xFFFFFFFFu, x > m + kRoom)) {
-        const float to = fmaxf(m, x), by = ex2(m - to);
-        m = to;
-        l *= by;
-        if (j > 0) {
-          wait(&C.o_done, (n - 1) & 1, C, a);   // at most one tile behind: the scores of this one came after the products of n - 2
-          tc_fence_after();
-#pragma unroll
-          for (int i = 0; i < Half; i += 32) {
-            uint32_t o[32];
-            tmem_ld32(lanes + kOCol + half * Half + i, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-            tmem_st32(lanes + kOCol + half * Half + i, o);
-          }
+        for (int i = 0; i < 32; i += 4) {
+          x = fmaxf(x, fmaxf(s[i], s[i + 1]));
+          y = fmaxf(y, fmaxf(s[i + 2], s[i + 3]));
         }
       }
-      uint32_t p[32];
+      x = fmaxf(x, y) * scale;
+      float before = m;                     // the maximum that O stands at
+      if constexpr (!S::Twin) {
+        if (j > 0) {
+          named_bar_sync(1 + (set ^ 1) * 4 + quarter, 64);
+          before = C.top[tile_row];
+        }
+      }
+      float now = before;
+      const bool grow = __any_sync(0xFFFFFFFFu, x > before + kRoom);
+      if (grow) now = fmaxf(before, x);
+      if constexpr (!S::Twin) {
+        C.top[tile_row] = now;
+        if (j + 1 < count) bar_arrive(1 + set * 4 + quarter, 64);
+      }
+      l *= ex2(m - now);
+      m = now;
+      if (grow && j > 0) {
+        // the products of the tile before are in O: where the sets take turns they may not be yet, but no other tile's are missing
+        if constexpr (!S::Twin) wait(&C.o_done, (n + j - 1) & 1, C, a);
+        tc_fence_after();
+        tmem_ld_wait();
+        const float by = ex2(before - now);
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          uint32_t o[32];
+          tmem_ld32(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+          tmem_st32(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
+        }
+      }
       float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float2 e = fma_f32x2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
-        e.x = ex2(e.x);
-        e.y = ex2(e.y);
-        sum = add_f32x2(sum, e);
-        p[i] = pack_bf16x2(e.x, e.y);
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld32(scores + (c + 1) * 32, raw[(c + 1) & 1]);
+        float* s = reinterpret_cast<float*>(raw[c & 1]);
+        if (mask) hide(s, c * 32);
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 e = fma_f32x2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          sum = add_f32x2(sum, e);
+          p[i] = pack_bf16x2(e.x, e.y);
+        }
+        tmem_st16(scores + c * 16, p);      // over scores that have been read: 16 columns of weights to 32
       }
       l += sum.x + sum.y;
-      tmem_st32(lanes + kSCol + (n & 1) * kKeys + half * 32, p);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&C.p_full[n & 1]);
+      mbar_arrive(&C.p_full[set]);
     }
-    // the two halves' sums
-    C.top[n & 1][half][row] = l;
-    named_bar_sync(1 + quarter, 64);
-    l += C.top[n & 1][half ^ 1][row];
-    named_bar_sync(1 + quarter, 64);        // read before the next segment's first maximum
-
+    n += count;
+    if constexpr (!S::Twin) {               // the sets' sums, at the last maximum
+      named_bar_sync(9, 256);
+      const float last = C.top[tile_row];
+      C.sum[set][tile_row] = l * ex2(m - last);
+      m = last;
+      named_bar_sync(9, 256);
+      l = C.sum[0][tile_row] + C.sum[1][tile_row];
+    }
     wait(&C.o_all, reader.n & 1, C, a);
     tc_fence_after();
     // groups that are not numbers and that this row sees
@@ -644,7 +784,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     }
     const bool whole = w.whole;
     const int c0 = w.c0, c1 = w.c1;
-    float* mine = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
+    float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
     auto write_out = [&](int rw, int d, const float (&x)[8], float inv) {       // eight dims, in the order of the operands
       const int tk = w.q_row + rw / a.group, hd = w.head * a.group + rw % a.group;
       float y[8] = {x[0] * inv, x[2] * inv, x[4] * inv, x[6] * inv, x[1] * inv, x[3] * inv, x[5] * inv, x[7] * inv};
@@ -656,52 +796,56 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       a.lse[static_cast<int64_t>(tk) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
     };
     const float inv = inverse(l);
+    if (!idle) {
+      __nv_bfloat16* to = a.out + (static_cast<int64_t>(w.q_row + row / a.group) * a.hq + w.head * a.group + row % a.group) * D + col0;
+#pragma unroll 1
+      for (int i = 0; i < S::Cols; i += 32) {
+        uint32_t o[32];
+        tmem_ld32(output + i, o);
+        tmem_ld_wait();
+        if (real) {
+          const bool nan = nans >> ((col0 + i) >> 6) & 1u;
 #pragma unroll
-    for (int i = 0; i < Half; i += 32) {
-      uint32_t o[32];
-      tmem_ld32(lanes + kOCol + half * Half + i, o);
-      tmem_ld_wait();
-      if (real) {
-        const bool nan = nans >> ((half * Half + i) >> 6) & 1u;
+          for (int k = 0; k < 32; k += 8) {
+            float x[8];
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          float x[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) x[c] = nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[k + c]);
-          if (whole) {
-            write_out(row, half * Half + i + k, x, inv);
-          } else {
-            __stcg(reinterpret_cast<float4*>(mine + row * D + half * Half + i + k), make_float4(x[0], x[1], x[2], x[3]));
-            __stcg(reinterpret_cast<float4*>(mine + row * D + half * Half + i + k + 4), make_float4(x[4], x[5], x[6], x[7]));
+            for (int c = 0; c < 8; ++c) x[c] = nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[k + c]);
+            if (whole) {
+              const float y[8] = {x[0] * inv, x[2] * inv, x[4] * inv, x[6] * inv, x[1] * inv, x[3] * inv, x[5] * inv, x[7] * inv};
+              *reinterpret_cast<uint4*>(to + i + k) = pack_bf16x8(y);
+            } else {
+              __stcg(reinterpret_cast<float4*>(part + row * D + col0 + i + k), make_float4(x[0], x[1], x[2], x[3]));
+              __stcg(reinterpret_cast<float4*>(part + row * D + col0 + i + k + 4), make_float4(x[4], x[5], x[6], x[7]));
+            }
           }
         }
       }
     }
     tc_fence_before();
-    named_bar_sync(5, 256);                 // everyone has read the list of this segment
+    named_bar_sync(9, 256);                 // everyone has read the list of this segment
     if (warp == 0 && lane < 4) { C.nan_count = 0; C.nan_first[lane] = INT_MAX; C.nan_last[lane] = -1; }
     __syncwarp();
     mbar_arrive(&C.o_free);
     if (whole) {
-      if (real && half == 0 && a.lse) write_lse(row, m, l);
+      if (real && col0 == 0 && a.lse) write_lse(row, m, l);
     } else {
-      if (real && half == 0) __stcg(reinterpret_cast<float2*>(mine + kRows * D + 2 * row), make_float2(m, l));
+      if (real && col0 == 0) __stcg(reinterpret_cast<float2*>(part + S::Rows * D + 2 * row), make_float2(m, l));
       __threadfence();
-      named_bar_sync(5, 256);
+      named_bar_sync(9, 256);
       if (warp == 0 && lane == 0) {
         const uint32_t before = atomicAdd(a.counters + c0, 1u);
         C.last = before == static_cast<uint32_t>(c1 - c0);
         if (C.last) a.counters[c0] = 0;
         __threadfence();
       }
-      named_bar_sync(5, 256);
+      named_bar_sync(9, 256);
       if (C.last) {
         for (int idx = warp * 32 + lane; idx < w.rows * (D / 8); idx += 256) {
           const int rw = idx / (D / 8), d = idx % (D / 8) * 8;
           float mx = kLow, sum = 0.0f, x[8] = {};
           for (int c = c0; c <= c1; ++c) {
             const float* from = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
-            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + kRows * D + 2 * rw));
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + S::Rows * D + 2 * rw));
             const float4 p0 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d)), p1 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d + 4));
             const float to = fmaxf(mx, ms.x), old = ex2(mx - to), by = ex2(ms.x - to);
             mx = to;
@@ -722,8 +866,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
 }
 
 // ---- the warp that lists the segments
+template <int Rows>
 __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per, int u0, int u1, int lane) {
-  Walk w;
+  Walk<Rows> w;
   w.b = C.found[0];
   w.load(a);
   w.u = u0;
@@ -747,12 +892,13 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per
   w.open();
   for (uint32_t n = 0;; ++n) {
     wait<true>(&C.seg_empty[n % kSegs], ((n / kSegs) & 1) ^ 1, C, a);
-    Walk v = w;
-    const bool more = w.next(a);
+    const bool none = w.t1 <= w.t0;         // a run of nothing but an item's own units
+    const Walk<Rows> v = w;
+    const bool more = !none && w.next(a);
     if (lane == 0) {
       const int tok = v.rb * v.it.tb;
       C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
-                          v.it.first_tile(v.rb) + v.t0, v.t1 - v.t0, v.i0 / per, (v.i0 + v.tiles - 1) / per,
+                          v.it.first_tile(v.rb) + v.t0, none ? 0 : v.t1 - v.t0, v.i0 / per, (v.i0 + v.tiles - 1) / per,
                           v.t1 - v.t0 == v.tiles, more};
       mbar_arrive(&C.seg_full[n % kSegs]);
     }
@@ -771,7 +917,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   const int chunk = (a.batch + kThreads - 1) / kThreads;
   int mine = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
-    const Item it = item_of(a, request_of(a, b, blockIdx.x == 0));
+    const Item it = item_of(a, request_of(a, b, blockIdx.x == 0), S::Rows);
     mine += static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
   }
   int upto = mine;
@@ -793,7 +939,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   if (upto - mine <= u0 && u0 < upto) {
     int at = upto - mine, b = tid * chunk;
     for (;; ++b) {
-      const Item it = item_of(a, request_of(a, b, false));
+      const Item it = item_of(a, request_of(a, b, false), S::Rows);
       const int cost = static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
       if (at + cost > u0) break;
       at += cost;
@@ -810,7 +956,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
     for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + 1); }
     mbar_init(&C.q_full, kFillWarps);
     mbar_init(&C.q_empty, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 32); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 16); }
     mbar_init(&C.o_done, 1);
     mbar_init(&C.o_all, 1);
     mbar_init(&C.o_free, kSoftmaxWarps * 32);
@@ -832,7 +978,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   } else {
     reg_dec<kRestRegs>();
     if (warp == kMmaWarp) mma_role<D>(a, smem, C);
-    else if (warp == kPlanWarp) plan_role(a, C, per, u0, u1, lane);
+    else if (warp == kPlanWarp) plan_role<S::Rows>(a, C, per, u0, u1, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -864,7 +1010,7 @@ static_assert(smem_bytes<256>() <= 232448 && smem_bytes<128>() <= 232448, "share
 }  // namespace
 
 namespace kv4 {
-size_t prompt_partial_floats() { return static_cast<size_t>(MONO_ATTN_SMS) * 2 * Shape<256>::Part; }
+size_t prompt_partial_floats() { return static_cast<size_t>(MONO_ATTN_SMS) * 2 * (Shape<128>::Part > Shape<256>::Part ? Shape<128>::Part : Shape<256>::Part); }
 int prompt(const AttnArgs& a, int head_dim, cudaStream_t stream) {
   return head_dim == 64 ? launch<64>(a, stream) : head_dim == 128 ? launch<128>(a, stream) : launch<256>(a, stream);
 }
