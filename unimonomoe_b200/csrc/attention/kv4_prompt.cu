@@ -26,8 +26,9 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kSoftmaxWarps = 8, kFillWarps = 8, kMmaWarp = 16, kPlanWarp = 17;
-constexpr int kThreads = 20 * 32;          // two warps are only there to make up a warpgroup
+constexpr int kSoftmaxWarps = 8, kFillWarps = 8;
+constexpr int kMmaWarp = 0, kPlanWarp = 1, kFirstSoftmax = 4, kFirstFill = kFirstSoftmax + kSoftmaxWarps;   // warps 2 and 3 only make up a warpgroup
+constexpr int kThreads = 20 * 32;
 // registers of a thread: 96 at launch; softmax, filling, the rest: 256 * 112 + 256 * 96 + 128 * 64 = 640 * 96
 constexpr int kSoftmaxRegs = 112, kFillRegs = 96, kRestRegs = 64;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
@@ -72,8 +73,9 @@ struct Control {
   uint32_t tmem, abort, last;
   uint32_t nan_count;                       // value groups that are not numbers: key and group of the first kNanList of a segment,
   int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
-  int found[2];
-  int wsum[20];
+  int found;
+  long long found_at;
+  long long wsum[20];
   Segment seg[kSegs];
   int32_t nan_list[kNanList];               // key * 16 + groups
   float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
@@ -82,18 +84,19 @@ struct Control {
 template <int D>
 constexpr int smem_bytes() { return Shape<D>::Q + Shape<D>::Slots * Shape<D>::Slot + static_cast<int>(sizeof(Control)); }
 
-// sum of floor((a i + b) / m), i < n; a, b >= 0 (by Euclid's algorithm on a and m)
-__device__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t sum = 0;
+// sum of floor((a i + b) / m), i < n (by Euclid's algorithm on a and m). All of it fits 32 bits: it is the tiles of a request.
+__device__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  uint32_t sum = 0;
   while (n > 0) {
-    sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
-    a %= m;
-    b %= m;
-    const int64_t y = a * n + b;
+    const uint32_t qa = a / m, qb = b / m;
+    sum += qa * (n * (n - 1) / 2) + qb * n;
+    a -= qa * m;
+    b -= qb * m;
+    const uint32_t y = a * n + b;
     if (y < m) break;
     n = y / m;
-    b = y % m;
-    const int64_t t = m;
+    b = y - n * m;
+    const uint32_t t = m;
     m = a;
     a = t;
   }
@@ -116,18 +119,18 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r, int
 
 // Tiles, and kOwn for each block, of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
 // one only where the first queries have no place in the sequence.
-__device__ __forceinline__ int64_t tiles_before(const Item& it, int rb) {
-  int64_t sum = static_cast<int64_t>(rb) * kOwn;
+__device__ __forceinline__ int tiles_before(const Item& it, int rb) {
+  int sum = rb * kOwn;
   if (it.place0 < 0) {
     for (int i = 0; i < rb; ++i) sum += it.tiles(i);
     return sum;
   }
   const int full = min(rb, it.n / it.tb);                // blocks of tb tokens; a shorter one is the last
-  sum += floor_sum(full, kKeys, it.tb, static_cast<int64_t>(it.place0) + it.tb + kKeys - 1);
+  sum += floor_sum(full, kKeys, it.tb, it.place0 + it.tb + kKeys - 1);
   if (it.window > 0) {
-    const int64_t begin = static_cast<int64_t>(it.place0) + 1 - it.window;      // of the first row; blocks with a negative one begin at 0
-    const int64_t skip = begin < 0 ? min((-begin + it.tb - 1) / it.tb, static_cast<int64_t>(full)) : 0;
-    sum -= floor_sum(full - skip, kKeys, it.tb, max(begin + skip * it.tb, static_cast<int64_t>(0)));
+    const int begin = it.place0 + 1 - it.window;         // of the first row; blocks with a negative one begin at 0
+    const int skip = begin < 0 ? min((-begin + it.tb - 1) / it.tb, full) : 0;
+    sum -= floor_sum(full - skip, kKeys, it.tb, max(begin + skip * it.tb, 0));
   }
   if (rb > full) sum += it.tiles(full);
   return sum;
@@ -136,7 +139,8 @@ __device__ __forceinline__ int64_t tiles_before(const Item& it, int rb) {
 // The segments of a CTA's run, one after another: tiles [t0, t1) of an item.
 template <int Rows>
 struct Walk {
-  int b, head, rb, blocks, tiles, at, u, u1, t0, t1, i0;
+  int b, head, rb, blocks, tiles, t0, t1;
+  int64_t at, u, u1, i0;                    // in units of the whole launch
   Request r;
   Item it;
   __device__ __forceinline__ void load(const AttnArgs& a) {
@@ -148,8 +152,8 @@ struct Walk {
   __device__ __forceinline__ void open() {
     tiles = it.tiles(rb);
     i0 = at + kOwn;
-    t0 = max(u - i0, 0);
-    t1 = min(tiles, u1 - i0);               // t1 <= t0: the run ends before its tiles
+    t0 = static_cast<int>(max(u - i0, static_cast<int64_t>(0)));
+    t1 = static_cast<int>(min(static_cast<int64_t>(tiles), u1 - i0));   // t1 <= t0: the run ends before its tiles
   }
   __device__ __forceinline__ bool next(const AttnArgs& a) {   // false behind the run's end
     u = i0 + t1;
@@ -336,6 +340,20 @@ struct Raw {
       }
     }
   }
+  // The groups of the next slot in the place of this one's: one slot's code for all of them, which the instruction cache holds.
+  __device__ __forceinline__ void next_slot() {
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int i = 0; i < Tok; ++i) scale[i][0] = scale[i][1];
+      if constexpr (VALUE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { code[i].x = code[i].z; code[i].y = code[i].w; }
+      } else {
+        code[0] = code[1];
+        code[2] = code[3];
+      }
+    }
+  }
   // Keys: word k (0, 1) of group gi of token g + 8 h. Values: the word of group gi of the u-th token.
   __device__ __forceinline__ uint32_t key_word(int h, int gi, int k) const {
     const int w = h * 2 * NG + 2 * gi + k;
@@ -423,7 +441,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
     if (lane == 0) mbar_arrive(&C.q_full);
 
     auto store_keys = [&]() {
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < S::PerTile; ++s) {
         const uint32_t base = ring + slot * S::Slot + k_off;
         wait(&C.empty[slot], (round & 1) ^ 1, C, a);
@@ -431,12 +449,12 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int p = 0; p < S::Panels; ++p) {
-            const int gi = s * S::Panels + p;
-            const Scale sc(k.scale[h][gi >> 1], gi);
+            const Scale sc(k.scale[h][0], p);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) sts128((base ^ (i * k_flip)) + p * kPanel + h * 1024, values8(k.key_word(h, gi, i), sc));
+            for (int i = 0; i < 2; ++i) sts128((base ^ (i * k_flip)) + p * kPanel + h * 1024, values8(k.key_word(h, p, i), sc));
           }
         filled();
+        k.next_slot();
       }
     };
     auto store_values = [&](int j) {
@@ -474,18 +492,17 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
           }
         __syncwarp();
       }
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < S::PerTile; ++s) {
         const uint32_t base = ring + slot * S::Slot;
         wait(&C.empty[slot], (round & 1) ^ 1, C, a);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int p = 0; p < S::Panels; ++p) {
-            const int gi = s * S::Panels + p;
-            sts128(base + (u & 1 ? v_off1 : v_off0) + p * kPanel + (u >> 1) * 1024, values8(v.value_word(u, gi), Scale(v.scale[u][gi >> 1], gi)));
-          }
+          for (int p = 0; p < S::Panels; ++p)
+            sts128(base + (u & 1 ? v_off1 : v_off0) + p * kPanel + (u >> 1) * 1024, values8(v.value_word(u, p), Scale(v.scale[u][0], p)));
         filled();
+        v.next_slot();
       }
     };
     // in the order in which the products take them; what is stored is loaded again at once, for the tile after
@@ -687,20 +704,27 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         for (int i = 0; i < 32; ++i)
           if (base + i < from || base + i >= to) s[i] = -INFINITY;
       };
-      uint32_t raw[2][32];
-      tmem_ld32(scores, raw[0]);
+      uint32_t r0[32], r1[32];              // 32 columns in work, 32 on their way
+      float *s0 = reinterpret_cast<float*>(r0), *s1 = reinterpret_cast<float*>(r1);
       float x = -INFINITY, y = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait();
-        tmem_ld32(scores + ((c + 1) & 3) * 32, raw[(c + 1) & 1]);     // after the last the first again
-        float* s = reinterpret_cast<float*>(raw[c & 1]);
-        if (mask) hide(s, c * 32);
+      auto most = [&](const float* s) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           x = fmaxf(x, fmaxf(s[i], s[i + 1]));
           y = fmaxf(y, fmaxf(s[i + 2], s[i + 3]));
         }
+      };
+      tmem_ld32(scores, r0);
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 64) {
+        tmem_ld_wait();
+        tmem_ld32(scores + c + 32, r1);
+        if (mask) hide(s0, c);
+        most(s0);
+        tmem_ld_wait();
+        tmem_ld32(scores + (c ^ 64), r0);   // after the last the first again
+        if (mask) hide(s1, c + 32);
+        most(s1);
       }
       x = fmaxf(x, y) * scale;
       float before = m;                     // the maximum that O stands at
@@ -736,12 +760,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         }
       }
       float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait();
-        if (c < 3) tmem_ld32(scores + (c + 1) * 32, raw[(c + 1) & 1]);
-        float* s = reinterpret_cast<float*>(raw[c & 1]);
-        if (mask) hide(s, c * 32);
+      auto weigh = [&](const float* s, uint32_t to) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -751,7 +770,18 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
           sum = add_f32x2(sum, e);
           p[i] = pack_bf16x2(e.x, e.y);
         }
-        tmem_st16(scores + c * 16, p);      // over scores that have been read: 16 columns of weights to 32
+        tmem_st16(to, p);                   // over scores that have been read: 16 columns of weights to 32
+      };
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 64) {
+        tmem_ld_wait();
+        tmem_ld32(scores + c + 32, r1);
+        if (mask) hide(s0, c);
+        weigh(s0, scores + c / 2);
+        tmem_ld_wait();
+        if (c == 0) tmem_ld32(scores + 64, r0);
+        if (mask) hide(s1, c + 32);
+        weigh(s1, scores + c / 2 + 16);
       }
       l += sum.x + sum.y;
       tmem_st_wait();
@@ -867,17 +897,17 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
 
 // ---- the warp that lists the segments
 template <int Rows>
-__device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per, int u0, int u1, int lane) {
+__device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int64_t per, int64_t u0, int64_t u1, int lane) {
   Walk<Rows> w;
-  w.b = C.found[0];
+  w.b = C.found;
   w.load(a);
   w.u = u0;
   w.u1 = u1;
   {  // the head and row block that u0 lies in: the lanes bisect together, 32 places at a time
-    const int64_t each = tiles_before(w.it, w.blocks);
-    const int64_t off = u0 - C.found[1];
+    const int each = tiles_before(w.it, w.blocks);
+    const int64_t off = u0 - C.found_at;
     w.head = static_cast<int>(off / each);
-    const int64_t rest = off - w.head * each;
+    const int rest = static_cast<int>(off - static_cast<int64_t>(w.head) * each);
     int low = 0, high = w.blocks;           // tiles_before(low) <= rest < tiles_before(high)
     while (high - low > 1) {
       const int step = (high - low + 31) / 32, at = min(low + lane * step, high);
@@ -887,7 +917,7 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per
       low += k * step;
     }
     w.rb = low;
-    w.at = C.found[1] + static_cast<int>(w.head * each + tiles_before(w.it, low));
+    w.at = C.found_at + static_cast<int64_t>(w.head) * each + tiles_before(w.it, low);
   }
   w.open();
   for (uint32_t n = 0;; ++n) {
@@ -898,7 +928,7 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int per
     if (lane == 0) {
       const int tok = v.rb * v.it.tb;
       C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
-                          v.it.first_tile(v.rb) + v.t0, none ? 0 : v.t1 - v.t0, v.i0 / per, (v.i0 + v.tiles - 1) / per,
+                          v.it.first_tile(v.rb) + v.t0, none ? 0 : v.t1 - v.t0, static_cast<int>(v.i0 / per), static_cast<int>((v.i0 + v.tiles - 1) / per),
                           v.t1 - v.t0 == v.tiles, more};
       mbar_arrive(&C.seg_full[n % kSegs]);
     }
@@ -915,37 +945,38 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
 
   // this CTA's run of all tiles
   const int chunk = (a.batch + kThreads - 1) / kThreads;
-  int mine = 0;
+  long long mine = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     const Item it = item_of(a, request_of(a, b, blockIdx.x == 0), S::Rows);
-    mine += static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
+    mine += static_cast<long long>(tiles_before(it, it.blocks())) * a.hk;
   }
-  int upto = mine;
+  long long upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    const long long x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
     if (lane >= d) upto += x;
   }
   if (lane == 31) C.wsum[warp] = upto;
   __syncthreads();
-  int total = 0;
+  long long total = 0;
   for (int i = 0; i < kThreads / 32; ++i) {
     if (i < warp) upto += C.wsum[i];
     total += C.wsum[i];
   }
-  const int per = (total + gridDim.x - 1) / static_cast<int>(gridDim.x);
-  const int u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  const long long per = (total + gridDim.x - 1) / gridDim.x, u0 = blockIdx.x * per, u1 = min(u0 + per, total);
   if (u0 >= u1) return;                     // the whole CTA, before anything is allocated
   if (upto - mine <= u0 && u0 < upto) {
-    int at = upto - mine, b = tid * chunk;
-    for (;; ++b) {
-      const Item it = item_of(a, request_of(a, b, false), S::Rows);
-      const int cost = static_cast<int>(tiles_before(it, it.blocks())) * a.hk;
-      if (at + cost > u0) break;
-      at += cost;
-    }
-    C.found[0] = b;
-    C.found[1] = at;
+    long long at = upto - mine;
+    int b = tid * chunk;
+    if (chunk > 1)
+      for (;; ++b) {
+        const Item it = item_of(a, request_of(a, b, false), S::Rows);
+        const long long cost = static_cast<long long>(tiles_before(it, it.blocks())) * a.hk;
+        if (at + cost > u0) break;
+        at += cost;
+      }
+    C.found = b;
+    C.found_at = at;
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&C.tmem, 512);
@@ -969,12 +1000,12 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   __syncthreads();
   tc_fence_after();
 
-  if (warp < kSoftmaxWarps) {
-    reg_inc<kSoftmaxRegs>();
-    softmax_role<D>(a, C, warp, lane);
-  } else if (warp < kSoftmaxWarps + kFillWarps) {
+  if (warp >= kFirstFill) {
     reg_dec<kFillRegs>();
-    fill_role<D>(a, smem, C, warp - kSoftmaxWarps, lane);
+    fill_role<D>(a, smem, C, warp - kFirstFill, lane);
+  } else if (warp >= kFirstSoftmax) {
+    reg_inc<kSoftmaxRegs>();
+    softmax_role<D>(a, C, warp - kFirstSoftmax, lane);
   } else {
     reg_dec<kRestRegs>();
     if (warp == kMmaWarp) mma_role<D>(a, smem, C);
