@@ -22,7 +22,13 @@ def test_every_declared_symbol_is_exported(attention_lib):
 
 
 def test_return_codes_before_any_cuda_call(attention_lib):
-    lib = A._load()
+    lib = ctypes.CDLL(attention_lib)
+    vp, i, i64, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+    lib.mono_attn_plan.argtypes = [vp, vp, i, vp, i, vp, i, vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mono_attn_qk_norm_rope.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, i, i, f, vp, i, i, i, vp, i, i, i, i, vp, vp, vp, i64, i64, vp, i64, i,
+                                           vp, vp, vp]
+    lib.mono_attn_kv4_append.argtypes = [vp, i64, i64, vp, i64, i64, i, i, i, vp, i64, i, vp, vp, vp]
+    lib.mono_attn_kv4_attention.argtypes = [vp, i64, i64, vp, i64, i, vp, i, vp, vp, i, i, i, i, i, i, f, i, vp, vp, vp, z, vp, vp]
     p = ctypes.addressof(ctypes.create_string_buffer(64))
     good = [p, p, 2, p, 4, p, 8, p, 16, 5, p, p, p, p, p, p, p, 0]
     for at, value, code in ((2, 0, -202), (2, A.MAX_REQUESTS + 1, -202), (8, 24, -202), (8, 8, -202), (0, 0, -201), (12, 0, -201), (16, 0, -201)):
@@ -87,7 +93,7 @@ def test_cache_refuses_other_types_sizes_and_strides():
             A.KV4Cache.empty(1, 1, dim, page, "cpu")
 
 
-def test_operators_refuse_cpu_tensors():
+def test_operators_refuse_cpu_tensors(attention_lib):
     i = torch.zeros(1, dtype=torch.int32)
     x = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
     cache = A.KV4Cache.empty(1, 1, 64, 16, "cpu")

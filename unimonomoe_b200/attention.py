@@ -5,14 +5,15 @@
 * ``kv4_append``, ``kv4_read``   keys and values into the cache by slot, and back
 * ``kv4_attention``   attention of single tokens, guessed tokens, chunks and whole prompts over the cache
 
-Host side of ``libmono_attention.so`` (include/mono_attention.h): arguments are checked, outputs and workspaces made, the
-launch goes to the current stream. Shapes, types and devices raise ValueError before anything is launched. What only the
-device knows (slots, pages, lengths) is checked there: the access is left out and the first fault kept in a status word, which
+Host side of ``libmono_attention.so`` (include/mono_attention.h): arguments are checked, outputs and workspaces made (in C++,
+csrc/attention/binding.cpp), the launch goes to the current stream. Shapes, types and devices raise ValueError before anything is
+launched. The workspace of ``kv4_attention`` is kept for each stream: launches on one stream, or graphs captured on it, must
+not overlap. What only the device knows (slots, pages, lengths) is checked there: the access is left out and the first fault kept in a status word, which
 ``check_status`` reads. There is no CPU or library fallback.
 """
 from __future__ import annotations
 
-import ctypes
+import importlib.util
 import os
 from typing import NamedTuple, Optional
 
@@ -28,7 +29,7 @@ BLOCK = 16                                   # tokens of a block
 HEAD_DIMS = (64, 128, 256)
 MAX_REQUESTS = 16384
 
-_lib = None
+_C = None
 
 
 def attention_lib_path() -> str:
@@ -37,104 +38,30 @@ def attention_lib_path() -> str:
 
 
 def _load():
-    global _lib
-    if _lib is None:
-        path = attention_lib_path()
+    """The Python module next to the library (csrc/attention/binding.cpp): checks, outputs, launches."""
+    global _C
+    if _C is None:
+        path = os.path.join(os.path.dirname(attention_lib_path()), "_mono_attention.so")
         try:
-            lib = ctypes.CDLL(path)
-        except OSError as e:
+            spec = importlib.util.spec_from_file_location("_mono_attention", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
             raise RuntimeError(f"{path} cannot be loaded; build it with `python -m unimonomoe_b200.build attention`") from e
-        p, i, l, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
-        lib.mono_attn_plan.argtypes = [p, p, i, p, i, p, i, p, i, i, p, p, p, p, p, p, p, p]
-        lib.mono_attn_qk_norm_rope.argtypes = [p, l, l, p, l, l, p, p, i, i, f, p, i, i, i, p, i, i, i, i, p, p, p, l, l, p, l, i,
-                                               p, p, p]
-        lib.mono_attn_kv4_append.argtypes = [p, l, l, p, l, l, i, i, i, p, l, i, p, p, p]
-        lib.mono_attn_kv4_read.argtypes = [p, l, i, p, i, i, i, p, p, p, p]
-        lib.mono_attn_kv4_attention.argtypes = [p, l, l, p, l, i, p, i, p, p, i, i, i, i, i, i, f, i, p, p, p, z, p, p]
-        lib.mono_attn_workspace_bytes.restype = z
-        _lib = lib
-    return _lib
-
-
-_ERRORS = {-201: "a required pointer is null", -202: "a size is out of its range", -203: "head size is not 64, 128 or 256",
-           -204: "workspace too small"}
-
-
-def _launched(name: str, rc: int) -> None:
-    if rc != 0:
-        raise RuntimeError(f"{name} failed: rc={rc}" + (f" ({_ERRORS[rc]})" if rc in _ERRORS else ""))
-
-
-# ---------------------------------------------------------------------- device state
-_status = {}
-_workspaces = {}
-
-
-def _status_word(device: torch.device) -> torch.Tensor:
-    s = _status.get(device.index)
-    if s is None:
-        s = _status[device.index] = torch.zeros(2, dtype=torch.int32, device=device)
-    return s
+        _C = module
+    return _C
 
 
 def check_status(device=None) -> None:
     """Synchronise and raise if a launch on this device has reported a fault since the last call."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    word = _status.get(torch.cuda.current_device() if dev.index is None else dev.index)
-    if word is None:
-        return
-    torch.cuda.synchronize(word.device)
+    dev = torch.device("cuda" if device is None else device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    word = _load().status_tensor(index)
+    torch.cuda.synchronize(index)
     code, where = word.tolist()
     if code:
         word.zero_()
         raise RuntimeError(f"attention device status: {STATUS_CODES.get(code, code)} (code {code}, at {where})")
-
-
-def _workspace(device: torch.device, stream: int) -> torch.Tensor:
-    """Scratch of the attention launches, one per device and stream, its counters zero between launches. A capture that finds
-    none gets buffers of its own, so that the capture's memory pool owns them."""
-    key = (device.index, stream)
-    ws = _workspaces.get(key)
-    if ws is None:
-        ws = torch.empty(_load().mono_attn_workspace_bytes(), dtype=torch.uint8, device=device)
-        ws[:1 << 16].zero_()
-        if not torch.cuda.is_current_stream_capturing():
-            _workspaces[key] = ws
-    return ws
-
-
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _cuda(name: str, t: torch.Tensor, dtype=None, device=None) -> torch.Tensor:
-    if not t.is_cuda:
-        raise ValueError(f"{name} is on {t.device}; these operators need a CUDA device, there is no CPU path")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    return t
-
-
-def _ints(name: str, t: torch.Tensor, shape, device, dtype=torch.int32) -> torch.Tensor:
-    _cuda(name, t, dtype, device)
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _rows(name: str, t: torch.Tensor, device=None) -> torch.Tensor:
-    """bf16 [tokens, heads, head_dim] with 16-byte rows; any other layout is copied into one."""
-    _cuda(name, t, torch.bfloat16, device)
-    if t.dim() != 3:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [tokens, heads, head_dim]")
-    a, b, c = t.stride()
-    if c != 1 or (a | b) & 7 or t.data_ptr() & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
-    return t
 
 
 def _head_dim(d: int) -> int:
@@ -147,23 +74,6 @@ def _page_size(p: int) -> int:
     if p < 16 or p > 1024 or p & (p - 1):
         raise ValueError(f"page size {p}; a power of two from 16 to 1024 is needed")
     return p
-
-
-class _On:
-    """The tensor's device as the current one, where it is not already."""
-
-    def __init__(self, device):
-        self.device, self.before = device, None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.device.index:
-            self.before = now
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
 
 
 # ---------------------------------------------------------------------- the cache
@@ -238,35 +148,8 @@ def plan_batch(cached_lens, new_lens, block_table, free_pages, taken, page_size:
     ``taken`` (int32 [1]) are in use. New pages are taken from the list in the order of the requests and entered into
     ``block_table`` in place. ``num_tokens`` is the number of rows of the result: rows behind the last token hold position
     0, slot -1, request -1, so a captured graph serves any smaller step. Nothing is read back to the host."""
-    dev = _cuda("cached_lens", cached_lens, torch.int32).device
-    B = cached_lens.numel()
-    if not 1 <= B <= MAX_REQUESTS:
-        raise ValueError(f"{B} requests; 1 to {MAX_REQUESTS} are planned at a time")
-    cached_lens, new_lens = _ints("cached_lens", cached_lens, (B,), dev), _ints("new_lens", new_lens, (B,), dev)
-    _cuda("block_table", block_table, torch.int32, dev)
-    if block_table.dim() != 2 or block_table.size(0) != B or block_table.size(1) < 1 or not block_table.is_contiguous():
-        raise ValueError(f"block_table must be contiguous int32 [{B}, pages], got {tuple(block_table.shape)}")
-    free_pages, taken = _ints("free_pages", free_pages, (free_pages.numel(),), dev), _ints("taken", taken, (1,), dev)
-    num_tokens = int(num_tokens)
-    if num_tokens < 0:
-        raise ValueError(f"num_tokens is {num_tokens}")
-    _page_size(page_size)
-    lib = _load()
-    with _On(dev):
-        new = lambda n, dt=torch.int32: torch.empty(n, dtype=dt, device=dev)  # noqa: E731
-        p = BatchPlan(new(B + 1), new(B), new(num_tokens), new(num_tokens, torch.int64), new(num_tokens), new(1))
-        _launched("mono_attn_plan", lib.mono_attn_plan(
-            cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), block_table.size(1), free_pages.data_ptr(),
-            free_pages.numel(), taken.data_ptr(), page_size, num_tokens, p.query_start.data_ptr(), p.seq_lens.data_ptr(),
-            p.positions.data_ptr(), p.slots.data_ptr(), p.requests.data_ptr(), p.taken.data_ptr(), _status_word(dev).data_ptr(),
-            _stream(dev)))
-    return p
+    return BatchPlan(*(_C or _load()).plan(cached_lens, new_lens, block_table, free_pages, taken, page_size, num_tokens))
 
-
-def _check_cache(cache: KV4Cache, kv_heads: int, head_dim: int, device) -> None:
-    if cache.kv_heads != kv_heads or cache.head_dim != head_dim or cache.device != device:
-        raise ValueError(f"cache holds {cache.kv_heads} KV heads of {cache.head_dim} on {cache.device}, the call has {kv_heads} of "
-                         f"{head_dim} on {device}")
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps: float = 1e-6, interleaved: bool = False,
@@ -278,85 +161,22 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps: float = 1e-6
 
     With ``cache``, ``v`` and ``slots`` the rotated keys and the values are stored in the cache in the same launch, the same
     codes as ``kv4_append`` of the results; only q is returned."""
-    q = _rows("q", q)
-    dev = q.device
-    k = _rows("k", k, dev)
-    T, H, D = q.shape
-    K = k.size(1)
-    _head_dim(D)
-    if k.size(0) != T or k.size(2) != D or not H or not K:
-        raise ValueError(f"q is {tuple(q.shape)}, k is {tuple(k.shape)}: tokens and head size must agree")
-    if q_weight.dtype not in (torch.bfloat16, torch.float32) or k_weight.dtype != q_weight.dtype:
-        raise ValueError(f"norm weights must both be bfloat16 or float32, got {q_weight.dtype} and {k_weight.dtype}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if _cuda(name, w, None, dev).shape != (D,) or not w.is_contiguous() or w.data_ptr() & 15:
-            raise ValueError(f"{name} must be contiguous [{D}] on a 16-byte boundary, got {tuple(w.shape)}")
-    _cuda("cos_sin", cos_sin, torch.float32, dev)
-    if cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15:
-        raise ValueError(f"cos_sin must be contiguous fp32 [positions, rotary_dim], got {tuple(cos_sin.shape)}")
-    R = cos_sin.size(1)
-    if R % 16 or R > D:
-        raise ValueError(f"rotary dim {R}; a multiple of 16 up to the head size {D} is needed")
-    if R and not cos_sin.size(0):
-        raise ValueError("cos_sin has no rows")
-    positions = _ints("positions", positions, (T,), dev)
-    stored = (0, 0, 0, 0, 0, 16, 0)
-    if cache is not None:
-        if v is None or slots is None:
-            raise ValueError("storing into a cache needs v and slots")
-        v = _rows("v", v, dev)
-        if v.shape != k.shape:
-            raise ValueError(f"v is {tuple(v.shape)}, k is {tuple(k.shape)}")
-        _check_cache(cache, K, D, dev)
-        slots = _ints("slots", slots, (T,), dev, torch.int64)
-        stored = (v.data_ptr(), v.stride(0), v.stride(1), cache.data.data_ptr(), cache.num_pages, cache.page_size, slots.data_ptr())
-    elif v is not None or slots is not None:
-        raise ValueError("v and slots are stored in a cache, and none is given")
-    lib = _load()
-    with _On(dev):
-        q_out = torch.empty((T, H, D), dtype=torch.bfloat16, device=dev)
-        k_out = None if cache is not None else torch.empty((T, K, D), dtype=torch.bfloat16, device=dev)
-        _launched("mono_attn_qk_norm_rope", lib.mono_attn_qk_norm_rope(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), q_weight.data_ptr(), k_weight.data_ptr(),
-            q_weight.dtype == torch.float32, bool(unit_offset), float(eps), cos_sin.data_ptr(), cos_sin.size(0), R, bool(interleaved),
-            positions.data_ptr(), T, H, K, D, q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), *stored,
-            _status_word(dev).data_ptr(), _stream(dev)) if T else 0)
-    return q_out if k_out is None else (q_out, k_out)
+    return (_C or _load()).qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, unit_offset, v,
+                                        None if cache is None else cache.data, slots)
+
 
 
 def kv4_append(k, v, cache: KV4Cache, slots) -> None:
     """Stores ``k`` and ``v`` (bf16 [tokens, kv_heads, head_dim], any strides) in the cache at ``slots`` (int64 [tokens], -1: not
     stored). No slot may be given twice."""
-    k = _rows("k", k)
-    dev = k.device
-    v = _rows("v", v, dev)
-    T, K, D = k.shape
-    if v.shape != k.shape:
-        raise ValueError(f"v is {tuple(v.shape)}, k is {tuple(k.shape)}")
-    _check_cache(cache, K, D, dev)
-    slots = _ints("slots", slots, (T,), dev, torch.int64)
-    if not T:
-        return
-    lib = _load()
-    with _On(dev):
-        _launched("mono_attn_kv4_append", lib.mono_attn_kv4_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), T, K, D, cache.data.data_ptr(),
-            cache.num_pages, cache.page_size, slots.data_ptr(), _status_word(dev).data_ptr(), _stream(dev)))
+    (_C or _load()).kv4_append(k, v, cache.data, slots)
+
 
 
 def kv4_read(cache: KV4Cache, slots):
     """What the cache holds at ``slots`` (int64 [tokens]) as (k, v), bf16 [tokens, kv_heads, head_dim], exactly; zeros at -1."""
-    dev = _cuda("cache", cache.data).device
-    T = slots.numel()
-    slots = _ints("slots", slots, (T,), dev, torch.int64)
-    lib = _load()
-    with _On(dev):
-        k, v = (torch.empty((T, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=dev) for _ in range(2))
-        if T:
-            _launched("mono_attn_kv4_read", lib.mono_attn_kv4_read(
-                cache.data.data_ptr(), cache.num_pages, cache.page_size, slots.data_ptr(), T, cache.kv_heads, cache.head_dim,
-                k.data_ptr(), v.data_ptr(), _status_word(dev).data_ptr(), _stream(dev)))
-    return k, v
+    return (_C or _load()).kv4_read(cache.data, slots)
+
 
 
 def kv4_attention(q, cache: KV4Cache, block_table, seq_lens, query_start, max_query_len: int, scale: Optional[float] = None,
@@ -370,35 +190,4 @@ def kv4_attention(q, cache: KV4Cache, block_table, seq_lens, query_start, max_qu
     heads]. A query that sees no key gets zeros and -inf. Rows that belong to no request are left as they are.
 
     ``max_query_len``: the largest number of queries of a request, or anything above; it chooses kernels, never results."""
-    q = _rows("q", q)
-    dev = q.device
-    T, H, D = q.shape
-    K = cache.kv_heads
-    _check_cache(cache, K, D, dev)
-    if not H or H % K:
-        raise ValueError(f"{H} query heads over {K} KV heads")
-    B = seq_lens.numel()
-    _cuda("block_table", block_table, torch.int32, dev)
-    if block_table.dim() != 2 or block_table.size(0) != B or not block_table.size(1) or not block_table.is_contiguous():
-        raise ValueError(f"block_table must be contiguous int32 [{B}, pages], got {tuple(block_table.shape)}")
-    if B > MAX_REQUESTS:
-        raise ValueError(f"{B} requests; up to {MAX_REQUESTS} are taken at a time")
-    seq_lens, query_start = _ints("seq_lens", seq_lens, (B,), dev), _ints("query_start", query_start, (B + 1,), dev)
-    if window < 0 or max_query_len < 0:
-        raise ValueError(f"window is {window}, max_query_len is {max_query_len}")
-    if out is None:
-        out = torch.empty((T, H, D), dtype=torch.bfloat16, device=dev)
-    elif out.shape != (T, H, D) or _cuda("out", out, torch.bfloat16, dev).data_ptr() & 15 or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous bfloat16 [{T}, {H}, {D}] on a 16-byte boundary, got {tuple(out.shape)}")
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-    if T and B:
-        lib = _load()
-        with _On(dev):
-            stream = _stream(dev)
-            ws = _workspace(dev, stream)
-            _launched("mono_attn_kv4_attention", lib.mono_attn_kv4_attention(
-                q.data_ptr(), q.stride(0), q.stride(1), cache.data.data_ptr(), cache.num_pages, cache.page_size,
-                block_table.data_ptr(), block_table.size(1), seq_lens.data_ptr(), query_start.data_ptr(), B, T, int(max_query_len),
-                H, K, D, D ** -0.5 if scale is None else float(scale), int(window), out.data_ptr(),
-                0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), _status_word(dev).data_ptr(), stream))
-    return (out, lse) if return_lse else out
+    return (_C or _load()).kv4_attention(q, cache.data, block_table, seq_lens, query_start, max_query_len, scale, window, out, return_lse)

@@ -108,11 +108,44 @@ def attention_lib_path() -> str:
     return os.path.join(LIBDIR, "libmono_attention.so")
 
 
+def attention_binding_path() -> str:
+    return os.path.join(LIBDIR, "_mono_attention.so")
+
+
+def _run(what: str, cmd: list) -> None:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stdout}{r.stderr}")
+
+
+def _compile_binding() -> str:
+    """The Python module of csrc/attention/binding.cpp, against torch's own headers and ABI."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    obj, abi = os.path.join(LIBDIR, "binding.o"), int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
+    include = [*cpp_extension.include_paths(), os.path.join(home, "include"), sysconfig.get_paths()["include"]]
+    _run("g++ for binding.cpp", [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_CUDA",
+                                 *(f"-isystem{i}" for i in dict.fromkeys(include)), "-c", os.path.join(ATTENTION, "binding.cpp"), "-o", obj])
+    return obj
+
+
+def _link_binding(obj: str) -> None:
+    from torch.utils import cpp_extension
+    libs = cpp_extension.library_paths()
+    _run("linking _mono_attention.so", [os.environ.get("CXX", "g++"), "-shared", obj, "-o", attention_binding_path(), *(f"-L{p}" for p in libs),
+                                        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{LIBDIR}", "-lmono_attention",
+                                        "-Wl,-rpath,$ORIGIN"])
+
+
 def build_attention(force: bool = False, verbose: bool = False) -> str:
-    """The attention half of the layer (include/mono_attention.h): one library for every geometry."""
+    """The attention half of the layer (include/mono_attention.h): one library for every geometry, and its Python module."""
     out, header = attention_lib_path(), os.path.join(HERE, "..", "include", "mono_attention.h")
     used = [os.path.join(ATTENTION, f) for f in os.listdir(ATTENTION)] + [os.path.join(CSRC, "ptx_sm100.cuh"), header, __file__]
-    if not force and os.path.exists(out) and all(os.path.getmtime(f) <= os.path.getmtime(out) for f in used):
+    outs = (out, attention_binding_path())
+    if not force and all(os.path.exists(o) and all(os.path.getmtime(f) <= os.path.getmtime(o) for f in used) for o in outs):
         return out
     os.makedirs(LIBDIR, exist_ok=True)
     nvcc = [os.environ.get("NVCC", "nvcc"), "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -125,9 +158,13 @@ def build_attention(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}{r.stderr}")
         return obj, r.stdout + r.stderr
 
-    with ThreadPoolExecutor(max_workers=len(ATTENTION_SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(ATTENTION_SOURCES) + 1) as ex:
+        binding = ex.submit(_compile_binding)
         built = list(ex.map(compile_one, ATTENTION_SOURCES))
+        binding_obj = binding.result()
     r = subprocess.run([*nvcc, "-shared", *(obj for obj, _ in built), "-o", out], capture_output=True, text=True)
+    if r.returncode == 0:
+        _link_binding(binding_obj)
     log = "".join(text for _, text in built) + r.stdout + r.stderr
     with open(out + ".log", "w") as f:
         f.write(log)
