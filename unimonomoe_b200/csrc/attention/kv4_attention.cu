@@ -24,6 +24,7 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   if (batch < 0 || tokens < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || table_width < 1 || num_pages < 1 ||
       window < 0 || max_query_len < 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
     return MONO_ATTN_BAD_SIZE;
+  if (static_cast<int64_t>(kv_heads) * page_size / 16 * block_bytes(head_dim) > INT32_MAX) return MONO_ATTN_BAD_SIZE;   // bytes of a page
   if (batch == 0 || tokens == 0) return 0;
   if (!q || !cache || !block_table || !seq_lens || !query_start || !out || !workspace || !status) return MONO_ATTN_NULL;
   if (workspace_bytes < mono_attn_workspace_bytes()) return MONO_ATTN_WORKSPACE;

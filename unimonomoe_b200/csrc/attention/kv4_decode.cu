@@ -39,10 +39,11 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1,
+                                         float c2, float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ void mma16816_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -60,8 +61,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 // c + 8 in the low four bits of both halves, to c as bf16.
-__device__ __forceinline__ uint32_t signed_code(uint32_t x) {
-  const uint32_t y = (x & 0x000F000Fu) | 0x43004300u, off = 0x43084308u;
+// (mask and exponent in registers: with both as immediates it is two instructions)
+__device__ __forceinline__ uint32_t signed_code(uint32_t x, uint32_t mask, uint32_t magic) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(magic));   // (x & mask) | magic
+  const uint32_t off = 0x43084308u;
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -77,8 +81,11 @@ struct Shape {
   static constexpr int Stages = D == 256 ? 2 : 3;
   static constexpr int Ring = Stages * Stage;           // of a warp
   static constexpr int Part = Rows * (D + 2);           // floats of a warp's or a CTA's state: output, maximum, sum
-  static constexpr int Smem = kWarps * (Ring > Part * 4 ? Ring : (Part * 4 + 15) / 16 * 16);
   static constexpr int PerSm = D == 256 ? 3 : NT == 2 && D == 128 ? 3 : 4;
+  static constexpr int Ctas = MONO_ATTN_SMS * PerSm;
+  static constexpr int Warp = Ring > Part * 4 ? Ring : (Part * 4 + 15) / 16 * 16;   // shared memory of a warp: its ring, then its state
+  static constexpr int Join = (Rows * Ctas * 4 + 15) / 16 * 16;   // the weights of all CTAs' states
+  static constexpr int Smem = kWarps * Warp > Join ? kWarps * Warp : Join;
 };
 
 // Steps of one item of a request; 0 if the request is not this kernel's.
@@ -98,8 +105,12 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
   __shared__ int s_sum[kWarps];
   __shared__ int s_found[2];
   __shared__ int s_last;
+  __shared__ float s_ms[S::Rows][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * (S::Smem / kWarps);
+  uint32_t mask4, magic;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask4));
+  asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
+  uint8_t* ring = smem + warp * S::Warp;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
 
   // this CTA's run [u0, u1) of all steps, and the request that it begins in
@@ -164,8 +175,9 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
     const int clear_hi = max(place0 + tok_first + 1, 0), clear_lo = a.window > 0 ? max(place0 + tok_last + 1 - a.window, 0) : 0;
 
     // query: B operand, row n = g of each tile; scaled by a power of two to an fp16 with its largest value near 2^14
+    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // the query carries the scale's sign
     uint32_t qf[NT][4 * NG][2];
-    float fac[NT][2], qs[NT][NG][2];
+    float fac[NT][2], room[NT][2], qs[NT][NG][2];
     int hi_r[NT][2], lo_r[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -179,7 +191,9 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p + 64 * gi + 16 * t + 8 * w)), x[gi][w]);
+            uint4 raw = __ldg(reinterpret_cast<const uint4*>(p + 64 * gi + 16 * t + 8 * w));
+            raw = make_uint4(raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip);
+            unpack_bf16x8(raw, x[gi][w]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[gi][w][j]) & 0x7FFFFFFFu);
           }
@@ -193,7 +207,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const int ex = min(max(static_cast<int>(top >> 23) - 127, -100), 100);
       const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
-      const float f = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(24 - 14 + ex + 127) << 23);
+      const float f = fmaxf(fabsf(a.scale_log2), 1e-37f) * __uint_as_float(static_cast<uint32_t>(24 - 14 + ex + 127) << 23);
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
         float sum = 0.0f;
@@ -215,6 +229,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       }
       fac[nt][0] = __shfl_sync(0xFFFFFFFFu, f, 8 * t);
       fac[nt][1] = __shfl_sync(0xFFFFFFFFu, f, 8 * t + 4);
+      room[nt][0] = kRoom / fac[nt][0];
+      room[nt][1] = kRoom / fac[nt][1];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {          // what row 2t + c of the tile sees: [lo_r, hi_r)
         const int rr = nt * 8 + 2 * t + c, place = place0 + (rb * S::Rows + rr) / a.group;
@@ -223,7 +239,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       }
     }
 
-    float o[NT][4 * NG][4], l[NT][2], m[NT][2];
+    // running maximum of the unscaled scores, and what it takes off the scaled ones (nothing before there is one)
+    float o[NT][4 * NG][4], l[NT][2], m[NT][2], off[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -232,55 +249,53 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.0f;
       l[nt][0] = l[nt][1] = 0.0f;
       m[nt][0] = m[nt][1] = kLow;
+      off[nt][0] = off[nt][1] = 0.0f;
     }
 
     // this warp's pairs of blocks: the warp-th, the (warp + 4)-th, ... of [k0, k1)
     const int pairs = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;
     const int count = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
-    const int per_page = 1 << (a.shift - 4);
-    auto fetch = [&](int i, int (&pg)[2]) {  // pages of the i-th pair
-      const int blk = (k0 >> 4) + 2 * (warp + kWarps * i);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) pg[h] = i < count && (blk + h) * 16 < k1 ? page_of(a, b, (blk + h) >> (a.shift - 4)) : -1;
+    const int page_shift = a.shift - 4, in_page = (1 << page_shift) - 1, blk0 = (k0 >> 4) + 2 * warp;
+    const uint8_t* head_at = a.cache + static_cast<int64_t>(head << page_shift) * S::Block + lane * 16;
+    const int page_bytes = (a.hk << page_shift) * S::Block;
+    // pages of 16 pairs at a time, those of the next 16 on their way: lane 2 i + h has block h of pair i
+    auto pages_of = [&](int i0) {
+      const int blk = blk0 + 2 * kWarps * (i0 + (lane >> 1)) + (lane & 1);
+      return blk * 16 < k1 ? page_of(a, b, blk >> page_shift) : 0;
     };
-    auto issue = [&](int i, const int (&pg)[2]) {
-      const int blk = (k0 >> 4) + 2 * (warp + kWarps * i);
+    int pages = pages_of(0), later = count > 16 ? pages_of(16) : 0, wstage = 0, rstage = 0;
+    auto issue = [&](int i) {
+      if (i < count) {
+        if ((i & 15) == 0 && i > 0) {
+          pages = later;
+          if (i + 16 < count) later = pages_of(i + 16);
+        }
+        const int blk = blk0 + 2 * kWarps * i;
+        const uint32_t to = ring_at + wstage * S::Stage + lane * 16;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (pg[h] >= 0) {
-          const uint8_t* src = a.cache + ((static_cast<int64_t>(pg[h]) * a.hk + head) * per_page + ((blk + h) & (per_page - 1))) * S::Block;
-          const uint32_t dst = ring_at + (i % S::Stages) * S::Stage + h * S::Block;
+        for (int h = 0; h < 2; ++h) {
+          const int pg = __shfl_sync(0xFFFFFFFFu, pages, (i & 15) * 2 + h);
+          if (h == 0 || (blk + 1) * 16 < k1) {
+            const uint8_t* src = head_at + static_cast<int64_t>(pg) * page_bytes + ((blk + h) & in_page) * S::Block;
 #pragma unroll
-          for (int j = 0; j < (S::Block + 511) / 512; ++j) {
-            const int off = j * 512 + lane * 16;
-            if (off < S::Block) cp16(dst + off, src + off);
+            for (int j = 0; j < (S::Block + 511) / 512; ++j)
+              if ((j + 1) * 512 <= S::Block || lane < (S::Block - j * 512) / 16) cp16(to + h * S::Block + j * 512, src + j * 512);
           }
         }
+        if (++wstage == S::Stages) wstage = 0;
+      }
       cp_commit();
     };
-    int pg[2];
-    fetch(0, pg);
 #pragma unroll
-    for (int i = 0; i < S::Stages - 1; ++i) {
-      int nx[2];
-      fetch(i + 1, nx);
-      issue(i, pg);
-      pg[0] = nx[0];
-      pg[1] = nx[1];
-    }
+    for (int i = 0; i < S::Stages - 1; ++i) issue(i);
 
     for (int i = 0; i < count; ++i) {
-      {
-        int nx[2];
-        fetch(i + S::Stages, nx);
-        __syncwarp();                        // all lanes are done with the stage that is written now
-        issue(i + S::Stages - 1, pg);
-        pg[0] = nx[0];
-        pg[1] = nx[1];
-      }
+      __syncwarp();                          // all lanes are done with the stage that is written now
+      issue(i + S::Stages - 1);
       cp_wait<S::Stages - 1>();
       __syncwarp();
-      const uint8_t* stage = ring + (i % S::Stages) * S::Stage;
+      const uint8_t* stage = ring + rstage * S::Stage;
+      if (++rstage == S::Stages) rstage = 0;
       const int key0 = k0 + 32 * (warp + kWarps * i);
       const bool mask = key0 < clear_lo || key0 + 32 > clear_hi || key0 + 32 > k1;
 
@@ -320,17 +335,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[h][nt][c] = 0.0f;
-#pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
           float acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = acc[nt][2] = qs[nt][gi][0];
-            acc[nt][1] = acc[nt][3] = qs[nt][gi][1];
-          }
 #pragma unroll
           for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -338,8 +344,13 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
               const uint32_t x0 = kw[0][2 * gi + w] >> (8 * st), x1 = kw[1][2 * gi + w] >> (8 * st);
               const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u, a3 = x1 & 0x00F000F0u;
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816(acc[nt], a0, a1, a2, a3, qf[nt][gi * 4 + w * 2 + st][0], qf[nt][gi * 4 + w * 2 + st][1]);
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t b0 = qf[nt][gi * 4 + w * 2 + st][0], b1 = qf[nt][gi * 4 + w * 2 + st][1];
+                if (w == 0 && st == 0)
+                  mma16816(acc[nt], a0, a1, a2, a3, b0, b1, qs[nt][gi][0], qs[nt][gi][1], qs[nt][gi][0], qs[nt][gi][1]);
+                else
+                  mma16816(acc[nt], a0, a1, a2, a3, b0, b1, acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+              }
             }
           float f[2];
 #pragma unroll
@@ -347,12 +358,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[h][nt][c] = fmaf(acc[nt][c], f[c >> 1], s[h][nt][c]);
+            for (int c = 0; c < 4; ++c) s[h][nt][c] = gi == 0 ? acc[nt][c] * f[c >> 1] : fmaf(acc[nt][c], f[c >> 1], s[h][nt][c]);
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[h][nt][c] *= fac[nt][c & 1];
       }
       if (mask) {
 #pragma unroll
@@ -364,13 +371,57 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
               const int key = key0 + 16 * h + g + 8 * (c >> 1);
               if (key < lo_r[nt][c & 1] || key >= min(hi_r[nt][c & 1], k1)) s[h][nt][c] = -INFINITY;
             }
+        // Behind the last key there may be anything, and a value that is not a number must not reach the rows that do not see it (0
+        // times it is not 0): its scale becomes 0, and the output of the rows that see it what it would have become.
+        uint32_t bad = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr) {
+            const bool behind = key0 + 16 * h + g + 8 * rr >= k1;
+#pragma unroll
+            for (int j = 0; j < (NG + 1) / 2; ++j) {
+              if (behind) vs[h][rr][j] = 0;
+              if ((vs[h][rr][j] & 0x7FFFu) > 0x7F80u) bad |= 1u << ((h * 2 + rr) * 4 + 2 * j);
+              if ((vs[h][rr][j] & 0x7FFF0000u) > 0x7F800000u) bad |= 2u << ((h * 2 + rr) * 4 + 2 * j);
+            }
+          }
+        if (__any_sync(0xFFFFFFFFu, bad != 0)) {
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            uint32_t rows_hit = 0;           // bit 2 nt + c: row 2t + c of the tile sees a group gi that is not a number
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int rr = 0; rr < 2; ++rr)
+                if (bad >> ((h * 2 + rr) * 4 + gi) & 1u) {
+                  vs[h][rr][gi >> 1] &= gi & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                      const int key = key0 + 16 * h + g + 8 * rr;
+                      if (key >= lo_r[nt][c] && key < hi_r[nt][c]) rows_hit |= 1u << (2 * nt + c);
+                    }
+                }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) rows_hit |= __shfl_xor_sync(0xFFFFFFFFu, rows_hit, d);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                if (rows_hit >> (2 * nt + c) & 1u)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) o[nt][4 * gi + j][c] = o[nt][4 * gi + j][c + 2] = __uint_as_float(0x7FC00000u);
+          }
+        }
       }
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          grow |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + kRoom;
+          grow |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + room[nt][c];
       if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -380,8 +431,9 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
             x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
-            const float to = fmaxf(m[nt][c], x), by = ex2(m[nt][c] - to);
+            const float to = fmaxf(m[nt][c], x), by = ex2((m[nt][c] - to) * fac[nt][c]);
             m[nt][c] = to;
+            off[nt][c] = to > kLow ? -to * fac[nt][c] : 0.0f;
             l[nt][c] *= by;
 #pragma unroll
             for (int j = 0; j < 4 * NG; ++j) {
@@ -398,7 +450,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            p[nt][c] = ex2(s[h][nt][c] - m[nt][c & 1]);
+            p[nt][c] = ex2(fmaf(s[h][nt][c], fac[nt][c & 1], off[nt][c & 1]));
             l[nt][c & 1] += p[nt][c];
           }
         uint32_t vw[4][NG];
@@ -430,11 +482,6 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
             float w[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) w[c] = p[nt][c] * f[c >> 1];
-            if (mask) {                      // what lies behind the sequence, or is hidden from a row, may hold anything
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                if (s[h][nt][c] == -INFINITY) w[c] = 0.0f;
-            }
             pb[nt][0] = transpose8(pack_bf16x2(w[0], w[1]));
             pb[nt][1] = transpose8(pack_bf16x2(w[2], w[3]));
           }
@@ -444,8 +491,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
             const uint32_t y = __byte_perm(vw[2][gi], vw[3][gi], half ? 0x7632 : 0x5410);
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-              const uint32_t a0 = signed_code(x >> (8 * st)), a1 = signed_code(x >> (8 * st + 4));
-              const uint32_t a2 = signed_code(y >> (8 * st)), a3 = signed_code(y >> (8 * st + 4));
+              const uint32_t a0 = signed_code(x >> (8 * st), mask4, magic), a1 = signed_code(x >> (8 * st + 4), mask4, magic);
+              const uint32_t a2 = signed_code(y >> (8 * st), mask4, magic), a3 = signed_code(y >> (8 * st + 4), mask4, magic);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816_bf16(o[nt][gi * 4 + half * 2 + st], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
@@ -468,7 +515,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
         const int row = nt * 8 + 2 * t + c;
         if (g == 0) {
-          ml[2 * row] = m[nt][c];
+          ml[2 * row] = m[nt][c] > kLow ? m[nt][c] * fac[nt][c] : kLow;
           ml[2 * row + 1] = x;
         }
 #pragma unroll
@@ -489,7 +536,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
           make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
       if (d == 0 && a.lse) a.lse[static_cast<int64_t>(tok) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
     };
-    constexpr int Wf = S::Smem / kWarps / 4;             // floats from one warp's state to the next
+    constexpr int Wf = S::Warp / 4;             // floats from one warp's state to the next
     for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
       const int row = idx / (D / 4), d = idx % (D / 4) * 4;
       const float* base = reinterpret_cast<const float*>(smem);
@@ -522,22 +569,41 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       }
       __syncthreads();
       if (s_last) {
+        // the CTAs' weights first (one for each row and CTA, in shared memory), then their outputs, whose loads
+        // do not wait for one another
+        float* weight = reinterpret_cast<float*>(smem);
+        const int n = c1 - c0 + 1;
+        auto from = [&](int i) { return a.partial + (static_cast<int64_t>(c0 + i) * 2 + (i == 0 ? 1 : 0)) * S::Part; };
+        for (int row = warp; row < rows; row += kWarps) {
+          float mx = kLow, sum = 0.0f;
+          for (int i = lane; i < n; i += 32) mx = fmaxf(mx, __ldcg(from(i) + S::Rows * D + 2 * row));
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+          for (int i = lane; i < n; i += 32) {
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from(i) + S::Rows * D + 2 * row));
+            const float by = ex2(ms.x - mx);
+            weight[row * S::Ctas + i] = by;
+            sum = fmaf(ms.y, by, sum);
+          }
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+          if (lane == 0) {
+            s_ms[row][0] = mx;
+            s_ms[row][1] = sum;
+          }
+        }
+        __syncthreads();
         for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
           const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-          float mx = kLow, sum = 0.0f;
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const float* from = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
-            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + S::Rows * D + 2 * row));
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from + row * D + d));
-            const float to = fmaxf(mx, ms.x), old = ex2(mx - to), by = ex2(ms.x - to);
-            mx = to;
-            sum = fmaf(ms.y, by, sum * old);
-            x.x = fmaf(y.x, by, x.x * old); x.y = fmaf(y.y, by, x.y * old);
-            x.z = fmaf(y.z, by, x.z * old); x.w = fmaf(y.w, by, x.w * old);
+#pragma unroll 8
+          for (int i = 0; i < n; ++i) {
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(from(i) + row * D + d));
+            const float by = weight[row * S::Ctas + i];
+            x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y);
+            x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
           }
-          finish(row, d, x, mx, sum);
+          finish(row, d, x, s_ms[row][0], s_ms[row][1]);
         }
       }
     }
@@ -558,7 +624,7 @@ int launch(const AttnArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  decode_kernel<D, NT><<<MONO_ATTN_SMS * S::PerSm, kThreads, S::Smem, stream>>>(a);
+  decode_kernel<D, NT><<<S::Ctas, kThreads, S::Smem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -239,10 +239,22 @@ struct Scale {
 };
 // Eight codes of a word times their scale, dims 0 4 1 5 2 6 3 7: a code c + 8 as the top four bits of the mantissa under the
 // exponent of 16 is 24 + c, and (24 + c) s - 24 s is exact in one fused multiply-add.
-__device__ __forceinline__ uint4 values8(uint32_t w, const Scale& s) {
+// (Mask and exponent come in registers: with both as immediates masking is two instructions.)
+struct Codes { uint32_t mask, magic; };
+__device__ __forceinline__ Codes codes() {
+  Codes c;
+  asm volatile("mov.b32 %0, 0x00780078;" : "=r"(c.mask));
+  asm volatile("mov.b32 %0, 0x41804180;" : "=r"(c.magic));
+  return c;
+}
+__device__ __forceinline__ uint4 values8(uint32_t w, const Scale& s, const Codes& c) {
   uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = fma2(((i ? w >> (4 * i - 3) : w << 3) & 0x00780078u) | 0x41804180u, s.s, s.n);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(i ? w >> (4 * i - 3) : w << 3), "r"(c.mask), "r"(c.magic));   // (w & mask) | magic
+    v[i] = fma2(y, s.s, s.n);
+  }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 // Pairs of fp32 in one instruction.
@@ -377,6 +389,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
   // where a lane stores: the two pieces of a key's row (tokens 8 further on 1024 bytes further), values of tokens 2t and 2t + 1
   const uint32_t k_off = (warp * 16 + g) * 128 + (((2 * t) ^ g) << 4), k_flip = 16;   // 2t and 2t + 1 differ in the lowest bit
   const uint32_t v_off0 = (warp * 16 + 2 * t) * 128 + ((g ^ (2 * t)) << 4), v_off1 = (warp * 16 + 2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4);
+  const Codes code = codes();
   uint32_t slot = 0, round = 0;                         // ring position
   Reader reader;
   auto filled = [&]() {
@@ -451,7 +464,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
           for (int p = 0; p < S::Panels; ++p) {
             const Scale sc(k.scale[h][0], p);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) sts128((base ^ (i * k_flip)) + p * kPanel + h * 1024, values8(k.key_word(h, p, i), sc));
+            for (int i = 0; i < 2; ++i) sts128((base ^ (i * k_flip)) + p * kPanel + h * 1024, values8(k.key_word(h, p, i), sc, code));
           }
         filled();
         k.next_slot();
@@ -500,7 +513,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int p = 0; p < S::Panels; ++p)
-            sts128(base + (u & 1 ? v_off1 : v_off0) + p * kPanel + (u >> 1) * 1024, values8(v.value_word(u, p), Scale(v.scale[u][0], p)));
+            sts128(base + (u & 1 ? v_off1 : v_off0) + p * kPanel + (u >> 1) * 1024, values8(v.value_word(u, p), Scale(v.scale[u][0], p), code));
         filled();
         v.next_slot();
       }
