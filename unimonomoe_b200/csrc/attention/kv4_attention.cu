@@ -41,6 +41,7 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   a.num_pages = num_pages;
   a.tokens = tokens; a.batch = batch; a.width = table_width; a.hq = q_heads; a.hk = kv_heads;
   a.group = q_heads / kv_heads;
+  a.group_inv = 0xFFFFFFFFu / static_cast<uint32_t>(a.group);
   a.shift = __builtin_ctz(page_size);
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -24,11 +24,18 @@ struct AttnArgs {
   int64_t q_ts, q_hs, num_pages;
   int tokens, batch, width, hq, hk, group, shift, window, split_rows;
   float scale_log2;                          // scale * log2(e)
+  uint32_t group_inv;                        // (2^32 - 1) / group
 };
 
 struct Request {
   int first, n, len;                         // first query row, queries, length of the sequence
 };
+
+// x / group for 0 <= x < 2^31: the product with the reciprocal is at most one too low.
+__device__ __forceinline__ int by_group(const AttnArgs& a, int x) {
+  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_inv));
+  return x - q * a.group >= a.group ? q + 1 : q;
+}
 
 // The lengths of request b, whatever the arrays hold within the buffers that there are.
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int b, bool tell) {

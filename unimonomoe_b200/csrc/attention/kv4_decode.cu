@@ -16,9 +16,12 @@
 //    them eight times finer and lose those below 2^-31 of the largest, which a dim of that kind shows too.
 //  * The maximum is only moved when a weight would pass 2^8: one vote per step instead of a reduction.
 //
-// The work, all (request, KV head, row block) items in steps of 128 tokens, is cut into equal runs, one to a CTA; an item that
-// lies in several runs is joined by whoever of its CTAs finishes last, in the order of the runs, so the result does not depend on
-// which one that is. Each warp has every fourth pair of blocks, its own ring of copies in flight, and its own softmax state.
+// The work is all (request, KV head, row block) items, in steps of 256 tokens. Where there are fewer items than CTAs each gets an equal
+// number of CTAs, which share its steps evenly; else, or where that leaves too much to the longest item, all steps are cut
+// into equal runs, one to a CTA (kOwn steps more for an item's own cost), whatever items they lie in. An item that several CTAs
+// have is joined by whoever of them finishes last, in the order of its tokens, so the result does not depend on which one that
+// is. Each warp has every eighth pair of blocks, its own ring of copies in flight, and its own softmax state; the copies of a
+// CTA's next item are on their way while the states of one are joined.
 #include "kv4_attention.cuh"
 
 namespace mono {
@@ -26,9 +29,11 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32 * kWarps;          // tokens of one step of a CTA
+// in steps: what an item costs beside them in a run; what joining costs
+constexpr int kOwn = 1, kJoin = 6;
 constexpr float kLow = -1e38f;              // below every score
 constexpr float kRoom = 8.0f;               // log2 of what a weight may grow to before the maximum is moved
 
@@ -78,14 +83,14 @@ struct Shape {
   static constexpr int Rows = 8 * NT;                   // query rows of an item
   static constexpr int Block = block_bytes(D);
   static constexpr int Stage = 2 * Block;               // a pair of blocks
-  static constexpr int Stages = D == 256 ? 2 : 3;
+  static constexpr int Stages = D == 64 ? 3 : 2;
   static constexpr int Ring = Stages * Stage;           // of a warp
   static constexpr int Part = Rows * (D + 2);           // floats of a warp's or a CTA's state: output, maximum, sum
-  static constexpr int PerSm = D == 256 ? 3 : NT == 2 && D == 128 ? 3 : 4;
+  static constexpr int State = (Part * 4 + 15) / 16 * 16;
+  static constexpr int Smem = kWarps * (Ring + State);
+  // 16 warps on an SM where their registers allow it, 8 of up to 255 registers where not
+  static constexpr int PerSm = D == 64 || (D == 128 && NT == 1) ? 2 : 1;
   static constexpr int Ctas = MONO_ATTN_SMS * PerSm;
-  static constexpr int Warp = Ring > Part * 4 ? Ring : (Part * 4 + 15) / 16 * 16;   // shared memory of a warp: its ring, then its state
-  static constexpr int Join = (Rows * Ctas * 4 + 15) / 16 * 16;   // the weights of all CTAs' states
-  static constexpr int Smem = kWarps * Warp > Join ? kWarps * Warp : Join;
 };
 
 // Steps of one item of a request; 0 if the request is not this kernel's.
@@ -97,82 +102,186 @@ __device__ __forceinline__ void cost_of(const AttnArgs& a, const Request& r, int
   steps = max(1, (r.len - lo + kStep - 1) / kStep);
 }
 
+// Tokens [k0, k1) of an item: a block of `rows` query rows of a KV head.
+struct Part {
+  int b, head, rb, rows, k0, k1;
+  int i0, i1, u, e;                          // steps of the item, and of this part
+  int c0, c1;                                // the CTAs that share the item
+  int first, place0, len;                    // of the request: its first query row, the place of it, the length
+};
+
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(const AttnArgs a) {
   using S = Shape<D, NT>;
   constexpr int NG = S::NG;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_sum[kWarps];
+  __shared__ int s_sum[kWarps][3];
   __shared__ int s_found[2];
   __shared__ int s_last;
-  __shared__ float s_ms[S::Rows][2];
+  __shared__ Part s_part;                    // the part whose states are joined
+  __shared__ float s_weight[S::Rows][32], s_old[S::Rows], s_sums[S::Rows], s_top[S::Rows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint32_t mask4, magic;
   asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask4));
   asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
-  uint8_t* ring = smem + warp * S::Warp;
+  uint8_t* ring = smem + warp * S::Ring;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  float* states = reinterpret_cast<float*>(smem + kWarps * S::Ring);
 
-  // this CTA's run [u0, u1) of all steps, and the request that it begins in
+  // All steps, all items and the longest item; the sums before each thread's requests.
   const int chunk = (a.batch + kThreads - 1) / kThreads;
-  int mine = 0;
+  int mine = 0, mine_items = 0, longest = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     int items, steps, lo;
     cost_of<S::Rows>(a, request_of(a, b, blockIdx.x == 0), items, steps, lo);
-    mine += items * steps;
+    mine += items * (steps + kOwn);
+    mine_items += items;
+    if (items) longest = max(longest, steps);
   }
-  int upto = mine;
+  int upto = mine, upto_items = mine_items;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-    if (lane >= d) upto += x;
+    const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d), y = __shfl_up_sync(0xFFFFFFFFu, upto_items, d);
+    longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, d));
+    if (lane >= d) { upto += x; upto_items += y; }
   }
-  if (lane == 31) s_sum[warp] = upto;
+  if (lane == 31) { s_sum[warp][0] = upto; s_sum[warp][1] = upto_items; s_sum[warp][2] = longest; }
   __syncthreads();
-  int total = 0;
+  int total = 0, all_items = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += s_sum[w];
-    total += s_sum[w];
+    if (w < warp) { upto += s_sum[w][0]; upto_items += s_sum[w][1]; }
+    total += s_sum[w][0];
+    all_items += s_sum[w][1];
+    longest = max(longest, s_sum[w][2]);
   }
-  const int per = (total + gridDim.x - 1) / static_cast<int>(gridDim.x);
-  const int u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  const int ctas = static_cast<int>(gridDim.x), per = (total + ctas - 1) / ctas;
+  // CTAs for each item (0: equal runs), from what the slowest CTA then has
+  int share = 0;
+  if (all_items > 0 && all_items <= ctas) {
+    const int most = min(ctas / all_items, longest), split = (longest + most - 1) / most + kJoin;
+    share = split < longest ? most : 1;
+    if (min(split, longest) > per + kJoin) share = 0;
+  }
+  // where this CTA begins: its run [u0, u1) of all steps, or its item and its part of that
+  const int u0 = share ? static_cast<int>(blockIdx.x) / share : static_cast<int>(blockIdx.x) * per, u1 = share ? all_items : min(u0 + per, total);
   if (u0 >= u1) return;
-  if (upto - mine <= u0 && u0 < upto) {
-    int at = upto - mine, b = tid * chunk;
-    for (;; ++b) {
-      int items, steps, lo;
-      cost_of<S::Rows>(a, request_of(a, b, false), items, steps, lo);
-      if (at + items * steps > u0) break;
-      at += items * steps;
-    }
+  const int before = share ? upto_items - mine_items : upto - mine, behind = share ? upto_items : upto;
+  if (before <= u0 && u0 < behind) {
+    int at = before, b = tid * chunk;
+    if (chunk > 1)
+      for (;; ++b) {
+        int items, steps, lo;
+        cost_of<S::Rows>(a, request_of(a, b, false), items, steps, lo);
+        const int cost = share ? items : items * (steps + kOwn);
+        if (at + cost > u0) break;
+        at += cost;
+      }
     s_found[0] = b;
     s_found[1] = at;
   }
   __syncthreads();
-  int b = s_found[0], at = s_found[1];       // request, and the step that its items begin at
 
-  for (int u = u0; u < u1;) {
-    Request r = request_of(a, b, false);
-    int items, steps, lo;
-    cost_of<S::Rows>(a, r, items, steps, lo);
-    while (u >= at + items * steps) {
-      at += items * steps;
-      r = request_of(a, ++b, false);
-      cost_of<S::Rows>(a, r, items, steps, lo);
+  // the parts of the run, one after another, and the copies of a part's first blocks
+  int walk_b = s_found[0], walk_at = s_found[1], walk_u = u0;   // request, where its items begin, where the next part begins
+  Part p;
+  int count, pages, later, wstage = 0, rstage = 0;              // this warp's pairs of blocks; pages of 32 blocks and the 32 after
+  const int page_shift = a.shift - 4, in_page = (1 << page_shift) - 1;
+  const int page_bytes = (a.hk << page_shift) * S::Block;
+  // the 32 blocks that this warp's pairs i0 .. i0 + 15 are: lane 2 i + h has block h of pair i
+  auto pages_of = [&](int i0) {
+    const int blk = (p.k0 >> 4) + 2 * (warp + kWarps * (i0 + (lane >> 1))) + (lane & 1);
+    return blk * 16 < p.k1 ? page_of(a, p.b, blk >> page_shift) : 0;
+  };
+  auto issue = [&](int i) {
+    if (i < count) {
+      if ((i & 15) == 0 && i > 0) {
+        pages = later;
+        if (i + 16 < count) later = pages_of(i + 16);
+      }
+      const int blk = (p.k0 >> 4) + 2 * (warp + kWarps * i);
+      const uint8_t* head_at = a.cache + static_cast<int64_t>(p.head << page_shift) * S::Block + lane * 16;
+      const uint32_t to = ring_at + wstage * S::Stage + lane * 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int pg = __shfl_sync(0xFFFFFFFFu, pages, (i & 15) * 2 + h);
+        if (h == 0 || (blk + 1) * 16 < p.k1) {
+          const uint8_t* src = head_at + static_cast<int64_t>(pg) * page_bytes + ((blk + h) & in_page) * S::Block;
+#pragma unroll
+          for (int j = 0; j < (S::Block + 511) / 512; ++j)
+            if ((j + 1) * 512 <= S::Block || lane < (S::Block - j * 512) / 16) cp16(to + h * S::Block + j * 512, src + j * 512);
+        }
+      }
+      if (++wstage == S::Stages) wstage = 0;
     }
-    const int item = (u - at) / steps, i0 = at + item * steps, i1 = i0 + steps;
-    const int e = min(i1, u1);
-    const int row_blocks = items / a.hk, head = item / row_blocks, rb = item - head * row_blocks;
-    const int rows = min(S::Rows, r.n * a.group - rb * S::Rows);
+    cp_commit();
+  };
+  auto begin = [&]() {                       // false behind the last part
+    for (;;) {
+      if (walk_u >= u1) return false;
+      Request r = request_of(a, walk_b, false);
+      int items, steps, lo;
+      cost_of<S::Rows>(a, r, items, steps, lo);
+      while (!share && walk_u >= walk_at + items * (steps + kOwn)) {
+        walk_at += items * (steps + kOwn);
+        r = request_of(a, ++walk_b, false);
+        cost_of<S::Rows>(a, r, items, steps, lo);
+      }
+      int item;
+      if (share) {
+        item = u0 - walk_at;
+        const int parts = min(share, steps), part = static_cast<int>(blockIdx.x) - u0 * share;
+        walk_u = u1;                         // the only one
+        if (part >= parts) return false;
+        p.i0 = 0;
+        p.i1 = steps;
+        p.u = steps * part / parts;
+        p.e = steps * (part + 1) / parts;
+        p.c0 = u0 * share;
+        p.c1 = p.c0 + parts - 1;
+      } else {
+        item = (walk_u - walk_at) / (steps + kOwn);
+        p.i0 = walk_at + item * (steps + kOwn) + kOwn;   // an item's own steps come first, and belong to nobody
+        p.i1 = p.i0 + steps;
+        p.u = max(walk_u, p.i0);
+        p.e = min(p.i1, u1);
+        p.c0 = p.i0 / per;
+        p.c1 = (p.i1 - 1) / per;
+        walk_u = p.e;
+        if (p.u >= p.e) {                    // the run ends before the item's tokens
+          walk_u = u1;
+          return false;
+        }
+      }
+      p.b = walk_b;
+      const int row_blocks = items / a.hk;
+      p.head = item / row_blocks;
+      p.rb = item - p.head * row_blocks;
+      p.rows = min(S::Rows, r.n * a.group - p.rb * S::Rows);
+      p.first = r.first;
+      p.place0 = r.len - r.n;
+      p.len = r.len;
+      const int tok_last = by_group(a, p.rb * S::Rows + p.rows - 1), seen = min(r.len, max(p.place0 + tok_last + 1, 0));
+      p.k0 = lo + (p.u - p.i0) * kStep;
+      p.k1 = min(lo + (p.e - p.i0) * kStep, seen);
+      const int pairs = p.k1 > p.k0 ? (p.k1 - p.k0 + 31) / 32 : 0;
+      count = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
+      pages = count > 0 ? pages_of(0) : 0;
+      later = count > 16 ? pages_of(16) : 0;
+#pragma unroll
+      for (int i = 0; i < S::Stages - 1; ++i) issue(i);
+      return true;
+    }
+  };
 
-    // tokens of this run, and the last one (exclusive) that any row of the block sees
-    const int place0 = r.len - r.n;
-    const int tok_first = rb * S::Rows / a.group, tok_last = (rb * S::Rows + rows - 1) / a.group;
-    const int seen = min(r.len, max(place0 + tok_last + 1, 0));
-    const int k0 = lo + (u - i0) * kStep, k1 = min(lo + (e - i0) * kStep, seen);
+  bool more = begin();
+  while (more) {
+    const int here = count;
+    if (tid == 0) s_part = p;                // read behind a barrier, when p is the next one already
     // every row sees all of [clear_lo, clear_hi)
-    const int clear_hi = max(place0 + tok_first + 1, 0), clear_lo = a.window > 0 ? max(place0 + tok_last + 1 - a.window, 0) : 0;
+    const int tok_first = by_group(a, p.rb * S::Rows), tok_last = by_group(a, p.rb * S::Rows + p.rows - 1);
+    const int clear_hi = max(p.place0 + tok_first + 1, 0), clear_lo = a.window > 0 ? max(p.place0 + tok_last + 1 - a.window, 0) : 0;
+    const int k0 = p.k0, k1 = p.k1;
 
     // query: B operand, row n = g of each tile; scaled by a power of two to an fp16 with its largest value near 2^14
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // the query carries the scale's sign
@@ -181,17 +290,17 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
     int hi_r[NT][2], lo_r[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = rb * S::Rows + nt * 8 + g;
-      const bool real = nt * 8 + g < rows;
+      const int row = p.rb * S::Rows + nt * 8 + g, tok = by_group(a, row);
+      const bool real = nt * 8 + g < p.rows;
       float x[NG][2][8];
       uint32_t top = 0;
       if (real) {
-        const __nv_bfloat16* p = a.q + (r.first + row / a.group) * a.q_ts + (head * a.group + row % a.group) * a.q_hs;
+        const __nv_bfloat16* qp = a.q + (p.first + tok) * a.q_ts + (p.head * a.group + row - tok * a.group) * a.q_hs;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            uint4 raw = __ldg(reinterpret_cast<const uint4*>(p + 64 * gi + 16 * t + 8 * w));
+            uint4 raw = __ldg(reinterpret_cast<const uint4*>(qp + 64 * gi + 16 * t + 8 * w));
             raw = make_uint4(raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip);
             unpack_bf16x8(raw, x[gi][w]);
 #pragma unroll
@@ -233,8 +342,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       room[nt][1] = kRoom / fac[nt][1];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {          // what row 2t + c of the tile sees: [lo_r, hi_r)
-        const int rr = nt * 8 + 2 * t + c, place = place0 + (rb * S::Rows + rr) / a.group;
-        hi_r[nt][c] = rr < rows ? min(place + 1, r.len) : 0;
+        const int rr = nt * 8 + 2 * t + c, place = p.place0 + by_group(a, p.rb * S::Rows + rr);
+        hi_r[nt][c] = rr < p.rows ? min(place + 1, p.len) : 0;
         lo_r[nt][c] = a.window > 0 ? place + 1 - a.window : 0;
       }
     }
@@ -252,44 +361,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       off[nt][0] = off[nt][1] = 0.0f;
     }
 
-    // this warp's pairs of blocks: the warp-th, the (warp + 4)-th, ... of [k0, k1)
-    const int pairs = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;
-    const int count = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
-    const int page_shift = a.shift - 4, in_page = (1 << page_shift) - 1, blk0 = (k0 >> 4) + 2 * warp;
-    const uint8_t* head_at = a.cache + static_cast<int64_t>(head << page_shift) * S::Block + lane * 16;
-    const int page_bytes = (a.hk << page_shift) * S::Block;
-    // pages of 16 pairs at a time, those of the next 16 on their way: lane 2 i + h has block h of pair i
-    auto pages_of = [&](int i0) {
-      const int blk = blk0 + 2 * kWarps * (i0 + (lane >> 1)) + (lane & 1);
-      return blk * 16 < k1 ? page_of(a, b, blk >> page_shift) : 0;
-    };
-    int pages = pages_of(0), later = count > 16 ? pages_of(16) : 0, wstage = 0, rstage = 0;
-    auto issue = [&](int i) {
-      if (i < count) {
-        if ((i & 15) == 0 && i > 0) {
-          pages = later;
-          if (i + 16 < count) later = pages_of(i + 16);
-        }
-        const int blk = blk0 + 2 * kWarps * i;
-        const uint32_t to = ring_at + wstage * S::Stage + lane * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int pg = __shfl_sync(0xFFFFFFFFu, pages, (i & 15) * 2 + h);
-          if (h == 0 || (blk + 1) * 16 < k1) {
-            const uint8_t* src = head_at + static_cast<int64_t>(pg) * page_bytes + ((blk + h) & in_page) * S::Block;
-#pragma unroll
-            for (int j = 0; j < (S::Block + 511) / 512; ++j)
-              if ((j + 1) * 512 <= S::Block || lane < (S::Block - j * 512) / 16) cp16(to + h * S::Block + j * 512, src + j * 512);
-          }
-        }
-        if (++wstage == S::Stages) wstage = 0;
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < S::Stages - 1; ++i) issue(i);
-
-    for (int i = 0; i < count; ++i) {
+    for (int i = 0; i < here; ++i) {
       __syncwarp();                          // all lanes are done with the stage that is written now
       issue(i + S::Stages - 1);
       cp_wait<S::Stages - 1>();
@@ -445,13 +517,13 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint8_t* blk = stage + h * S::Block + 8 * D;
-        float p[NT][4];
+        float pr[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            p[nt][c] = ex2(fmaf(s[h][nt][c], fac[nt][c & 1], off[nt][c & 1]));
-            l[nt][c & 1] += p[nt][c];
+            pr[nt][c] = ex2(fmaf(s[h][nt][c], fac[nt][c & 1], off[nt][c & 1]));
+            l[nt][c & 1] += pr[nt][c];
           }
         uint32_t vw[4][NG];
         if constexpr (D == 64) {
@@ -481,7 +553,7 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
           for (int nt = 0; nt < NT; ++nt) {
             float w[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = p[nt][c] * f[c >> 1];
+            for (int c = 0; c < 4; ++c) w[c] = pr[nt][c] * f[c >> 1];
             pb[nt][0] = transpose8(pack_bf16x2(w[0], w[1]));
             pb[nt][1] = transpose8(pack_bf16x2(w[2], w[3]));
           }
@@ -500,10 +572,10 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         }
       }
     }
-    cp_wait<0>();
-    __syncthreads();                         // the rings become the warps' states
+    __syncwarp();                            // the ring is free
+    more = begin();                          // the next part's copies, while this one's states are joined
 
-    float* part = reinterpret_cast<float*>(ring);
+    float* part = states + warp * (S::State / 4);
     float* ml = part + S::Rows * D;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -526,29 +598,30 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       }
     __syncthreads();
 
-    const bool whole = u == i0 && e == i1;
-    const int c0 = i0 / per, c1 = (i1 - 1) / per;        // the CTAs that share the item
+    const Part& q = s_part;
+    const bool whole = q.u == q.i0 && q.e == q.i1;
+    const int c0 = q.c0, c1 = q.c1, rows = q.rows;
     float* mine_at = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
     auto finish = [&](int row, int d, float4 x, float mx, float sum) {
       const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;   // a sum that is not a number stays one
-      const int rr = rb * S::Rows + row, tok = r.first + rr / a.group, hd = head * a.group + rr % a.group;
+      const int rr = q.rb * S::Rows + row, in = by_group(a, rr), tok = q.first + in, hd = q.head * a.group + rr - in * a.group;
       *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(tok) * a.hq + hd) * D + d) =
           make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
       if (d == 0 && a.lse) a.lse[static_cast<int64_t>(tok) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
     };
-    constexpr int Wf = S::Warp / 4;             // floats from one warp's state to the next
-    for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
+    constexpr int Wf = S::State / 4, Work = S::Rows * D / 4, PerThread = (Work + kThreads - 1) / kThreads;
+    const int work = rows * (D / 4);
+    for (int idx = tid; idx < work; idx += kThreads) {
       const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-      const float* base = reinterpret_cast<const float*>(smem);
       float mx = kLow, sum = 0.0f;
       float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, base[w * Wf + S::Rows * D + 2 * row]);
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, states[w * Wf + S::Rows * D + 2 * row]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float by = ex2(base[w * Wf + S::Rows * D + 2 * row] - mx);
-        const float4 y = *reinterpret_cast<const float4*>(base + w * Wf + row * D + d);
-        sum = fmaf(base[w * Wf + S::Rows * D + 2 * row + 1], by, sum);
+        const float by = ex2(states[w * Wf + S::Rows * D + 2 * row] - mx);
+        const float4 y = *reinterpret_cast<const float4*>(states + w * Wf + row * D + d);
+        sum = fmaf(states[w * Wf + S::Rows * D + 2 * row + 1], by, sum);
         x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y); x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
       }
       if (whole) {
@@ -558,10 +631,10 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
         if (d == 0) __stcg(reinterpret_cast<float2*>(mine_at + S::Rows * D + 2 * row), make_float2(mx, sum));
       }
     }
+    __syncthreads();                         // the states may be written again; and the CTA's part is complete
     if (!whole) {
-      __threadfence();
-      __syncthreads();
       if (tid == 0) {
+        __threadfence();
         const uint32_t before = atomicAdd(a.counters + c0, 1u);
         s_last = before == static_cast<uint32_t>(c1 - c0);
         if (s_last) a.counters[c0] = 0;
@@ -569,47 +642,61 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       }
       __syncthreads();
       if (s_last) {
-        // the CTAs' weights first (one for each row and CTA, in shared memory), then their outputs, whose loads
-        // do not wait for one another
-        float* weight = reinterpret_cast<float*>(smem);
+        // 32 CTAs at a time: their weights, a lane to a CTA, then their outputs, whose loads do not wait for one another
         const int n = c1 - c0 + 1;
         auto from = [&](int i) { return a.partial + (static_cast<int64_t>(c0 + i) * 2 + (i == 0 ? 1 : 0)) * S::Part; };
-        for (int row = warp; row < rows; row += kWarps) {
-          float mx = kLow, sum = 0.0f;
-          for (int i = lane; i < n; i += 32) mx = fmaxf(mx, __ldcg(from(i) + S::Rows * D + 2 * row));
+        float4 x[PerThread];
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-          for (int i = lane; i < n; i += 32) {
-            const float2 ms = __ldcg(reinterpret_cast<const float2*>(from(i) + S::Rows * D + 2 * row));
-            const float by = ex2(ms.x - mx);
-            weight[row * S::Ctas + i] = by;
-            sum = fmaf(ms.y, by, sum);
-          }
+        for (int k = 0; k < PerThread; ++k) x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i0 = 0; i0 < n; i0 += 32) {
+          for (int row = warp; row < rows; row += kWarps) {
+            const float2 ms = i0 + lane < n ? __ldcg(reinterpret_cast<const float2*>(from(i0 + lane) + S::Rows * D + 2 * row)) : make_float2(kLow, 0.0f);
+            const float top = i0 ? s_top[row] : kLow;
+            float mx = fmaxf(ms.x, top);
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-          if (lane == 0) {
-            s_ms[row][0] = mx;
-            s_ms[row][1] = sum;
+            for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+            const float by = ex2(ms.x - mx), old = ex2(top - mx);
+            float sum = ms.y * by;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            s_weight[row][lane] = by;
+            if (lane == 0) {
+              s_sums[row] = i0 ? fmaf(s_sums[row], old, sum) : sum;
+              s_old[row] = old;
+              s_top[row] = mx;
+            }
           }
+          __syncthreads();
+          const int m = min(32, n - i0);
+#pragma unroll
+          for (int k = 0; k < PerThread; ++k) {
+            const int idx = tid + k * kThreads, row = idx / (D / 4), d = idx % (D / 4) * 4;
+            if (idx < work) {
+              if (i0) {
+                const float old = s_old[row];
+                x[k].x *= old; x[k].y *= old; x[k].z *= old; x[k].w *= old;
+              }
+#pragma unroll 8
+              for (int i = 0; i < m; ++i) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(from(i0 + i) + row * D + d));
+                const float by = s_weight[row][i];
+                x[k].x = fmaf(y.x, by, x[k].x); x[k].y = fmaf(y.y, by, x[k].y);
+                x[k].z = fmaf(y.z, by, x[k].z); x[k].w = fmaf(y.w, by, x[k].w);
+              }
+            }
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < PerThread; ++k) {
+          const int idx = tid + k * kThreads, row = idx / (D / 4), d = idx % (D / 4) * 4;
+          if (idx < work) finish(row, d, x[k], s_top[row], s_sums[row]);
         }
         __syncthreads();
-        for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
-          const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-          for (int i = 0; i < n; ++i) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from(i) + row * D + d));
-            const float by = weight[row * S::Ctas + i];
-            x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y);
-            x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
-          }
-          finish(row, d, x, s_ms[row][0], s_ms[row][1]);
-        }
       }
     }
-    __syncthreads();                         // the rings are free again
-    u = e;
   }
+  cp_wait<0>();
 }
 
 template <int D, int NT>

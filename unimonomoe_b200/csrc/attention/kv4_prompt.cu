@@ -436,7 +436,10 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
           const int row = warp * 16 + (i0 + i) * Step / 16 * kRows + (i0 + i) * Step % 16 + lane / Lanes;   // 16 rows of each Q tile
           x[i] = make_uint4(0, 0, 0, 0);
           if (row < rows)
-            x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + row / a.group) * a.q_ts + (w.head * a.group + row % a.group) * a.q_hs + 8 * col));
+            {
+              const int tok = by_group(a, row);
+              x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (w.q_row + tok) * a.q_ts + (w.head * a.group + row - tok * a.group) * a.q_hs + 8 * col));
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -701,9 +704,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     const int first = w.first, count = w.count, more = w.more;
     if (count == 0) break;
     const bool real = row < w.rows, idle = S::Twin && set == 1 && w.rows <= kRows;
-    const int place = w.place + row / a.group, hi = real ? place + 1 : 0, lo = a.window > 0 ? place + 1 - a.window : 0;
+    const int tok = by_group(a, row), place = w.place + tok, hi = real ? place + 1 : 0, lo = a.window > 0 ? place + 1 - a.window : 0;
     // every row of the block sees all of [clear_lo, clear_hi)
-    const int clear_hi = w.place + 1, clear_lo = a.window > 0 ? w.place + (w.rows - 1) / a.group + 1 - a.window : 0;
+    const int clear_hi = w.place + 1, clear_lo = a.window > 0 ? w.place + by_group(a, w.rows - 1) + 1 - a.window : 0;
     float m = kLow, l = 0.0f;
     // where the sets take turns, this one's next tile is the first or the second of the segment
     for (int j = idle ? count : S::Twin ? 0 : (n ^ set) & 1; j < count; j += S::Twin ? 1 : 2, ++mine) {
@@ -829,18 +832,18 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     const int c0 = w.c0, c1 = w.c1;
     float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
     auto write_out = [&](int rw, int d, const float (&x)[8], float inv) {       // eight dims, in the order of the operands
-      const int tk = w.q_row + rw / a.group, hd = w.head * a.group + rw % a.group;
+      const int in = by_group(a, rw), tk = w.q_row + in, hd = w.head * a.group + rw - in * a.group;
       float y[8] = {x[0] * inv, x[2] * inv, x[4] * inv, x[6] * inv, x[1] * inv, x[3] * inv, x[5] * inv, x[7] * inv};
       *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(tk) * a.hq + hd) * D + d) = pack_bf16x8(y);
     };
     auto inverse = [](float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; };
     auto write_lse = [&](int rw, float mx, float sum) {
-      const int tk = w.q_row + rw / a.group, hd = w.head * a.group + rw % a.group;
+      const int in = by_group(a, rw), tk = w.q_row + in, hd = w.head * a.group + rw - in * a.group;
       a.lse[static_cast<int64_t>(tk) * a.hq + hd] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
     };
     const float inv = inverse(l);
     if (!idle) {
-      __nv_bfloat16* to = a.out + (static_cast<int64_t>(w.q_row + row / a.group) * a.hq + w.head * a.group + row % a.group) * D + col0;
+      __nv_bfloat16* to = a.out + (static_cast<int64_t>(w.q_row + tok) * a.hq + w.head * a.group + row - tok * a.group) * D + col0;
 #pragma unroll 1
       for (int i = 0; i < S::Cols; i += 32) {
         uint32_t o[32];
