@@ -31,11 +31,7 @@ struct Request {
   int first, n, len;                         // first query row, queries, length of the sequence
 };
 
-// x / group for 0 <= x < 2^31: the product with the reciprocal is at most one too low.
-__device__ __forceinline__ int by_group(const AttnArgs& a, int x) {
-  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_inv));
-  return x - q * a.group >= a.group ? q + 1 : q;
-}
+__device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return divide(x, a.group, a.group_inv); }
 
 // The lengths of request b, whatever the arrays hold within the buffers that there are.
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int b, bool tell) {

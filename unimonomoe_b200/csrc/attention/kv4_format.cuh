@@ -61,27 +61,80 @@ __device__ __forceinline__ float round5(float s) {
   return __uint_as_float(b & ~0x7FFFFu);
 }
 
-// Eight values of a row, in the eight adjacent lanes that share a group: their codes as one word, and the group's scale.
-// The lanes of `mask` take part, whole groups of eight.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t mask, float& scale) {
-  uint32_t top = 0;                        // magnitudes as integers: a NaN is above infinity, infinity above the rest
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
+      "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+
+// Eight bf16 of a row, in the eight adjacent lanes that share a group: their codes as one word, and the group's scale.
+// All lanes of the warp take part.
+__device__ __forceinline__ uint32_t quantise8(const uint4& raw, float& scale) {
+  // largest magnitude, as integers: a NaN is above infinity, infinity above the rest
+  uint32_t m = __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(mask, top, d));
+  for (int d = 1; d < 8; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  const uint32_t top = max(m << 16, m & 0xFFFF0000u);
   if (top >= 0x7F800000u) {
     scale = __uint_as_float(0x7FC00000u);
     return 0x88888888u;
   }
-  const float s = fminf(fmaxf(round5(__fdiv_rn(__uint_as_float(top), 7.0f)), kScaleMin), kScaleMax);
+  const float seventh = __fdiv_rn(__uint_as_float(top), 7.0f);
+  const float s = fminf(fmaxf(round5(seventh), kScaleMin), kScaleMax);
   scale = s;
-  uint32_t w = 0;
+  // x / s by one step of Newton's method on the quotient with an exact residual (Markstein, 1990): a quotient halfway between two codes
+  // has few bits and comes out exactly, so that ties go to even as they are defined to. No quotient rounds to more than 7, unless
+  // the scale was cut. The integers are taken from the low bits of sums with 1.5 * 2^23 + 8, whose other bits are subtracted
+  // from the word at the end.
+  const float inv = __frcp_rn(s), most = seventh > kScaleMax ? 7.0f : 8.0f;
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t word = 0u - 0x4B400000u * 0x11111111u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.0f), 7.0f);
-    w |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = bf16x2(w[i]);
+    float2 y = mul2(x, both(inv));
+    y = fma2(fma2(make_float2(-y.x, -y.y), both(s), x), both(inv), y);
+    if (most == 7.0f) y = make_float2(fminf(fmaxf(y.x, -7.0f), 7.0f), fminf(fmaxf(y.y, -7.0f), 7.0f));
+    y = add2(y, both(12582920.0f));
+    word += __float_as_uint(y.x) * (1u << (8 * i)) + __float_as_uint(y.y) * (1u << (8 * i + 4));
   }
-  return w;
+  return word;
+}
+
+// What a word of eight codes and their scale stand for, in order, exactly.
+__device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t scale) {
+  // a code c + 8 as the top four bits of the mantissa under the exponent of 16 is 24 + c; (24 + c) s - 24 s in one step
+  const uint32_t even = (word << 3) & 0x78787878u, odd = (word >> 1) & 0x78787878u, s2 = scale | scale << 16;
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2), n = __hmul2(s, __float2bfloat162_rn(-24.0f));
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t y = __byte_perm(even, odd, i * 0x1111 + 0x4400);            // byte i of both, twice
+    y = (y & 0x00780078u) | 0x41804180u;
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&y), s, n);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// x / d for 0 <= x < 2^31 with inv = (2^32 - 1) / d: the product with the reciprocal is at most one too low.
+__device__ __forceinline__ int divide(int x, int d, uint32_t inv) {
+  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv));
+  return x - q * d >= d ? q + 1 : q;
 }
 
 // Stores dims 8 l .. 8 l + 7 of one row: `blk` is its block, r its token there.

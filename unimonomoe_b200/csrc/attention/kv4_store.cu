@@ -15,8 +15,9 @@ struct StoreArgs {
   uint8_t* cache;
   const int64_t* slots;
   uint32_t* status;
-  int64_t k_ts, k_hs, v_ts, v_hs, slot_count, rows;
-  int heads, shift;
+  int64_t k_ts, k_hs, v_ts, v_hs, slot_count;
+  int rows, heads, shift;
+  uint32_t per_inv;                         // of the rows of a token
 };
 
 // Rows are (token, head, key or value), D/8 lanes each; a warp does 32/(D/8) of them at a time, U times.
@@ -24,58 +25,57 @@ template <int D, int U, bool READ>
 __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
   constexpr int L = D / 8, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * R * U + sub;
+  const int first = (static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5)) * R * U + sub;
   if (first - sub >= a.rows) return;        // the whole warp
-  const uint32_t per = 2 * a.heads;
-  int64_t slot[U], token[U];
-  int head[U];
+  const int per = 2 * a.heads;
+  int64_t slot[U];
+  int token[U], head[U];
   bool value[U], fine[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int64_t row = first + i * R;
+    const int row = first + i * R;
     fine[i] = row < a.rows;
-    const int64_t r = fine[i] ? row : a.rows - 1;
-    token[i] = r / per;
-    const int h = static_cast<int>(r - token[i] * per);
+    const int r = fine[i] ? row : a.rows - 1;
+    token[i] = kv4::divide(r, per, a.per_inv);
+    const int h = r - token[i] * per;
     value[i] = h >= a.heads;
     head[i] = value[i] ? h - a.heads : h;
-    slot[i] = a.slots[token[i]];
+    slot[i] = __ldg(a.slots + token[i]);
+  }
+  uint4 raw[U];
+  if constexpr (!READ) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      raw[i] = __ldg(reinterpret_cast<const uint4*>((value[i] ? a.v + token[i] * a.v_ts + head[i] * a.v_hs : a.k + token[i] * a.k_ts + head[i] * a.k_hs) + 8 * l));
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i)
     if (slot[i] < -1 || slot[i] >= a.slot_count) {
       if (l == 0) kv4::report(a.status, kv4::kBadSlot, static_cast<uint32_t>(token[i]));
       slot[i] = -1;
     }
-  }
   if constexpr (READ) {
-    uint32_t word[U];
-    float scale[U];
+    uint32_t word[U], scale[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       word[i] = 0x88888888u;
-      scale[i] = 0.0f;
+      scale[i] = 0;
       if (slot[i] >= 0) {
         const uint8_t* blk = a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift);
         const int r = static_cast<int>(slot[i] & 15);
-        word[i] = *reinterpret_cast<const uint32_t*>(blk + (value[i] ? kv4::value_word<D>(r, l) : kv4::key_word<D>(r, l)));
-        scale[i] = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(blk + kv4::scale_at<D>(r, value[i], l >> 3))) << 16);
+        word[i] = __ldg(reinterpret_cast<const uint32_t*>(blk + (value[i] ? kv4::value_word<D>(r, l) : kv4::key_word<D>(r, l))));
+        scale[i] = __ldg(reinterpret_cast<const uint16_t*>(blk + kv4::scale_at<D>(r, value[i], l >> 3)));
       }
     }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = scale[i] * static_cast<float>(static_cast<int>((word[i] >> (4 * j)) & 15u) - 8);
-      if (fine[i]) *reinterpret_cast<uint4*>((value[i] ? a.v_out : a.k_out) + (token[i] * a.heads + head[i]) * D + 8 * l) = kv4::pack_bf16x8(x);
-    }
-  } else {
-    uint4 raw[U];
-#pragma unroll
     for (int i = 0; i < U; ++i)
-      raw[i] = *reinterpret_cast<const uint4*>((value[i] ? a.v + token[i] * a.v_ts + head[i] * a.v_hs : a.k + token[i] * a.k_ts + head[i] * a.k_hs) + 8 * l);
+      if (fine[i])
+        *reinterpret_cast<uint4*>((value[i] ? a.v_out : a.k_out) + (static_cast<int64_t>(token[i]) * a.heads + head[i]) * D + 8 * l) = kv4::dequantise8(word[i], scale[i]);
+  } else {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      float x[8], s;
-      kv4::unpack_bf16x8(raw[i], x);
-      const uint32_t word = kv4::quantise8(x, 0xFFFFFFFFu, s);
+      float s;
+      const uint32_t word = kv4::quantise8(raw[i], s);
       if (fine[i] && slot[i] >= 0)
         kv4::store8<D>(a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift), static_cast<int>(slot[i] & 15), value[i], l, word, s);
     }
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
 
 template <int D, bool READ>
 int launch(const StoreArgs& a, cudaStream_t stream) {
-  constexpr int U = 2;
+  constexpr int U = 4;
   const int64_t rows = 32 / (D / 8) * U * kWarps;
   store_kernel<D, U, READ><<<static_cast<unsigned>((a.rows + rows - 1) / rows), kWarps * 32, 0, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
@@ -93,7 +93,7 @@ int launch(const StoreArgs& a, cudaStream_t stream) {
 int check(int tokens, int heads, int head_dim, int64_t num_pages, int page_size) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
   if (tokens < 0 || heads < 1 || num_pages < 1 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return MONO_ATTN_BAD_SIZE;
-  return 0;
+  return static_cast<int64_t>(tokens) * heads * 2 > INT32_MAX - 4096 ? MONO_ATTN_BAD_SIZE : 0;
 }
 
 }  // namespace
@@ -113,7 +113,8 @@ extern "C" int mono_attn_kv4_append(const void* k, int64_t k_token_stride, int64
   a.cache = cache; a.slots = slots; a.status = status;
   a.k_ts = k_token_stride; a.k_hs = k_head_stride; a.v_ts = v_token_stride; a.v_hs = v_head_stride;
   a.slot_count = num_pages * page_size;
-  a.rows = static_cast<int64_t>(tokens) * kv_heads * 2;
+  a.rows = tokens * kv_heads * 2;
+  a.per_inv = 0xFFFFFFFFu / static_cast<uint32_t>(2 * kv_heads);
   a.heads = kv_heads;
   a.shift = __builtin_ctz(page_size);
   return head_dim == 64 ? launch<64, false>(a, stream) : head_dim == 128 ? launch<128, false>(a, stream) : launch<256, false>(a, stream);
@@ -131,7 +132,8 @@ extern "C" int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int p
   a.v_out = static_cast<__nv_bfloat16*>(v_out);
   a.cache = const_cast<uint8_t*>(cache); a.slots = slots; a.status = status;
   a.slot_count = num_pages * page_size;
-  a.rows = static_cast<int64_t>(tokens) * kv_heads * 2;
+  a.rows = tokens * kv_heads * 2;
+  a.per_inv = 0xFFFFFFFFu / static_cast<uint32_t>(2 * kv_heads);
   a.heads = kv_heads;
   a.shift = __builtin_ctz(page_size);
   return head_dim == 64 ? launch<64, true>(a, stream) : head_dim == 128 ? launch<128, true>(a, stream) : launch<256, true>(a, stream);

@@ -25,73 +25,93 @@ struct RopeArgs {
   const int64_t* slots;
   uint32_t* status;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, slot_count;
-  int tokens, hq, hk, heads, rotary, table_rows, shift;
+  int tokens, hq, hk, heads, rotary, table_rows, shift, q_units, per;   // units of a token: of its queries, all
+  uint32_t per_inv;
   float eps;
   bool interleaved, unit, w_fp32;
 };
 
-__device__ __forceinline__ void load_weight(const void* w, bool fp32, bool unit, int at, float (&x)[8]) {
-  if (fp32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// The lane's eight weights: four from `at`, four from `then`.
+__device__ __forceinline__ void load_weight(const RopeArgs& a, const void* w, int at, int then, float (&x)[8]) {
+  if (a.w_fp32) {
+    const float4 p = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at), q = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + then);
+    x[0] = p.x; x[1] = p.y; x[2] = p.z; x[3] = p.w; x[4] = q.x; x[5] = q.y; x[6] = q.z; x[7] = q.w;
   } else {
-    kv4::unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at), x);
+    const uint2 p = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at), q = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + then);
+    kv4::unpack_bf16x8(make_uint4(p.x, p.y, q.x, q.y), x);
   }
-  if (unit)
+  if (a.unit)
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] += 1.0f;
 }
 
-// A row (one head of one token) is held by D/8 lanes, eight dims each; a warp does 32/(D/8) heads of one token at a time, U times.
+// A row (one head of one token) is held by D/8 lanes, eight dims each; a warp does 32/(D/8) heads of one token at a time, U times, either of
+// the queries or of the keys (and values). Where halves turn against each other a lane below the rotary dims has four dims of each
+// half, so that both of a pair and their one cosine and sine are in one lane; else its eight dims are adjacent. What is stored in
+// the cache is brought into that order. Pairs (x0, x1) become r (x0 w0 c - x1 w1 s), r (x1 w1 c + x0 w0 s) with the products of the
+// weights made once for all heads; two pairs to an instruction.
 template <int D, int U, bool STORE>
 __global__ __launch_bounds__(kWarps * 32) void rope_kernel(const RopeArgs a) {
   constexpr int L = D / 8, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
-  const int per = (a.heads + R * U - 1) / (R * U);
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t token = unit / per;
+  const int unit = static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5);
+  const int token = kv4::divide(unit, a.per, a.per_inv);
   if (token >= a.tokens) return;            // the whole warp
-  const int h0 = static_cast<int>(unit - token * per) * R * U + sub;
+  const int part = unit - token * a.per;
+  const bool queries = part < a.q_units;
+  const int h0 = (queries ? part : part - a.q_units) * R * U + sub, heads = queries ? a.hq : a.heads - a.hq;   // of the queries, or of keys and values
+  const int half = a.rotary >> 1;
+  const bool turns = 8 * l < a.rotary, split = turns && !a.interleaved;
+  const int at = split ? 4 * l : 8 * l, then = split ? at + half : at + 4;
 
   uint4 raw[U];
+  if (queries) {
+    const __nv_bfloat16* p = a.q + token * a.q_ts;
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int h = min(h0 + i * R, a.heads - 1);
-    const __nv_bfloat16* p = h < a.hq          ? a.q + token * a.q_ts + h * a.q_hs
-                             : h < a.hq + a.hk ? a.k + token * a.k_ts + (h - a.hq) * a.k_hs
-                                               : a.v + token * a.v_ts + (h - a.hq - a.hk) * a.v_hs;
-    raw[i] = *reinterpret_cast<const uint4*>(p + 8 * l);
+    for (int i = 0; i < U; ++i) {
+      const __nv_bfloat16* x = p + min(h0 + i * R, heads - 1) * a.q_hs;
+      const uint2 y = __ldg(reinterpret_cast<const uint2*>(x + at)), z = __ldg(reinterpret_cast<const uint2*>(x + then));
+      raw[i] = make_uint4(y.x, y.y, z.x, z.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = min(h0 + i * R, heads - 1);
+      const bool is_v = STORE && h >= a.hk;
+      const __nv_bfloat16* x = is_v ? a.v + token * a.v_ts + (h - a.hk) * a.v_hs : a.k + token * a.k_ts + h * a.k_hs;
+      const uint2 y = __ldg(reinterpret_cast<const uint2*>(x + (is_v ? 8 * l : at))), z = __ldg(reinterpret_cast<const uint2*>(x + (is_v ? 8 * l + 4 : then)));
+      raw[i] = make_uint4(y.x, y.y, z.x, z.y);
+    }
   }
-
-  // cosines and sines of this lane's eight dims (four pairs in the interleaved form); outside the rotary dims 1 and 0
-  const int half = a.rotary >> 1, d0 = 8 * l;
-  const bool turns = d0 < a.rotary;
-  float co[8], si[8];
-  int pos = a.positions[token];
+  int pos = __ldg(a.positions + token);
   if (pos < 0 || pos >= a.table_rows) {
     if (lane == 0) kv4::report(a.status, kv4::kBadPosition, static_cast<uint32_t>(token));
     pos = 0;
   }
+  float4 co = make_float4(1.0f, 1.0f, 1.0f, 1.0f), si = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // of the lane's four pairs
   if (turns) {
-    const float* row = a.table + static_cast<int64_t>(pos) * a.rotary;
-    if (a.interleaved) {
-      const float4 c = *reinterpret_cast<const float4*>(row + d0 / 2), s = *reinterpret_cast<const float4*>(row + half + d0 / 2);
-      co[0] = co[1] = c.x; co[2] = co[3] = c.y; co[4] = co[5] = c.z; co[6] = co[7] = c.w;
-      si[0] = -s.x; si[1] = s.x; si[2] = -s.y; si[3] = s.y; si[4] = -s.z; si[5] = s.z; si[6] = -s.w; si[7] = s.w;
-    } else {
-      const float* c = row + (d0 < half ? d0 : d0 - half);
+    const float* row = a.table + static_cast<int64_t>(pos) * a.rotary + 4 * l;
+    co = __ldg(reinterpret_cast<const float4*>(row));
+    si = __ldg(reinterpret_cast<const float4*>(row + half));
+  }
+  // first and second of the pairs: (x[j], x[j + 4]), or neighbours; their weights times the cosines, times the sines
+  float2 c0[2], c1[2], s0[2], s1[2];
+  {
+    float w[8];
+    load_weight(a, queries ? a.wq : a.wk, at, then, w);
+    const float c[4] = {co.x, co.y, co.z, co.w}, s[4] = {si.x, si.y, si.z, si.w};
+    const bool near = a.interleaved;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 x = reinterpret_cast<const float4*>(c)[j], y = reinterpret_cast<const float4*>(c + half)[j];
-        const float sign = d0 < half ? -1.0f : 1.0f;
-        co[4 * j] = x.x; co[4 * j + 1] = x.y; co[4 * j + 2] = x.z; co[4 * j + 3] = x.w;
-        si[4 * j] = sign * y.x; si[4 * j + 1] = sign * y.y; si[4 * j + 2] = sign * y.z; si[4 * j + 3] = sign * y.w;
-      }
+    for (int j = 0; j < 2; ++j) {
+      const float2 w0 = near ? make_float2(w[4 * j], w[4 * j + 2]) : make_float2(w[2 * j], w[2 * j + 1]);
+      const float2 w1 = near ? make_float2(w[4 * j + 1], w[4 * j + 3]) : make_float2(w[2 * j + 4], w[2 * j + 5]);
+      const float2 cj = make_float2(c[2 * j], c[2 * j + 1]), sj = make_float2(s[2 * j], s[2 * j + 1]);
+      c0[j] = kv4::mul2(w0, cj);
+      c1[j] = kv4::mul2(w1, cj);
+      s0[j] = kv4::mul2(w0, sj);
+      s1[j] = kv4::mul2(w1, make_float2(-sj.x, -sj.y));
     }
   }
-  const int partner = a.interleaved ? l : d0 < half ? l + half / 8 : l - half / 8;
-  const int src = sub * L + (turns ? partner : l);
 
   int64_t slot = -1;
   if constexpr (STORE) {
@@ -101,62 +121,86 @@ __global__ __launch_bounds__(kWarps * 32) void rope_kernel(const RopeArgs a) {
       slot = -1;
     }
   }
+  __nv_bfloat16* out = queries ? a.q_out + static_cast<int64_t>(token) * a.hq * D : a.k_out + static_cast<int64_t>(token) * a.hk * D;
+  const int outs = queries ? a.hq : STORE && a.k_out == nullptr ? 0 : a.hk;   // heads that are written
 
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int h = h0 + i * R;
-    const bool is_v = STORE && h >= a.hq + a.hk, is_q = h < a.hq;
-    float x[8];
-    kv4::unpack_bf16x8(raw[i], x);
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
-    const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-    float w[8];
-    load_weight(is_q ? a.wq : a.wk, a.w_fp32, a.unit, d0, w);
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = x[j] * r * w[j];
+    const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float2 x0[2], x1[2];                    // first and second of pairs 2 j, 2 j + 1
     if (a.interleaved) {
-      if (turns) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float y0 = y[j], y1 = y[j + 1];
-          y[j] = fmaf(y0, co[j], y1 * si[j]);
-          y[j + 1] = fmaf(y1, co[j + 1], y0 * si[j + 1]);
-        }
+      for (int j = 0; j < 2; ++j) {
+        const float2 p = kv4::bf16x2(v[2 * j]), q = kv4::bf16x2(v[2 * j + 1]);
+        x0[j] = make_float2(p.x, q.x);
+        x1[j] = make_float2(p.y, q.y);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float other = __shfl_sync(0xFFFFFFFFu, y[j], src);
-        if (turns) y[j] = fmaf(y[j], co[j], other * si[j]);
+      for (int j = 0; j < 2; ++j) {
+        x0[j] = kv4::bf16x2(v[j]);
+        x1[j] = kv4::bf16x2(v[j + 2]);
       }
     }
-    const uint4 rounded = is_v ? raw[i] : kv4::pack_bf16x8(y);
-    if (is_q || (h < a.hq + a.hk && a.k_out)) {
-      __nv_bfloat16* o = is_q ? a.q_out + (token * a.hq + h) * D : a.k_out + (token * a.hk + h - a.hq) * D;
-      *reinterpret_cast<uint4*>(o + d0) = rounded;
+    float2 sq = kv4::mul2(x0[0], x0[0]);
+    sq = kv4::fma2(x0[1], x0[1], sq);
+    sq = kv4::fma2(x1[0], x1[0], sq);
+    sq = kv4::fma2(x1[1], x1[1], sq);
+    float ss = sq.x + sq.y;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
+    const float2 r = kv4::both(rsqrtf(ss * (1.0f / D) + a.eps));
+    float2 y0[2], y1[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      y0[j] = kv4::mul2(kv4::fma2(x0[j], c0[j], kv4::mul2(x1[j], s1[j])), r);
+      y1[j] = kv4::mul2(kv4::fma2(x1[j], c1[j], kv4::mul2(x0[j], s0[j])), r);
+    }
+    uint4 rounded;
+    if (a.interleaved)
+      rounded = make_uint4(kv4::pack_bf16x2(y0[0].x, y1[0].x), kv4::pack_bf16x2(y0[0].y, y1[0].y), kv4::pack_bf16x2(y0[1].x, y1[1].x), kv4::pack_bf16x2(y0[1].y, y1[1].y));
+    else
+      rounded = make_uint4(kv4::pack_bf16x2(y0[0].x, y0[0].y), kv4::pack_bf16x2(y0[1].x, y0[1].y), kv4::pack_bf16x2(y1[0].x, y1[0].y), kv4::pack_bf16x2(y1[1].x, y1[1].y));
+    if (h < outs) {
+      __nv_bfloat16* o = out + h * D;
+      *reinterpret_cast<uint2*>(o + at) = make_uint2(rounded.x, rounded.y);
+      *reinterpret_cast<uint2*>(o + then) = make_uint2(rounded.z, rounded.w);
     }
     if constexpr (STORE) {
-      float z[8], s;
-      kv4::unpack_bf16x8(rounded, z);
-      const uint32_t word = kv4::quantise8(z, 0xFFFFFFFFu, s);
-      if (slot >= 0 && !is_q && h < a.heads) {
-        const int head = is_v ? h - a.hq - a.hk : h - a.hq;
-        kv4::store8<D>(a.cache + kv4::block_at<D>(slot, head, a.hk, a.shift), static_cast<int>(slot & 15), is_v, l, word, s);
+      if (queries) continue;                // the whole warp
+      const bool is_v = h >= a.hk;
+      // dims 8 l .. 8 l + 7 of a key: the lower pieces of lanes 2 l and 2 l + 1, or the upper ones of those that lie half further back
+      uint4 row = is_v ? raw[i] : rounded;
+      if (!a.interleaved) {
+        const bool upper = 8 * l >= half;
+        const int from = sub * L + (upper ? (8 * l - half) / 4 : 2 * l), src = turns ? from : lane, src2 = turns ? from + 1 : lane;
+        uint32_t p[8];
+        p[0] = __shfl_sync(0xFFFFFFFFu, rounded.x, src); p[1] = __shfl_sync(0xFFFFFFFFu, rounded.y, src);
+        p[2] = __shfl_sync(0xFFFFFFFFu, rounded.x, src2); p[3] = __shfl_sync(0xFFFFFFFFu, rounded.y, src2);
+        p[4] = __shfl_sync(0xFFFFFFFFu, rounded.z, src); p[5] = __shfl_sync(0xFFFFFFFFu, rounded.w, src);
+        p[6] = __shfl_sync(0xFFFFFFFFu, rounded.z, src2); p[7] = __shfl_sync(0xFFFFFFFFu, rounded.w, src2);
+        if (turns && !is_v) row = upper ? make_uint4(p[4], p[5], p[6], p[7]) : make_uint4(p[0], p[1], p[2], p[3]);
+      }
+      float sc;
+      const uint32_t word = kv4::quantise8(row, sc);
+      if (slot >= 0 && h < heads) {
+        const int head = is_v ? h - a.hk : h;
+        kv4::store8<D>(a.cache + kv4::block_at<D>(slot, head, a.hk, a.shift), static_cast<int>(slot & 15), is_v, l, word, sc);
       }
     }
   }
 }
 
 template <int D, int U, bool STORE>
-int launch(const RopeArgs& a, cudaStream_t stream) {
-  const int rows = 32 / (D / 8) * U, per = (a.heads + rows - 1) / rows;
-  const int64_t blocks = (static_cast<int64_t>(a.tokens) * per + kWarps - 1) / kWarps;
-  rope_kernel<D, U, STORE><<<static_cast<unsigned>(blocks), kWarps * 32, 0, stream>>>(a);
+int launch(RopeArgs a, cudaStream_t stream) {
+  const int rows = 32 / (D / 8) * U;
+  a.q_units = (a.hq + rows - 1) / rows;
+  a.per = a.q_units + (a.heads - a.hq + rows - 1) / rows;
+  a.per_inv = 0xFFFFFFFFu / static_cast<uint32_t>(a.per);
+  const int64_t units = static_cast<int64_t>(a.tokens) * a.per;
+  if (units > INT32_MAX - 64) return MONO_ATTN_BAD_SIZE;
+  rope_kernel<D, U, STORE><<<static_cast<unsigned>((units + kWarps - 1) / kWarps), kWarps * 32, 0, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
