@@ -13,6 +13,7 @@
 #include <cmath>
 #include <map>
 #include <utility>
+#include <vector>
 
 #include "../../../include/mono_attention.h"
 
@@ -95,6 +96,30 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
 
+// Several one-dimensional tensors in one allocation: an allocation costs the host more than all the rest of one.
+class Block {
+ public:
+  Block(c10::Device device, std::initializer_list<std::pair<int64_t, at::ScalarType>> parts) {
+    int64_t bytes = 0;
+    for (const auto& [n, type] : parts) bytes += padded(n, type);
+    base_ = empty({bytes}, at::kByte, device);
+    int64_t at = 0;
+    for (const auto& [n, type] : parts) {
+      Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(), c10::scalarTypeToTypeMeta(type));
+      t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(type)));
+      t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+      tensors_.push_back(std::move(t));
+      at += padded(n, type);
+    }
+  }
+  const Tensor& operator[](size_t i) const { return tensors_[i]; }
+
+ private:
+  static int64_t padded(int64_t n, at::ScalarType type) { return (n * static_cast<int64_t>(c10::elementSize(type)) + 15) / 16 * 16; }
+  Tensor base_;
+  std::vector<Tensor> tensors_;
+};
+
 // ---- what is kept: a status word for each device, a workspace for each stream of a device. Never freed: a captured graph may
 // hold their addresses, and at exit the allocator is gone before them.
 Tensor& status_word(c10::DeviceIndex device) {
@@ -162,8 +187,8 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   page_size(page);
   const int tokens = size32(integer(a[6], "num_tokens"), "num_tokens");
   const c10::cuda::CUDAGuard guard(dev);
-  const Tensor start = empty({batch + 1}, at::kInt, dev), lens = empty({batch}, at::kInt, dev), positions = empty({tokens}, at::kInt, dev),
-               slots = empty({tokens}, at::kLong, dev), requests = empty({tokens}, at::kInt, dev), taken_out = empty({1}, at::kInt, dev);
+  const Block block(dev, {{batch + 1, at::kInt}, {batch, at::kInt}, {tokens, at::kInt}, {tokens, at::kLong}, {tokens, at::kInt}, {1, at::kInt}});
+  const Tensor &start = block[0], &lens = block[1], &positions = block[2], &slots = block[3], &requests = block[4], &taken_out = block[5];
   launched("mono_attn_plan",
            mono_attn_plan(ptr<int32_t>(cached), ptr<int32_t>(fresh), static_cast<int>(batch), ptr<int32_t>(table), size32(table.size(1), "pages of block_table"),
                           ptr<int32_t>(free), size32(free.numel(), "free_pages"), ptr<int32_t>(taken), static_cast<int>(page), tokens,
