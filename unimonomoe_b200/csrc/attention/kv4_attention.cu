@@ -48,7 +48,10 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   // max_query_len is only a bound: without the kernel of many rows the other one takes every request
   const int64_t most = static_cast<int64_t>(max_query_len < tokens ? max_query_len : tokens) * a.group;
   const bool many = most > kSplitRows && a.group <= 128;
-  a.split_rows = many ? kSplitRows : INT32_MAX;
+  // every request has the largest number of queries (as one alone does): all of them are the other kernel's
+  const bool all = many && static_cast<int64_t>(max_query_len) * batch <= tokens;
+  a.split_rows = all ? 0 : many ? kSplitRows : INT32_MAX;
+  if (all) return prompt(a, head_dim, stream);
   if (const int rc = decode(a, head_dim, most > kSplitRows ? kSplitRows : static_cast<int>(most), stream)) return rc;
   return many ? prompt(a, head_dim, stream) : 0;
 }

@@ -27,10 +27,8 @@ namespace {
 using namespace kv4;
 
 constexpr int kSoftmaxWarps = 8, kFillWarps = 8;
-constexpr int kMmaWarp = 0, kPlanWarp = 1, kFirstSoftmax = 4, kFirstFill = kFirstSoftmax + kSoftmaxWarps;   // warps 2 and 3 only make up a warpgroup
-constexpr int kThreads = 20 * 32;
-// registers of a thread: 96 at launch; softmax, filling, the rest: 256 * 112 + 256 * 96 + 128 * 64 = 640 * 96
-constexpr int kSoftmaxRegs = 112, kFillRegs = 96, kRestRegs = 64;
+constexpr int kMmaWarp = 0, kPlanWarp = 1, kFirstSoftmax = 2, kFirstFill = kFirstSoftmax + kSoftmaxWarps;
+constexpr int kThreads = (kFirstFill + kFillWarps) * 32;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
 constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
@@ -75,7 +73,7 @@ struct Control {
   int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
   int found;
   long long found_at;
-  long long wsum[20];
+  long long wsum[kThreads / 32];
   Segment seg[kSegs];
   int32_t nan_list[kNanList];               // key * 16 + groups
   float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
@@ -119,7 +117,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r, int
 
 // Tiles, and kOwn for each block, of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
 // one only where the first queries have no place in the sequence.
-__device__ __forceinline__ int tiles_before(const Item& it, int rb) {
+__device__ __noinline__ int tiles_before(const Item& it, int rb) {
   int sum = rb * kOwn;
   if (it.place0 < 0) {
     for (int i = 0; i < rb; ++i) sum += it.tiles(i);
@@ -292,23 +290,24 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b,
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+               "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
-      "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
-      "r"(v[30]), "r"(v[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void bar_arrive(int id, int count) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -428,7 +427,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
       const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
       const int col = lane % Lanes, rows = w.rows;
       const bool twin = rows > kRows;
-#pragma unroll
+#pragma unroll 1
       for (int i0 = 0; i0 < N; i0 += 8) {
         uint4 x[8];
 #pragma unroll
@@ -582,9 +581,9 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
     const uint64_t dq = umma_desc_sw128(q_at + (tile * S::NG + s * S::Panels) * kPanel), dk = umma_desc_sw128(ring + at * S::Slot);
     const uint32_t d = tmem + kSCol + buf * kKeys;
     if (elect_one_sync()) {
-#pragma unroll
+#pragma unroll 1
       for (int p = 0; p < S::Panels; ++p)
-#pragma unroll
+#pragma unroll 4
         for (int k = 0; k < 4; ++k) umma_bf16(d, dq + (p * kPanel + k * 32) / 16, dk + (p * kPanel + k * 32) / 16, qk, (s | p | k) != 0);
     }
     __syncwarp();
@@ -594,7 +593,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
     const uint64_t dv = desc_mn_sw128(ring + at * S::Slot);
     const uint32_t d = tmem + kOCol + tile * kRows + s * S::Panels * 64, p = tmem + kSCol + buf * kKeys;
     if (elect_one_sync()) {
-#pragma unroll
+#pragma unroll 4
       for (int k = 0; k < kKeys / 16; ++k) umma_bf16_ts(d, p + k * 8, dv + k * 2048 / 16, pv, add || k != 0);
     }
     __syncwarp();
@@ -652,7 +651,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
       }
     } else {
       auto next_scores = [&](uint32_t tile) {
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < S::PerTile; ++s) {
           filled();
           scores(0, tile & 1, s, slot);
@@ -669,7 +668,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
         if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
         wait_warp(&C.p_full[n[0] & 1], (n[0] >> 1) & 1, C, a);
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < S::PerTile; ++s) {
           filled();
           values(0, n[0] & 1, s, slot, j > 0);
@@ -689,9 +688,9 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
 
 // ---- the eight warps of the softmax
 template <int D>
-__device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int warp, int lane) {
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int warp, int quarter, int lane) {
   using S = Shape<D>;
-  const int quarter = warp & 3, set = warp >> 2;        // lanes of tensor memory; which four warps
+  const int set = warp >> 2;                            // which four warps; `quarter`: their lanes of tensor memory
   const int row = (S::Twin ? set * kRows : 0) + quarter * 32 + lane, tile_row = quarter * 32 + lane;
   const int col0 = S::Twin ? 0 : set * S::Cols;         // output columns of this thread, in the epilogue
   const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16), scores = lanes + kSCol + set * kKeys;
@@ -717,29 +716,29 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       const int from = lo - key0, to = hi - key0;
       auto hide = [&](float* s, int base) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 16; ++i)
           if (base + i < from || base + i >= to) s[i] = -INFINITY;
       };
-      uint32_t r0[32], r1[32];              // 32 columns in work, 32 on their way
+      uint32_t r0[16], r1[16];              // 16 columns in work, 16 on their way
       float *s0 = reinterpret_cast<float*>(r0), *s1 = reinterpret_cast<float*>(r1);
       float x = -INFINITY, y = -INFINITY;
       auto most = [&](const float* s) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
+        for (int i = 0; i < 16; i += 4) {
           x = fmaxf(x, fmaxf(s[i], s[i + 1]));
           y = fmaxf(y, fmaxf(s[i + 2], s[i + 3]));
         }
       };
-      tmem_ld32(scores, r0);
+      tmem_ld16(scores, r0);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 64) {
+      for (int c = 0; c < 128; c += 32) {
         tmem_ld_wait();
-        tmem_ld32(scores + c + 32, r1);
+        tmem_ld16(scores + c + 16, r1);
         if (mask) hide(s0, c);
         most(s0);
         tmem_ld_wait();
-        tmem_ld32(scores + (c ^ 64), r0);   // after the last the first again
-        if (mask) hide(s1, c + 32);
+        tmem_ld16(scores + ((c + 32) & 127), r0);       // after the last the first again
+        if (mask) hide(s1, c + 16);
         most(s1);
       }
       x = fmaxf(x, y) * scale;
@@ -766,38 +765,38 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         tmem_ld_wait();
         const float by = ex2(before - now);
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-          uint32_t o[32];
-          tmem_ld32(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
+        for (int i = 0; i < D; i += 16) {
+          uint32_t o[16];
+          tmem_ld16(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-          tmem_st32(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+          tmem_st16(lanes + kOCol + (S::Twin ? set * kRows : 0) + i, o);
         }
       }
       float2 sum = make_float2(0.0f, 0.0f);
       auto weigh = [&](const float* s, uint32_t to) {
-        uint32_t p[16];
+        uint32_t p[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 8; ++i) {
           float2 e = fma_f32x2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
           e.x = ex2(e.x);
           e.y = ex2(e.y);
           sum = add_f32x2(sum, e);
           p[i] = pack_bf16x2(e.x, e.y);
         }
-        tmem_st16(to, p);                   // over scores that have been read: 16 columns of weights to 32
+        tmem_st8(to, p);                    // over scores that have been read: 8 columns of weights to 16
       };
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 64) {
+      for (int c = 0; c < 128; c += 32) {
         tmem_ld_wait();
-        tmem_ld32(scores + c + 32, r1);
+        tmem_ld16(scores + c + 16, r1);
         if (mask) hide(s0, c);
         weigh(s0, scores + c / 2);
         tmem_ld_wait();
-        if (c == 0) tmem_ld32(scores + 64, r0);
-        if (mask) hide(s1, c + 32);
-        weigh(s1, scores + c / 2 + 16);
+        if (c + 32 < 128) tmem_ld16(scores + c + 32, r0);
+        if (mask) hide(s1, c + 16);
+        weigh(s1, scores + c / 2 + 8);
       }
       l += sum.x + sum.y;
       tmem_st_wait();
@@ -845,24 +844,26 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     if (!idle) {
       __nv_bfloat16* to = a.out + (static_cast<int64_t>(w.q_row + tok) * a.hq + w.head * a.group + row - tok * a.group) * D + col0;
 #pragma unroll 1
-      for (int i = 0; i < S::Cols; i += 32) {
-        uint32_t o[32];
-        tmem_ld32(output + i, o);
+      for (int i = 0; i < S::Cols; i += 16) {
+        uint32_t o[16];
+        tmem_ld16(output + i, o);
         tmem_ld_wait();
         if (real) {
-          const bool nan = nans >> ((col0 + i) >> 6) & 1u;
+          const float nan = nans >> ((col0 + i) >> 6) & 1u ? __uint_as_float(0x7FC00000u) : 0.0f;
+          if (whole) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float x[8];
+            for (int k = 0; k < 16; k += 8) {
+              float x[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] = nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[k + c]);
-            if (whole) {
-              const float y[8] = {x[0] * inv, x[2] * inv, x[4] * inv, x[6] * inv, x[1] * inv, x[3] * inv, x[5] * inv, x[7] * inv};
+              for (int c = 0; c < 8; ++c) x[c] = fmaf(__uint_as_float(o[k + c]), inv, nan);
+              const float y[8] = {x[0], x[2], x[4], x[6], x[1], x[3], x[5], x[7]};
               *reinterpret_cast<uint4*>(to + i + k) = pack_bf16x8(y);
-            } else {
-              __stcg(reinterpret_cast<float4*>(part + row * D + col0 + i + k), make_float4(x[0], x[1], x[2], x[3]));
-              __stcg(reinterpret_cast<float4*>(part + row * D + col0 + i + k + 4), make_float4(x[4], x[5], x[6], x[7]));
             }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              __stcg(reinterpret_cast<float4*>(part + row * D + col0 + i + k), make_float4(__uint_as_float(o[k]) + nan, __uint_as_float(o[k + 1]) + nan,
+                                                                                           __uint_as_float(o[k + 2]) + nan, __uint_as_float(o[k + 3]) + nan));
           }
         }
       }
@@ -1016,17 +1017,10 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   __syncthreads();
   tc_fence_after();
 
-  if (warp >= kFirstFill) {
-    reg_dec<kFillRegs>();
-    fill_role<D>(a, smem, C, warp - kFirstFill, lane);
-  } else if (warp >= kFirstSoftmax) {
-    reg_inc<kSoftmaxRegs>();
-    softmax_role<D>(a, C, warp - kFirstSoftmax, lane);
-  } else {
-    reg_dec<kRestRegs>();
-    if (warp == kMmaWarp) mma_role<D>(a, smem, C);
-    else if (warp == kPlanWarp) plan_role<S::Rows>(a, C, per, u0, u1, lane);
-  }
+  if (warp >= kFirstFill) fill_role<D>(a, smem, C, warp - kFirstFill, lane);
+  else if (warp >= kFirstSoftmax) softmax_role<D>(a, C, warp - kFirstSoftmax, warp & 3, lane);
+  else if (warp == kMmaWarp) mma_role<D>(a, smem, C);
+  else plan_role<S::Rows>(a, C, per, u0, u1, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
