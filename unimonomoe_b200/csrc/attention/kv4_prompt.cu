@@ -2,8 +2,9 @@
 //
 // A CTA takes row blocks (all query heads of one KV head for some tokens) against tiles of 128 keys:
 //   S = Q K^T and O += P V on tcgen05 (bf16, fp32 sums in tensor memory), the softmax between them in registers.
-// Heads of 64 and 128: two Q tiles of 128 rows, which share the operands made of the codes; one has its softmax while the other has the
-// tensor cores. Heads of 256, whose O alone takes half of tensor memory: one Q tile, and two tiles of keys at a time.
+// Heads of 64 and 128: two Q tiles of 128 rows, which share the operands made of the codes; the scores of half a tile of keys are made
+// while the other half's have their softmax. Heads of 256, whose O alone takes half of tensor memory: one Q tile, whose scores are
+// made a tile of keys ahead.
 // Eighteen warps, one CTA on an SM:
 //   8 turn codes into operands: a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
 //     128-byte-swizzled layout, keys for S with dims along K, values as they are (dims along N). A block's words are what a lane
@@ -49,6 +50,7 @@ struct Shape {
   static constexpr int Rows = Twin ? 2 * kRows : kRows; // of a row block
   static constexpr int Slots = D == 64 ? 8 : 5;
   static constexpr int Q = (Twin ? 2 : 1) * NG * kPanel;
+  static constexpr int Sub = Twin ? 64 : 128;           // keys of a score buffer
   static constexpr int Cols = Twin ? D : D / 2;         // output columns of a thread
   static constexpr int Part = Rows * (D + 2);           // floats of a CTA's state: output, maximum and sum
 };
@@ -66,8 +68,8 @@ struct Control {
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint64_t full[8], empty[8];               // ring slots
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2];
-  uint64_t o_done, o_all, o_free;           // a tile's products, a segment's; the segment's output has been read
+  uint64_t s_full[4], p_full[4];            // score buffers: 2 Q tile + half of the tile of keys, or tile of keys modulo 2
+  uint64_t o_done[2], o_all, o_free;        // a buffer's products with values (for each Q tile), a segment's; the segment's output has been read
   uint32_t tmem, abort, last;
   uint32_t nan_count;                       // value groups that are not numbers: key and group of the first kNanList of a segment,
   int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
@@ -316,6 +318,12 @@ constexpr uint32_t kSCol = 0, kOCol = 256;
 
 // ---- the eight warps that fill the ring
 // A lane's words and scales of a block of 16 tokens: of its keys (tokens g, g + 8), or of its values (2t, 2t+1, 2t+8, 2t+9).
+// 16 bytes that nobody else on this SM reads: not kept in what shared memory leaves of L1.
+__device__ __forceinline__ uint4 ldg_once(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 template <int D, bool VALUE>
 struct Raw {
   static constexpr int NG = D / kGroup, Tok = VALUE ? 4 : 2, SW = (NG + 1) / 2;
@@ -335,7 +343,7 @@ struct Raw {
     }
     const uint8_t* c = p + (VALUE ? 8 * D : 0) + lane * 16;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) code[i] = __ldg(reinterpret_cast<const uint4*>(c + i * 512));
+    for (int i = 0; i < NG; ++i) code[i] = ldg_once(c + i * 512);
 #pragma unroll
     for (int i = 0; i < Tok; ++i) {
       const int tok = VALUE ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i;
@@ -562,43 +570,31 @@ template <int D>
 __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Control& C) {
   using S = Shape<D>;
   const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q, tmem = uniform(C.tmem);
-  constexpr uint32_t qk = umma_idesc_bf16_f32(kRows, kKeys), pv = umma_idesc_bf16_f32(kRows, S::Panels * 64) | (1u << 16);
+  constexpr uint32_t qk = umma_idesc_bf16_f32(kRows, S::Sub), pv = umma_idesc_bf16_f32(kRows, S::Panels * 64) | (1u << 16);
   uint32_t slot = 0, round = 0;                         // ring position
   Reader reader;
+  // Everything between two waits is issued in one go by one lane: what the warp does beside issuing keeps the tensor cores waiting.
   auto advance = [&]() {
     if (++slot == S::Slots) { slot = 0; ++round; }
   };
-  auto filled = [&]() {
-    wait_warp(&C.full[slot], round & 1, C, a);
-    tc_fence_after();
+  auto filled = [&]() { wait_warp(&C.full[slot], round & 1, C, a); };
+  // Q tile `tile` against the keys from `key` on of the slot `at` (the s-th of a tile's keys), into the score buffers from `buf` on
+  auto scores = [&](int tile, int buf, int s, uint32_t at, int key) {
+    const uint64_t dq = umma_desc_sw128(q_at + (tile * S::NG + s * S::Panels) * kPanel), dk = umma_desc_sw128(ring + at * S::Slot + key * 128);
+    const uint32_t d = tmem + kSCol + buf * S::Sub;
+#pragma unroll
+    for (int p = 0; p < S::Panels; ++p)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) umma_bf16(d, dq + (p * kPanel + k * 32) / 16, dk + (p * kPanel + k * 32) / 16, qk, (s | p | k) != 0);
   };
-  auto commit = [&](uint64_t* bar) {
-    if (elect_one_sync()) umma_commit(bar);
-    __syncwarp();
+  // weights of buffer `buf` times the values from `key` on of the slot `at` (the s-th of a tile's values), onto the output of Q tile `tile`
+  auto values = [&](int tile, int buf, int s, uint32_t at, int key, bool add) {
+    const uint64_t dv = desc_mn_sw128(ring + at * S::Slot + key * 128);
+    const uint32_t d = tmem + kOCol + tile * kRows + s * S::Panels * 64, p = tmem + kSCol + buf * S::Sub;
+#pragma unroll
+    for (int k = 0; k < S::Sub / 16; ++k) umma_bf16_ts(d, p + k * 8, dv + k * 2048 / 16, pv, add || k != 0);
   };
-  // panels of a slot (the s-th of a tile's keys) against Q tile `tile`, into score buffer `buf`
-  auto scores = [&](int tile, int buf, int s, uint32_t at) {
-    const uint64_t dq = umma_desc_sw128(q_at + (tile * S::NG + s * S::Panels) * kPanel), dk = umma_desc_sw128(ring + at * S::Slot);
-    const uint32_t d = tmem + kSCol + buf * kKeys;
-    if (elect_one_sync()) {
-#pragma unroll 1
-      for (int p = 0; p < S::Panels; ++p)
-#pragma unroll 4
-        for (int k = 0; k < 4; ++k) umma_bf16(d, dq + (p * kPanel + k * 32) / 16, dk + (p * kPanel + k * 32) / 16, qk, (s | p | k) != 0);
-    }
-    __syncwarp();
-  };
-  // weights of buffer `buf` times the values of a slot (the s-th of a tile's values), onto the output of Q tile `tile`
-  auto values = [&](int tile, int buf, int s, uint32_t at, bool add) {
-    const uint64_t dv = desc_mn_sw128(ring + at * S::Slot);
-    const uint32_t d = tmem + kOCol + tile * kRows + s * S::Panels * 64, p = tmem + kSCol + buf * kKeys;
-    if (elect_one_sync()) {
-#pragma unroll 4
-      for (int k = 0; k < kKeys / 16; ++k) umma_bf16_ts(d, p + k * 8, dv + k * 2048 / 16, pv, add || k != 0);
-    }
-    __syncwarp();
-  };
-  uint32_t n[2] = {0, 0};                               // tiles so far in each score buffer
+  uint32_t n = 0, m = 0;                                // tiles of keys so far; those with a second Q tile
   for (;;) {
     const uint32_t seg = reader.n;
     wait_warp<true>(&C.seg_full[seg % kSegs], (seg / kSegs) & 1, C, a);
@@ -610,75 +606,103 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
     wait_warp(&C.q_full, seg & 1, C, a);
     if constexpr (S::Twin) {
       filled();
-      scores(0, 0, 0, slot);
-      commit(&C.s_full[0]);
-      if (twin) {
-        scores(1, 1, 0, slot);
-        commit(&C.s_full[1]);
+      tc_fence_after();
+      if (elect_one_sync()) {
+        scores(0, 0, 0, slot, 0);
+        umma_commit(&C.s_full[0]);
+        if (twin) {
+          scores(1, 2, 0, slot, 0);
+          umma_commit(&C.s_full[2]);
+        }
+        scores(0, 1, 0, slot, S::Sub);
+        umma_commit(&C.s_full[1]);
+        if (twin) {
+          scores(1, 3, 0, slot, S::Sub);
+          umma_commit(&C.s_full[3]);
+        }
+        umma_commit(&C.empty[slot]);
+        if (count == 1) umma_commit(&C.q_empty);
       }
-      commit(&C.empty[slot]);
-      if (count == 1) commit(&C.q_empty);
+      __syncwarp();
       advance();
-      for (int j = 0; j < count; ++j) {
+#pragma unroll 1
+      for (int j = 0; j < count; ++j, ++n) {
         const uint32_t v = slot;
+        const bool next = j + 1 < count;
         filled();
         advance();
-        if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
-        wait_warp(&C.p_full[0], n[0]++ & 1, C, a);
-        tc_fence_after();
-        values(0, 0, 0, v, j > 0);
         const uint32_t k = slot;
-        if (j + 1 < count) {
+        if (next) {
           filled();
-          scores(0, 0, 0, k);
-          commit(&C.s_full[0]);
-        }
-        if (twin) {
-          wait_warp(&C.p_full[1], n[1]++ & 1, C, a);
-          tc_fence_after();
-          values(1, 1, 0, v, j > 0);
-        }
-        commit(&C.empty[v]);
-        if (j + 1 < count) {
-          if (twin) {
-            scores(1, 1, 0, k);
-            commit(&C.s_full[1]);
-          }
-          commit(&C.empty[k]);
-          if (j + 2 == count) commit(&C.q_empty);
           advance();
         }
+        if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
+        // a half of the tile for a Q tile: its products with the values, then the scores of the next tile's half into its buffer
+        auto half_of = [&](int tile, int half, uint32_t parity, bool last) {
+          const int b = 2 * tile + half;
+          wait_warp(&C.p_full[b], parity, C, a);
+          tc_fence_after();
+          if (elect_one_sync()) {
+            values(tile, b, 0, v, half * S::Sub, j > 0 || half > 0);
+            umma_commit(&C.o_done[tile]);
+            if (last) umma_commit(&C.empty[v]);
+            if (next) {
+              scores(tile, b, 0, k, half * S::Sub);
+              umma_commit(&C.s_full[b]);
+              if (last) {
+                umma_commit(&C.empty[k]);
+                if (j + 2 == count) umma_commit(&C.q_empty);
+              }
+            }
+          }
+          __syncwarp();
+        };
+        half_of(0, 0, n & 1, false);
+        if (twin) half_of(1, 0, m & 1, false);
+        half_of(0, 1, n & 1, !twin);
+        if (twin) half_of(1, 1, m++ & 1, true);
       }
     } else {
-      auto next_scores = [&](uint32_t tile) {
+      // scores of a tile, its keys in PerTile slots
+      auto next_scores = [&](uint32_t tile, bool last) {
 #pragma unroll 1
         for (int s = 0; s < S::PerTile; ++s) {
           filled();
-          scores(0, tile & 1, s, slot);
-          commit(&C.empty[slot]);
+          tc_fence_after();
+          if (elect_one_sync()) {
+            scores(0, tile & 1, s, slot, 0);
+            umma_commit(&C.empty[slot]);
+            if (s + 1 == S::PerTile) {
+              umma_commit(&C.s_full[tile & 1]);
+              if (last) umma_commit(&C.q_empty);
+            }
+          }
+          __syncwarp();
           advance();
         }
-        commit(&C.s_full[tile & 1]);
       };
-      next_scores(n[0]);
-      if (count == 1) commit(&C.q_empty);
-      for (int j = 0; j < count; ++j, ++n[0]) {
-        if (j + 1 < count) next_scores(n[0] + 1);
-        if (j + 2 == count) commit(&C.q_empty);
+      next_scores(n, count == 1);
+#pragma unroll 1
+      for (int j = 0; j < count; ++j, ++n) {
+        if (j + 1 < count) next_scores(n + 1, j + 2 == count);
         if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
-        wait_warp(&C.p_full[n[0] & 1], (n[0] >> 1) & 1, C, a);
-        tc_fence_after();
+        wait_warp(&C.p_full[n & 1], (n >> 1) & 1, C, a);
 #pragma unroll 1
         for (int s = 0; s < S::PerTile; ++s) {
           filled();
-          values(0, n[0] & 1, s, slot, j > 0);
-          commit(&C.empty[slot]);
+          tc_fence_after();
+          if (elect_one_sync()) {
+            values(0, n & 1, s, slot, 0, j > 0);
+            umma_commit(&C.empty[slot]);
+            if (s + 1 == S::PerTile) umma_commit(&C.o_done[0]);
+          }
+          __syncwarp();
           advance();
         }
-        commit(&C.o_done);
       }
     }
-    commit(&C.o_all);
+    if (elect_one_sync()) umma_commit(&C.o_all);
+    __syncwarp();
     if (!more) {
       wait_warp(&C.o_all, seg & 1, C, a);        // nothing is in flight when tensor memory is given back
       break;
@@ -693,10 +717,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
   const int set = warp >> 2;                            // which four warps; `quarter`: their lanes of tensor memory
   const int row = (S::Twin ? set * kRows : 0) + quarter * 32 + lane, tile_row = quarter * 32 + lane;
   const int col0 = S::Twin ? 0 : set * S::Cols;         // output columns of this thread, in the epilogue
-  const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16), scores = lanes + kSCol + set * kKeys;
+  const uint32_t lanes = C.tmem + (static_cast<uint32_t>(quarter * 32) << 16), scores0 = lanes + kSCol + set * kKeys;   // its first buffer, or its only one
   const uint32_t output = lanes + kOCol + set * kRows;  // of its Q tile, or its half of the only one
   const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);     // the queries carry its sign; not 0, for -inf times it stays -inf
-  uint32_t n = 0, mine = 0;                             // tiles of keys so far (all, where sets take turns); this set's score buffers
+  uint32_t n = 0, mine = 0;                             // tiles of keys so far; uses of this set's buffers
   Reader reader;
   for (;;) {
     const Segment& w = reader.take(C, a);
@@ -707,12 +731,14 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     // every row of the block sees all of [clear_lo, clear_hi)
     const int clear_hi = w.place + 1, clear_lo = a.window > 0 ? w.place + by_group(a, w.rows - 1) + 1 - a.window : 0;
     float m = kLow, l = 0.0f;
-    // where the sets take turns, this one's next tile is the first or the second of the segment
-    for (int j = idle ? count : S::Twin ? 0 : (n ^ set) & 1; j < count; j += S::Twin ? 1 : 2, ++mine) {
-      const int key0 = (first + j) * kKeys;
-      wait(&C.s_full[set], mine & 1, C, a);
+    // halves of tiles of keys; or, where the sets take turns, every other tile: the first or the second of the segment first
+    const int steps = idle ? 0 : S::Twin ? 2 * count : count;
+    for (int j = S::Twin ? 0 : (n ^ set) & 1; j < steps; j += S::Twin ? 1 : 2, ++mine) {
+      const int key0 = first * kKeys + j * S::Sub, buf = S::Twin ? 2 * set + (j & 1) : set;
+      const uint32_t scores = scores0 + (S::Twin ? (j & 1) * S::Sub : 0);
+      wait(&C.s_full[buf], (S::Twin ? mine >> 1 : mine) & 1, C, a);
       tc_fence_after();
-      const bool mask = key0 < clear_lo || key0 + kKeys > clear_hi;
+      const bool mask = key0 < clear_lo || key0 + S::Sub > clear_hi;
       const int from = lo - key0, to = hi - key0;
       auto hide = [&](float* s, int base) {
 #pragma unroll
@@ -731,13 +757,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       };
       tmem_ld16(scores, r0);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = 0; c < S::Sub; c += 32) {
         tmem_ld_wait();
         tmem_ld16(scores + c + 16, r1);
         if (mask) hide(s0, c);
         most(s0);
         tmem_ld_wait();
-        tmem_ld16(scores + ((c + 32) & 127), r0);       // after the last the first again
+        tmem_ld16(scores + ((c + 32) & (S::Sub - 1)), r0);   // after the last the first again
         if (mask) hide(s1, c + 16);
         most(s1);
       }
@@ -759,8 +785,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       l *= ex2(m - now);
       m = now;
       if (grow && j > 0) {
-        // the products of the tile before are in O: where the sets take turns they may not be yet, but no other tile's are missing
-        if constexpr (!S::Twin) wait(&C.o_done, (n + j - 1) & 1, C, a);
+        // the products of the buffer before have to be in O; no others are missing, for this one's scores came after them
+        if constexpr (S::Twin) wait(&C.o_done[set], (mine - 1) & 1, C, a);
+        else wait(&C.o_done[0], (n + j - 1) & 1, C, a);
         tc_fence_after();
         tmem_ld_wait();
         const float by = ex2(before - now);
@@ -788,20 +815,20 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         tmem_st8(to, p);                    // over scores that have been read: 8 columns of weights to 16
       };
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = 0; c < S::Sub; c += 32) {
         tmem_ld_wait();
         tmem_ld16(scores + c + 16, r1);
         if (mask) hide(s0, c);
         weigh(s0, scores + c / 2);
         tmem_ld_wait();
-        if (c + 32 < 128) tmem_ld16(scores + c + 32, r0);
+        if (c + 32 < S::Sub) tmem_ld16(scores + c + 32, r0);
         if (mask) hide(s1, c + 16);
         weigh(s1, scores + c / 2 + 8);
       }
       l += sum.x + sum.y;
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&C.p_full[set]);
+      mbar_arrive(&C.p_full[buf]);
     }
     n += count;
     if constexpr (!S::Twin) {               // the sets' sums, at the last maximum
@@ -1004,8 +1031,9 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
     for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + 1); }
     mbar_init(&C.q_full, kFillWarps);
     mbar_init(&C.q_empty, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 16); }
-    mbar_init(&C.o_done, 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 16); }
+    mbar_init(&C.o_done[0], 1);
+    mbar_init(&C.o_done[1], 1);
     mbar_init(&C.o_all, 1);
     mbar_init(&C.o_free, kSoftmaxWarps * 32);
     mbar_init_fence();
