@@ -5,13 +5,13 @@
 // Heads of 64 and 128: two Q tiles of 128 rows, which share the operands made of the codes; the scores of half a tile of keys are made
 // while the other half's have their softmax. Heads of 256, whose O alone takes half of tensor memory: one Q tile, whose scores are
 // made a tile of keys ahead.
-// Eighteen warps, one CTA on an SM:
+// Nineteen warps, one CTA on an SM:
 //   8 turn codes into operands: a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
 //     128-byte-swizzled layout, keys for S with dims along K, values as they are (dims along N). A block's words are what a lane
 //     stores as 16 bytes, eight dims in the order 0 4 1 5 2 6 3 7 in which masking leaves them; queries are stored in the same
 //     order, and the output is put back from it.
 //   1 lists the segments of the CTA's run, a few ahead of the others.
-//   1 issues the products.
+//   2 issue the products, one those of each Q tile (the second has nothing to do for heads of 256).
 //   8 do the softmax, a thread to a row: four warps have one Q tile each, or every other tile of keys (the running maximum
 //     then goes through shared memory). S is read twice, for the maximum and for the weights, instead of being kept in
 //     128 registers. P goes back to tensor memory over S. O is only rescaled when a row's maximum has grown by more than 2^8 (by
@@ -28,7 +28,7 @@ namespace {
 using namespace kv4;
 
 constexpr int kSoftmaxWarps = 8, kFillWarps = 8;
-constexpr int kMmaWarp = 0, kPlanWarp = 1, kFirstSoftmax = 2, kFirstFill = kFirstSoftmax + kSoftmaxWarps;
+constexpr int kMmaWarp = 0, kMmaWarps = 2, kPlanWarp = 2, kFirstSoftmax = 3, kFirstFill = kFirstSoftmax + kSoftmaxWarps;
 constexpr int kThreads = (kFirstFill + kFillWarps) * 32;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
 constexpr int kKeys = 128, kRows = 128;    // of a product's tile
@@ -565,9 +565,9 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
   }
 }
 
-// ---- the warp that issues the products
+// ---- the warps that issue the products: each its Q tile's, or the first one all of them
 template <int D>
-__device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Control& C) {
+__device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Control& C, int tile) {
   using S = Shape<D>;
   const uint32_t q_at = smem_u32(smem), ring = q_at + S::Q, tmem = uniform(C.tmem);
   constexpr uint32_t qk = umma_idesc_bf16_f32(kRows, S::Sub), pv = umma_idesc_bf16_f32(kRows, S::Panels * 64) | (1u << 16);
@@ -594,13 +594,13 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
 #pragma unroll
     for (int k = 0; k < S::Sub / 16; ++k) umma_bf16_ts(d, p + k * 8, dv + k * 2048 / 16, pv, add || k != 0);
   };
-  uint32_t n = 0, m = 0;                                // tiles of keys so far; those with a second Q tile
+  uint32_t n = 0;                                       // tiles of keys so far (of this warp's Q tile)
   for (;;) {
     const uint32_t seg = reader.n;
     wait_warp<true>(&C.seg_full[seg % kSegs], (seg / kSegs) & 1, C, a);
     const Segment& w = C.seg[seg % kSegs];
     const int count = uniform(w.count), more = uniform(w.more);
-    const bool twin = S::Twin && uniform(w.rows) > kRows;
+    const bool mine = tile == 0 || uniform(w.rows) > kRows;    // else only the ring's slots are handed on
     if (count == 0) break;
     reader.done(C);
     wait_warp(&C.q_full, seg & 1, C, a);
@@ -608,25 +608,19 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
       filled();
       tc_fence_after();
       if (elect_one_sync()) {
-        scores(0, 0, 0, slot, 0);
-        umma_commit(&C.s_full[0]);
-        if (twin) {
-          scores(1, 2, 0, slot, 0);
-          umma_commit(&C.s_full[2]);
-        }
-        scores(0, 1, 0, slot, S::Sub);
-        umma_commit(&C.s_full[1]);
-        if (twin) {
-          scores(1, 3, 0, slot, S::Sub);
-          umma_commit(&C.s_full[3]);
-        }
+        if (mine)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            scores(tile, 2 * tile + half, 0, slot, half * S::Sub);
+            umma_commit(&C.s_full[2 * tile + half]);
+          }
         umma_commit(&C.empty[slot]);
         if (count == 1) umma_commit(&C.q_empty);
       }
       __syncwarp();
       advance();
 #pragma unroll 1
-      for (int j = 0; j < count; ++j, ++n) {
+      for (int j = 0; j < count; ++j) {
         const uint32_t v = slot;
         const bool next = j + 1 < count;
         filled();
@@ -637,30 +631,32 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, uint8_t* smem, Contr
           advance();
         }
         if (j == 0) wait_warp(&C.o_free, (seg & 1) ^ 1, C, a);
-        // a half of the tile for a Q tile: its products with the values, then the scores of the next tile's half into its buffer
-        auto half_of = [&](int tile, int half, uint32_t parity, bool last) {
+        // half a tile: its products with the values, then the scores of the next tile's half into its buffer
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
           const int b = 2 * tile + half;
-          wait_warp(&C.p_full[b], parity, C, a);
+          if (mine) wait_warp(&C.p_full[b], n & 1, C, a);
           tc_fence_after();
           if (elect_one_sync()) {
-            values(tile, b, 0, v, half * S::Sub, j > 0 || half > 0);
-            umma_commit(&C.o_done[tile]);
-            if (last) umma_commit(&C.empty[v]);
+            if (mine) {
+              values(tile, b, 0, v, half * S::Sub, j > 0 || half > 0);
+              umma_commit(&C.o_done[tile]);
+            }
+            if (half) umma_commit(&C.empty[v]);
             if (next) {
-              scores(tile, b, 0, k, half * S::Sub);
-              umma_commit(&C.s_full[b]);
-              if (last) {
+              if (mine) {
+                scores(tile, b, 0, k, half * S::Sub);
+                umma_commit(&C.s_full[b]);
+              }
+              if (half) {
                 umma_commit(&C.empty[k]);
                 if (j + 2 == count) umma_commit(&C.q_empty);
               }
             }
           }
           __syncwarp();
-        };
-        half_of(0, 0, n & 1, false);
-        if (twin) half_of(1, 0, m & 1, false);
-        half_of(0, 1, n & 1, !twin);
-        if (twin) half_of(1, 1, m++ & 1, true);
+        }
+        n += mine;
       }
     } else {
       // scores of a tile, its keys in PerTile slots
@@ -1027,14 +1023,15 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < S::Slots; ++i) { mbar_init(&C.full[i], kFillWarps); mbar_init(&C.empty[i], 1); }
-    for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + 1); }
+    constexpr int issuers = S::Twin ? kMmaWarps : 1;
+    for (int i = 0; i < S::Slots; ++i) { mbar_init(&C.full[i], kFillWarps); mbar_init(&C.empty[i], issuers); }
+    for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + issuers); }
     mbar_init(&C.q_full, kFillWarps);
-    mbar_init(&C.q_empty, 1);
+    mbar_init(&C.q_empty, issuers);
     for (int i = 0; i < 4; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 16); }
     mbar_init(&C.o_done[0], 1);
     mbar_init(&C.o_done[1], 1);
-    mbar_init(&C.o_all, 1);
+    mbar_init(&C.o_all, issuers);
     mbar_init(&C.o_free, kSoftmaxWarps * 32);
     mbar_init_fence();
     C.abort = 0;
@@ -1047,7 +1044,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
 
   if (warp >= kFirstFill) fill_role<D>(a, smem, C, warp - kFirstFill, lane);
   else if (warp >= kFirstSoftmax) softmax_role<D>(a, C, warp - kFirstSoftmax, warp & 3, lane);
-  else if (warp == kMmaWarp) mma_role<D>(a, smem, C);
+  else if (warp < kMmaWarp + kMmaWarps) { if (S::Twin || warp == kMmaWarp) mma_role<D>(a, smem, C, S::Twin ? uniform(warp - kMmaWarp) : 0); }
   else plan_role<S::Rows>(a, C, per, u0, u1, lane);
   tc_fence_before();
   __syncthreads();
