@@ -736,11 +736,19 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       tc_fence_after();
       const bool mask = key0 < clear_lo || key0 + S::Sub > clear_hi;
       const int from = lo - key0, to = hi - key0;
-      auto hide = [&](float* s, int base) {
+      if (mask) {                           // written back, so that what follows needs no masks
+#pragma unroll 1
+        for (int c = 0; c < S::Sub; c += 16) {
+          uint32_t s[16];
+          tmem_ld16(scores + c, s);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (base + i < from || base + i >= to) s[i] = -INFINITY;
-      };
+          for (int i = 0; i < 16; ++i)
+            if (c + i < from || c + i >= to) s[i] = 0xFF800000u;
+          tmem_st16(scores + c, s);
+        }
+        tmem_st_wait();
+      }
       uint32_t r0[16], r1[16];              // 16 columns in work, 16 on their way
       float *s0 = reinterpret_cast<float*>(r0), *s1 = reinterpret_cast<float*>(r1);
       float x = -INFINITY, y = -INFINITY;
@@ -756,11 +764,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       for (int c = 0; c < S::Sub; c += 32) {
         tmem_ld_wait();
         tmem_ld16(scores + c + 16, r1);
-        if (mask) hide(s0, c);
         most(s0);
         tmem_ld_wait();
         tmem_ld16(scores + ((c + 32) & (S::Sub - 1)), r0);   // after the last the first again
-        if (mask) hide(s1, c + 16);
         most(s1);
       }
       x = fmaxf(x, y) * scale;
@@ -814,11 +820,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       for (int c = 0; c < S::Sub; c += 32) {
         tmem_ld_wait();
         tmem_ld16(scores + c + 16, r1);
-        if (mask) hide(s0, c);
         weigh(s0, scores + c / 2);
         tmem_ld_wait();
         if (c + 32 < S::Sub) tmem_ld16(scores + c + 32, r0);
-        if (mask) hide(s1, c + 16);
         weigh(s1, scores + c / 2 + 8);
       }
       l += sum.x + sum.y;
