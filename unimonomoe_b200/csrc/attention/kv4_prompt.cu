@@ -19,6 +19,7 @@
 // Work is cut into equal runs of tiles, one to a CTA; items that lie in several runs are joined as in kv4_decode.cu.
 // All waits are bounded.
 #include <climits>
+#include <type_traits>
 #include "kv4_attention.cuh"
 #include "../ptx_sm100.cuh"
 
@@ -27,9 +28,8 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kSoftmaxWarps = 8, kFillWarps = 8;
+constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 0, kMmaWarps = 2, kPlanWarp = 2, kFirstSoftmax = 3, kFirstFill = kFirstSoftmax + kSoftmaxWarps;
-constexpr int kThreads = (kFirstFill + kFillWarps) * 32;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
 constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
@@ -48,6 +48,8 @@ struct Shape {
   static constexpr int PerTile = NG / Panels;           // slots of a tile's keys, or of its values
   static constexpr bool Twin = D <= 128;                // two Q tiles; else one, and the softmax warps take turns at the keys
   static constexpr int Rows = Twin ? 2 * kRows : kRows; // of a row block
+  static constexpr bool Split = !Twin;                  // keys and values are filled in by eight warps each, else by the same eight
+  static constexpr int FillWarps = Split ? 16 : 8, Threads = (kFirstFill + FillWarps) * 32;
   static constexpr int Slots = D == 64 ? 8 : 5;
   static constexpr int Q = (Twin ? 2 : 1) * NG * kPanel;
   static constexpr int Sub = Twin ? 64 : 128;           // keys of a score buffer
@@ -75,7 +77,7 @@ struct Control {
   int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
   int found;
   long long found_at;
-  long long wsum[kThreads / 32];
+  long long wsum[32];
   Segment seg[kSegs];
   int32_t nan_list[kNanList];               // key * 16 + groups
   float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
@@ -386,7 +388,9 @@ struct Raw {
   }
 };
 
-template <int D>
+// `warp`: which of the eight blocks of 16 tokens of a tile. A ring is in the order in which the products take it:
+// K0 V0 K1 V1 .., or with scores a tile ahead K0 K1 V0 K2 V1 .. V(last). What is stored is loaded again at once, for the tile after.
+template <int D, bool KEYS, bool VALUES>
 __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Control& C, int warp, int lane) {
   using S = Shape<D>;
   constexpr int NG = S::NG;
@@ -397,6 +401,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
   const uint32_t k_off = (warp * 16 + g) * 128 + (((2 * t) ^ g) << 4), k_flip = 16;   // 2t and 2t + 1 differ in the lowest bit
   const uint32_t v_off0 = (warp * 16 + 2 * t) * 128 + ((g ^ (2 * t)) << 4), v_off1 = (warp * 16 + 2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4);
   const Codes code = codes();
+  struct Nothing {};
   uint32_t slot = 0, round = 0;                         // ring position
   Reader reader;
   auto filled = [&]() {
@@ -404,6 +409,10 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
     __syncwarp();
     if (lane == 0) mbar_arrive(&C.full[slot]);
     if (++slot == S::Slots) { slot = 0; ++round; }
+  };
+  auto skip = [&]() {                                   // a tile of the other kind
+    slot += S::PerTile;
+    if (slot >= S::Slots) { slot -= S::Slots; ++round; }
   };
   for (;;) {
     const Segment& w = reader.take(C, a);
@@ -422,16 +431,17 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
       const int blk = (first + j) * (kKeys / 16) + warp, pg = __shfl_sync(0xFFFFFFFFu, pages, j & 31);
       return blk * 16 < end ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
     };
-    Raw<D, false> k;
-    Raw<D, true> v;
-    const uint8_t *at = block(0), *then = nullptr;      // blocks whose values, whose keys are loaded next
-    k.load(at, g, t, lane);
-    v.load(at, g, t, lane);
+    std::conditional_t<KEYS, Raw<D, false>, Nothing> k;
+    std::conditional_t<VALUES, Raw<D, true>, Nothing> v;
+    const uint8_t* at = block(0);                       // block whose values are loaded next
+    if constexpr (KEYS) k.load(at, g, t, lane);
+    if constexpr (VALUES) v.load(at, g, t, lane);
 
     // queries, in the order of the operands
     wait(&C.q_empty, (seg & 1) ^ 1, C, a);
     {
-      constexpr int Lanes = D / 8, Step = 32 / Lanes, Mine = S::Rows / kFillWarps, N = Mine / Step;
+      constexpr int Lanes = D / 8, Step = 32 / Lanes, N = S::Rows / S::FillWarps / Step, Each = kRows / S::FillWarps;
+      const int part = (warp + (KEYS ? 0 : 8)) * Each;  // rows of each Q tile
       const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
       const int col = lane % Lanes, rows = w.rows;
       const bool twin = rows > kRows;
@@ -440,7 +450,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         uint4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int row = warp * 16 + (i0 + i) * Step / 16 * kRows + (i0 + i) * Step % 16 + lane / Lanes;   // 16 rows of each Q tile
+          const int row = part + (i0 + i) * Step / Each * kRows + (i0 + i) * Step % Each + lane / Lanes;
           x[i] = make_uint4(0, 0, 0, 0);
           if (row < rows)
             {
@@ -450,7 +460,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int row = warp * 16 + (i0 + i) * Step % 16 + lane / Lanes, tile = (i0 + i) * Step / 16;
+          const int row = part + (i0 + i) * Step % Each + lane / Lanes, tile = (i0 + i) * Step / Each;
           if (tile == 0 || twin)
             sts128(q_at + (tile * NG + (col >> 3)) * kPanel + row * 128 + (((col & 7) ^ (row & 7)) << 4),
                    make_uint4(__byte_perm(x[i].x, x[i].z, 0x5410) ^ flip, __byte_perm(x[i].x, x[i].z, 0x7632) ^ flip,
@@ -464,6 +474,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
     if (lane == 0) mbar_arrive(&C.q_full);
 
     auto store_keys = [&]() {
+      if constexpr (KEYS) {
 #pragma unroll 1
       for (int s = 0; s < S::PerTile; ++s) {
         const uint32_t base = ring + slot * S::Slot + k_off;
@@ -479,8 +490,10 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         filled();
         k.next_slot();
       }
+      }
     };
     auto store_values = [&](int j) {
+      if constexpr (VALUES) {
       // behind the sequence there may be anything; a group that is not a number must not reach the rows that do not see it
       const int key0 = (first + j) * kKeys + warp * 16;
       if (key0 + 16 > end) {
@@ -527,39 +540,40 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         filled();
         v.next_slot();
       }
-    };
-    // in the order in which the products take them; what is stored is loaded again at once, for the tile after
-    store_keys();
-    if (count > 1) {
-      then = block(1);
-      k.load(then, g, t, lane);
-    }
-    for (int j = 0; j < count; ++j) {
-      const bool keys = j + 1 < count;
-      const uint8_t* after = nullptr;
-      auto values = [&]() {
-        store_values(j);
-        if (keys) {
-          at = then;
-          v.load(at, g, t, lane);
-        }
-      };
-      auto next_keys = [&]() {
-        if (keys) store_keys();
-        if (j + 2 < count) {
-          const uint8_t* p = block(j + 2);
-          k.load(p, g, t, lane);
-          after = p;
-        }
-      };
-      if constexpr (S::Twin) {
-        values();
-        next_keys();
-      } else {
-        next_keys();
-        values();
       }
-      then = after;
+    };
+    if constexpr (S::Split) {
+      for (int j = 0; j < count; ++j) {
+        const uint8_t* next = j + 1 < count ? block(j + 1) : nullptr;
+        if constexpr (KEYS) {
+          store_keys();
+          if (j > 0) skip();
+          if (j + 1 == count) skip();
+          else k.load(next, g, t, lane);
+        } else {
+          if (j == 0) skip();
+          if (j + 1 < count) skip();
+          store_values(j);
+          if (j + 1 < count) v.load(next, g, t, lane);
+        }
+      }
+    } else {
+      store_keys();
+      if (count > 1) {
+        at = block(1);
+        k.load(at, g, t, lane);
+      }
+      for (int j = 0; j < count; ++j) {
+        store_values(j);
+        if (j + 1 < count) {
+          v.load(at, g, t, lane);
+          store_keys();
+          if (j + 2 < count) {
+            at = block(j + 2);
+            k.load(at, g, t, lane);
+          }
+        }
+      }
     }
     if (!more) break;
   }
@@ -981,14 +995,14 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int64_t
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const AttnArgs a) {
   using S = Shape<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Control& C = *reinterpret_cast<Control*>(smem + S::Q + S::Slots * S::Slot);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   // this CTA's run of all tiles
-  const int chunk = (a.batch + kThreads - 1) / kThreads;
+  const int chunk = (a.batch + S::Threads - 1) / S::Threads;
   long long mine = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     const Item it = item_of(a, request_of(a, b, blockIdx.x == 0), S::Rows);
@@ -1003,7 +1017,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   if (lane == 31) C.wsum[warp] = upto;
   __syncthreads();
   long long total = 0;
-  for (int i = 0; i < kThreads / 32; ++i) {
+  for (int i = 0; i < S::Threads / 32; ++i) {
     if (i < warp) upto += C.wsum[i];
     total += C.wsum[i];
   }
@@ -1028,9 +1042,9 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   }
   if (tid == 0) {
     constexpr int issuers = S::Twin ? kMmaWarps : 1;
-    for (int i = 0; i < S::Slots; ++i) { mbar_init(&C.full[i], kFillWarps); mbar_init(&C.empty[i], issuers); }
-    for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + kFillWarps + issuers); }
-    mbar_init(&C.q_full, kFillWarps);
+    for (int i = 0; i < S::Slots; ++i) { mbar_init(&C.full[i], 8); mbar_init(&C.empty[i], issuers); }
+    for (int i = 0; i < kSegs; ++i) { mbar_init(&C.seg_full[i], 1); mbar_init(&C.seg_empty[i], kSoftmaxWarps + S::FillWarps + issuers); }
+    mbar_init(&C.q_full, S::FillWarps);
     mbar_init(&C.q_empty, issuers);
     for (int i = 0; i < 4; ++i) { mbar_init(&C.s_full[i], 1); mbar_init(&C.p_full[i], kSoftmaxWarps * 16); }
     mbar_init(&C.o_done[0], 1);
@@ -1046,7 +1060,8 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const AttnArgs a) {
   __syncthreads();
   tc_fence_after();
 
-  if (warp >= kFirstFill) fill_role<D>(a, smem, C, warp - kFirstFill, lane);
+  if (warp >= kFirstFill + 8) { if constexpr (S::Split) fill_role<D, false, true>(a, smem, C, warp - kFirstFill - 8, lane); }
+  else if (warp >= kFirstFill) fill_role<D, true, !S::Split>(a, smem, C, warp - kFirstFill, lane);
   else if (warp >= kFirstSoftmax) softmax_role<D>(a, C, warp - kFirstSoftmax, warp & 3, lane);
   else if (warp < kMmaWarp + kMmaWarps) { if (S::Twin || warp == kMmaWarp) mma_role<D>(a, smem, C, S::Twin ? uniform(warp - kMmaWarp) : 0); }
   else plan_role<S::Rows>(a, C, per, u0, u1, lane);
@@ -1071,7 +1086,7 @@ int launch(const AttnArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  prompt_kernel<D><<<MONO_ATTN_SMS, kThreads, smem_bytes<D>(), stream>>>(a);
+  prompt_kernel<D><<<MONO_ATTN_SMS, Shape<D>::Threads, smem_bytes<D>(), stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
