@@ -49,10 +49,21 @@ __device__ __forceinline__ int scale_at(int r, bool value, int gi) {
 // First byte of the block of `slot` (page * page_size + offset) for one head; page_shift = log2(page_size).
 template <int D>
 __device__ __forceinline__ int64_t block_at(int64_t slot, int head, int heads, int page_shift) {
-  const int64_t page = slot >> page_shift;
-  const int sub = static_cast<int>(slot & ((1 << page_shift) - 1)) >> 4;
-  return (((page * heads + head) << (page_shift - 4)) + sub) * block_bytes(D);
+  // numbers of blocks fit 32 bits: 2^32 of the smallest ones are 4 TB
+  const int shift = page_shift - 4;
+  const uint32_t sub = static_cast<uint32_t>(slot >> 4), page = sub >> shift;
+  return static_cast<int64_t>(sub + page * (static_cast<uint32_t>(heads - 1) << shift) + (static_cast<uint32_t>(head) << shift)) * block_bytes(D);
 }
+
+// key_word or value_word of a lane whose row is a key (or a value) throughout, for many tokens: linear in three parts of r.
+template <int D>
+struct WordPlace {
+  int first, pair, odd;                     // the place for r = 0; what a step of r >> 1 & 3, of r & 1 adds
+  __device__ __forceinline__ WordPlace(bool value, int l)
+      : first(value ? value_word<D>(0, l) : key_word<D>(0, l)), pair(value ? value_word<D>(2, 0) - value_word<D>(0, 0) : key_word<D>(2, 0)),
+        odd(value ? value_word<D>(1, 0) - value_word<D>(0, 0) : key_word<D>(1, 0)) {}
+  __device__ __forceinline__ int at(int r) const { return first + (r >> 3) * key_word<D>(8, 0) + (r >> 1 & 3) * pair + (r & 1) * odd; }
+};
 
 // To five significant bits, ties to even. Finite, normal s.
 __device__ __forceinline__ float round5(float s) {
@@ -93,22 +104,26 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& raw, float& scale) {
     scale = __uint_as_float(0x7FC00000u);
     return 0x88888888u;
   }
-  const float seventh = __fdiv_rn(__uint_as_float(top), 7.0f);
+  // top / 7 and x / s by one step of Newton's method on the quotient with an exact residual (Markstein, 1990). With the rounded reciprocal
+  // of 7 it is the rounded quotient.
+  const float seven = 0.14285714924335479736f, about = __uint_as_float(top) * seven, seventh = fmaf(fmaf(about, -7.0f, __uint_as_float(top)), seven, about);
   const float s = fminf(fmaxf(round5(seventh), kScaleMin), kScaleMax);
   scale = s;
-  // x / s by one step of Newton's method on the quotient with an exact residual (Markstein, 1990): a quotient halfway between two codes
-  // has few bits and comes out exactly, so that ties go to even as they are defined to. No quotient rounds to more than 7, unless
-  // the scale was cut. The integers are taken from the low bits of sums with 1.5 * 2^23 + 8, whose other bits are subtracted
-  // from the word at the end.
-  const float inv = __frcp_rn(s), most = seventh > kScaleMax ? 7.0f : 8.0f;
+  // A quotient x / s halfway between two codes has few bits and comes out exactly with any reciprocal that is right to some 2^-20,
+  // so that ties go to even as they are defined to; the others are further from there than the error. No quotient rounds to more
+  // than 7, unless the scale was cut. The integers are taken from the low bits of sums with 1.5 * 2^23 + 8, whose other bits are
+  // subtracted from the word at the end.
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const bool cut = seventh > kScaleMax;
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t word = 0u - 0x4B400000u * 0x11111111u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 x = bf16x2(w[i]);
     float2 y = mul2(x, both(inv));
-    y = fma2(fma2(make_float2(-y.x, -y.y), both(s), x), both(inv), y);
-    if (most == 7.0f) y = make_float2(fminf(fmaxf(y.x, -7.0f), 7.0f), fminf(fmaxf(y.y, -7.0f), 7.0f));
+    y = fma2(fma2(y, both(-s), x), both(inv), y);
+    if (cut) y = make_float2(fminf(fmaxf(y.x, -7.0f), 7.0f), fminf(fmaxf(y.y, -7.0f), 7.0f));
     y = add2(y, both(12582920.0f));
     word += __float_as_uint(y.x) * (1u << (8 * i)) + __float_as_uint(y.y) * (1u << (8 * i + 4));
   }

@@ -16,42 +16,39 @@ struct StoreArgs {
   const int64_t* slots;
   uint32_t* status;
   int64_t k_ts, k_hs, v_ts, v_hs, slot_count;
-  int rows, heads, shift;
+  int tokens, step, heads, shift;           // step: a quarter of the tokens
   uint32_t per_inv;                         // of the rows of a token
 };
 
-// Rows are (token, head, key or value), D/8 lanes each; a warp does 32/(D/8) of them at a time, U times.
+// Rows are (token, head, key or value), D/8 lanes each. A thread has U rows, of the same head of tokens `step` apart, so that what
+// belongs to the head is worked out once: the kernels are bound by instructions before they are by memory.
 template <int D, int U, bool READ>
 __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
-  constexpr int L = D / 8, R = 32 / L;
-  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
-  const int first = (static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5)) * R * U + sub;
-  if (first - sub >= a.rows) return;        // the whole warp
-  const int per = 2 * a.heads;
+  constexpr int L = D / 8, Scales = 4 * D / kv4::kGroup;      // bytes of a token's scales
+  const int l = threadIdx.x % L, row = static_cast<int>((blockIdx.x * kWarps * 32 + threadIdx.x) / L), per = 2 * a.heads;
+  if (row - static_cast<int>(threadIdx.x % 32) / L >= a.step * per) return;   // the whole warp
+  const int first = kv4::divide(min(row, a.step * per - 1), per, a.per_inv), h = min(row, a.step * per - 1) - first * per;
+  const bool value = h >= a.heads, real = row < a.step * per;
+  const int head = value ? h - a.heads : h, scale_to = kv4::scale_at<D>(0, value, l >> 3);
+  const kv4::WordPlace<D> place(value, l);
   int64_t slot[U];
-  int token[U], head[U];
-  bool value[U], fine[U];
+  bool fine[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int row = first + i * R;
-    fine[i] = row < a.rows;
-    const int r = fine[i] ? row : a.rows - 1;
-    token[i] = kv4::divide(r, per, a.per_inv);
-    const int h = r - token[i] * per;
-    value[i] = h >= a.heads;
-    head[i] = value[i] ? h - a.heads : h;
-    slot[i] = __ldg(a.slots + token[i]);
+    fine[i] = real && first + i * a.step < a.tokens;
+    slot[i] = fine[i] ? __ldg(a.slots + first + i * a.step) : -1;
   }
   uint4 raw[U];
   if constexpr (!READ) {
+    const int64_t ts = value ? a.v_ts : a.k_ts;
+    const __nv_bfloat16* from = (value ? a.v + head * a.v_hs : a.k + head * a.k_hs) + first * ts + 8 * l;
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      raw[i] = __ldg(reinterpret_cast<const uint4*>((value[i] ? a.v + token[i] * a.v_ts + head[i] * a.v_hs : a.k + token[i] * a.k_ts + head[i] * a.k_hs) + 8 * l));
+    for (int i = 0; i < U; ++i) raw[i] = fine[i] ? __ldg(reinterpret_cast<const uint4*>(from + i * (a.step * ts))) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < U; ++i)
-    if (slot[i] < -1 || slot[i] >= a.slot_count) {
-      if (l == 0) kv4::report(a.status, kv4::kBadSlot, static_cast<uint32_t>(token[i]));
+    if (static_cast<uint64_t>(slot[i]) >= static_cast<uint64_t>(a.slot_count)) {
+      if (slot[i] != -1 && l == 0) kv4::report(a.status, kv4::kBadSlot, static_cast<uint32_t>(first + i * a.step));
       slot[i] = -1;
     }
   if constexpr (READ) {
@@ -61,32 +58,37 @@ __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
       word[i] = 0x88888888u;
       scale[i] = 0;
       if (slot[i] >= 0) {
-        const uint8_t* blk = a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift);
-        const int r = static_cast<int>(slot[i] & 15);
-        word[i] = __ldg(reinterpret_cast<const uint32_t*>(blk + (value[i] ? kv4::value_word<D>(r, l) : kv4::key_word<D>(r, l))));
-        scale[i] = __ldg(reinterpret_cast<const uint16_t*>(blk + kv4::scale_at<D>(r, value[i], l >> 3)));
+        const uint8_t* blk = a.cache + kv4::block_at<D>(slot[i], head, a.heads, a.shift);
+        const int r = static_cast<int>(slot[i]) & 15;
+        word[i] = __ldg(reinterpret_cast<const uint32_t*>(blk + place.at(r)));
+        scale[i] = __ldg(reinterpret_cast<const uint16_t*>(blk + scale_to + r * Scales));
       }
     }
+    __nv_bfloat16* to = (value ? a.v_out : a.k_out) + (static_cast<int64_t>(first) * a.heads + head) * D + 8 * l;
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (fine[i])
-        *reinterpret_cast<uint4*>((value[i] ? a.v_out : a.k_out) + (static_cast<int64_t>(token[i]) * a.heads + head[i]) * D + 8 * l) = kv4::dequantise8(word[i], scale[i]);
+      if (fine[i]) *reinterpret_cast<uint4*>(to + i * (static_cast<int64_t>(a.step) * a.heads * D)) = kv4::dequantise8(word[i], scale[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       float s;
       const uint32_t word = kv4::quantise8(raw[i], s);
-      if (fine[i] && slot[i] >= 0)
-        kv4::store8<D>(a.cache + kv4::block_at<D>(slot[i], head[i], a.heads, a.shift), static_cast<int>(slot[i] & 15), value[i], l, word, s);
+      if (slot[i] >= 0) {
+        uint8_t* blk = a.cache + kv4::block_at<D>(slot[i], head, a.heads, a.shift);
+        const int r = static_cast<int>(slot[i]) & 15;
+        *reinterpret_cast<uint32_t*>(blk + place.at(r)) = word;
+        if ((l & 7) == 0)
+          *reinterpret_cast<uint16_t*>(blk + scale_to + r * Scales) = static_cast<uint16_t>(__float_as_uint(s) >> 16);
+      }
     }
   }
 }
 
 template <int D, bool READ>
-int launch(const StoreArgs& a, cudaStream_t stream) {
-  constexpr int U = 4;
-  const int64_t rows = 32 / (D / 8) * U * kWarps;
-  store_kernel<D, U, READ><<<static_cast<unsigned>((a.rows + rows - 1) / rows), kWarps * 32, 0, stream>>>(a);
+int launch(StoreArgs& a, cudaStream_t stream) {
+  constexpr int U = 4, Rows = kWarps * 32 / (D / 8);
+  a.step = (a.tokens + U - 1) / U;
+  store_kernel<D, U, READ><<<static_cast<unsigned>((static_cast<int64_t>(a.step) * 2 * a.heads + Rows - 1) / Rows), kWarps * 32, 0, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -113,7 +115,7 @@ extern "C" int mono_attn_kv4_append(const void* k, int64_t k_token_stride, int64
   a.cache = cache; a.slots = slots; a.status = status;
   a.k_ts = k_token_stride; a.k_hs = k_head_stride; a.v_ts = v_token_stride; a.v_hs = v_head_stride;
   a.slot_count = num_pages * page_size;
-  a.rows = tokens * kv_heads * 2;
+  a.tokens = tokens;
   a.per_inv = 0xFFFFFFFFu / static_cast<uint32_t>(2 * kv_heads);
   a.heads = kv_heads;
   a.shift = __builtin_ctz(page_size);
@@ -132,7 +134,7 @@ extern "C" int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int p
   a.v_out = static_cast<__nv_bfloat16*>(v_out);
   a.cache = const_cast<uint8_t*>(cache); a.slots = slots; a.status = status;
   a.slot_count = num_pages * page_size;
-  a.rows = tokens * kv_heads * 2;
+  a.tokens = tokens;
   a.per_inv = 0xFFFFFFFFu / static_cast<uint32_t>(2 * kv_heads);
   a.heads = kv_heads;
   a.shift = __builtin_ctz(page_size);
