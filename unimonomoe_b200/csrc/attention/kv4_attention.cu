@@ -3,8 +3,12 @@
 
 namespace mono {
 namespace kv4 {
-// Query rows for a KV head up to which a request goes to the kernel of few rows.
-constexpr int kSplitRows = 64;
+// Query rows for a KV head up to which a request goes to the kernel of few rows, whose time grows with the rows, while the other
+// one's hardly does up to its 128 or 256. Few (request, KV head) items leave each to many CTAs, whose states the kernel of many rows takes
+// longer to join. Measured, in us (kernel of few rows / of many, heads of 128, groups of 8): 32 requests to 8192 with 4 KV heads, 32
+// rows 79 / 95, 48 rows 106 / 98; 16 such requests, 48 rows 60 / 61; 4 requests to 16384, 64 rows 46 / 52, 128 rows 68 / 68;
+// one to 65536, 128 rows 95 / 115. Heads of 256: 32 rows 85 / 76, 16 requests 48 rows 68 / 62; 4 to 16384, 128 rows 79 / 128.
+constexpr int kSplitRows = 40, kSplitRowsFew = 128, kFewItems = 32;
 }  // namespace kv4
 }  // namespace mono
 
@@ -47,11 +51,12 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   a.scale_log2 = scale * 1.4426950408889634f;
   // max_query_len is only a bound: without the kernel of many rows the other one takes every request
   const int64_t most = static_cast<int64_t>(max_query_len < tokens ? max_query_len : tokens) * a.group;
-  const bool many = most > kSplitRows && a.group <= 128;
+  const int split = batch * static_cast<int64_t>(kv_heads) < kFewItems ? kSplitRowsFew : kSplitRows;
+  const bool many = most > split && a.group <= 128;
   // every request has the largest number of queries (as one alone does): all of them are the other kernel's
   const bool all = many && static_cast<int64_t>(max_query_len) * batch <= tokens;
-  a.split_rows = all ? 0 : many ? kSplitRows : INT32_MAX;
+  a.split_rows = all ? 0 : many ? split : INT32_MAX;
   if (all) return prompt(a, head_dim, stream);
-  if (const int rc = decode(a, head_dim, most > kSplitRows ? kSplitRows : static_cast<int>(most), stream)) return rc;
+  if (const int rc = decode(a, head_dim, most > split ? split : static_cast<int>(most), stream)) return rc;
   return many ? prompt(a, head_dim, stream) : 0;
 }

@@ -33,7 +33,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32 * kWarps;          // tokens of one step of a CTA
 // in steps: what an item costs beside them in a run; what joining costs
-constexpr int kOwn = 1, kJoin = 6;
+constexpr int kOwn = 1, kJoin = 3;
 constexpr float kLow = -1e38f;              // below every score
 constexpr float kRoom = 8.0f;               // log2 of what a weight may grow to before the maximum is moved
 
