@@ -18,6 +18,15 @@
 //     the warps of that row themselves; sums are fp32, so nothing is lost by a maximum that is a little old).
 // Work is cut into equal runs of tiles, one to a CTA; items that lie in several runs are joined as in kv4_decode.cu.
 // All waits are bounded.
+//
+// Bound by the tensor cores, 4 D operations for each pair of a query and a key it sees, and behind them by what surrounds them. Seven
+// chunks of 350 to 700 tokens behind contexts to 4096 (32 query and 4 KV heads of 128): 241 us, 0.74 PFLOP/s; a prompt of 8192 (16 query and 2 KV
+// heads of 256): 640 us, 0.86 PFLOP/s (690 us, 0.80 in a long loop). Once the pipeline runs, a tile of 256 rows and 128 keys takes 2050 ns for heads of 128,
+// where its products alone would take 1100: the softmax of each half tile takes 1850 cycles of the 2050 that pass between two, on two warps
+// of each scheduler that exchange 64 x 32 exponentials a warp and wait for tensor memory. Replacing some of the exponentials by
+// polynomials made it slower (243 -> 251 us for one pair in eight), as did keeping the scores in registers (247 -> 265 us), 16
+// softmax warps (245 -> 261 us) and their 27 warps' registers (243 -> 263 us). Heads of 256 take 2500 ns for 128 rows and 128 keys:
+// their operands, twice as many for each product, pass shared memory three times, 2560 cycles of its bandwidth in 4600.
 #include <climits>
 #include <type_traits>
 #include "kv4_attention.cuh"
@@ -46,9 +55,11 @@ struct Shape {
   static constexpr int Panels = D == 64 ? 1 : 2;        // of a slot
   static constexpr int Slot = Panels * kPanel;
   static constexpr int PerTile = NG / Panels;           // slots of a tile's keys, or of its values
-  static constexpr bool Twin = D <= 128;                // two Q tiles; else one, and the softmax warps take turns at the keys
+  static constexpr bool Twin = D <= 128;                // two Q tiles (their outputs and scores fill 512 columns); else one, and the softmax warps take turns at the keys
   static constexpr int Rows = Twin ? 2 * kRows : kRows; // of a row block
-  static constexpr bool Split = !Twin;                  // keys and values are filled in by eight warps each, else by the same eight
+  // Keys and values are filled in by eight warps each, else by the same eight. Heads of 256 (prompt of 8192): 640 us, else 686; heads of 128
+  // (chunks of 700) 263 us, else 243: they do not wait for operands, and 27 warps leave 72 registers.
+  static constexpr bool Split = !Twin;
   static constexpr int FillWarps = Split ? 16 : 8, Threads = (kFirstFill + FillWarps) * 32;
   static constexpr int Slots = D == 64 ? 8 : 5;
   static constexpr int Q = (Twin ? 2 : 1) * NG * kPanel;
@@ -222,11 +233,11 @@ struct Reader {
   }
 };
 
-__device__ __forceinline__ uint32_t fma2(uint32_t x, uint32_t y, uint32_t z) {
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t x, uint32_t y, uint32_t z) {
   const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&z));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t add2(uint32_t x, uint32_t y) {
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t x, uint32_t y) {
   const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -255,21 +266,9 @@ __device__ __forceinline__ uint4 values8(uint32_t w, const Scale& s, const Codes
   for (int i = 0; i < 4; ++i) {
     uint32_t y;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(i ? w >> (4 * i - 3) : w << 3), "r"(c.mask), "r"(c.magic));   // (w & mask) | magic
-    v[i] = fma2(y, s.s, s.n);
+    v[i] = fma_bf16x2(y, s.s, s.n);
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
-}
-// Pairs of fp32 in one instruction.
-__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
-      "l"(*reinterpret_cast<const uint64_t*>(&c)));
-  return *reinterpret_cast<const float2*>(&r);
-}
-__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
-  return *reinterpret_cast<const float2*>(&r);
 }
 __device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -507,7 +506,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < Raw<D, true>::SW; ++i) sum = add2(sum, v.scale[u][i]);
+        for (int i = 0; i < Raw<D, true>::SW; ++i) sum = add_bf16x2(sum, v.scale[u][i]);
       if (__any_sync(0xFFFFFFFFu, (sum & 0x7FFFu) > 0x7F80u || (sum & 0x7FFF0000u) > 0x7F800000u)) {
         wait(&C.o_free, (seg & 1) ^ 1, C, a);           // the list of the segment before has been read
 #pragma unroll
@@ -822,10 +821,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
         uint32_t p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float2 e = fma_f32x2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
+          float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale), make_float2(-m, -m));
           e.x = ex2(e.x);
           e.y = ex2(e.y);
-          sum = add_f32x2(sum, e);
+          sum = add2(sum, e);
           p[i] = pack_bf16x2(e.x, e.y);
         }
         tmem_st8(to, p);                    // over scores that have been read: 8 columns of weights to 16

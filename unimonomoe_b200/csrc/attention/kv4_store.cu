@@ -1,5 +1,8 @@
 // Keys and values into the 4-bit cache, and what they stand for back out of it, by slot.
-// Bound by memory: 2 bytes a value on one side, 17/32 on the other; a lane has eight dims, one word of the cache.
+// 2 bytes a value on one side, 17/32 on the other; a lane has eight dims, one word of the cache. 16384 tokens with 4 heads of 128, 42.6 MB,
+// take 16 us to store and 10.5 us to read; a copy of as many bytes takes 7.5 us. Bound by instructions: the issue slots are 79%
+// used, 160 instructions for eight dims that are stored (the largest magnitude and scale of a group, eight quotients, a place),
+// 95 for eight that are read. That values of a token lie 64 bytes apart costs nothing: stored like keys they take as long.
 #include <cuda_runtime.h>
 #include "kv4_format.cuh"
 #include "../../../include/mono_attention.h"
@@ -86,6 +89,7 @@ __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
 
 template <int D, bool READ>
 int launch(StoreArgs& a, cudaStream_t stream) {
+  // 16384 tokens stored, read: U = 1 18.6, 14.1 us; 2 16.6, 11.2; 4 15.9, 10.5; 8 16.5, 10.6
   constexpr int U = 4, Rows = kWarps * 32 / (D / 8);
   a.step = (a.tokens + U - 1) / U;
   store_kernel<D, U, READ><<<static_cast<unsigned>((static_cast<int64_t>(a.step) * 2 * a.heads + Rows - 1) / Rows), kWarps * 32, 0, stream>>>(a);
