@@ -457,3 +457,41 @@ def test_the_whole_step_against_its_parts_in_64_bits():
             values[b].append(ref.quantised(qkv[starts[b]:starts[b + 1], H + K:]))
             cached[b] += news[b]
         close(out, None, ref.attention(q, [torch.cat(x) for x in keys], [torch.cat(x) for x in values], starts, 0, D ** -0.5))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 64])
+def test_not_finite_keys_and_values_in_prompts_of_all_head_sizes(D, window):
+    H, K, n = 4, 2, 300
+    cache, table, ln, st, q, _, _, starts = make([n], [200], H, K, D, 16, seed=14)
+    k, v = randn((n, K, D), 41), randn((n, K, D), 42)
+    v[n - 1, 0, D - 1] = math.nan                            # only the last query sees these
+    v[130, 1, 0] = -math.inf                                 # queries from 130 on, or to 193 with the window
+    k[n - 1, 1, 3] = math.inf
+    i = torch.arange(n, device=DEV)
+    A.kv4_append(k, v, cache, table[0].long()[i // 16] * 16 + i % 16)
+    out = A.kv4_attention(q, cache, table, ln, st, 200, window=window)
+    close(out, None, ref.attention(q, [ref.quantised(k)], [ref.quantised(v)], starts, window, D ** -0.5))
+    bad = torch.isnan(out).flatten(2).any(-1)[:, 2:].any(-1)
+    assert not bad[:30].any() and bad[30:94].all() and bad[-1] and (window == 0 or not bad[94:-1].any())
+
+
+@pytest.mark.parametrize("H,K,D,page", [(8, 2, 64, 16), (16, 2, 128, 32), (16, 2, 256, 16)])
+@pytest.mark.parametrize("bound", [0, 7])
+def test_batches_of_many_items_of_few_and_many_rows(H, K, D, page, bound):
+    """40 (request, KV head) items and more: requests of one token, of a few, and of chunks side by side, some of them empty."""
+    news = [1, 5, 6, 40, 0, 11, 1, 3, 64, 17, 10, 2, 1, 33, 5, 1, 0, 12, 9, 30]
+    lens = [n + 37 * i * (i % 3) for i, n in enumerate(news)]
+    cache, table, ln, st, q, keys, values, starts = make(lens, news, H, K, D, page, seed=D)
+    out, lse = A.kv4_attention(q, cache, table, ln, st, max(news) + bound, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))
+
+
+@pytest.mark.parametrize("H,K,D", [(2, 1, 64), (4, 2, 128), (2, 1, 256)])
+def test_chunks_over_long_contexts_are_joined_the_same_way_every_time(H, K, D):
+    cache, table, ln, st, q, keys, values, starts = make([9000, 300], [150, 270], H, K, D, 64, seed=15)
+    q = q * 3
+    out, lse = A.kv4_attention(q, cache, table, ln, st, 270, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))
+    for _ in range(5):
+        assert torch.equal(out, A.kv4_attention(q, cache, table, ln, st, 270))

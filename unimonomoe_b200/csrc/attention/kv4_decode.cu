@@ -36,8 +36,8 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 32 * kWarps;          // tokens of one step of a CTA
 // In steps: what an item costs beside them in a run; what joining costs. With kJoin 12 one sequence of 1500 to 3000 tokens is not divided
-// and takes 21 us instead of 13; with 6 sixteen of 1000 to 2000 (heads of 256) take 23 us, with 3 or less 17.
-constexpr int kOwn = 1, kJoin = 3;
+// and takes 21 us instead of 13; with 6 sixteen of 1000 to 2000 (heads of 256) take 23 us, with 3 or less 17; one of 777 takes 15.1 with 3, 14.6 with 2.
+constexpr int kOwn = 1, kJoin = 2;
 constexpr float kLow = -1e38f;              // below every score
 constexpr float kRoom = 8.0f;               // log2 of what a weight may grow to before the maximum is moved
 
