@@ -60,7 +60,8 @@ int mono_attn_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_s
                          int64_t v_head_stride, int tokens, int kv_heads, int head_dim, uint8_t* cache, int64_t num_pages,
                          int page_size, const int64_t* slots, uint32_t* status, mono_attn_stream_t stream);
 
-/* What the cache holds at slots, as contiguous bf16 [tokens, kv_heads, head_dim]; zeros for slot -1. */
+/* What the cache holds at slots, as contiguous bf16 [tokens, kv_heads, head_dim] (fastest on 32-byte
+ * boundaries); zeros for slot -1. */
 int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, const int64_t* slots, int tokens, int kv_heads,
                        int head_dim, void* k_out, void* v_out, uint32_t* status, mono_attn_stream_t stream);
 

@@ -1,4 +1,5 @@
 """The attention operators against their definitions in 64 bits: sizes, layouts and masks where they can go wrong."""
+import ctypes
 import math
 import random
 
@@ -495,3 +496,23 @@ def test_chunks_over_long_contexts_are_joined_the_same_way_every_time(H, K, D):
     close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))
     for _ in range(5):
         assert torch.equal(out, A.kv4_attention(q, cache, table, ln, st, 270))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_reading_into_outputs_on_16_byte_boundaries(D):
+    """The C ABI takes outputs on any 16-byte boundary; those on 32 are written in wider pieces."""
+    lib = ctypes.CDLL(A.attention_lib_path())
+    K, n = 3, 37
+    cache = A.KV4Cache.empty(4, K, D, 16, DEV)
+    k, v, slots = randn((n, K, D), 1), randn((n, K, D), 2), torch.randperm(64, generator=gen(3), device=DEV)[:n].contiguous()
+    A.kv4_append(k, v, cache, slots)
+    want = A.kv4_read(cache, slots)
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    room = torch.full((2, n * K * D + 16), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = [x[8:8 + n * K * D] for x in room]
+    assert got[0].data_ptr() % 32 == 16
+    rc = lib.mono_attn_kv4_read(p(cache.data), ctypes.c_int64(4), 16, p(slots), n, K, D, p(got[0]), p(got[1]), p(status),
+                                ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0 and torch.equal(got[0].view(n, K, D), want[0]) and torch.equal(got[1].view(n, K, D), want[1])
+    assert (room[:, :8] == 7).all() and (room[:, 8 + n * K * D:] == 7).all() and not status.any()

@@ -92,17 +92,23 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
 
-// Eight bf16 of a row, in the eight adjacent lanes that share a group: their codes as one word, and the group's scale.
+// 8 N bf16 of a row, in the 8 / N adjacent lanes that share a group: their codes as N words, and the group's scale.
 // All lanes of the warp take part.
-__device__ __forceinline__ uint32_t quantise8(const uint4& raw, float& scale) {
+template <int N>
+__device__ __forceinline__ void quantise(const uint4 (&raw)[N], uint32_t (&words)[N], float& scale) {
   // largest magnitude, as integers: a NaN is above infinity, infinity above the rest
-  uint32_t m = __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
+  uint32_t m = 0;
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  for (int n = 0; n < N; ++n)
+    m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[n].x & 0x7FFF7FFFu, raw[n].y & 0x7FFF7FFFu), __vmaxu2(raw[n].z & 0x7FFF7FFFu, raw[n].w & 0x7FFF7FFFu)));
+#pragma unroll
+  for (int d = 1; d < 8 / N; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
   const uint32_t top = max(m << 16, m & 0xFFFF0000u);
   if (top >= 0x7F800000u) {
     scale = __uint_as_float(0x7FC00000u);
-    return 0x88888888u;
+#pragma unroll
+    for (int n = 0; n < N; ++n) words[n] = 0x88888888u;
+    return;
   }
   // top / 7 and x / s by one step of Newton's method on the quotient with an exact residual (Markstein, 1990). With the rounded reciprocal
   // of 7 it is the rounded quotient.
@@ -116,18 +122,27 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& raw, float& scale) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   const bool cut = seventh > kScaleMax;
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t word = 0u - 0x4B400000u * 0x11111111u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = bf16x2(w[i]);
-    float2 y = mul2(x, both(inv));
-    y = fma2(fma2(y, both(-s), x), both(inv), y);
-    if (cut) y = make_float2(fminf(fmaxf(y.x, -7.0f), 7.0f), fminf(fmaxf(y.y, -7.0f), 7.0f));
-    y = add2(y, both(12582920.0f));
-    word += __float_as_uint(y.x) * (1u << (8 * i)) + __float_as_uint(y.y) * (1u << (8 * i + 4));
+  for (int n = 0; n < N; ++n) {
+    const uint32_t w[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+    uint32_t word = 0u - 0x4B400000u * 0x11111111u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = bf16x2(w[i]);
+      float2 y = mul2(x, both(inv));
+      y = fma2(fma2(y, both(-s), x), both(inv), y);
+      if (cut) y = make_float2(fminf(fmaxf(y.x, -7.0f), 7.0f), fminf(fmaxf(y.y, -7.0f), 7.0f));
+      y = add2(y, both(12582920.0f));
+      word += __float_as_uint(y.x) * (1u << (8 * i)) + __float_as_uint(y.y) * (1u << (8 * i + 4));
+    }
+    words[n] = word;
   }
-  return word;
+}
+__device__ __forceinline__ uint32_t quantise8(const uint4& raw, float& scale) {
+  const uint4 r[1] = {raw};
+  uint32_t w[1];
+  quantise(r, w, scale);
+  return w[0];
 }
 
 // What a word of eight codes and their scale stand for, in order, exactly.
