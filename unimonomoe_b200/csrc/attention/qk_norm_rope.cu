@@ -7,8 +7,9 @@
 // Sums and products in fp32, one rounding to bf16 at the end. The cache quantises the key after that rounding, so that it
 // holds the same codes as a key stored from the tensor.
 //
-// Bound by memory: 4 bytes a value, read and written once. 8192 tokens of 36 heads of 128 take 35.4 us, 4.4 TB/s, where a copy
-// of as many bytes takes 26.8; the rest is the tables' and the weights' reads and instructions (a lane's eight dims take some 70).
+// Bound by memory: 4 bytes a value, read and written once. 8192 tokens of 36 heads of 128 take 33.1 us, 4.7 TB/s, where a copy
+// of as many bytes takes 26.8; behind memory it is instructions, some 130 for a lane's eight dims with what it shares among four heads. With the
+// keys and values stored in the cache, a fifth of the rows, 45 us.
 #include <cuda_runtime.h>
 #include "kv4_format.cuh"
 #include "../../../include/mono_attention.h"
@@ -53,8 +54,9 @@ __device__ __forceinline__ void load_weight(const RopeArgs& a, const void* w, in
 // half, so that both of a pair and their one cosine and sine are in one lane; else its eight dims are adjacent. What is stored in
 // the cache is brought into that order. Pairs (x0, x1) become r (x0 w0 c - x1 w1 s), r (x1 w1 c + x0 w0 s) with the products of the
 // weights made once for all heads; two pairs to an instruction.
+// Five CTAs to an SM (48 registers, one of them spilled for heads of 128): 8192 tokens of 36 heads of 128 33.1 us; four 35.5; six 37.3.
 template <int D, int U, bool STORE>
-__global__ __launch_bounds__(kWarps * 32) void rope_kernel(const RopeArgs a) {
+__global__ __launch_bounds__(kWarps * 32, 5) void rope_kernel(const RopeArgs a) {
   constexpr int L = D / 8, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
   const int unit = static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5);
@@ -209,7 +211,7 @@ int launch(RopeArgs a, cudaStream_t stream) {
 
 template <int D>
 int launch_d(const RopeArgs& a, bool store, cudaStream_t stream) {
-  constexpr int U = 4;                      // 8192 tokens of 36 heads of 128: 1: 55 us, 2: 39, 4: 35.5, 8: 37
+  constexpr int U = 4;                      // 8192 tokens of 36 heads of 128, four CTAs to an SM: 1: 55 us, 2: 39, 4: 35.5, 8: 37
   return store ? launch<D, U, true>(a, stream) : launch<D, U, false>(a, stream);
 }
 
