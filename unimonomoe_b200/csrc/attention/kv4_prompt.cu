@@ -44,6 +44,9 @@ constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
 constexpr float kLow = -1e38f, kRoom = 8.0f;
 constexpr int kNanList = 64;
+// States that one CTA joins. 256 rows over 65536 tokens (4 KV heads of 128, 37 states): 208 us alone, 123 in two steps; four requests of 64 tokens over 16384
+// (5 to 7 states) 111, with 6 here 126; 32 tokens (10 states) 137 alone, 114.
+constexpr int kJoinAlone = 8;
 // What an item costs beside its tiles, in tiles: loading its queries, filling and draining the pipeline, writing its output.
 // It counts where work is divided, for the first blocks of a prompt are many and short.
 constexpr int kOwn = 2;
@@ -917,21 +920,36 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       if (real && col0 == 0 && a.lse) write_lse(row, m, l);
     } else {
       if (real && col0 == 0) __stcg(reinterpret_cast<float2*>(part + S::Rows * D + 2 * row), make_float2(m, l));
-      __threadfence();
-      named_bar_sync(9, 256);
-      if (warp == 0 && lane == 0) {
-        const uint32_t before = atomicAdd(a.counters + c0, 1u);
-        C.last = before == static_cast<uint32_t>(c1 - c0);
-        if (C.last) a.counters[c0] = 0;
+      // Whoever comes last joins. Where more than kJoinAlone CTAs have the item, first the last of each `group` of them joins the group's
+      // states into the one of its first CTA, then the last group's last CTA those of the groups.
+      const int all = c1 - c0 + 1;
+      int group = all;
+      if (all > kJoinAlone)
+        for (group = 1; group * group < all;) ++group;
+      const int groups = (all + group - 1) / group;
+      int first = c0 + (static_cast<int>(blockIdx.x) - c0) / group * group, n = min(group, c1 + 1 - first), step = 1;
+      bool final = groups == 1;
+      uint32_t* counter = a.counters + MONO_ATTN_SMS + 2 * first + (first == c0 ? 1 : 0);
+      for (;;) {
         __threadfence();
-      }
-      named_bar_sync(9, 256);
-      if (C.last) {
+        named_bar_sync(9, 256);
+        if (warp == 0 && lane == 0) {
+          const uint32_t before = atomicAdd(counter, 1u);
+          C.last = before == static_cast<uint32_t>(n - 1);
+          if (C.last) *counter = 0;
+          __threadfence();
+        }
+        named_bar_sync(9, 256);
+        if (!C.last) break;
+        auto state = [&](int i) {
+          const int c = first + i * step;
+          return a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
+        };
         for (int idx = warp * 32 + lane; idx < w.rows * (D / 8); idx += 256) {
           const int rw = idx / (D / 8), d = idx % (D / 8) * 8;
           float mx = kLow, sum = 0.0f, x[8] = {};
-          for (int c = c0; c <= c1; ++c) {
-            const float* from = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::Part;
+          for (int i = 0; i < n; ++i) {
+            const float* from = state(i);
             const float2 ms = __ldcg(reinterpret_cast<const float2*>(from + S::Rows * D + 2 * rw));
             const float4 p0 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d)), p1 = __ldcg(reinterpret_cast<const float4*>(from + rw * D + d + 4));
             const float to = fmaxf(mx, ms.x), old = ex2(mx - to), by = ex2(ms.x - to);
@@ -942,9 +960,31 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
             x[4] = fmaf(p1.x, by, x[4] * old); x[5] = fmaf(p1.y, by, x[5] * old);
             x[6] = fmaf(p1.z, by, x[6] * old); x[7] = fmaf(p1.w, by, x[7] * old);
           }
-          write_out(rw, d, x, inverse(sum));
-          if (d == 0 && a.lse) write_lse(rw, mx, sum);
+          if (final) {
+            write_out(rw, d, x, inverse(sum));
+            if (d == 0 && a.lse) write_lse(rw, mx, sum);
+          } else {                          // nobody else reads these eight
+            __stcg(reinterpret_cast<float4*>(state(0) + rw * D + d), make_float4(x[0], x[1], x[2], x[3]));
+            __stcg(reinterpret_cast<float4*>(state(0) + rw * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
+          }
         }
+        if (final) break;
+        named_bar_sync(9, 256);             // all have read the maxima and sums that are written now
+        for (int rw = warp * 32 + lane; rw < w.rows; rw += 256) {
+          float mx = kLow, sum = 0.0f;
+          for (int i = 0; i < n; ++i) {
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(state(i) + S::Rows * D + 2 * rw));
+            const float to = fmaxf(mx, ms.x);
+            sum = fmaf(ms.y, ex2(ms.x - to), sum * ex2(mx - to));
+            mx = to;
+          }
+          __stcg(reinterpret_cast<float2*>(state(0) + S::Rows * D + 2 * rw), make_float2(mx, sum));
+        }
+        first = c0;
+        step = group;
+        n = groups;
+        final = true;
+        counter = a.counters + c0;
       }
     }
     reader.done(C);
