@@ -16,12 +16,14 @@
 //     then goes through shared memory). S is read twice, for the maximum and for the weights, instead of being kept in
 //     128 registers. P goes back to tensor memory over S. O is only rescaled when a row's maximum has grown by more than 2^8 (by
 //     the warps of that row themselves; sums are fp32, so nothing is lost by a maximum that is a little old).
-// Work is cut into equal runs of tiles, one to a CTA; items that lie in several runs are joined as in kv4_decode.cu.
+// Where there are no more (request, KV head, row block) items than CTAs, each gets an equal number of CTAs; else, or where that leaves too much
+// to the longest, all tiles are cut into equal runs, one to a CTA. Items that several CTAs have are joined in a fixed order, so results do
+// not depend on timing.
 // All waits are bounded.
 //
 // Bound by the tensor cores, 4 D operations for each pair of a query and a key it sees, and behind them by what surrounds them. Seven
-// chunks of 350 to 700 tokens behind contexts to 4096 (32 query and 4 KV heads of 128): 241 us, 0.74 PFLOP/s; a prompt of 8192 (16 query and 2 KV
-// heads of 256): 640 us, 0.86 PFLOP/s (690 us, 0.80 in a long loop). Once the pipeline runs, a tile of 256 rows and 128 keys takes 2050 ns for heads of 128,
+// chunks of 350 to 700 tokens behind contexts to 4096 (32 query and 4 KV heads of 128): 241 to 250 us, 0.72 PFLOP/s; a prompt of 8192 (16 query and 2 KV
+// heads of 256): 630 us, 0.87 PFLOP/s (688 us, 0.80 in a long loop). Once the pipeline runs, a tile of 256 rows and 128 keys takes 2050 ns for heads of 128,
 // where its products alone would take 1100: the softmax of each half tile takes 1850 cycles of the 2050 that pass between two, on two warps
 // of each scheduler that exchange 64 x 32 exponentials a warp and wait for tensor memory. Replacing some of the exponentials by
 // polynomials made it slower (243 -> 251 us for one pair in eight), as did keeping the scores in registers (247 -> 265 us), 16
@@ -44,12 +46,24 @@ constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
 constexpr float kLow = -1e38f, kRoom = 8.0f;
 constexpr int kNanList = 64;
-// States that one CTA joins. 256 rows over 65536 tokens (4 KV heads of 128, 37 states): 208 us alone, 123 in two steps; four requests of 64 tokens over 16384
-// (5 to 7 states) 111, with 6 here 126; 32 tokens (10 states) 137 alone, 114.
-constexpr int kJoinAlone = 8;
 // What an item costs beside its tiles, in tiles: loading its queries, filling and draining the pipeline, writing its output.
 // It counts where work is divided, for the first blocks of a prompt are many and short.
 constexpr int kOwn = 2;
+// States that one CTA joins. 256 rows over 65536 tokens (4 KV heads of 128, 37 states): 208 us alone, 123 in two steps; four requests of 64 tokens over 16384
+// (5 to 7 states) 111, with 6 here 126; 32 tokens (10 states) 137 alone, 114.
+constexpr int kJoinAlone = 8;
+// In tiles: what joining the states of s CTAs takes, and what runs that begin and end inside items cost beyond parts of one item. One request
+// of 200, 400, 800 tokens (32 query and 4 KV heads of 128) takes 21, 23, 32 us in parts of items, 40, 42, 62 in equal runs; one of 3000, with
+// more items than CTAs, or of 1600, whose last item is many times its first, 72 us in equal runs. With kCut 4 a chunk of 256 tokens over 4096 goes
+// to runs, 70 us instead of 58; with 14 one of 64 over 4096 to parts, 71 instead of
+// 63, one of 24 too, 58 instead of 68 (both with 2 + 1.5 t for joining; with 2 + t two of 64 over 2000 take 52 instead of 64).
+constexpr int kCut = 8;
+__device__ __forceinline__ int join_cost(int s) {
+  int t = s;
+  if (s > kJoinAlone)
+    for (t = 2; t * t < 4 * s;) ++t;        // two steps of sqrt(s)
+  return s == 1 ? 0 : 2 + t;
+}
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D>
@@ -92,6 +106,7 @@ struct Control {
   int found;
   long long found_at;
   long long wsum[32];
+  int witems[32], wlongest[32];
   Segment seg[kSegs];
   int32_t nan_list[kNanList];               // key * 16 + groups
   float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
@@ -994,10 +1009,29 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
 
 // ---- the warp that lists the segments
 template <int Rows>
-__device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int64_t per, int64_t u0, int64_t u1, int lane) {
+__device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int share, int64_t per, int64_t u0, int64_t u1, int lane) {
   Walk<Rows> w;
   w.b = C.found;
   w.load(a);
+  auto publish = [&](uint32_t n, const Walk<Rows>& v, int c0, int c1, bool more) {
+    if (lane == 0) {
+      const int tok = v.rb * v.it.tb;
+      C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
+                          v.it.first_tile(v.rb) + v.t0, max(v.t1 - v.t0, 0), c0, c1, v.t1 - v.t0 == v.tiles, more};
+      mbar_arrive(&C.seg_full[n % kSegs]);
+    }
+  };
+  if (share) {                              // this CTA's part of item u0
+    const int item = static_cast<int>(u0 - C.found_at);
+    w.head = item / w.blocks;
+    w.rb = item - w.head * w.blocks;
+    w.tiles = w.it.tiles(w.rb);
+    const int parts = min(share, w.tiles), c0 = static_cast<int>(u0) * share, part = static_cast<int>(blockIdx.x) - c0;
+    w.t0 = part < parts ? w.tiles * part / parts : 0;
+    w.t1 = part < parts ? w.tiles * (part + 1) / parts : 0;
+    publish(0, w, c0, c0 + parts - 1, false);
+    return;
+  }
   w.u = u0;
   w.u1 = u1;
   {  // the head and row block that u0 lies in: the lanes bisect together, 32 places at a time
@@ -1019,16 +1053,9 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int64_t
   w.open();
   for (uint32_t n = 0;; ++n) {
     wait<true>(&C.seg_empty[n % kSegs], ((n / kSegs) & 1) ^ 1, C, a);
-    const bool none = w.t1 <= w.t0;         // a run of nothing but an item's own units
     const Walk<Rows> v = w;
-    const bool more = !none && w.next(a);
-    if (lane == 0) {
-      const int tok = v.rb * v.it.tb;
-      C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
-                          v.it.first_tile(v.rb) + v.t0, none ? 0 : v.t1 - v.t0, static_cast<int>(v.i0 / per), static_cast<int>((v.i0 + v.tiles - 1) / per),
-                          v.t1 - v.t0 == v.tiles, more};
-      mbar_arrive(&C.seg_full[n % kSegs]);
-    }
+    const bool more = w.t1 > w.t0 && w.next(a);   // else: a run of nothing but an item's own units
+    publish(n, v, static_cast<int>(v.i0 / per), static_cast<int>((v.i0 + v.tiles - 1) / per), more);
     if (!more) break;
   }
 }
@@ -1043,32 +1070,54 @@ __global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const Attn
   // this CTA's run of all tiles
   const int chunk = (a.batch + S::Threads - 1) / S::Threads;
   long long mine = 0;
+  int mine_items = 0, longest = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     const Item it = item_of(a, request_of(a, b, blockIdx.x == 0), S::Rows);
-    mine += static_cast<long long>(tiles_before(it, it.blocks())) * a.hk;
+    const int blocks = it.blocks();
+    mine += static_cast<long long>(tiles_before(it, blocks)) * a.hk;
+    mine_items += blocks * a.hk;
+    if (blocks) longest = max(longest, max(it.tiles(blocks - 1), it.tiles(max(blocks - 2, 0))));
   }
   long long upto = mine;
+  int upto_items = mine_items;
+  longest = __reduce_max_sync(0xFFFFFFFFu, longest);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const long long x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-    if (lane >= d) upto += x;
+    const int y = __shfl_up_sync(0xFFFFFFFFu, upto_items, d);
+    if (lane >= d) { upto += x; upto_items += y; }
   }
-  if (lane == 31) C.wsum[warp] = upto;
+  if (lane == 31) { C.wsum[warp] = upto; C.witems[warp] = upto_items; C.wlongest[warp] = longest; }
   __syncthreads();
   long long total = 0;
+  int items = 0;
   for (int i = 0; i < S::Threads / 32; ++i) {
-    if (i < warp) upto += C.wsum[i];
+    if (i < warp) { upto += C.wsum[i]; upto_items += C.witems[i]; }
     total += C.wsum[i];
+    items += C.witems[i];
+    longest = max(longest, C.wlongest[i]);
   }
-  const long long per = (total + gridDim.x - 1) / gridDim.x, u0 = blockIdx.x * per, u1 = min(u0 + per, total);
+  const int ctas = static_cast<int>(gridDim.x);
+  const long long per = (total + ctas - 1) / ctas;
+  // CTAs for each item, by what the longest item then takes (0: equal runs)
+  int share = 0;
+  if (items > 0 && items <= ctas) {
+    uint32_t best = 0xFFFFFFFFu;
+    for (int s = 1 + lane; s <= min(ctas / items, longest); s += 32) best = min(best, static_cast<uint32_t>((longest + s - 1) / s + join_cost(s)) << 8 | s);
+    best = __reduce_min_sync(0xFFFFFFFFu, best);
+    if ((best >> 8) <= per + kCut) share = best & 255;
+  }
+  // where this CTA begins: its run of all tiles, or its item
+  const long long u0 = share ? blockIdx.x / share : blockIdx.x * per, u1 = share ? items : min(u0 + per, total);
   if (u0 >= u1) return;                     // the whole CTA, before anything is allocated
-  if (upto - mine <= u0 && u0 < upto) {
-    long long at = upto - mine;
+  const long long before = share ? upto_items - mine_items : upto - mine, behind = share ? upto_items : upto;
+  if (before <= u0 && u0 < behind) {
+    long long at = before;
     int b = tid * chunk;
     if (chunk > 1)
       for (;; ++b) {
         const Item it = item_of(a, request_of(a, b, false), S::Rows);
-        const long long cost = static_cast<long long>(tiles_before(it, it.blocks())) * a.hk;
+        const long long cost = static_cast<long long>(share ? it.blocks() : tiles_before(it, it.blocks())) * a.hk;
         if (at + cost > u0) break;
         at += cost;
       }
@@ -1103,7 +1152,7 @@ __global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const Attn
   else if (warp >= kFirstFill) fill_role<D, true, !S::Split>(a, smem, C, warp - kFirstFill, lane);
   else if (warp >= kFirstSoftmax) softmax_role<D>(a, C, warp - kFirstSoftmax, warp & 3, lane);
   else if (warp < kMmaWarp + kMmaWarps) { if (S::Twin || warp == kMmaWarp) mma_role<D>(a, smem, C, S::Twin ? uniform(warp - kMmaWarp) : 0); }
-  else plan_role<S::Rows>(a, C, per, u0, u1, lane);
+  else plan_role<S::Rows>(a, C, share, per, u0, u1, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
