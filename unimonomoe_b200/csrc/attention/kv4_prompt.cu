@@ -5,8 +5,8 @@
 // Heads of 64 and 128: two Q tiles of 128 rows, which share the operands made of the codes; the scores of half a tile of keys are made
 // while the other half's have their softmax. Heads of 256, whose O alone takes half of tensor memory: one Q tile, whose scores are
 // made a tile of keys ahead.
-// Nineteen warps, one CTA on an SM:
-//   8 turn codes into operands: a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
+// Nineteen warps, 27 for heads of 256, one CTA on an SM:
+//   8 turn codes into operands (8 those of keys, 8 those of values for heads of 256): a block of 16 tokens each, s * c exact in bf16, into a ring of [128 keys x 128 dims] slots in the
 //     128-byte-swizzled layout, keys for S with dims along K, values as they are (dims along N). A block's words are what a lane
 //     stores as 16 bytes, eight dims in the order 0 4 1 5 2 6 3 7 in which masking leaves them; queries are stored in the same
 //     order, and the output is put back from it.
@@ -27,8 +27,8 @@
 // where its products alone would take 1100: the softmax of each half tile takes 1850 cycles of the 2050 that pass between two, on two warps
 // of each scheduler that exchange 64 x 32 exponentials a warp and wait for tensor memory. Replacing some of the exponentials by
 // polynomials made it slower (243 -> 251 us for one pair in eight), as did keeping the scores in registers (247 -> 265 us), 16
-// softmax warps (245 -> 261 us) and their 27 warps' registers (243 -> 263 us). Heads of 256 take 2500 ns for 128 rows and 128 keys:
-// their operands, twice as many for each product, pass shared memory three times, 2560 cycles of its bandwidth in 4600.
+// softmax warps (245 -> 261 us) and their 27 warps' registers (243 -> 263 us). Heads of 256 take 2100 ns for 128 rows and 128 keys:
+// their operands, twice as many for each product, pass shared memory three times, 2560 cycles of its bandwidth in 4000.
 #include <climits>
 #include <type_traits>
 #include "kv4_attention.cuh"
@@ -335,7 +335,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 constexpr uint32_t kSCol = 0, kOCol = 256;
 
-// ---- the eight warps that fill the ring
+// ---- the warps that fill the ring
 // A lane's words and scales of a block of 16 tokens: of its keys (tokens g, g + 8), or of its values (2t, 2t+1, 2t+8, 2t+9).
 // 16 bytes that nobody else on this SM reads: not kept in what shared memory leaves of L1.
 __device__ __forceinline__ uint4 ldg_once(const uint8_t* p) {
