@@ -1,0 +1,62 @@
+"""The attention operators where something is missing, not finite or out of range, in shapes that the tests by size do not have."""
+import math
+
+import pytest
+import torch
+
+from tests import attention_ref as ref
+from tests.test_gpu_attention import DEV, close, gen, make, randn
+from unimonomoe_b200 import attention as A
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    A.check_status(DEV)
+
+
+def store(cache, table, b, k, v, page):
+    """Keys and values of request b, from its first token on."""
+    i = torch.arange(len(k), device=DEV)
+    A.kv4_append(k, v, cache, table[b].long()[i // page] * page + i % page)
+
+
+# ---------------------------------------------------------------------- values that are not numbers
+@pytest.mark.parametrize("H,K,D", [(4, 4, 64), (8, 2, 64), (8, 4, 128), (16, 2, 128), (8, 4, 256)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_values_that_are_not_numbers_in_many_short_prompts(H, K, D, window):
+    """CTAs have many items of a single tile of keys one after another: a group that is not a number reaches the rows of its own
+    request that see it, all of them, and no other request's."""
+    count = 500
+    lens = [60 + (37 * i) % 69 for i in range(count)]
+    cache, table, ln, st, q, keys, values, starts = make(lens, lens, H, K, D, 16, seed=D + K)
+    for b in range(0, count, 3):
+        v = randn((lens[b], K, D), 500 + D + K + b)          # what make() has stored, with one value in it that is not finite
+        at, head, dim = (11 * b) % lens[b], b % K, (29 * b) % D
+        v[at, head, dim] = (math.nan, math.inf, -math.inf)[b % 3]
+        store(cache, table, b, randn((lens[b], K, D), 100 + D + K + b), v, 16)
+        values[b] = ref.quantised(v)
+    want = ref.attention(q, keys, values, starts, window, D ** -0.5)
+    assert torch.isnan(want[0]).any()
+    for _ in range(3):
+        out, lse = A.kv4_attention(q, cache, table, ln, st, 128, window=window, return_lse=True)
+        close(out, lse, want)
+
+
+@pytest.mark.parametrize("H,K,D", [(2, 1, 64), (8, 1, 128), (8, 2, 256)])
+@pytest.mark.parametrize("window", [0, 60, 97])
+def test_values_that_are_not_numbers_far_apart_in_a_window(H, K, D, window):
+    """Two hundred of them in two places: with a window the rows between see none."""
+    n = 500
+    cache, table, ln, st, q, keys, values, starts = make([n, n], [n, 300], H, K, D, 16, seed=D)
+    for b in range(2):
+        v = randn((n, K, D), 500 + D + b)
+        v[60:160, 0, 3] = math.inf
+        v[390:490, K - 1, D - 1] = math.nan
+        store(cache, table, b, randn((n, K, D), 100 + D + b), v, 16)
+        values[b] = ref.quantised(v)
+    want = ref.attention(q, keys, values, starts, window, D ** -0.5)
+    close(A.kv4_attention(q, cache, table, ln, st, n, window=window), None, want)
+    assert window == 0 or not torch.isnan(want[0][260:390]).any()

@@ -45,7 +45,7 @@ constexpr int kSegs = 4;                    // segments that the roles may be ap
 constexpr int kKeys = 128, kRows = 128;    // of a product's tile
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
 constexpr float kLow = -1e38f, kRoom = 8.0f;
-constexpr int kNanList = 64;
+constexpr int kHits = 16;                   // words of the rows that see values that are not numbers
 // What an item costs beside its tiles, in tiles: loading its queries, filling and draining the pipeline, writing its output.
 // It counts where work is divided, for the first blocks of a prompt are many and short.
 constexpr int kOwn = 2;
@@ -83,6 +83,8 @@ struct Shape {
   static constexpr int Sub = Twin ? 64 : 128;           // keys of a score buffer
   static constexpr int Cols = Twin ? D : D / 2;         // output columns of a thread
   static constexpr int Part = Rows * (D + 2);           // floats of a CTA's state: output, maximum and sum
+  static constexpr int HitWords = kHits / NG;           // for each group of dims
+  static_assert(HitWords * 32 >= Rows, "a bit for each token of a row block");
 };
 
 // Tiles [first, first + count) of keys for a row block: all query heads of a KV head for some tokens of a request.
@@ -101,14 +103,12 @@ struct Control {
   uint64_t s_full[4], p_full[4];            // score buffers: 2 Q tile + half of the tile of keys, or tile of keys modulo 2
   uint64_t o_done[2], o_all, o_free;        // a buffer's products with values (for each Q tile), a segment's; the segment's output has been read
   uint32_t tmem, abort, last;
-  uint32_t nan_count;                       // value groups that are not numbers: key and group of the first kNanList of a segment,
-  int nan_first[4], nan_last[4];            // and for each group the keys that they lie between
   int found;
   long long found_at;
   long long wsum[32];
   int witems[32], wlongest[32];
   Segment seg[kSegs];
-  int32_t nan_list[kNanList];               // key * 16 + groups
+  uint32_t hit[kSegs][kHits];               // for each group of dims, the segment's tokens that see a value there which is not a number
   float top[kRows], sum[2][kRows];          // running maxima; the sums of the two sets of warps
 };
 
@@ -405,6 +405,15 @@ struct Raw {
   }
 };
 
+// Marks the tokens of a row block that see the key `at` places behind its first token (before it where negative).
+__device__ __noinline__ void seen_by(uint32_t* hit, int words, int at, int window) {
+  const int to = window > 0 ? at + window : INT_MAX;
+  for (int i = 0; i < words; ++i) {
+    const int lo = min(max(at - 32 * i, 0), 32), hi = min(max(to - 32 * i, 0), 32);
+    if (lo < hi) atomicOr(hit + i, (0xFFFFFFFFu >> (32 - (hi - lo))) << lo);
+  }
+}
+
 // `warp`: which of the eight blocks of 16 tokens of a tile. A ring is in the order in which the products take it:
 // K0 V0 K1 V1 .., or with scores a tile ahead K0 K1 V0 K2 V1 .. V(last). What is stored is loaded again at once, for the tile after.
 template <int D, bool KEYS, bool VALUES>
@@ -434,7 +443,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
   for (;;) {
     const Segment& w = reader.take(C, a);
     const uint32_t seg = reader.n;
-    const int first = w.first, count = w.count, end = w.end, more = w.more, request = w.request;
+    const int first = w.first, count = w.count, end = w.end, more = w.more, request = w.request, place = w.place;
     if (count == 0) break;
     const int64_t head_at = static_cast<int64_t>(w.head) << page_shift, page_blocks = static_cast<int64_t>(a.hk) << page_shift;
 
@@ -526,7 +535,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
 #pragma unroll
         for (int i = 0; i < Raw<D, true>::SW; ++i) sum = add_bf16x2(sum, v.scale[u][i]);
       if (__any_sync(0xFFFFFFFFu, (sum & 0x7FFFu) > 0x7F80u || (sum & 0x7FFF0000u) > 0x7F800000u)) {
-        wait(&C.o_free, (seg & 1) ^ 1, C, a);           // the list of the segment before has been read
+        // in the segment's own list: the one before may still be read, and the one before that, where a single tile lies between
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -534,13 +543,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
             uint32_t& x = v.scale[u][gi >> 1];
             if ((x >> (gi & 1) * 16 & 0x7FFFu) > 0x7F80u) {
               x &= gi & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-              if (g == 0) {
-                const int key = key0 + 2 * t + (u & 1) + 8 * (u >> 1);
-                atomicMin(&C.nan_first[gi], key);
-                atomicMax(&C.nan_last[gi], key);
-                const uint32_t to = atomicAdd(&C.nan_count, 1u);
-                if (to < kNanList) C.nan_list[to] = key * 4 + gi;
-              }
+              if (g == 0) seen_by(C.hit[seg % kSegs] + gi * S::HitWords, S::HitWords, key0 + 2 * t + (u & 1) + 8 * (u >> 1) - place, a.window);
             }
           }
         __syncwarp();
@@ -874,17 +877,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
     tc_fence_after();
     // groups that are not numbers and that this row sees
     uint32_t nans = 0;
-    const uint32_t listed = *static_cast<volatile uint32_t*>(&C.nan_count);
-    if (listed) {
-      for (uint32_t i = 0; i < min(listed, static_cast<uint32_t>(kNanList)); ++i) {
-        const int key = C.nan_list[i] >> 2;
-        if (key >= lo && key < hi) nans |= 1u << (C.nan_list[i] & 3);
-      }
-      // more than the list holds: all keys between the first and the last count (which only a window can tell apart)
-      if (listed > kNanList)
-        for (int gi = 0; gi < S::NG; ++gi)
-          if (*static_cast<volatile int*>(&C.nan_first[gi]) < hi && *static_cast<volatile int*>(&C.nan_last[gi]) >= lo) nans |= 1u << gi;
-    }
+#pragma unroll
+    for (int gi = 0; gi < S::NG; ++gi)
+      nans |= (*static_cast<volatile uint32_t*>(&C.hit[reader.n % kSegs][gi * S::HitWords + (tok >> 5)]) >> (tok & 31) & 1u) << gi;
     const bool whole = w.whole;
     const int c0 = w.c0, c1 = w.c1;
     float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0 ? 1 : 0)) * S::Part;
@@ -927,9 +922,6 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Control& C, int 
       }
     }
     tc_fence_before();
-    named_bar_sync(9, 256);                 // everyone has read the list of this segment
-    if (warp == 0 && lane < 4) { C.nan_count = 0; C.nan_first[lane] = INT_MAX; C.nan_last[lane] = -1; }
-    __syncwarp();
     mbar_arrive(&C.o_free);
     if (whole) {
       if (real && col0 == 0 && a.lse) write_lse(row, m, l);
@@ -1014,6 +1006,8 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int sha
   w.b = C.found;
   w.load(a);
   auto publish = [&](uint32_t n, const Walk<Rows>& v, int c0, int c1, bool more) {
+    if (lane < kHits) C.hit[n % kSegs][lane] = 0;
+    __syncwarp();
     if (lane == 0) {
       const int tok = v.rb * v.it.tb;
       C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
@@ -1141,8 +1135,6 @@ __global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const Attn
     mbar_init(&C.o_free, kSoftmaxWarps * 32);
     mbar_init_fence();
     C.abort = 0;
-    C.nan_count = 0;
-    for (int i = 0; i < 4; ++i) { C.nan_first[i] = INT_MAX; C.nan_last[i] = -1; }
   }
   tc_fence_before();
   __syncthreads();
