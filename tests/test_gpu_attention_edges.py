@@ -60,3 +60,19 @@ def test_values_that_are_not_numbers_far_apart_in_a_window(H, K, D, window):
     want = ref.attention(q, keys, values, starts, window, D ** -0.5)
     close(A.kv4_attention(q, cache, table, ln, st, n, window=window), None, want)
     assert window == 0 or not torch.isnan(want[0][260:390]).any()
+
+
+# ---------------------------------------------------------------------- pages that are not there
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("H,K,D", [(2, 2, 64), (16, 2, 128), (8, 2, 256)])
+@pytest.mark.parametrize("news", [[1, 2], [5, 1], [150, 70], [300, 40]])
+@pytest.mark.parametrize("window", [1, 30, 200])
+def test_pages_before_the_window_may_be_gone(page, H, K, D, news, window):
+    """A server that gives back what no later token sees: its entries are -1, and nothing is reported."""
+    lens = [n + 600 + 77 * i for i, n in enumerate(news)]
+    cache, table, ln, st, q, keys, values, starts = make(lens, news, H, K, D, page, seed=D)
+    for b, (n, m) in enumerate(zip(lens, news)):
+        table[b, :max(n - m + 1 - window, 0) // page] = -1
+    out, lse = A.kv4_attention(q, cache, table, ln, st, max(news), window=window, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, window, D ** -0.5))
+    A.check_status(DEV)

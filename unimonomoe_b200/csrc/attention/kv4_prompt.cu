@@ -90,7 +90,7 @@ struct Shape {
 // Tiles [first, first + count) of keys for a row block: all query heads of a KV head for some tokens of a request.
 struct Segment {
   int request, head, q_row, rows;           // first query row; query rows of the block
-  int place, end;                           // place of the first token; keys that any row sees
+  int place, begin, end;                    // place of the first token; [begin, end): keys that any row sees
   int first, count;
   int c0, c1;                               // the CTAs that share the item: more than one where count is not all of it
   int whole, more;
@@ -138,7 +138,8 @@ __device__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
 struct Item {
   int place0, n, len, tb, window;
   __device__ __forceinline__ int blocks() const { return (n + tb - 1) / tb; }
-  __device__ __forceinline__ int first_tile(int rb) const { return window > 0 ? max(place0 + rb * tb + 1 - window, 0) / kKeys : 0; }
+  __device__ __forceinline__ int begin(int rb) const { return window > 0 ? max(place0 + rb * tb + 1 - window, 0) : 0; }
+  __device__ __forceinline__ int first_tile(int rb) const { return begin(rb) / kKeys; }
   __device__ __forceinline__ int seen(int rb) const { return min(len, max(place0 + min((rb + 1) * tb, n), 0)); }
   // tiles of row block rb, at least one
   __device__ __forceinline__ int tiles(int rb) const { return max(1, (seen(rb) + kKeys - 1) / kKeys - first_tile(rb)); }
@@ -349,7 +350,7 @@ struct Raw {
   uint4 code[NG];
   uint32_t scale[Tok][SW];
 
-  // The block at p; null: one behind all keys, read as zeros.
+  // The block at p; null: one before or behind all keys, read as zeros.
   __device__ __forceinline__ void load(const uint8_t* p, int g, int t, int lane) {
     if (p == nullptr) {
 #pragma unroll
@@ -443,19 +444,20 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
   for (;;) {
     const Segment& w = reader.take(C, a);
     const uint32_t seg = reader.n;
-    const int first = w.first, count = w.count, end = w.end, more = w.more, request = w.request, place = w.place;
+    const int first = w.first, count = w.count, begin = w.begin, end = w.end, more = w.more, request = w.request, place = w.place;
     if (count == 0) break;
     const int64_t head_at = static_cast<int64_t>(w.head) << page_shift, page_blocks = static_cast<int64_t>(a.hk) << page_shift;
 
-    // page of this warp's block of tile `lane` of each 32 tiles
+    // page of this warp's block of tile `lane` of each 32 tiles; none for a block that no row sees, whose entry may be gone
     int pages = 0;
+    auto seen = [&](int blk) { return blk * 16 < end && blk * 16 + 16 > begin; };
     auto block = [&](int j) -> const uint8_t* {
       if ((j & 31) == 0) {
         const int blk = (first + j + lane) * (kKeys / 16) + warp;
-        pages = blk * 16 < end ? page_of(a, request, blk >> page_shift) : 0;
+        pages = seen(blk) ? page_of(a, request, blk >> page_shift) : 0;
       }
       const int blk = (first + j) * (kKeys / 16) + warp, pg = __shfl_sync(0xFFFFFFFFu, pages, j & 31);
-      return blk * 16 < end ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
+      return seen(blk) ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
     };
     std::conditional_t<KEYS, Raw<D, false>, Nothing> k;
     std::conditional_t<VALUES, Raw<D, true>, Nothing> v;
@@ -1010,7 +1012,7 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int sha
     __syncwarp();
     if (lane == 0) {
       const int tok = v.rb * v.it.tb;
-      C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.seen(v.rb),
+      C.seg[n % kSegs] = {v.b, v.head, v.r.first + tok, min(v.it.tb, v.it.n - tok) * a.group, v.it.place0 + tok, v.it.begin(v.rb), v.it.seen(v.rb),
                           v.it.first_tile(v.rb) + v.t0, max(v.t1 - v.t0, 0), c0, c1, v.t1 - v.t0 == v.tiles, more};
       mbar_arrive(&C.seg_full[n % kSegs]);
     }
