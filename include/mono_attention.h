@@ -36,7 +36,8 @@ typedef struct CUstream_st* mono_attn_stream_t; /* cudaStream_t */
 
 /* Positions, slots, requests and block-table entries of a step's tokens. cached, fresh: int32 [batch], tokens in the cache
  * and tokens of this step. table: int32 [batch, width]; the entries of the pages that a request has are read, those of the
- * pages that it gets are written. free_pages: int32 [free_count]; the next one handed out is free_pages[*taken].
+ * pages that it gets are written. free_pages: int32 [free_count]; the next one handed out is free_pages[*taken],
+ * entries for which there is none left become -1 (*taken_out is then above free_count).
  * Out: query_start int32 [batch + 1], seq_lens int32 [batch], positions int32, slots int64 and requests int32 [tokens]
  * (rows behind the last token: 0, -1, -1), taken_out int32 [1]. A token without a page gets slot -1. */
 int mono_attn_plan(const int32_t* cached, const int32_t* fresh, int batch, int32_t* table, int width, const int32_t* free_pages,
@@ -67,7 +68,8 @@ int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, c
 
 /* Attention of q [tokens, q_heads, head_dim] over the cache, into contiguous bf16 out and, unless null, fp32 lse [tokens,
  * q_heads] (natural log). Rows query_start[b] .. query_start[b + 1] are the last ones of sequence b, seq_lens[b] long with them;
- * each sees the keys up to its own place, with window > 0 the last `window` of them. Rows of no request are not written.
+ * each sees the keys up to its own place, with window > 0 the last `window` of them. Keys and values of a page that is missing from block_table (an
+ * entry outside the cache, which is reported) are zeros. Rows of no request are not written.
  * max_query_len: an upper bound of the queries of a request; it chooses kernels, results do not depend on it.
  * workspace: mono_attn_workspace_bytes(), its first 4 * MONO_ATTN_COUNTERS bytes zero before the first launch (each launch
  * leaves them zero); launches that share it must not overlap. */

@@ -76,3 +76,29 @@ def test_pages_before_the_window_may_be_gone(page, H, K, D, news, window):
     out, lse = A.kv4_attention(q, cache, table, ln, st, max(news), window=window, return_lse=True)
     close(out, lse, ref.attention(q, keys, values, starts, window, D ** -0.5))
     A.check_status(DEV)
+
+
+@pytest.mark.parametrize("H,K,D", [(8, 2, 64), (16, 2, 128), (10, 2, 256)])
+@pytest.mark.parametrize("entry", [-1, 10 ** 6])
+@pytest.mark.parametrize("news", [1, 3, 250])
+def test_a_missing_page_is_zeros_and_no_other_requests_page(H, K, D, entry, news):
+    lens = [400, 400]
+    cache, table, ln, st, q, keys, values, starts = make(lens, [news] * 2, H, K, D, 32, seed=D)
+    for b, col in ((0, 2), (0, 3), (1, 12)):
+        table[b, col] = entry
+        keys[b][32 * col:32 * (col + 1)] = 0
+        values[b][32 * col:32 * (col + 1)] = 0
+    out, lse = A.kv4_attention(q, cache, table, ln, st, news, return_lse=True)
+    with pytest.raises(RuntimeError, match="block-table entry"):
+        A.check_status(DEV)
+    close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))
+
+
+def test_plan_without_pages_enters_none():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = i32([[1, 90, 91, 92], [2, 93, 94, 95]])            # both rows hold what earlier requests had
+    p = A.plan_batch(i32([16, 16]), i32([20, 17]), table, i32([5, 6, 7]), i32([0]), 16, 37)
+    with pytest.raises(RuntimeError, match="more pages"):
+        A.check_status(DEV)
+    assert table.tolist() == [[1, 5, 6, 92], [2, 7, -1, 95]] and p.taken.tolist() == [4]
+    assert p.slots.tolist() == [*range(80, 100), *range(112, 128), -1]

@@ -146,7 +146,7 @@ def plan_batch(cached_lens, new_lens, block_table, free_pages, taken, page_size:
     """Where the tokens of a step go. ``cached_lens`` and ``new_lens`` (int32 [batch]) are each request's tokens in the cache and
     in this step, ``block_table`` (int32 [batch, width]) its pages, ``free_pages`` (int32) the free list, of which the first
     ``taken`` (int32 [1]) are in use. New pages are taken from the list in the order of the requests and entered into
-    ``block_table`` in place. ``num_tokens`` is the number of rows of the result: rows behind the last token hold position
+    ``block_table`` in place; where the list is too short, -1 is entered and ``taken`` of the result lies behind its end. ``num_tokens`` is the number of rows of the result: rows behind the last token hold position
     0, slot -1, request -1, so a captured graph serves any smaller step. Nothing is read back to the host."""
     return BatchPlan(*(_C or _load()).plan(cached_lens, new_lens, block_table, free_pages, taken, page_size, num_tokens))
 
@@ -184,7 +184,7 @@ def kv4_attention(q, cache: KV4Cache, block_table, seq_lens, query_start, max_qu
     """Attention of ``q`` (bf16 [tokens, heads, head_dim]) over the cache. Rows ``query_start[b]`` to ``query_start[b + 1]`` (int32
     [batch + 1]) are the last tokens of sequence b, which is ``seq_lens[b]`` (int32 [batch]) long with them and lies in the pages
     ``block_table[b]`` (int32 [batch, width]). Each query sees the keys up to its own place; with ``window`` > 0, the last
-    ``window`` of those. heads / kv_heads query heads share a KV head. ``scale`` is 1 / sqrt(head_dim) unless given.
+    ``window`` of those. A page that is missing from the table is reported, its keys and values are zeros. heads / kv_heads query heads share a KV head. ``scale`` is 1 / sqrt(head_dim) unless given.
 
     Returns ``out`` (bf16 [tokens, heads, head_dim], made unless given) or (out, lse) with the fp32 natural log-sum-exp [tokens,
     heads]. A query that sees no key gets zeros and -inf. Rows that belong to no request are left as they are.

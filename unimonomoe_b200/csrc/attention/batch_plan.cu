@@ -91,8 +91,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
     if (held + f > a.width && lane == 0 && n > 0) kv4::report(a.status, kv4::kTooLong, b);
     for (int j = lane; j < f; j += 32) {
       const int at = taken + first[b] + j;
-      if (held + j < a.width && at >= 0 && at < a.free_count)
-        a.table[static_cast<int64_t>(b) * a.width + held + j] = a.free_pages[at];
+      if (held + j < a.width)               // none left: not what the row held for an earlier request
+        a.table[static_cast<int64_t>(b) * a.width + held + j] = at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
     }
   }
 

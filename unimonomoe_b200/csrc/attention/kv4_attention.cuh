@@ -46,12 +46,13 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int b, bool tel
   return {s, e - s, min(max(len, 0), cap)};
 }
 
-// Page of column `col` of request b. An entry outside the cache is reported and read as page 0.
+// Page of column `col` of request b. An entry outside the cache is reported: -1, whose keys and values are zeros. Any page that there is might be
+// another request's.
 __device__ __forceinline__ int page_of(const AttnArgs& a, int b, int col) {
   const int p = __ldg(a.table + static_cast<int64_t>(b) * a.width + min(col, a.width - 1));
   if (p >= 0 && p < a.num_pages) return p;
   report(a.status, kBadPage, b);
-  return 0;
+  return -1;
 }
 
 // The two kernels: requests of up to a.split_rows query rows for a KV head, and those of more.

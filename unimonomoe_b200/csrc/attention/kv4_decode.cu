@@ -41,8 +41,9 @@ constexpr int kOwn = 1, kJoin = 2;
 constexpr float kLow = -1e38f;              // below every score
 constexpr float kRoom = 8.0f;               // log2 of what a weight may grow to before the maximum is moved
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes, of which the first `bytes` are read and the others zeros.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -210,10 +211,11 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       for (int h = 0; h < 2; ++h) {
         const int pg = __shfl_sync(0xFFFFFFFFu, pages, (i & 15) * 2 + h);
         if (h == 0 || (blk + 1) * 16 < p.k1) {
-          const uint8_t* src = head_at + static_cast<int64_t>(pg) * page_bytes + ((blk + h) & in_page) * S::Block;
+          const uint32_t bytes = pg < 0 ? 0 : 16;                 // no page: zeros
+          const uint8_t* src = head_at + static_cast<int64_t>(max(pg, 0)) * page_bytes + ((blk + h) & in_page) * S::Block;
 #pragma unroll
           for (int j = 0; j < (S::Block + 511) / 512; ++j)
-            if ((j + 1) * 512 <= S::Block || lane < (S::Block - j * 512) / 16) cp16(to + h * S::Block + j * 512, src + j * 512);
+            if ((j + 1) * 512 <= S::Block || lane < (S::Block - j * 512) / 16) cp16(to + h * S::Block + j * 512, src + j * 512, bytes);
         }
       }
       if (++wstage == S::Stages) wstage = 0;

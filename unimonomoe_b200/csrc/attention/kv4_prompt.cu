@@ -350,7 +350,7 @@ struct Raw {
   uint4 code[NG];
   uint32_t scale[Tok][SW];
 
-  // The block at p; null: one before or behind all keys, read as zeros.
+  // The block at p; null: one before or behind all keys, or without a page, read as zeros.
   __device__ __forceinline__ void load(const uint8_t* p, int g, int t, int lane) {
     if (p == nullptr) {
 #pragma unroll
@@ -457,7 +457,7 @@ __device__ __forceinline__ void fill_role(const AttnArgs& a, uint8_t* smem, Cont
         pages = seen(blk) ? page_of(a, request, blk >> page_shift) : 0;
       }
       const int blk = (first + j) * (kKeys / 16) + warp, pg = __shfl_sync(0xFFFFFFFFu, pages, j & 31);
-      return seen(blk) ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
+      return pg >= 0 && seen(blk) ? a.cache + (pg * page_blocks + head_at + (blk & ((1 << page_shift) - 1))) * block_bytes(D) : nullptr;
     };
     std::conditional_t<KEYS, Raw<D, false>, Nothing> k;
     std::conditional_t<VALUES, Raw<D, true>, Nothing> v;
