@@ -102,3 +102,16 @@ def test_plan_without_pages_enters_none():
         A.check_status(DEV)
     assert table.tolist() == [[1, 5, 6, 92], [2, 7, -1, 95]] and p.taken.tolist() == [4]
     assert p.slots.tolist() == [*range(80, 100), *range(112, 128), -1]
+
+
+# ---------------------------------------------------------------------- scales
+@pytest.mark.parametrize("H,K,D", [(4, 2, 64), (12, 2, 128), (10, 2, 256)])
+@pytest.mark.parametrize("lens,news", [([700, 3], [1, 1]), ([300, 9], [5, 7]), ([260, 200], [250, 200])])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-38, -1e-30, 0.1])
+def test_no_scale_and_queries_of_next_to_nothing_weigh_all_alike(H, K, D, lens, news, scale):
+    cache, table, ln, st, q, keys, values, starts = make(lens, news, H, K, D, 16, seed=D)
+    q[:, ::3] = 0
+    q[:, 1::3] *= 2.0 ** -115
+    for window in (0, 6):
+        out, lse = A.kv4_attention(q, cache, table, ln, st, max(news), scale=scale, window=window, return_lse=True)
+        close(out, lse, ref.attention(q, keys, values, starts, window, scale))

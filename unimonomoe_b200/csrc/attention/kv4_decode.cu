@@ -322,7 +322,8 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const int ex = min(max(static_cast<int>(top >> 23) - 127, -100), 100);
       const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
-      const float f = fmaxf(fabsf(a.scale_log2), 1e-37f) * __uint_as_float(static_cast<uint32_t>(24 - 14 + ex + 127) << 23);
+      // not 0 (a scale of 0, a row of zeros), for -inf times it stays -inf: below 1e-37 it makes no weight differ from 1
+      const float f = fmaxf(fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(24 - 14 + ex + 127) << 23), 1e-37f);
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
         float sum = 0.0f;
