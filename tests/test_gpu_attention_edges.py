@@ -1,5 +1,8 @@
 """The attention operators where something is missing, not finite or out of range, in shapes that the tests by size do not have."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -115,3 +118,62 @@ def test_no_scale_and_queries_of_next_to_nothing_weigh_all_alike(H, K, D, lens, 
     for window in (0, 6):
         out, lse = A.kv4_attention(q, cache, table, ln, st, max(news), scale=scale, window=window, return_lse=True)
         close(out, lse, ref.attention(q, keys, values, starts, window, scale))
+
+
+# ---------------------------------------------------------------------- the status word, graphs
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from unimonomoe_b200 import attention as A
+dev = torch.device("cuda:0")
+junk = [torch.full((1 << k,), -1, dtype=torch.int32, device=dev) for k in range(1, 24)]     # what a word made from freed memory would hold
+del junk
+x = torch.ones(1, 1, 64, dtype=torch.bfloat16, device=dev)
+cache = A.KV4Cache(torch.zeros(2, 1, 1, 17 * 64, dtype=torch.uint8, device=dev))
+good, bad = torch.zeros(1, dtype=torch.int64, device=dev), torch.full((1,), 99, dtype=torch.int64, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    k, v = A.kv4_read(cache, good)                           # the first call of the process
+A.check_status(dev)                                          # nothing has run yet
+def faulty():
+    A.kv4_append(x, x, cache, bad)
+def told():
+    try:
+        A.check_status(dev)
+    except RuntimeError as e:
+        assert "slot outside" in str(e), e
+        return True
+    return False
+graph.replay()
+assert not told()
+faulty()
+graph.replay()
+assert told() and not told()
+graph.replay()
+faulty()
+assert told() and not told()
+print("fine")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    got = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], capture_output=True, text=True, timeout=300,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert got.returncode == 0 and got.stdout.strip() == "fine", got.stdout + got.stderr
+
+
+def test_graphs_captured_on_a_stream_without_a_workspace_run_one_after_another():
+    H, K, D = 8, 2, 128
+    cache, table, ln, st, q, keys, values, starts = make([3000, 900], [1, 60], H, K, D, 16, seed=6)
+    want = [A.kv4_attention(x, cache, table, ln, st, 60) for x in (q, -q)]
+    stream, graphs, outs = torch.cuda.Stream(), [], []
+    for x in (q, -q):
+        graphs.append(torch.cuda.CUDAGraph())
+        outs.append(torch.full_like(q, math.nan))
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            A.kv4_attention(x, cache, table, ln, st, 60, out=outs[-1])
+    for _ in range(3):
+        for graph, out in zip(graphs, outs):
+            out.fill_(math.nan)
+            graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))

@@ -122,11 +122,19 @@ class Block {
 
 // ---- what is kept: a status word for each device, a workspace for each stream of a device. Never freed: a captured graph may
 // hold their addresses, and at exit the allocator is gone before them.
+//
+// The word is zeroed once, before any launch that may report into it, whatever stream that goes to; and not as a part of a graph, each replay of which
+// would wipe what was reported before. So it is made on a stream that is not being captured, and waited for.
 Tensor& status_word(c10::DeviceIndex device) {
   static auto* words = new std::array<Tensor, 64>();
   Tensor& t = words->at(device);
-  if (!t.defined()) t = at::zeros({2}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
-  return t;
+  if (t.defined()) return t;
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);   // allocating and waiting beside a capture
+  c10::cuda::CUDAStreamGuard side(c10::cuda::getStreamFromPool(true, device));
+  while (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) side.reset_stream(c10::cuda::getStreamFromPool(true, device));
+  const Tensor w = at::zeros({2}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
+  side.current_stream().synchronize();
+  return t = w;
 }
 uint32_t* status(c10::DeviceIndex device) { return static_cast<uint32_t*>(status_word(device).data_ptr()); }
 
