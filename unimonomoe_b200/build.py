@@ -133,10 +133,12 @@ def _compile_binding() -> str:
 
 
 def _link_binding(obj: str) -> None:
+    """Against the C++ runtime that torch's libraries use. A compiler without a shared one of its own takes the archive; the module then has a
+    second runtime in it, and an exception whose message was put together by both crashes the process instead of reaching Python."""
     from torch.utils import cpp_extension
     libs = cpp_extension.library_paths()
     _run("linking _mono_attention.so", [os.environ.get("CXX", "g++"), "-shared", obj, "-o", attention_binding_path(), *(f"-L{p}" for p in libs),
-                                        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{LIBDIR}", "-lmono_attention",
+                                        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-l:libstdc++.so.6", f"-L{LIBDIR}", "-lmono_attention",
                                         "-Wl,-rpath,$ORIGIN"])
 
 
