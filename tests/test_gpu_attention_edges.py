@@ -177,3 +177,37 @@ def test_graphs_captured_on_a_stream_without_a_workspace_run_one_after_another()
             out.fill_(math.nan)
             graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+# ---------------------------------------------------------------------- refusals
+def _views():
+    data = torch.zeros(4, 2, 2, 17 * 64, dtype=torch.uint8, device=DEV)
+    yield "every other page", data[::2]
+    yield "one page many times", data[:1].expand(9, -1, -1, -1)
+    yield "half of the heads", data[:, :1]
+    yield "flat", data.flatten(2)
+    yield "another type", data.view(torch.int8)
+    yield "no pages", data[:0]
+    yield "a page size of 48", torch.zeros(4, 2, 3, 17 * 64, dtype=torch.uint8, device=DEV)
+    yield "a page size of 2048", torch.zeros(1, 2, 128, 17 * 64, dtype=torch.uint8, device=DEV)
+    yield "a head size of 96", torch.zeros(4, 2, 1, 17 * 96, dtype=torch.uint8, device=DEV)
+    yield "not 17 bytes a dim", torch.zeros(4, 2, 1, 17 * 64 + 8, dtype=torch.uint8, device=DEV)
+    yield "off its boundary", torch.zeros(4 * 2 * 17 * 64 + 8, dtype=torch.uint8, device=DEV)[8:].view(4, 2, 1, 17 * 64)
+
+
+@pytest.mark.parametrize("what", ["every other page", "one page many times", "half of the heads", "flat", "another type", "no pages", "a page size of 48",
+                                  "a page size of 2048", "a head size of 96", "not 17 bytes a dim", "off its boundary"])
+def test_what_is_not_a_cache_is_refused_by_every_operator(what):
+    class Looks:                                             # anything with `data`, as a tensor has too
+        pass
+    cache = Looks()
+    cache.data = dict(_views())[what]
+    x, slots = randn((1, 2, 64), 1), torch.zeros(1, dtype=torch.int64, device=DEV)
+    one, w, cs = torch.ones(1, dtype=torch.int32, device=DEV), randn((64,), 2), torch.ones(4, 64, device=DEV)
+    start = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for c in (cache, cache.data):
+        for call in (lambda: A.kv4_append(x, x, c, slots), lambda: A.kv4_read(c, slots),
+                     lambda: A.qk_norm_rope(x, x, w, w, cs, one, v=x, cache=c, slots=slots),
+                     lambda: A.kv4_attention(x, c, one[None], one, start, 1)):
+            with pytest.raises(ValueError):
+                call()

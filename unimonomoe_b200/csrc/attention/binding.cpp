@@ -9,6 +9,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <map>
@@ -80,11 +81,22 @@ void page_size(int64_t p) {
   TORCH_CHECK_VALUE(p >= 16 && p <= 1024 && !(p & (p - 1)), "page size ", p, "; a power of two from 16 to 1024 is needed");
 }
 
+// The cache's tensor, checked as KV4Cache does when it is made: here is where its pointer and sizes are used.
 struct Cache {
   const Tensor& data;
   int64_t pages, heads, dim;
   int page;
-  explicit Cache(const Tensor& d) : data(d), pages(d.size(0)), heads(d.size(1)), dim(d.size(3) / 17), page(static_cast<int>(d.size(2)) * 16) {}
+  explicit Cache(const Tensor& d) : data(d) {
+    TORCH_CHECK_VALUE(d.dim() == 4 && d.scalar_type() == at::kByte && d.is_contiguous() && d.size(0) > 0 && d.size(1) > 0 && d.size(3) % 17 == 0 && aligned(d),
+                      "cache must be contiguous uint8 [num_pages, kv_heads, page_size / 16, 17 * head_dim] on a 16-byte boundary, got ", d.sizes(), " ",
+                      d.scalar_type());
+    pages = d.size(0);
+    heads = d.size(1);
+    dim = d.size(3) / 17;
+    head_dim(dim);
+    page_size(std::min<int64_t>(d.size(2), 1 << 20) * 16);
+    page = static_cast<int>(d.size(2)) * 16;
+  }
   uint8_t* ptr() const { return static_cast<uint8_t*>(data.data_ptr()); }
   void check(int64_t kv_heads, int64_t d, c10::Device device) const {
     TORCH_CHECK_VALUE(heads == kv_heads && dim == d && data.device() == device, "cache holds ", heads, " KV heads of ", dim, " on ",
