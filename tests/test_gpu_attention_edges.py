@@ -1,4 +1,5 @@
 """The attention operators where something is missing, not finite or out of range, in shapes that the tests by size do not have."""
+import ctypes
 import math
 import os
 import subprocess
@@ -211,3 +212,74 @@ def test_what_is_not_a_cache_is_refused_by_every_operator(what):
                      lambda: A.kv4_attention(x, c, one[None], one, start, 1)):
             with pytest.raises(ValueError):
                 call()
+
+
+# ---------------------------------------------------------------------- plans of what cannot be
+def raw_plan(cached, new, table, free, taken, page, tokens):
+    """The C entry with every output, and the table, inside one buffer of 0x5A bytes, 256 to each side: (outputs, table, what was reported); nothing else has
+    been written."""
+    lib = ctypes.CDLL(A.attention_lib_path())
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    batch, width = len(cached), len(table[0])
+    sizes = {"table": 4 * batch * width, "start": 4 * (batch + 1), "lens": 4 * batch, "positions": 4 * tokens, "slots": 8 * tokens, "requests": 4 * tokens,
+             "taken": 4}
+    room = torch.full((sum(256 + (n + 255) // 256 * 256 for n in sizes.values()) + 256,), 0x5A, dtype=torch.uint8, device=DEV)
+    view, at, mine = {}, 256, torch.zeros(room.numel(), dtype=torch.bool, device=DEV)
+    for name, n in sizes.items():
+        view[name] = room[at:at + n].view(torch.int64 if name == "slots" else torch.int32)
+        mine[at:at + n] = True
+        at += (n + 255) // 256 * 256 + 256
+    view["table"].copy_(i32(table).flatten())
+    given = i32(cached), i32(new), i32(free), i32([taken])
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    rc = lib.mono_attn_plan(p(given[0]), p(given[1]), batch, p(view["table"]), width, p(given[2]), len(free), p(given[3]), page, tokens, p(view["start"]),
+                            p(view["lens"]), p(view["positions"]), p(view["slots"]), p(view["requests"]), p(view["taken"]), p(status),
+                            ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    got = {name: x.tolist() for name, x in view.items()}
+    assert (room[~mine] == 0x5A).all()
+    return got, [got["table"][i * width:(i + 1) * width] for i in range(batch)], A.STATUS_CODES[status.tolist()[0]]
+
+
+TOP = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("cached,new,taken,said", [
+    ([TOP], [1], 0, "longer"), ([TOP - 20], [40], 0, "longer"), ([TOP - 16], [TOP], 0, "longer"), ([0, TOP - 5], [TOP, TOP], 0, ""),
+    ([40] * 1100, [TOP - 70000] * 1100, 0, ""), ([40] * 600, [2 ** 22] * 600, 0, ""), ([3, 70], [20, 5], TOP, "more pages"),
+    ([3, 70], [20, 5], -TOP, "more pages"), ([3, 70], [20, 5], -1, "more pages"), ([TOP - 70000, 3], [60000, 20], TOP, "")])
+@pytest.mark.parametrize("page", [16, 1024])
+def test_lengths_at_the_end_of_32_bits_stay_in_bounds(cached, new, taken, said, page):
+    width, tokens = 6, 200
+    table = [[1, 2, 3, 4, 5, 6]] * len(cached)
+    got, after, told = raw_plan(cached, new, table, [7, 8, 9], taken, page, tokens)
+    assert said in told and told != "ok"
+    assert all(-1 <= s < 10 * page for s in got["slots"])
+    assert all(0 <= p < 2 ** 31 for p in got["positions"]) and all(-1 <= r < len(cached) for r in got["requests"])
+    assert got["start"][0] == 0 and got["start"] == sorted(got["start"]) and all(0 <= n < 2 ** 31 for n in got["lens"])
+    assert all(e in range(-1, 10) for row in after for e in row)
+
+
+@pytest.mark.parametrize("what,code", [("pages", "more pages"), ("table", "longer than"), ("tokens", "more tokens"), ("negative", "negative"),
+                                       ("entry", "block-table entry")])
+def test_plan_faults_touch_nothing_but_the_outputs(what, code):
+    cached, new, free, tokens, width = [10, 40], [20, 30], [5, 6, 7, 8], 50, 5
+    table = [[1, -1, -1, -1, -1], [2, 3, 4, -1, -1]]
+    want = [[1, 5, -1, -1, -1], [2, 3, 4, 6, 7]]
+    if what == "pages":
+        free, want[1][4] = [5, 6], -1
+    elif what == "table":
+        width, table, want = 4, [r[:4] for r in table], [r[:4] for r in want]
+    elif what == "tokens":
+        tokens = 49
+    elif what == "negative":
+        new, want[1][3:] = [20, -30], [-1, -1]
+    elif what == "entry":
+        table[0][0] = want[0][0] = -1
+    got, after, told = raw_plan(cached, new, table, free, 0, 16, tokens)
+    assert code in told and after == want
+    ref_table = [r[:] for r in table]
+    if what == "tokens":                                     # all but the token that has no row
+        start, lens, pos, slot, req, taken = ref.plan(cached, new, ref_table, free, 0, 16, 50)
+        assert (got["start"], got["lens"], got["positions"], got["slots"], got["requests"], got["taken"]) == (start, lens, pos[:49], slot[:49], req[:49], [taken])

@@ -17,6 +17,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = MONO_ATTN_MAX_REQUESTS;
+// Longest sequence; longer ones are reported and cut. Then no place, page or column leaves 32 bits, whatever the lengths are, and sums over requests
+// stay at the largest integer instead of turning negative (starts that fall would give a token a place outside its request).
+constexpr int kLongest = 0x7FFF0000;
+__device__ __forceinline__ int add(int x, int y) { return static_cast<int>(min(static_cast<uint32_t>(x) + static_cast<uint32_t>(y), 0x7FFFFFFFu)); }
 
 struct PlanArgs {
   const int32_t *cached, *fresh;
@@ -36,7 +40,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int page = 1 << a.shift;
   int base_t = 0, base_p = 0;
-  bool bad = false;
+  bool bad = false, too_long = false;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + tid;
     int n = 0, f = 0;
@@ -46,13 +50,16 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
       bad |= c < 0 || n < 0;
       c = max(c, 0);
       n = max(n, 0);
+      too_long |= c > kLongest || n > kLongest - c;
+      c = min(c, kLongest);
+      n = min(n, kLongest - c);
       f = ((c + n + page - 1) >> a.shift) - ((c + page - 1) >> a.shift);
     }
     int sn = n, sf = f;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int x = __shfl_up_sync(0xFFFFFFFFu, sn, d), y = __shfl_up_sync(0xFFFFFFFFu, sf, d);
-      if (lane >= d) { sn += x; sf += y; }
+      if (lane >= d) { sn = add(sn, x); sf = add(sf, y); }
     }
     if (lane == 31) { wsum[0][warp] = sn; wsum[1][warp] = sf; }
     __syncthreads();
@@ -60,39 +67,42 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const int x = wsum[0][w], y = wsum[1][w];
-      if (w < warp) { on += x; of += y; }
-      tn += x;
-      tf += y;
+      if (w < warp) { on = add(on, x); of = add(of, y); }
+      tn = add(tn, x);
+      tf = add(tf, y);
     }
-    if (b < a.batch) { start[b] = on + sn - n; first[b] = of + sf - f; }
-    base_t += tn;
-    base_p += tf;
+    const int n_before = __shfl_up_sync(0xFFFFFFFFu, sn, 1), f_before = __shfl_up_sync(0xFFFFFFFFu, sf, 1);
+    if (b < a.batch) { start[b] = lane ? add(on, n_before) : on; first[b] = lane ? add(of, f_before) : of; }
+    base_t = add(base_t, tn);
+    base_p = add(base_p, tf);
     __syncthreads();
   }
   if (tid == 0) { start[a.batch] = base_t; first[a.batch] = base_p; }
   __syncthreads();
   const int total = base_t, taken = a.taken[0];
   if (blockIdx.x == 0 && tid == 0) {
-    a.taken_out[0] = taken + base_p;
+    const int64_t behind = static_cast<int64_t>(taken) + base_p;
+    a.taken_out[0] = static_cast<int>(min(behind, static_cast<int64_t>(INT32_MAX)));
     a.query_start[a.batch] = total;
     if (total > a.tokens) kv4::report(a.status, kv4::kTooManyTokens, total);
-    if (taken < 0 || taken + base_p > a.free_count) kv4::report(a.status, kv4::kNoPages, taken + base_p);
+    if (taken < 0 || behind > a.free_count) kv4::report(a.status, kv4::kNoPages, static_cast<uint32_t>(behind));
   }
   if (bad && blockIdx.x == 0) kv4::report(a.status, kv4::kBadLength, tid);
+  if (too_long && blockIdx.x == 0) kv4::report(a.status, kv4::kTooLong, tid);
 
   // one warp for a request: its length, its start, the entries of its new pages
   for (int b = blockIdx.x * kWarps + warp; b < a.batch; b += gridDim.x * kWarps) {
-    const int c = max(a.cached[b], 0), n = start[b + 1] - start[b];
+    const int c = min(max(a.cached[b], 0), kLongest), n = start[b + 1] - start[b];
     if (lane == 0) {
       a.seq_lens[b] = c + n;
       a.query_start[b] = start[b];
     }
     const int held = (c + page - 1) >> a.shift, f = first[b + 1] - first[b];
     if (held + f > a.width && lane == 0 && n > 0) kv4::report(a.status, kv4::kTooLong, b);
-    for (int j = lane; j < f; j += 32) {
-      const int at = taken + first[b] + j;
-      if (held + j < a.width)               // none left: not what the row held for an earlier request
-        a.table[static_cast<int64_t>(b) * a.width + held + j] = at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
+    for (int j = lane; j < min(f, a.width - held); j += 32) {
+      const int64_t at = static_cast<int64_t>(taken) + first[b] + j;
+      // none left: not what the row held for an earlier request
+      a.table[static_cast<int64_t>(b) * a.width + held + j] = at >= 0 && at < a.free_count ? a.free_pages[at] : -1;
     }
   }
 
@@ -107,7 +117,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
         if (start[mid] <= t) lo = mid; else hi = mid;
       }
       req = lo;
-      const int c = max(a.cached[req], 0), held = (c + page - 1) >> a.shift;
+      const int c = min(max(a.cached[req], 0), kLongest), held = (c + page - 1) >> a.shift;
       pos = c + t - start[req];
       const int col = pos >> a.shift;
       int pg = -1;
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const PlanArgs a) {
         if (col < a.width) pg = a.table[static_cast<int64_t>(req) * a.width + col];
         if (pg < 0) kv4::report(a.status, col < a.width ? kv4::kBadPage : kv4::kTooLong, req);
       } else {
-        const int at = taken + first[req] + col - held;
+        const int64_t at = static_cast<int64_t>(taken) + first[req] + col - held;
         if (col < a.width && at >= 0 && at < a.free_count) pg = a.free_pages[at];
       }
       if (pg >= 0) slot = (static_cast<int64_t>(pg) << a.shift) + (pos & (page - 1));
