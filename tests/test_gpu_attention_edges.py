@@ -283,3 +283,45 @@ def test_plan_faults_touch_nothing_but_the_outputs(what, code):
     if what == "tokens":                                     # all but the token that has no row
         start, lens, pos, slot, req, taken = ref.plan(cached, new, ref_table, free, 0, 16, 50)
         assert (got["start"], got["lens"], got["positions"], got["slots"], got["requests"], got["taken"]) == (start, lens, pos[:49], slot[:49], req[:49], [taken])
+
+
+# ---------------------------------------------------------------------- sizes past 32 bits
+def test_more_rows_than_32_bits_of_threads():
+    """2^28 + 5 tokens of one head of 256, the same row for all of them (strides of 0), of which a few are stored."""
+    T = 2 ** 28 + 5
+    cache = A.KV4Cache.empty(1, 1, 256, 16, DEV)
+    cache.data.fill_(0x88)
+    k, v = randn((1, 1, 256), 1), randn((1, 1, 256), 2)
+    slots = torch.full((T,), -1, dtype=torch.int64, device=DEV)
+    for i, at in enumerate((0, T // 2 - 1, T // 2, T // 2 + 1, T - 2, T - 1)):
+        slots[at] = 2 * i
+    A.kv4_append(k.expand(T, 1, 256), v.expand(T, 1, 256), cache, slots)
+    got = A.kv4_read(cache, torch.arange(12, device=DEV))
+    for x, y in zip(got, (k, v)):
+        assert torch.equal(x[::2].double(), ref.quantised(y).expand(6, 1, 256))
+
+
+@pytest.mark.parametrize("news", [1, 200])
+def test_a_cache_of_more_than_4_gib(news):
+    """Pages on both sides of byte 2^32 and of element 2^32 / 2, read and written by every operator."""
+    H, K, D, page, n = 8, 2, 128, 1024, 5000
+    pages = 2 ** 32 // (K * page * 17 * D // 16) + 40            # of 278 528 bytes
+    cache = A.KV4Cache.empty(pages, K, D, page, DEV)
+    assert cache.data.numel() > 2 ** 32
+    edge = [i * 2 ** 31 // (K * page * 17 * D // 16) for i in (1, 2)]
+    table = torch.tensor([[edge[0], pages - 1, edge[1], edge[1] + 1, edge[0] + 1, 0]], dtype=torch.int32, device=DEV)
+    i = torch.arange(n, device=DEV)
+    slots = table[0].long()[i // page] * page + i % page
+    k, v, q = randn((n, K, D), 1), randn((n, K, D), 2), randn((news, H, D), 3)
+    cs, w = torch.cat([torch.ones(1, 32, device=DEV), torch.zeros(1, 32, device=DEV)], 1), randn((D,), 4)
+    A.kv4_append(k[1000:], v[1000:], cache, slots[1000:])
+    raw = randn((1000, K, D), 5)                                # the first page's keys come by way of their norm
+    zeros = torch.zeros(1000, dtype=torch.int32, device=DEV)
+    _, k0 = A.qk_norm_rope(raw, raw, w, w, cs, zeros)
+    A.qk_norm_rope(raw, raw, w, w, cs, zeros, v=v[:1000], cache=cache, slots=slots[:1000])
+    keys, values = ref.quantised(torch.cat([k0, k[1000:]])), ref.quantised(v)
+    got = A.kv4_read(cache, slots)
+    assert torch.equal(got[0].double(), keys) and torch.equal(got[1].double(), values)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    out, lse = A.kv4_attention(q, cache, table, i32([n]), i32([0, news]), news, return_lse=True)
+    close(out, lse, ref.attention(q, [keys], [values], [0, news], 0, D ** -0.5))

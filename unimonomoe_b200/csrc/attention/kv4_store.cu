@@ -41,7 +41,7 @@ __device__ __forceinline__ void store32(__nv_bfloat16* p, const uint4& v, const 
 template <int D, int U, bool READ>
 __global__ __launch_bounds__(kWarps * 32) void store_kernel(const StoreArgs a) {
   constexpr int L = D / 16, Scales = 4 * D / kv4::kGroup;    // lanes of a row; bytes of a token's scales
-  const int l = threadIdx.x % L, row = static_cast<int>((blockIdx.x * kWarps * 32 + threadIdx.x) / L), per = 2 * a.heads;
+  const int l = threadIdx.x % L, row = static_cast<int>(blockIdx.x * (kWarps * 32 / L) + threadIdx.x / L), per = 2 * a.heads;
   if (row - static_cast<int>(threadIdx.x % 32) / L >= a.step * per) return;   // the whole warp
   const int first = kv4::divide(min(row, a.step * per - 1), per, a.per_inv), h = min(row, a.step * per - 1) - first * per;
   const bool value = h >= a.heads, real = row < a.step * per;
