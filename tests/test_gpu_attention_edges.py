@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from tests import attention_ref as ref
-from tests.test_gpu_attention import DEV, close, gen, make, randn
+from tests.test_gpu_attention import DEV, _rope_inputs, close, gen, make, randn
 from unimonomoe_b200 import attention as A
 
 pytestmark = pytest.mark.gpu
@@ -325,3 +325,36 @@ def test_a_cache_of_more_than_4_gib(news):
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
     out, lse = A.kv4_attention(q, cache, table, i32([n]), i32([0, news]), news, return_lse=True)
     close(out, lse, ref.attention(q, [keys], [values], [0, news], 0, D ** -0.5))
+
+
+# ---------------------------------------------------------------------- norms and rotation
+@pytest.mark.parametrize("D,R", [(64, 0), (64, 32), (128, 48), (256, 64), (256, 256)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_an_infinity_reaches_what_turns_with_it_and_nothing_else(D, R, interleaved):
+    q, k = randn((D, 3, D), D), randn((D, 1, D), D + 1)
+    i = torch.arange(D, device=DEV)
+    q[i, 1, i], k[i, 0, i] = math.inf, -math.inf                # token t: dim t
+    q[5, 0, 7] = math.nan
+    w = randn((2, D), 3)
+    angle = torch.rand(9, R // 2, generator=gen(4), device=DEV) + 0.1
+    table, pos = torch.cat([angle.cos(), angle.sin()], 1).contiguous(), torch.randint(0, 9, (D,), generator=gen(5), device=DEV).to(torch.int32)
+    for got, x, y in zip(A.qk_norm_rope(q, k, w[0], w[1], table, pos, 1e-6, interleaved), (q, k), w):
+        want = ref.norm_rope(x, y, table, pos, 1e-6, interleaved, False)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        bad = torch.isinf(x).any(-1)
+        assert not got[bad].nan_to_num(0.0).any()
+
+
+@pytest.mark.parametrize("D,H,K,R,T", [(64, 4, 1, 64, 7), (64, 5, 5, 16, 33), (128, 7, 3, 48, 19), (128, 32, 4, 128, 3), (256, 16, 2, 64, 9)])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_neighbours_into_the_cache_are_append_of_their_results(D, H, K, R, T, fp32):
+    q, k, v, wq, wk, table, pos = _rope_inputs(D, H, K, R, T, fp32)
+    caches = [A.KV4Cache.empty(T // 32 + 2, K, D, 32, DEV) for _ in range(2)]
+    slots = torch.randperm((T // 32 + 2) * 32, generator=gen(1), device=DEV)[:T]
+    slots[1] = -1
+    for c in caches:
+        c.data.zero_()
+    q1, k1 = A.qk_norm_rope(q, k, wq, wk, table, pos, 1e-5, True, True)
+    A.kv4_append(k1, v, caches[0], slots)
+    q2 = A.qk_norm_rope(q, k, wq, wk, table, pos, 1e-5, True, True, v=v, cache=caches[1], slots=slots)
+    assert torch.equal(q1, q2) and torch.equal(caches[0].data, caches[1].data)

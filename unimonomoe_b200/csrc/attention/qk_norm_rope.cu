@@ -7,9 +7,9 @@
 // Sums and products in fp32, one rounding to bf16 at the end. The cache quantises the key after that rounding, so that it
 // holds the same codes as a key stored from the tensor.
 //
-// Bound by memory: 4 bytes a value, read and written once. 8192 tokens of 36 heads of 128 take 33.1 us, 4.7 TB/s, where a copy
+// Bound by memory: 4 bytes a value, read and written once. 8192 tokens of 36 heads of 128 take 33.2 us, 4.7 TB/s, where a copy
 // of as many bytes takes 26.8; behind memory it is instructions, some 130 for a lane's eight dims with what it shares among four heads. With the
-// keys and values stored in the cache, a fifth of the rows, 45 us.
+// keys and values stored in the cache, a fifth of the rows, 47 us.
 #include <cuda_runtime.h>
 #include "kv4_format.cuh"
 #include "../../../include/mono_attention.h"
@@ -49,14 +49,44 @@ __device__ __forceinline__ void load_weight(const RopeArgs& a, const void* w, in
     for (int i = 0; i < 8; ++i) x[i] += 1.0f;
 }
 
+// An infinity reaches the dim that it turns against; dims that do not turn only share a lane's products (0 times it) with it, and are done again here, each
+// on its own. (A NaN reaches them all.) The cache's groups of 64 need it not: one value that is not a number makes all of a group so.
+// A call that begins anew, so that the kernel keeps nothing for it but a predicate.
+template <int D, int U>
+__device__ __noinline__ void beside_infinity(const RopeArgs& a) {
+  constexpr int L = D / 8, R = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane % L, unit = static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5);
+  const int token = unit / a.per, part = unit % a.per;
+  const bool queries = part < a.q_units;
+  __nv_bfloat16* const out = queries ? a.q_out + static_cast<int64_t>(token) * a.hq * D : a.k_out ? a.k_out + static_cast<int64_t>(token) * a.hk * D : nullptr;
+  const __nv_bfloat16* const in = queries ? a.q + token * a.q_ts : a.k + token * a.k_ts;
+  float w[8];
+  load_weight(a, queries ? a.wq : a.wk, 8 * l, 8 * l + 4, w);
+  for (int i = 0; i < U; ++i) {
+    const int h = (queries ? part : part - a.q_units) * R * U + lane / L + i * R;
+    if (h >= (queries ? a.hq : a.hk) || !out) continue;
+    const uint4* row = reinterpret_cast<const uint4*>(in + h * (queries ? a.q_hs : a.k_hs));
+    float x[8], sum = 0.0f;                 // of magnitudes: infinite only with an infinity and no NaN
+    for (int n = 0; n < L; ++n) {
+      kv4::unpack_bf16x8(row[n], x);
+      for (int d = 0; d < 8; ++d) sum += fabsf(x[d]) * 0x1p-10f;
+    }
+    if (sum != INFINITY) continue;
+    kv4::unpack_bf16x8(row[l], x);
+    for (int d = 0; d < 8; ++d) x[d] = x[d] * 0.0f * w[d];
+    *reinterpret_cast<uint4*>(out + h * D + 8 * l) = kv4::pack_bf16x8(x);
+  }
+}
+
 // A row (one head of one token) is held by D/8 lanes, eight dims each; a warp does 32/(D/8) heads of one token at a time, U times, either of
 // the queries or of the keys (and values). Where halves turn against each other a lane below the rotary dims has four dims of each
 // half, so that both of a pair and their one cosine and sine are in one lane; else its eight dims are adjacent. What is stored in
 // the cache is brought into that order. Pairs (x0, x1) become r (x0 w0 c - x1 w1 s), r (x1 w1 c + x0 w0 s) with the products of the
 // weights made once for all heads; two pairs to an instruction.
-// Five CTAs to an SM (48 registers, one of them spilled for heads of 128): 8192 tokens of 36 heads of 128 33.1 us; four 35.5; six 37.3.
+// Five CTAs to an SM (48 registers, one of them spilled for heads of 128 and 256): 8192 tokens of 36 heads of 128 33.2 us; four 35.5; six 37.3. Storing,
+// four (64 registers, none spilled): 47.4 us, of 40 heads of 64 with 8 stored 31.0; five (100 to 116 bytes spilled) 47.2 and 33.0.
 template <int D, int U, bool STORE>
-__global__ __launch_bounds__(kWarps * 32, 5) void rope_kernel(const RopeArgs a) {
+__global__ __launch_bounds__(kWarps * 32, STORE ? 4 : 5) void rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int L = D / 8, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
   const int unit = static_cast<int>(blockIdx.x) * kWarps + static_cast<int>(threadIdx.x >> 5);
@@ -128,6 +158,7 @@ __global__ __launch_bounds__(kWarps * 32, 5) void rope_kernel(const RopeArgs a) 
   }
   __nv_bfloat16* out = queries ? a.q_out + static_cast<int64_t>(token) * a.hq * D : a.k_out + static_cast<int64_t>(token) * a.hk * D;
   const int outs = queries ? a.hq : STORE && a.k_out == nullptr ? 0 : a.hk;   // heads that are written
+  bool infinite = false;                    // a head with an infinity in it (or squares beyond fp32): a root of infinity, everything times 0
 
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -156,6 +187,7 @@ __global__ __launch_bounds__(kWarps * 32, 5) void rope_kernel(const RopeArgs a) 
 #pragma unroll
     for (int d = 1; d < L; d <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
     const float2 r = kv4::both(rsqrtf(ss * (1.0f / D) + a.eps));
+    infinite |= r.x == 0.0f;
     float2 y0[2], y1[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -195,6 +227,7 @@ __global__ __launch_bounds__(kWarps * 32, 5) void rope_kernel(const RopeArgs a) 
       }
     }
   }
+  if (infinite && !turns) beside_infinity<D, U>(a);
 }
 
 template <int D, int U, bool STORE>
