@@ -358,3 +358,24 @@ def test_neighbours_into_the_cache_are_append_of_their_results(D, H, K, R, T, fp
     A.kv4_append(k1, v, caches[0], slots)
     q2 = A.qk_norm_rope(q, k, wq, wk, table, pos, 1e-5, True, True, v=v, cache=caches[1], slots=slots)
     assert torch.equal(q1, q2) and torch.equal(caches[0].data, caches[1].data)
+
+
+def test_more_steps_than_32_bits_are_reported_and_not_begun():
+    B, K, D, page, width = 16384, 8, 64, 1024, 5000              # 2.6e9 steps of 256 tokens, all in one page
+    cache = A.KV4Cache(torch.zeros(1, K, page // 16, 17 * D, dtype=torch.uint8, device=DEV))
+    table = torch.zeros(B, width, dtype=torch.int32, device=DEV)
+    lens = torch.full((B,), width * page, dtype=torch.int32, device=DEV)
+    out = torch.full((B, K, D), 3.0, dtype=torch.bfloat16, device=DEV)
+    A.kv4_attention(torch.zeros_like(out), cache, table, lens, torch.arange(B + 1, dtype=torch.int32, device=DEV), 1, out=out)
+    with pytest.raises(RuntimeError, match="longer than"):
+        A.check_status(DEV)
+    assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("news", [1, 100])
+@pytest.mark.parametrize("window", [400, 4096, 2 ** 31, 2 ** 62])
+def test_windows_as_wide_as_the_sequence_and_wider(news, window):
+    H, K, D = 8, 2, 128
+    cache, table, ln, st, q, keys, values, starts = make([400], [news], H, K, D, 16, seed=3)
+    out, lse = A.kv4_attention(q, cache, table, ln, st, news, window=window, return_lse=True)
+    close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))

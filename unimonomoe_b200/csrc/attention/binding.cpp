@@ -354,7 +354,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                      size32(table.size(1), "pages of block_table"), ptr<int32_t>(lens), ptr<int32_t>(start), static_cast<int>(B),
                                      size32(T, "tokens"), static_cast<int>(std::min<int64_t>(longest, INT32_MAX)), size32(H, "heads"),
                                      static_cast<int>(cache.heads), static_cast<int>(D), static_cast<float>(scale),
-                                     static_cast<int>(std::min<int64_t>(window, 1 << 30)), out.data_ptr(), want_lse ? ptr<float>(lse) : nullptr, ws.data_ptr(),
+                                     static_cast<int>(std::min<int64_t>(window, INT32_MAX)), out.data_ptr(), want_lse ? ptr<float>(lse) : nullptr, ws.data_ptr(),
                                      static_cast<size_t>(ws.numel()), status(dev.index()), stream));
   }
   PyObject* o = a[8] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[8]);

@@ -47,7 +47,8 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   a.group = q_heads / kv_heads;
   a.group_inv = 0xFFFFFFFFu / static_cast<uint32_t>(a.group);
   a.shift = __builtin_ctz(page_size);
-  a.window = window;
+  const int64_t longest = static_cast<int64_t>(table_width) * page_size;
+  a.window = window >= longest ? 0 : window;  // as wide as any sequence: none
   a.scale_log2 = scale * 1.4426950408889634f;
   // max_query_len is only a bound: without the kernel of many rows the other one takes every request
   const int64_t most = static_cast<int64_t>(max_query_len < tokens ? max_query_len : tokens) * a.group;

@@ -135,11 +135,13 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
 
   // All steps, all items and the longest item; the sums before each thread's requests.
   const int chunk = (a.batch + kThreads - 1) / kThreads;
+  // Sums of steps stay at the largest integer: more than a launch could do in seconds, and reported (2^31 steps are 34 TB of a cache of heads of 64).
+  auto add = [](int x, int y) { return static_cast<int>(min(static_cast<uint32_t>(x) + static_cast<uint32_t>(y), 0x7FFFFFFFu)); };
   int mine = 0, mine_items = 0, longest = 0;
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     int items, steps, lo;
     cost_of<S::Rows>(a, request_of(a, b, blockIdx.x == 0), items, steps, lo);
-    mine += items * (steps + kOwn);
+    mine = add(mine, static_cast<int>(min(static_cast<int64_t>(items) * (steps + kOwn), static_cast<int64_t>(INT32_MAX))));
     mine_items += items;
     if (items) longest = max(longest, steps);
   }
@@ -148,17 +150,21 @@ __global__ __launch_bounds__(kThreads, Shape<D, NT>::PerSm) void decode_kernel(c
   for (int d = 1; d < 32; d <<= 1) {
     const int x = __shfl_up_sync(0xFFFFFFFFu, upto, d), y = __shfl_up_sync(0xFFFFFFFFu, upto_items, d);
     longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, d));
-    if (lane >= d) { upto += x; upto_items += y; }
+    if (lane >= d) { upto = add(upto, x); upto_items += y; }
   }
   if (lane == 31) { s_sum[warp][0] = upto; s_sum[warp][1] = upto_items; s_sum[warp][2] = longest; }
   __syncthreads();
   int total = 0, all_items = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) { upto += s_sum[w][0]; upto_items += s_sum[w][1]; }
-    total += s_sum[w][0];
+    if (w < warp) { upto = add(upto, s_sum[w][0]); upto_items += s_sum[w][1]; }
+    total = add(total, s_sum[w][0]);
     all_items += s_sum[w][1];
     longest = max(longest, s_sum[w][2]);
+  }
+  if (total == INT32_MAX) {
+    if (blockIdx.x == 0 && tid == 0) report(a.status, kTooLong, 0);
+    return;
   }
   const int ctas = static_cast<int>(gridDim.x), per = (total + ctas - 1) / ctas;
   // CTAs for each item (0: equal runs), from what the slowest CTA then has

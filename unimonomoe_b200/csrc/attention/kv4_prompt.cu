@@ -32,6 +32,7 @@
 #include <climits>
 #include <type_traits>
 #include "kv4_attention.cuh"
+#include "kv4_tiles.cuh"
 #include "../ptx_sm100.cuh"
 
 namespace mono {
@@ -42,13 +43,10 @@ using namespace kv4;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 0, kMmaWarps = 2, kPlanWarp = 2, kFirstSoftmax = 3, kFirstFill = kFirstSoftmax + kSoftmaxWarps;
 constexpr int kSegs = 4;                    // segments that the roles may be apart
-constexpr int kKeys = 128, kRows = 128;    // of a product's tile
+constexpr int kRows = 128;                  // of a product's tile, as kKeys
 constexpr int kPanel = kKeys * 128;         // bytes of [128 rows x 64 dims]
 constexpr float kLow = -1e38f, kRoom = 8.0f;
 constexpr int kHits = 16;                   // words of the rows that see values that are not numbers
-// What an item costs beside its tiles, in tiles: loading its queries, filling and draining the pipeline, writing its output.
-// It counts where work is divided, for the first blocks of a prompt are many and short.
-constexpr int kOwn = 2;
 // States that one CTA joins. 256 rows over 65536 tokens (4 KV heads of 128, 37 states): 208 us alone, 123 in two steps; four requests of 64 tokens over 16384
 // (5 to 7 states) 111, with 6 here 126; 32 tokens (10 states) 137 alone, 114.
 constexpr int kJoinAlone = 8;
@@ -115,57 +113,8 @@ struct Control {
 template <int D>
 constexpr int smem_bytes() { return Shape<D>::Q + Shape<D>::Slots * Shape<D>::Slot + static_cast<int>(sizeof(Control)); }
 
-// sum of floor((a i + b) / m), i < n (by Euclid's algorithm on a and m). All of it fits 32 bits: it is the tiles of a request.
-__device__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  uint32_t sum = 0;
-  while (n > 0) {
-    const uint32_t qa = a / m, qb = b / m;
-    sum += qa * (n * (n - 1) / 2) + qb * n;
-    a -= qa * m;
-    b -= qb * m;
-    const uint32_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y - n * m;
-    const uint32_t t = m;
-    m = a;
-    a = t;
-  }
-  return sum;
-}
-
-// The row blocks of a request: `tb` tokens each, all query heads of a KV head.
-struct Item {
-  int place0, n, len, tb, window;
-  __device__ __forceinline__ int blocks() const { return (n + tb - 1) / tb; }
-  __device__ __forceinline__ int begin(int rb) const { return window > 0 ? max(place0 + rb * tb + 1 - window, 0) : 0; }
-  __device__ __forceinline__ int first_tile(int rb) const { return begin(rb) / kKeys; }
-  __device__ __forceinline__ int seen(int rb) const { return min(len, max(place0 + min((rb + 1) * tb, n), 0)); }
-  // tiles of row block rb, at least one
-  __device__ __forceinline__ int tiles(int rb) const { return max(1, (seen(rb) + kKeys - 1) / kKeys - first_tile(rb)); }
-};
-
 __device__ __forceinline__ Item item_of(const AttnArgs& a, const Request& r, int rows) {
   return {r.len - r.n, r.n * a.group > a.split_rows ? r.n : 0, r.len, rows / a.group, a.window};
-}
-
-// Tiles, and kOwn for each block, of the row blocks before rb: the ends of what they see less its beginnings, each a sum of floors; counted one by
-// one only where the first queries have no place in the sequence.
-__device__ __noinline__ int tiles_before(const Item& it, int rb) {
-  int sum = rb * kOwn;
-  if (it.place0 < 0) {
-    for (int i = 0; i < rb; ++i) sum += it.tiles(i);
-    return sum;
-  }
-  const int full = min(rb, it.n / it.tb);                // blocks of tb tokens; a shorter one is the last
-  sum += floor_sum(full, kKeys, it.tb, it.place0 + it.tb + kKeys - 1);
-  if (it.window > 0) {
-    const int begin = it.place0 + 1 - it.window;         // of the first row; blocks with a negative one begin at 0
-    const int skip = begin < 0 ? min((-begin + it.tb - 1) / it.tb, full) : 0;
-    sum -= floor_sum(full - skip, kKeys, it.tb, max(begin + skip * it.tb, 0));
-  }
-  if (rb > full) sum += it.tiles(full);
-  return sum;
 }
 
 // The segments of a CTA's run, one after another: tiles [t0, t1) of an item.
@@ -1031,10 +980,9 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int sha
   w.u = u0;
   w.u1 = u1;
   {  // the head and row block that u0 lies in: the lanes bisect together, 32 places at a time
-    const int each = tiles_before(w.it, w.blocks);
-    const int64_t off = u0 - C.found_at;
+    const int64_t each = tiles_before(w.it, w.blocks), off = u0 - C.found_at;
     w.head = static_cast<int>(off / each);
-    const int rest = static_cast<int>(off - static_cast<int64_t>(w.head) * each);
+    const int64_t rest = off - w.head * each;
     int low = 0, high = w.blocks;           // tiles_before(low) <= rest < tiles_before(high)
     while (high - low > 1) {
       const int step = (high - low + 31) / 32, at = min(low + lane * step, high);
@@ -1044,7 +992,7 @@ __device__ __forceinline__ void plan_role(const AttnArgs& a, Control& C, int sha
       low += k * step;
     }
     w.rb = low;
-    w.at = C.found_at + static_cast<int64_t>(w.head) * each + tiles_before(w.it, low);
+    w.at = C.found_at + w.head * each + tiles_before(w.it, low);
   }
   w.open();
   for (uint32_t n = 0;; ++n) {
@@ -1070,7 +1018,7 @@ __global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const Attn
   for (int b = tid * chunk; b < min((tid + 1) * chunk, a.batch); ++b) {
     const Item it = item_of(a, request_of(a, b, blockIdx.x == 0), S::Rows);
     const int blocks = it.blocks();
-    mine += static_cast<long long>(tiles_before(it, blocks)) * a.hk;
+    mine += tiles_before(it, blocks) * a.hk;
     mine_items += blocks * a.hk;
     if (blocks) longest = max(longest, max(it.tiles(blocks - 1), it.tiles(max(blocks - 2, 0))));
   }
@@ -1113,7 +1061,7 @@ __global__ __launch_bounds__(Shape<D>::Threads, 1) void prompt_kernel(const Attn
     if (chunk > 1)
       for (;; ++b) {
         const Item it = item_of(a, request_of(a, b, false), S::Rows);
-        const long long cost = static_cast<long long>(share ? it.blocks() : tiles_before(it, it.blocks())) * a.hk;
+        const long long cost = (share ? it.blocks() : tiles_before(it, it.blocks())) * a.hk;
         if (at + cost > u0) break;
         at += cost;
       }
