@@ -70,7 +70,7 @@ int mono_attn_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, c
  * q_heads] (natural log). Rows query_start[b] .. query_start[b + 1] are the last ones of sequence b, seq_lens[b] long with them;
  * each sees the keys up to its own place, with window > 0 the last `window` of them. Keys and values of a page that is missing from block_table (an
  * entry outside the cache, which is reported) are zeros. Rows of no request are not written.
- * max_query_len: an upper bound of the queries of a request; it chooses kernels, results do not depend on it.
+ * scale is finite. max_query_len: an upper bound of the queries of a request; it chooses kernels, results do not depend on it.
  * workspace: mono_attn_workspace_bytes(), its first 4 * MONO_ATTN_COUNTERS bytes zero before the first launch (each launch
  * leaves them zero); launches that share it must not overlap. */
 size_t mono_attn_workspace_bytes(void);

@@ -1,4 +1,6 @@
 """What the attention operators refuse, and how: an exception that Python can catch, in a process that lives on."""
+import ctypes
+import math
 import os
 import shutil
 import subprocess
@@ -87,3 +89,23 @@ print("fine")
 def test_every_wrong_argument_is_a_python_exception(attention_lib):
     got = subprocess.run([sys.executable, "-c", CALLS], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert got.returncode == 0 and got.stdout.strip() == "fine", f"{got.returncode}: {got.stdout}{got.stderr}"
+
+
+def test_the_c_entry_refuses_scales_that_are_not_numbers(attention_lib):
+    lib = ctypes.CDLL(attention_lib)
+    vp, i, i64, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+    lib.mono_attn_kv4_attention.argtypes = [vp, i64, i64, vp, i64, i, vp, i, vp, vp, i, i, i, i, i, i, f, i, vp, vp, vp, z, vp, vp]
+    p = ctypes.addressof(ctypes.create_string_buffer(64))
+    for scale, code in ((math.nan, -202), (math.inf, -202), (-math.inf, -202), (0.1, -204)):
+        assert lib.mono_attn_kv4_attention(p, 128, 128, p, 4, 16, p, 4, p, p, 1, 1, 1, 4, 2, 128, scale, 0, p, 0, p, 100, p, 0) == code
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39])
+def test_scales_that_are_not_numbers_are_refused(attention_lib, scale):
+    import torch
+    from unimonomoe_b200 import attention as A
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    cache, x = A.KV4Cache.empty(1, 1, 64), torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="scale"):
+        A.kv4_attention(x, cache, one[None] * 0, one, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1, scale=scale)

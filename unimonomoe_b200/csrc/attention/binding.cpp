@@ -334,6 +334,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t longest = integer(a[5], "max_query_len"), window = integer(a[7], "window");
   TORCH_CHECK_VALUE(window >= 0 && longest >= 0, "window is ", window, ", max_query_len is ", longest);
   const double scale = a[6] == Py_None ? 1.0 / std::sqrt(static_cast<double>(D)) : number(a[6], "scale");
+  TORCH_CHECK_VALUE(std::isfinite(static_cast<float>(scale)), "scale is ", scale, "; a finite number of 32 bits is needed");
   const bool want_lse = truth(a[9]);
   const c10::cuda::CUDAGuard guard(dev);
   Tensor out;

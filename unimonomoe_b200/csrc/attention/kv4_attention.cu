@@ -1,4 +1,6 @@
 // Entry of the attention over the 4-bit cache: checks, and which kernels are launched.
+#include <cfloat>
+#include <cmath>
 #include "kv4_attention.cuh"
 
 namespace mono {
@@ -26,7 +28,7 @@ extern "C" int mono_attn_kv4_attention(const void* q, int64_t q_token_stride, in
   using namespace mono::kv4;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MONO_ATTN_BAD_HEAD_DIM;
   if (batch < 0 || tokens < 0 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || table_width < 1 || num_pages < 1 ||
-      window < 0 || max_query_len < 0 || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+      window < 0 || max_query_len < 0 || !(fabsf(scale) <= FLT_MAX) || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
     return MONO_ATTN_BAD_SIZE;
   if (static_cast<int64_t>(kv_heads) * page_size / 16 * block_bytes(head_dim) > INT32_MAX) return MONO_ATTN_BAD_SIZE;   // bytes of a page
   if (batch == 0 || tokens == 0) return 0;
