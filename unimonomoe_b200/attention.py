@@ -9,7 +9,7 @@ Host side of ``libmono_attention.so`` (include/mono_attention.h): arguments are 
 csrc/attention/binding.cpp), the launch goes to the current stream. Shapes, types and devices raise ValueError before anything is
 launched. The workspace of ``kv4_attention`` is kept for each stream: launches on one stream, or graphs captured on it, must
 not overlap. What only the device knows (slots, pages, lengths) is checked there: the access is left out and the first fault kept in a status word, which
-``check_status`` reads. There is no CPU or library fallback.
+``check_status`` reads. Forward only: results carry no graph. There is no CPU or library fallback.
 """
 from __future__ import annotations
 
@@ -187,7 +187,8 @@ def kv4_attention(q, cache: KV4Cache, block_table, seq_lens, query_start, max_qu
     ``window`` of those. A page that is missing from the table is reported, its keys and values are zeros. heads / kv_heads query heads share a KV head. ``scale`` is 1 / sqrt(head_dim) unless given.
 
     Returns ``out`` (bf16 [tokens, heads, head_dim], made unless given) or (out, lse) with the fp32 natural log-sum-exp [tokens,
-    heads]. A query that sees no key gets zeros and -inf. Rows that belong to no request are left as they are.
+    heads]. A query that sees no key gets zeros and -inf. Rows that belong to no request are left as they are (what
+    is made here is unset there).
 
     ``max_query_len``: the largest number of queries of a request, or anything above; it chooses kernels, never results."""
     return (_C or _load()).kv4_attention(q, cache.data, block_table, seq_lens, query_start, max_query_len, scale, window, out, return_lse)

@@ -2,8 +2,8 @@
 // that share a KV head are taken together, in blocks of 8 or 16.
 //
 // What bounds it is the cache, read once: 17/16 bytes for each key and value dim of a token. With 32 query and 4 KV heads of 128, 64
-// sequences of 4096 to 8192 tokens take 63.5 us, 3.4 TB/s, two of 131072 take 45.3 us. Each 65536 tokens more in both add 13.5 us, 5.3 TB/s
-// (a copy has 6.55): what lies between is the launch, the division of the work, the first copies' way and the join, some 14 us,
+// sequences of 4096 to 8192 tokens take 63.5 us, 3.4 TB/s, two of 131072 take 45.9 us. Each 65536 tokens more in both add 13.5 us, 5.3 TB/s
+// (a copy has 6.55): what lies between is the launch, the division of the work, the first copies' way and the join, some 13.8 us,
 // which is also what one token after 777 others takes. A CTA-wide product of 64 or more
 // rows on tcgen05 would be nearly all padding here, so the products go through mma.sync with the keys (and the dims of the
 // values) as its 16 rows and the query rows as its 8 columns, and what is made cheap is the way of a code into an operand:

@@ -5,7 +5,8 @@
 // A group x of 64 values is stored as a scale s and codes c in [-7, 7], kept as c + 8 in half a byte:
 //   s = round to five significant bits of max|x| / 7, within [2^-60, 2^60];   c = clamp(rint(x / s), -7, 7);   value s * c
 // Five bits of s and three of c make s * c exact in bfloat16: nothing is rounded when a key or value is read back, and
-// the matrix unit works on the values themselves. Rounding s costs at most 1/32 of a step of the largest code.
+// the matrix unit works on the values themselves. Rounding s moves it by at most 1/32, the largest value of a
+// group by at most 7/32 of a step.
 // A group that holds an infinity or a NaN gets the scale NaN: what reads it sees that it was not finite.
 //
 // Codes lie in the order in which the lanes of a warp use them as the A operand of mma.m16n8k16 (lane = 4 g + t holds rows g

@@ -22,8 +22,8 @@
 // All waits are bounded.
 //
 // Bound by the tensor cores, 4 D operations for each pair of a query and a key it sees, and behind them by what surrounds them. Seven
-// chunks of 350 to 700 tokens behind contexts to 4096 (32 query and 4 KV heads of 128): 241 to 250 us, 0.72 PFLOP/s; a prompt of 8192 (16 query and 2 KV
-// heads of 256): 630 us, 0.87 PFLOP/s (688 us, 0.80 in a long loop). Once the pipeline runs, a tile of 256 rows and 128 keys takes 2050 ns for heads of 128,
+// chunks of 350 to 700 tokens behind contexts to 4096 (32 query and 4 KV heads of 128): 245 to 250 us, 0.72 PFLOP/s; a prompt of 8192 (16 query and 2 KV
+// heads of 256): 671 to 690 us, 0.80 to 0.82 PFLOP/s. Once the pipeline runs, a tile of 256 rows and 128 keys takes 2050 ns for heads of 128,
 // where its products alone would take 1100: the softmax of each half tile takes 1850 cycles of the 2050 that pass between two, on two warps
 // of each scheduler that exchange 64 x 32 exponentials a warp and wait for tensor memory. Replacing some of the exponentials by
 // polynomials made it slower (243 -> 251 us for one pair in eight), as did keeping the scores in registers (247 -> 265 us), 16

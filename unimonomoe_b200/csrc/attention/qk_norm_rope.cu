@@ -9,7 +9,8 @@
 //
 // Bound by memory: 4 bytes a value, read and written once. 8192 tokens of 36 heads of 128 take 33.2 us, 4.7 TB/s, where a copy
 // of as many bytes takes 26.8; behind memory it is instructions, some 130 for a lane's eight dims with what it shares among four heads. With the
-// keys and values stored in the cache, a fifth of the rows, 47 us.
+// keys and values stored in the cache, a fifth of the rows, 47 us: more than the two apart (33.2 and 8.3), for eight dims to a lane take more
+// instructions to quantise than kv4_append's sixteen, and value rows run through the norm as well. What it saves is a launch, where tokens are few.
 #include <cuda_runtime.h>
 #include "kv4_format.cuh"
 #include "../../../include/mono_attention.h"
