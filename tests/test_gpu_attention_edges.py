@@ -379,3 +379,32 @@ def test_windows_as_wide_as_the_sequence_and_wider(news, window):
     cache, table, ln, st, q, keys, values, starts = make([400], [news], H, K, D, 16, seed=3)
     out, lse = A.kv4_attention(q, cache, table, ln, st, news, window=window, return_lse=True)
     close(out, lse, ref.attention(q, keys, values, starts, 0, D ** -0.5))
+
+
+FIRST_CALL_IN_INFERENCE_MODE = """
+import torch
+from unimonomoe_b200 import attention as A
+dev = torch.device("cuda:0")
+x = torch.ones(1, 1, 64, dtype=torch.bfloat16, device=dev)
+cache, bad = A.KV4Cache.empty(2, 1, 64, 16, dev), torch.full((1,), 99, dtype=torch.int64, device=dev)
+def told():
+    try:
+        A.check_status(dev)
+    except RuntimeError as e:
+        assert "slot outside" in str(e), e
+        return True
+    return False
+with torch.inference_mode():
+    A.kv4_append(x, x, cache, bad)                           # the first call of the process
+assert told() and not told()
+A.kv4_append(x, x, cache, bad)
+with torch.inference_mode():
+    assert told() and not told()
+print("fine")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_in_inference_mode():
+    got = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_INFERENCE_MODE], capture_output=True, text=True, timeout=300,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert got.returncode == 0 and got.stdout.strip() == "fine", got.stdout + got.stderr

@@ -3,6 +3,7 @@
 // documentation. In C++ because a call is to cost the host a few microseconds: in Python the checks and allocations alone took
 // fifteen to twenty, several times what the small launches take on the GPU.
 #include <ATen/ATen.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -136,11 +137,13 @@ class Block {
 // hold their addresses, and at exit the allocator is gone before them.
 //
 // The word is zeroed once, before any launch that may report into it, whatever stream that goes to; and not as a part of a graph, each replay of which
-// would wipe what was reported before. So it is made on a stream that is not being captured, and waited for.
+// would wipe what was reported before. So it is made on a stream that is not being captured, and waited for. Nor as an inference tensor, which
+// check_status could not write outside of that mode.
 Tensor& status_word(c10::DeviceIndex device) {
   static auto* words = new std::array<Tensor, 64>();
   Tensor& t = words->at(device);
   if (t.defined()) return t;
+  const c10::InferenceMode normal(false);
   const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);   // allocating and waiting beside a capture
   c10::cuda::CUDAStreamGuard side(c10::cuda::getStreamFromPool(true, device));
   while (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) side.reset_stream(c10::cuda::getStreamFromPool(true, device));
