@@ -3,8 +3,8 @@
 geometry the division of a batch among them (``plan``), their products over ragged runs of rows (``experts``) and the weighted
 sum of each token's results (``combine``). From the one token of a quiet server to prefill batches of 16384 tokens.
 
-Numbers. A row is cut into groups of 128 that share a scale: with m the largest magnitude (1 where that is below the smallest
-normal fp32 number), codes are e4m3 of x * (448 / m), to nearest, and the scale is m / 448. Weights [N, K] in e4m3 have one fp32
+Numbers. A row is cut into groups of 128 that share a scale: with m the largest magnitude (1 where that is below 2^-100, so that
+448 / m stays finite), codes are e4m3 of x * (448 / m), to nearest, and the scale is m / 448. Weights [N, K] in e4m3 have one fp32
 scale for each block of 128 x 128. A product sums codes * codes over a group of K, times both scales, over the groups.
 """
 import math
@@ -125,7 +125,7 @@ def _codes(x):
     k = x.shape[-1]
     g = torch.nn.functional.pad(x, (0, -k % 128)).unflatten(-1, (-1, 128))
     m = g.abs().amax(-1)
-    m = torch.where(m < torch.finfo(torch.float32).tiny, 1.0, m)
+    m = torch.where(m < 2.0 ** -100, 1.0, m)
     q = (g * _over(448.0, m)[..., None]).clamp(-448, 448).to(E4M3).flatten(-2)[..., :k]
     return q.contiguous(), _over(m, 448.0)
 
@@ -300,7 +300,7 @@ def _exact_codes(x):
     codes, scales = [], []
     for g in x.split(128, -1):
         m = g.abs().amax(-1, keepdim=True)
-        m = torch.where(m < 2.0 ** -126, torch.ones_like(m), m)
+        m = torch.where(m < 2.0 ** -100, torch.ones_like(m), m)
         codes.append(_exact_e4m3(g * 448.0 / m))
         scales.append(m / 448.0)
     return torch.cat(codes, -1), torch.cat(scales, -1)
