@@ -26,6 +26,12 @@ def attention_lib():
 
 
 @pytest.fixture(scope="session")
+def linear_lib():
+    from unimonomoe_b200 import build
+    return build.build_linear()
+
+
+@pytest.fixture(scope="session")
 def oracle():
     from oracle import cpu_oracle
     cpu_oracle.build()

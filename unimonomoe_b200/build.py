@@ -7,6 +7,7 @@ binary); here the variants share one source and differ by -D macros.
     python -m unimonomoe_b200.build            # every variant
     python -m unimonomoe_b200.build qwen_w1    # one
     python -m unimonomoe_b200.build attention  # the attention half (also built with every variant)
+    python -m unimonomoe_b200.build linear     # the block-FP8 products (likewise)
 """
 from __future__ import annotations
 
@@ -100,16 +101,28 @@ def build_variant(variant: str, force: bool = False, verbose: bool = False) -> s
     return out
 
 
-ATTENTION = os.path.join(CSRC, "attention")
-ATTENTION_SOURCES = ["batch_plan.cu", "qk_norm_rope.cu", "kv4_store.cu", "kv4_attention.cu", "kv4_decode.cu", "kv4_prompt.cu"]
+# The two halves of a layer around the MoE kernel: one library each for every geometry, with a Python module of its own
+# (csrc/<name>/binding.cpp), sources in csrc/<name>, C ABI in include/mono_<name>.h.
+PARTS = {
+    "attention": ["batch_plan.cu", "qk_norm_rope.cu", "kv4_store.cu", "kv4_attention.cu", "kv4_decode.cu", "kv4_prompt.cu"],
+    "linear": ["linear.cu", "linear_few.cu", "linear_many.cu", "fp8_quantize.cu", "expert_plan.cu", "expert_combine.cu"],
+}
+
+
+def part_lib_path(part: str) -> str:
+    return os.path.join(LIBDIR, f"libmono_{part}.so")
+
+
+def part_binding_path(part: str) -> str:
+    return os.path.join(LIBDIR, f"_mono_{part}.so")
 
 
 def attention_lib_path() -> str:
-    return os.path.join(LIBDIR, "libmono_attention.so")
+    return part_lib_path("attention")
 
 
 def attention_binding_path() -> str:
-    return os.path.join(LIBDIR, "_mono_attention.so")
+    return part_binding_path("attention")
 
 
 def _run(what: str, cmd: list) -> None:
@@ -118,35 +131,35 @@ def _run(what: str, cmd: list) -> None:
         raise RuntimeError(f"{what} failed:\n{r.stdout}{r.stderr}")
 
 
-def _compile_binding() -> str:
-    """The Python module of csrc/attention/binding.cpp, against torch's own headers and ABI."""
+def _compile_binding(part: str) -> str:
+    """The Python module of csrc/<part>/binding.cpp, against torch's own headers and ABI."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
-    obj, abi = os.path.join(LIBDIR, "binding.o"), int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    obj, abi = os.path.join(LIBDIR, f"{part}_binding.o"), int(torch._C._GLIBCXX_USE_CXX11_ABI)
     home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
     include = [*cpp_extension.include_paths(), os.path.join(home, "include"), sysconfig.get_paths()["include"]]
     _run("g++ for binding.cpp", [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_CUDA",
-                                 *(f"-isystem{i}" for i in dict.fromkeys(include)), "-c", os.path.join(ATTENTION, "binding.cpp"), "-o", obj])
+                                 *(f"-isystem{i}" for i in dict.fromkeys(include)), "-c", os.path.join(CSRC, part, "binding.cpp"), "-o", obj])
     return obj
 
 
-def _link_binding(obj: str) -> None:
+def _link_binding(part: str, obj: str) -> None:
     """Against the C++ runtime that torch's libraries use. A compiler without a shared one of its own takes the archive; the module then has a
     second runtime in it, and an exception whose message was put together by both crashes the process instead of reaching Python."""
     from torch.utils import cpp_extension
     libs = cpp_extension.library_paths()
-    _run("linking _mono_attention.so", [os.environ.get("CXX", "g++"), "-shared", obj, "-o", attention_binding_path(), *(f"-L{p}" for p in libs),
-                                        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-l:libstdc++.so.6", f"-L{LIBDIR}", "-lmono_attention",
-                                        "-Wl,-rpath,$ORIGIN"])
+    _run(f"linking _mono_{part}.so", [os.environ.get("CXX", "g++"), "-shared", obj, "-o", part_binding_path(part), *(f"-L{p}" for p in libs),
+                                      "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-l:libstdc++.so.6", f"-L{LIBDIR}", f"-lmono_{part}",
+                                      "-Wl,-rpath,$ORIGIN"])
 
 
-def build_attention(force: bool = False, verbose: bool = False) -> str:
-    """The attention half of the layer (include/mono_attention.h): one library for every geometry, and its Python module."""
-    out, header = attention_lib_path(), os.path.join(HERE, "..", "include", "mono_attention.h")
-    used = [os.path.join(ATTENTION, f) for f in os.listdir(ATTENTION)] + [os.path.join(CSRC, "ptx_sm100.cuh"), header, __file__]
-    outs = (out, attention_binding_path())
+def build_part(part: str, force: bool = False, verbose: bool = False) -> str:
+    """libmono_<part>.so and its Python module."""
+    source, out, header = os.path.join(CSRC, part), part_lib_path(part), os.path.join(HERE, "..", "include", f"mono_{part}.h")
+    used = [os.path.join(source, f) for f in os.listdir(source)] + [os.path.join(CSRC, f) for f in ("ptx_sm100.cuh", "pair_sm100.cuh")] + [header, __file__]
+    outs = (out, part_binding_path(part))
     if not force and all(os.path.exists(o) and all(os.path.getmtime(f) <= os.path.getmtime(o) for f in used) for o in outs):
         return out
     os.makedirs(LIBDIR, exist_ok=True)
@@ -155,18 +168,18 @@ def build_attention(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(src):
         obj = os.path.join(LIBDIR, os.path.splitext(src)[0] + ".o")
-        r = subprocess.run([*nvcc, "-c", os.path.join(ATTENTION, src), "-o", obj], capture_output=True, text=True)
+        r = subprocess.run([*nvcc, "-c", os.path.join(source, src), "-o", obj], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}{r.stderr}")
         return obj, r.stdout + r.stderr
 
-    with ThreadPoolExecutor(max_workers=len(ATTENTION_SOURCES) + 1) as ex:
-        binding = ex.submit(_compile_binding)
-        built = list(ex.map(compile_one, ATTENTION_SOURCES))
+    with ThreadPoolExecutor(max_workers=len(PARTS[part]) + 1) as ex:
+        binding = ex.submit(_compile_binding, part)
+        built = list(ex.map(compile_one, PARTS[part]))
         binding_obj = binding.result()
     r = subprocess.run([*nvcc, "-shared", *(obj for obj, _ in built), "-o", out], capture_output=True, text=True)
     if r.returncode == 0:
-        _link_binding(binding_obj)
+        _link_binding(part, binding_obj)
     log = "".join(text for _, text in built) + r.stdout + r.stderr
     with open(out + ".log", "w") as f:
         f.write(log)
@@ -175,8 +188,18 @@ def build_attention(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         for line in log.splitlines():
             if "registers" in line or "spill" in line:
-                print(f"[attention] {line.strip()}")
+                print(f"[{part}] {line.strip()}")
     return out
+
+
+def build_attention(force: bool = False, verbose: bool = False) -> str:
+    """The attention half of the layer (include/mono_attention.h)."""
+    return build_part("attention", force, verbose)
+
+
+def build_linear(force: bool = False, verbose: bool = False) -> str:
+    """The block-FP8 products (include/mono_linear.h)."""
+    return build_part("linear", force, verbose)
 
 
 def build_microbench() -> str:
@@ -205,11 +228,12 @@ if __name__ == "__main__":
         sel.remove("microbench")
         if not sel:
             sys.exit(0)
-    if "attention" in sel or not sel:
-        print("attention ->", build_attention(force="--force" in sys.argv, verbose=True))
-        if sel == ["attention"]:
-            sys.exit(0)
-        sel = [s for s in sel if s != "attention"]
+    asked = [p for p in PARTS if p in sel or not sel]
+    for p in asked:
+        print(p, "->", build_part(p, force="--force" in sys.argv, verbose=True))
+    if sel and all(s in PARTS for s in sel):
+        sys.exit(0)
+    sel = [s for s in sel if s not in PARTS]
     res = build_all(sel or None, force="--force" in sys.argv, verbose=True)
     for k, v in res.items():
         print(k, "->", v)

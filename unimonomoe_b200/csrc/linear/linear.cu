@@ -1,0 +1,134 @@
+// Entries of the block-FP8 products: checks, tensor maps, and which kernel is launched.
+#include "linear.cuh"
+
+namespace mono {
+namespace {
+
+using namespace lin;
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Through the runtime, so that the library loads on a machine without a driver.
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (fn == nullptr) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(sym);
+  }
+  return fn;
+}
+
+// Bytes [matrices][rows][k], boxes of 128 rows x 128 with the 128-byte swizzle; what lies outside a matrix reads as zero.
+bool map_bytes(CUtensorMap* m, const void* base, int rank, uint64_t k, uint64_t rows, uint64_t matrices) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {k, rows, matrices}, strides[2] = {k, k * rows};
+  const cuuint32_t box[3] = {kGroup, kGroup, 1}, steps[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Cycles that a group of K takes, about: of a tile of the kernel of many rows, and of those of the kernel of few.
+constexpr int kManyGroup = 700, kManyStart = 3000;
+int few_group(int tile, bool gate) { return (tile <= 16 ? 400 : tile <= 32 ? 430 : tile <= 64 ? 520 : 800) * (gate ? 2 : 1) * 4 / 4; }
+
+struct Choice {
+  int tile, split;                           // of the kernel of few rows; tile 0: the kernel of many
+  int64_t clusters;
+};
+
+// `tiles(t)`: an upper bound of the row tiles of t rows.
+template <typename Tiles>
+Choice choose(const Product& p, int few_tile, bool may_many, Tiles tiles) {
+  const bool gate = p.codes != nullptr;
+  const int64_t few_cols = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup), many_cols = gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup);
+  const int64_t units = tiles(few_tile) * few_cols;
+  int split = 1;
+  while (split < 8 && split * 2 <= p.groups && units * split * 2 <= kSms) split *= 2;
+  const int64_t clusters = split > 1 ? units : units < kSms ? units : kSms;
+  if (may_many) {
+    const int64_t many = div_up(tiles(256) * many_cols, kSms / 2) * p.groups * kManyGroup + kManyStart;
+    const int64_t few = div_up(units * split, kSms) * div_up(p.groups, split) * few_group(few_tile, gate);
+    if (many < few) return {0, 1, 0};
+  }
+  return {few_tile, split, clusters};
+}
+
+int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream) {
+  CUtensorMap w, x;
+  if (!map_bytes(&w, weight, 3, p.k, p.n, p.experts)) return MONO_LIN_DRIVER;
+  const bool gate = p.codes != nullptr;
+  if (c.tile) {
+    p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, kGroup));
+    return launch_few(p, w, c.tile, c.split, c.clusters, stream);
+  }
+  if (!map_bytes(&x, p.x, 2, p.k, p.x_rows, 1)) return MONO_LIN_DRIVER;
+  p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup));
+  return launch_many(p, w, x, stream);
+}
+
+// What every product checks; fills in what follows from the sizes.
+int check(Product& p, const uint8_t* weight) {
+  if (p.n < 1 || p.k < 16 || p.k % 16 || p.n > (1 << 24) || p.k > (1 << 24) || p.rows < 0 || p.rows > INT32_MAX || p.x_rows < 0 || p.x_rows > INT32_MAX)
+    return MONO_LIN_BAD_SIZE;
+  if (p.codes && p.n % (2 * kGroup)) return MONO_LIN_BAD_SIZE;
+  p.groups = (p.k + kGroup - 1) / kGroup;
+  p.blocks = (p.n + kGroup - 1) / kGroup;
+  if (p.rows == 0) return 0;
+  if (!p.x || !p.xs || !weight || !p.ws || !p.status || (p.out == nullptr) == (p.codes == nullptr) || (p.codes == nullptr) != (p.scales == nullptr)) return MONO_LIN_NULL;
+  if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(p.codes)) & 15) return MONO_LIN_ALIGNMENT;
+  p.vec = p.n % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual)) & 15) == 0;
+  return 0;
+}
+
+}  // namespace
+}  // namespace mono
+
+extern "C" int mono_lin_product(const uint8_t* codes, const float* scales, int64_t rows, const uint8_t* weight, const float* weight_scale, int n, int k,
+                                void* out, int out_fp32, const void* residual, uint8_t* codes_out, float* scales_out, int after_quantize,
+                                uint32_t* status, mono_lin_stream_t stream) {
+  using namespace mono;
+  Product p{};
+  p.x = codes; p.xs = scales; p.ws = weight_scale;
+  p.residual = static_cast<const __nv_bfloat16*>(residual);
+  p.out = out; p.codes = codes_out; p.scales = scales_out; p.status = status;
+  p.rows = p.x_rows = rows;
+  p.n = n; p.k = k; p.experts = 1;
+  p.fp32 = out_fp32;
+  p.after = after_quantize;
+  if (const int rc = check(p, weight)) return rc;
+  if (rows == 0) return 0;
+  const bool gate = codes_out != nullptr;
+  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || gate ? 64 : 128;
+  const Choice c = choose(p, tile, rows > 64, [&](int t) { return div_up(rows, t); });
+  if (!c.tile) p.after = 0;
+  return run(p, weight, c, stream);
+}
+
+extern "C" int mono_lin_experts(const uint8_t* codes, const float* scales, int64_t x_rows, const int32_t* tokens, const int32_t* offsets, int64_t rows,
+                                int experts, const uint8_t* weight, const float* weight_scale, int n, int k, void* out, uint8_t* codes_out,
+                                float* scales_out, uint32_t* status, mono_lin_stream_t stream) {
+  using namespace mono;
+  if (experts < 1 || experts > MONO_LIN_MAX_EXPERTS) return MONO_LIN_BAD_SIZE;
+  Product p{};
+  p.x = codes; p.xs = scales; p.ws = weight_scale;
+  p.offsets = offsets; p.tokens = tokens;
+  p.out = out; p.codes = codes_out; p.scales = scales_out; p.status = status;
+  p.rows = rows; p.x_rows = x_rows;
+  p.n = n; p.k = k; p.experts = experts;
+  if (const int rc = check(p, weight)) return rc;
+  if (rows == 0) return 0;
+  if (!offsets) return MONO_LIN_NULL;
+  if (!tokens && x_rows < rows) return MONO_LIN_BAD_SIZE;
+  if (x_rows == 0) return MONO_LIN_BAD_SIZE;
+  const bool gate = codes_out != nullptr;
+  const int64_t each = div_up(rows, experts);
+  const int tile = each <= 4 ? 16 : each <= 16 ? 32 : each <= 48 || gate ? 64 : 128;
+  const Choice c = choose(p, tile, each > 48, [&](int t) { return rows < experts ? rows : experts + rows / t; });
+  return run(p, weight, c, stream);
+}

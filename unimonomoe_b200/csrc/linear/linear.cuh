@@ -1,0 +1,229 @@
+// What the block-FP8 operators share: status codes, bounded waits, packing, the arguments of a product and the division of its
+// work into units.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include "../../../include/mono_linear.h"
+#include "../ptx_sm100.cuh"
+
+namespace mono {
+namespace lin {
+
+constexpr int kGroup = 128;                  // columns that share a scale, rows too in a weight
+constexpr int kSms = 148;
+
+enum Status : uint32_t {
+  kBadExpert = 1,                            // expert id past the last expert
+  kBadOffsets = 2,                           // offsets out of order or outside the rows
+  kBadToken = 3,                             // row outside the rows that there are
+  kBadPosition = 4,                          // position outside the partial rows
+  kWaitTimeout = 5,
+};
+
+__device__ __forceinline__ void report(uint32_t* status, uint32_t code, uint32_t where) {
+  if (atomicCAS(status, 0u, code) == 0u) status[1] = where;
+}
+
+// ---- waits
+// Phase `parity` of a barrier. One that does not come is reported, and from then on no wait of the CTA waits: every role runs
+// through its loop, whatever is in memory, and the launch ends. The clock is only read once in 64 polls.
+constexpr uint64_t kWaitNs = 2000000000ull;
+struct Waits {
+  uint32_t* stop;                            // of the CTA, in shared memory
+  uint32_t* status;
+  __device__ __forceinline__ bool gave_up(uint32_t polls, uint64_t& since) const {
+    if ((polls & 63u) != 0u) return false;
+    volatile uint32_t* s = stop;
+    if (*s) return true;
+    const uint64_t now = globaltimer_ns();
+    if (since == 0) since = now;
+    if (now - since <= kWaitNs) return false;
+    report(status, kWaitTimeout, blockIdx.x);
+    *s = 1u;
+    return true;
+  }
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) const {
+    uint64_t since = 0;
+    for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up(polls, since); ++polls) {}
+    __syncwarp();
+  }
+  // By one lane alone.
+  __device__ __forceinline__ void wait_lane(uint64_t* bar, uint32_t parity) const {
+    uint64_t since = 0;
+    for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up(polls, since); ++polls) {}
+  }
+  // With a result that the compiler sees to be the same for the whole warp: the warp that issues the products stays in uniform
+  // control flow, its descriptors in uniform registers.
+  __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity) const {
+    uint64_t since = 0;
+    for (uint32_t polls = 1; !__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity)); ++polls)
+      if (__any_sync(0xFFFFFFFFu, gave_up(polls, since))) break;
+  }
+};
+// Time for what a CTA that gave up has in flight; it takes microseconds.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 200000) __nanosleep(10000);
+}
+
+// ---- values
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
+      "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+// Four values as e4m3, to nearest, the first in the lowest byte; NaN stays NaN, what is past 448 becomes 448.
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+}
+// silu(a) * b. Exponential and division are the exact ones: with the fast ones one code in 10^5 is another.
+__device__ __forceinline__ float gated(float a, float b) { return __fdiv_rn(a, 1.0f + expf(-a)) * b; }
+// The scale of a group whose largest magnitude has the bits `m` (a NaN's are above infinity's), and what its values are multiplied by.
+struct GroupScale {
+  float scale, inverse;
+  __device__ __forceinline__ explicit GroupScale(uint32_t m) {
+    const float top = m < 0x0D800000u ? 1.0f : __uint_as_float(m);      // 2^-100
+    if (m >= 0x7F800000u) {
+      scale = inverse = __uint_as_float(0x7FC00000u);
+    } else {
+      scale = __fdiv_rn(top, 448.0f);
+      inverse = __fdiv_rn(448.0f, top);
+    }
+  }
+};
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// ---- launches one after another without a gap
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ---- products
+struct Product {
+  const uint8_t* x;                          // codes [x_rows, k]
+  const float* xs;                           // their scales [x_rows, groups]
+  const float* ws;                           // [experts][blocks][groups]
+  const int32_t* offsets;                    // of the experts' runs, or null: one run of all rows
+  const int32_t* tokens;                     // row of x for each row, or null: the same
+  const __nv_bfloat16* residual;
+  void* out;
+  uint8_t* codes;
+  float* scales;
+  uint32_t* status;
+  int64_t rows, x_rows;
+  int n, k, experts, groups, blocks;
+  int cols;                                  // units along n
+  int fp32, vec, after;                      // out is fp32; its rows begin on 16-byte boundaries; launched beside the launch before
+};
+
+struct Run {
+  int64_t row;                               // first row of the unit
+  int rows, expert, col;
+};
+
+// Units of `Tile` rows: units of a run of n rows are ceil(n / Tile), times p.cols along n. `first` (shared memory, experts + 1 words)
+// holds the number of row tiles in the runs before each; filled by all threads of the CTA.
+template <int Tile>
+struct Division {
+  const Product& p;
+  const int* first;
+  __device__ __forceinline__ Division(const Product& p, const int* first) : p(p), first(first) {}
+
+  static __device__ __forceinline__ void run(const Product& p, int e, int64_t& a, int64_t& b) {
+    a = __ldg(p.offsets + e);
+    b = __ldg(p.offsets + e + 1);
+  }
+  // By all threads, `threads` of them a multiple of 32, at most 1024; `sums` has 32 words. Where offsets are out of order or
+  // outside the rows, there are no units.
+  static __device__ __forceinline__ void fill(const Product& p, int* first, int* sums, int threads) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int base = 0;
+    bool bad = false;
+    for (int e0 = 0; e0 < p.experts; e0 += threads) {
+      int n = 0;
+      if (e0 + t < p.experts) {
+        int64_t a, b;
+        run(p, e0 + t, a, b);
+        if (a < 0 || b < a || b > p.rows) {
+          report(p.status, kBadOffsets, e0 + t);
+          bad = true;
+        } else {
+          n = static_cast<int>((b - a + Tile - 1) / Tile);
+        }
+      }
+      int s = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+        if (lane >= d) s += o;
+      }
+      if (lane == 31) sums[warp] = s;
+      __syncthreads();
+      int before = base;
+      for (int w = 0; w < warp; ++w) before += sums[w];
+      if (e0 + t < p.experts) first[e0 + t] = before + s - n;
+      for (int w = 0; w < threads / 32; ++w) base += sums[w];
+      __syncthreads();
+    }
+    if (__syncthreads_or(bad)) base = 0;
+    if (t == 0) first[p.experts] = base;
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ int64_t row_tiles() const { return p.offsets ? first[p.experts] : (p.rows + Tile - 1) / Tile; }
+  __device__ __forceinline__ int64_t units() const { return row_tiles() * p.cols; }
+  // Unit u. Experts' units follow one another along n, so that a weight is read once for the row tiles of its run; those of one
+  // dense product are taken in bands of eight row tiles, whose rows and the weight's both stay in L2.
+  __device__ __forceinline__ Run unit(int64_t u) const {
+    Run r;
+    if (p.offsets) {
+      const int tile = static_cast<int>(u / p.cols);
+      r.col = static_cast<int>(u - static_cast<int64_t>(tile) * p.cols);
+      int lo = 0, hi = p.experts;            // first[lo] <= tile < first[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= tile) lo = mid; else hi = mid;
+      }
+      int64_t a, b;
+      run(p, lo, a, b);
+      r.expert = lo;
+      r.row = a + static_cast<int64_t>(tile - first[lo]) * Tile;
+      r.rows = static_cast<int>(b - r.row < Tile ? (b > r.row ? b - r.row : 0) : Tile);
+      return r;
+    }
+    constexpr int kBand = 8;
+    const int64_t tiles = row_tiles(), band = u / (kBand * p.cols), left = tiles - band * kBand;
+    const int high = static_cast<int>(left < kBand ? left : kBand), in = static_cast<int>(u - band * kBand * p.cols);
+    r.expert = 0;
+    r.col = in / high;
+    r.row = (band * kBand + in % high) * Tile;
+    r.rows = static_cast<int>(p.rows - r.row < Tile ? p.rows - r.row : Tile);
+    return r;
+  }
+};
+
+// Row of x that row i has; -1 (reported) where there is none.
+__device__ __forceinline__ int64_t source_row(const Product& p, int64_t i) {
+  if (!p.tokens) return i;
+  const int64_t t = __ldg(p.tokens + i);
+  if (t >= 0 && t < p.x_rows) return t;
+  report(p.status, kBadToken, static_cast<uint32_t>(i));
+  return -1;
+}
+
+// The two kernels (linear_few.cu, linear_many.cu).
+int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream);
+int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, cudaStream_t stream);
+
+}  // namespace lin
+}  // namespace mono
