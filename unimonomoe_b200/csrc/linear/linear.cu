@@ -21,21 +21,33 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Bytes [matrices][rows][k], boxes of 128 rows x 128 with the 128-byte swizzle; what lies outside a matrix reads as zero.
-bool map_bytes(CUtensorMap* m, const void* base, int rank, uint64_t k, uint64_t rows, uint64_t matrices) {
+// Bytes [matrices][rows][k], boxes of `box_rows` rows x 128 with the 128-byte swizzle; what lies outside a matrix reads as zero.
+bool map_bytes(CUtensorMap* m, const void* base, int rank, uint64_t k, uint64_t rows, uint64_t matrices, uint32_t box_rows) {
   const EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[3] = {k, rows, matrices}, strides[2] = {k, k * rows};
-  const cuuint32_t box[3] = {kGroup, kGroup, 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {kGroup, box_rows, 1}, steps[3] = {1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// bf16 [rows][n], boxes of 32 rows x 64 columns with the 128-byte swizzle.
+bool map_out(CUtensorMap* m, void* base, uint64_t n, uint64_t rows) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {n, rows}, strides[1] = {2 * n};
+  const cuuint32_t box[2] = {64, 32}, steps[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Cycles that a group of K takes, about: of a tile of the kernel of many rows, and of those of the kernel of few.
-constexpr int kManyGroup = 700, kManyStart = 3000;
-int few_group(int tile, bool gate) { return (tile <= 16 ? 400 : tile <= 32 ? 430 : tile <= 64 ? 520 : 800) * (gate ? 2 : 1) * 4 / 4; }
+// About how many cycles things take: a group of K of a tile of the kernel of many rows, a stage of the kernel of few; what a unit has
+// around that, and what joining the CTAs of a cluster adds.
+constexpr int kManyGroup = 1300, kManyUnit = 3000, kStart = 3000, kJoin = 2500;
+int few_stage(int tile, bool gate) { return tile <= 16 ? 450 : tile <= 32 ? 550 : tile <= 64 ? (gate ? 1000 : 1100) : 900; }
+int few_unit(int tile) { return 300 + 15 * tile; }
 
 struct Choice {
   int tile, split;                           // of the kernel of few rows; tile 0: the kernel of many
@@ -44,32 +56,35 @@ struct Choice {
 
 // `tiles(t)`: an upper bound of the row tiles of t rows.
 template <typename Tiles>
-Choice choose(const Product& p, int few_tile, bool may_many, Tiles tiles) {
+Choice choose(const Product& p, int tile, bool may_many, Tiles tiles) {
   const bool gate = p.codes != nullptr;
   const int64_t few_cols = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup), many_cols = gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup);
-  const int64_t units = tiles(few_tile) * few_cols;
-  int split = 1;
-  while (split < 8 && split * 2 <= p.groups && units * split * 2 <= kSms) split *= 2;
-  const int64_t clusters = split > 1 ? units : units < kSms ? units : kSms;
-  if (may_many) {
-    const int64_t many = div_up(tiles(256) * many_cols, kSms / 2) * p.groups * kManyGroup + kManyStart;
-    const int64_t few = div_up(units * split, kSms) * div_up(p.groups, split) * few_group(few_tile, gate);
-    if (many < few) return {0, 1, 0};
+  const int64_t units = tiles(tile) * few_cols, steps = div_up(p.groups, few_groups(tile, gate));
+  Choice best{tile, 1, units < kSms ? units : kSms};
+  int64_t cost = kStart + div_up(units, kSms) * (steps * few_stage(tile, gate) + few_unit(tile));
+  for (int split = 2; split <= 8 && split <= steps && units * split <= kSms; ++split) {
+    const int64_t c = div_up(units, few_clusters(split)) * (kStart + div_up(steps, split) * few_stage(tile, gate) + kJoin + few_unit(tile) / split);
+    if (c < cost) {
+      cost = c;
+      best = {tile, split, units};
+    }
   }
-  return {few_tile, split, clusters};
+  if (may_many && kStart + div_up(tiles(256) * many_cols, kSms / 2) * (p.groups * kManyGroup + kManyUnit) < cost) return {0, 1, 0};
+  return best;
 }
 
 int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream) {
-  CUtensorMap w, x;
-  if (!map_bytes(&w, weight, 3, p.k, p.n, p.experts)) return MONO_LIN_DRIVER;
+  CUtensorMap w, x, out{};
+  if (!map_bytes(&w, weight, 3, p.k, p.n, p.experts, c.tile ? 128 : 64)) return MONO_LIN_DRIVER;
   const bool gate = p.codes != nullptr;
   if (c.tile) {
     p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, kGroup));
     return launch_few(p, w, c.tile, c.split, c.clusters, stream);
   }
-  if (!map_bytes(&x, p.x, 2, p.k, p.x_rows, 1)) return MONO_LIN_DRIVER;
+  if (!map_bytes(&x, p.x, 2, p.k, p.x_rows, 1, 128)) return MONO_LIN_DRIVER;
   p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup));
-  return launch_many(p, w, x, stream);
+  if (!gate && p.vec && !p.fp32 && !map_out(&out, p.out, p.n, p.rows)) return MONO_LIN_DRIVER;
+  return launch_many(p, w, x, out, stream);
 }
 
 // What every product checks; fills in what follows from the sizes.
@@ -79,6 +94,7 @@ int check(Product& p, const uint8_t* weight) {
   if (p.codes && p.n % (2 * kGroup)) return MONO_LIN_BAD_SIZE;
   p.groups = (p.k + kGroup - 1) / kGroup;
   p.blocks = (p.n + kGroup - 1) / kGroup;
+  if ((p.rows / 16 + p.experts + 1) * p.blocks > INT32_MAX) return MONO_LIN_BAD_SIZE;      // units are counted in 32 bits
   if (p.rows == 0) return 0;
   if (!p.x || !p.xs || !weight || !p.ws || !p.status || (p.out == nullptr) == (p.codes == nullptr) || (p.codes == nullptr) != (p.scales == nullptr)) return MONO_LIN_NULL;
   if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(p.codes)) & 15) return MONO_LIN_ALIGNMENT;
@@ -129,6 +145,8 @@ extern "C" int mono_lin_experts(const uint8_t* codes, const float* scales, int64
   const bool gate = codes_out != nullptr;
   const int64_t each = div_up(rows, experts);
   const int tile = each <= 4 ? 16 : each <= 16 ? 32 : each <= 48 || gate ? 64 : 128;
-  const Choice c = choose(p, tile, each > 48, [&](int t) { return rows < experts ? rows : experts + rows / t; });
+  // the kernel of many rows counts gathered rows in 32 bits, 16 bytes at a time
+  const bool may_many = each > 48 && (!tokens || x_rows * (k / 16) <= UINT32_MAX);
+  const Choice c = choose(p, tile, may_many, [&](int t) { return rows < experts ? rows : experts + rows / t; });
   return run(p, weight, c, stream);
 }

@@ -26,6 +26,13 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t code, uint32_t
 }
 
 // ---- waits
+// Whether phase `parity` is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 // Phase `parity` of a barrier. One that does not come is reported, and from then on no wait of the CTA waits: every role runs
 // through its loop, whatever is in memory, and the launch ends. The clock is only read once in 64 polls.
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -47,6 +54,19 @@ struct Waits {
     uint64_t since = 0;
     for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up(polls, since); ++polls) {}
     __syncwarp();
+  }
+  // Two barriers, looked at together: each look takes some hundred cycles, ready or not.
+  __device__ __forceinline__ void wait(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) const {
+    const bool first = mbar_test(a, pa), second = mbar_test(b, pb);
+    if (!first) wait(a, pa);
+    if (!second) wait(b, pb);
+    __syncwarp();
+  }
+  __device__ __forceinline__ void wait_warp(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) const {
+    const bool first = mbar_test(a, pa), second = mbar_test(b, pb);
+    if (__all_sync(0xFFFFFFFFu, first && second)) return;
+    wait_warp(a, pa);
+    wait_warp(b, pb);
   }
   // By one lane alone.
   __device__ __forceinline__ void wait_lane(uint64_t* bar, uint32_t parity) const {
@@ -89,6 +109,9 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
 }
 // silu(a) * b. Exponential and division are the exact ones: with the fast ones one code in 10^5 is another.
 __device__ __forceinline__ float gated(float a, float b) { return __fdiv_rn(a, 1.0f + expf(-a)) * b; }
+// The same of a product's sums, which are themselves off by more than the fast exponential and division are. Where exp(-a) is infinite
+// or close to it (a under -87) the quotient is -0.
+__device__ __forceinline__ float gated_sums(float a, float b) { return __fdividef(a, 1.0f + __expf(-a)) * b; }
 // The scale of a group whose largest magnitude has the bits `m` (a NaN's are above infinity's), and what its values are multiplied by.
 struct GroupScale {
   float scale, inverse;
@@ -127,8 +150,7 @@ struct Product {
 };
 
 struct Run {
-  int64_t row;                               // first row of the unit
-  int rows, expert, col;
+  int row, rows, expert, col;                // first row of the unit, its rows
 };
 
 // Units of `Tile` rows: units of a run of n rows are ceil(n / Tile), times p.cols along n. `first` (shared memory, experts + 1 words)
@@ -139,10 +161,6 @@ struct Division {
   const int* first;
   __device__ __forceinline__ Division(const Product& p, const int* first) : p(p), first(first) {}
 
-  static __device__ __forceinline__ void run(const Product& p, int e, int64_t& a, int64_t& b) {
-    a = __ldg(p.offsets + e);
-    b = __ldg(p.offsets + e + 1);
-  }
   // By all threads, `threads` of them a multiple of 32, at most 1024; `sums` has 32 words. Where offsets are out of order or
   // outside the rows, there are no units.
   static __device__ __forceinline__ void fill(const Product& p, int* first, int* sums, int threads) {
@@ -152,8 +170,7 @@ struct Division {
     for (int e0 = 0; e0 < p.experts; e0 += threads) {
       int n = 0;
       if (e0 + t < p.experts) {
-        int64_t a, b;
-        run(p, e0 + t, a, b);
+        const int64_t a = __ldg(p.offsets + e0 + t), b = __ldg(p.offsets + e0 + t + 1);
         if (a < 0 || b < a || b > p.rows) {
           report(p.status, kBadOffsets, e0 + t);
           bad = true;
@@ -180,50 +197,81 @@ struct Division {
     __syncthreads();
   }
 
-  __device__ __forceinline__ int64_t row_tiles() const { return p.offsets ? first[p.experts] : (p.rows + Tile - 1) / Tile; }
-  __device__ __forceinline__ int64_t units() const { return row_tiles() * p.cols; }
+  __device__ __forceinline__ int row_tiles() const { return p.offsets ? first[p.experts] : static_cast<int>((p.rows + Tile - 1) / Tile); }
+  __device__ __forceinline__ int units() const { return row_tiles() * p.cols; }
   // Unit u. Experts' units follow one another along n, so that a weight is read once for the row tiles of its run; those of one
   // dense product are taken in bands of eight row tiles, whose rows and the weight's both stay in L2.
-  __device__ __forceinline__ Run unit(int64_t u) const {
+  __device__ __forceinline__ Run unit(int u) const {
     Run r;
     if (p.offsets) {
-      const int tile = static_cast<int>(u / p.cols);
-      r.col = static_cast<int>(u - static_cast<int64_t>(tile) * p.cols);
+      const int tile = u / p.cols;
+      r.col = u - tile * p.cols;
       int lo = 0, hi = p.experts;            // first[lo] <= tile < first[hi]
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (first[mid] <= tile) lo = mid; else hi = mid;
       }
-      int64_t a, b;
-      run(p, lo, a, b);
+      const int a = __ldg(p.offsets + lo), b = __ldg(p.offsets + lo + 1);
       r.expert = lo;
-      r.row = a + static_cast<int64_t>(tile - first[lo]) * Tile;
-      r.rows = static_cast<int>(b - r.row < Tile ? (b > r.row ? b - r.row : 0) : Tile);
+      r.row = a + (tile - first[lo]) * Tile;
+      r.rows = max(0, min(Tile, b - r.row));
       return r;
     }
     constexpr int kBand = 8;
-    const int64_t tiles = row_tiles(), band = u / (kBand * p.cols), left = tiles - band * kBand;
-    const int high = static_cast<int>(left < kBand ? left : kBand), in = static_cast<int>(u - band * kBand * p.cols);
+    const int band = u / (kBand * p.cols), high = min(kBand, row_tiles() - band * kBand), in = u - band * kBand * p.cols;
     r.expert = 0;
     r.col = in / high;
-    r.row = (band * kBand + in % high) * Tile;
-    r.rows = static_cast<int>(p.rows - r.row < Tile ? p.rows - r.row : Tile);
+    r.row = (band * kBand + in - r.col * high) * Tile;
+    r.rows = min(Tile, static_cast<int>(p.rows) - r.row);
     return r;
   }
 };
 
-// Row of x that row i has; -1 (reported) where there is none.
-__device__ __forceinline__ int64_t source_row(const Product& p, int64_t i) {
-  if (!p.tokens) return i;
-  const int64_t t = __ldg(p.tokens + i);
-  if (t >= 0 && t < p.x_rows) return t;
-  report(p.status, kBadToken, static_cast<uint32_t>(i));
-  return -1;
+// ---- results
+// Four columns of a row of the result, from column n on. Out of line, like all that is not the usual case: what a unit runs through
+// once it finds in no cache, and every 128 bytes of code then cost it as much as some hundred cycles.
+static __device__ __noinline__ void store_any(const __nv_bfloat16* residual, void* out, int cols, int fp32, int64_t at, int n, float4 v) {
+  float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < cols) {
+      if (residual) x[i] += __bfloat162float(residual[at + i]);
+      if (fp32) static_cast<float*>(out)[at + i] = x[i];
+      else static_cast<__nv_bfloat16*>(out)[at + i] = __float2bfloat16_rn(x[i]);
+    }
+}
+__device__ __forceinline__ void store4(const Product& p, int64_t row, int n, const float4& v) {
+  const int64_t at = row * p.n + n;
+  if (p.vec && !p.fp32 && !p.residual) {     // n is a multiple of 8
+    if (n < p.n) *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  } else {
+    store_any(p.residual, p.out, p.n, p.fp32, at, n, v);
+  }
 }
 
-// The two kernels (linear_few.cu, linear_many.cu).
+// Row of x that row i has; where there is none that is reported, and the first one is taken.
+__device__ __forceinline__ int source_row(const Product& p, int64_t i) {
+  if (!p.tokens) return static_cast<int>(i);
+  const int t = __ldg(p.tokens + i);
+  if (t >= 0 && t < p.x_rows) return t;
+  report(p.status, kBadToken, static_cast<uint32_t>(i));
+  return 0;
+}
+
+// ---- copies into shared memory
+// 16 bytes, or zeros where `bytes` is 0.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The two kernels (linear_few.cu, linear_many.cu). Groups of K in a stage of the first, and how many clusters of `split` of its CTAs run at once.
+constexpr int few_groups(int tile, bool gate) { return gate || tile > 64 ? 1 : 2; }
+int few_clusters(int split);
 int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream);
-int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, cudaStream_t stream);
+int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, cudaStream_t stream);
 
 }  // namespace lin
 }  // namespace mono
