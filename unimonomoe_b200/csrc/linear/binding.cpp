@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
+#include <utility>
 
 #include "../../../include/mono_linear.h"
 
@@ -68,6 +69,34 @@ void inner(int64_t k, const char* name) {
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
+// Several tensors in one allocation: an allocation costs the host more than all the rest of one.
+class Block {
+ public:
+  using Part = std::pair<c10::SmallVector<int64_t, 6>, at::ScalarType>;
+  Block(c10::Device device, std::initializer_list<Part> parts) {
+    int64_t bytes = 0;
+    for (const Part& p : parts) bytes += padded(p);
+    base_ = empty({bytes}, at::kByte, device);
+    int64_t at = 0;
+    for (const Part& p : parts) {
+      Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(), c10::scalarTypeToTypeMeta(p.second));
+      t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(p.second)));
+      t.unsafeGetTensorImpl()->set_sizes_contiguous(p.first);
+      tensors_.push_back(std::move(t));
+      at += padded(p);
+    }
+  }
+  const Tensor& operator[](size_t i) const { return tensors_[i]; }
+
+ private:
+  static int64_t padded(const Part& p) {
+    int64_t n = static_cast<int64_t>(c10::elementSize(p.second));
+    for (const int64_t s : p.first) n *= s;
+    return (n + 15) / 16 * 16;
+  }
+  Tensor base_;
+  c10::SmallVector<Tensor, 4> tensors_;
+};
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
@@ -195,7 +224,8 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   inner(k, silu ? "each half of x" : "x");
   const c10::Device dev = x.t.device();
   const c10::cuda::CUDAGuard guard(dev);
-  const Tensor q = empty(with_last(x.t, k), at::kFloat8_e4m3fn, dev), s = empty(with_last(x.t, groups(k)), at::kFloat, dev);
+  const Block block(dev, {{with_last(x.t, k), at::kFloat8_e4m3fn}, {with_last(x.t, groups(k)), at::kFloat}});
+  const Tensor &q = block[0], &s = block[1];
   launched("mono_lin_quantize", mono_lin_quantize(x.t.data_ptr(), x.stride, x.rows, static_cast<int>(k), silu, ptr<uint8_t>(q), ptr<float>(s), stream_of(dev)));
   return tuple({q, s});
   END_HANDLE_TH_ERRORS
@@ -243,8 +273,14 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     codes = ptr<uint8_t>(q);
     scales = ptr<float>(s);
   }
-  const Tensor out = silu ? empty(with_last(x, w.n / 2), at::kFloat8_e4m3fn, dev) : empty(with_last(x, w.n), fp32 ? at::kFloat : at::kBFloat16, dev);
-  const Tensor out_s = silu ? empty(with_last(x, w.n / 256), at::kFloat, dev) : Tensor();
+  Tensor out, out_s;
+  if (silu) {
+    const Block block(dev, {{with_last(x, w.n / 2), at::kFloat8_e4m3fn}, {with_last(x, w.n / 256), at::kFloat}});
+    out = block[0];
+    out_s = block[1];
+  } else {
+    out = empty(with_last(x, w.n), fp32 ? at::kFloat : at::kBFloat16, dev);
+  }
   launched("mono_lin_product",
            mono_lin_product(codes, scales, rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), static_cast<int>(w.n), static_cast<int>(w.k), silu ? nullptr : out.data_ptr(),
                             fp32, ptr<void>(residual), silu ? ptr<uint8_t>(out) : nullptr, ptr<float>(out_s), quantise, status(dev), stream_of(dev)));
@@ -266,7 +302,8 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(experts >= 1 && experts <= MONO_LIN_MAX_EXPERTS, experts, " experts; 1 to ", MONO_LIN_MAX_EXPERTS, " are taken");
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor ids = in.is_contiguous() ? in : in.contiguous();
-  const Tensor offsets = empty({experts + 1}, at::kInt, dev), rows = empty({tokens * top}, at::kInt, dev), positions = empty({tokens, top}, at::kInt, dev);
+  const Block block(dev, {{{experts + 1}, at::kInt}, {{tokens * top}, at::kInt}, {{tokens, top}, at::kInt}});
+  const Tensor &offsets = block[0], &rows = block[1], &positions = block[2];
   launched("mono_lin_plan", mono_lin_plan(ids.data_ptr(), ids.scalar_type() == at::kLong, tokens, static_cast<int>(top), static_cast<int>(experts),
                                           ptr<int32_t>(offsets), ptr<int32_t>(rows), ptr<int32_t>(positions), status(dev), stream_of(dev)));
   return tuple({offsets, rows, positions});
@@ -295,13 +332,20 @@ PyObject* experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(gather || x.size(0) == rows, "x has ", x.size(0), " rows, the plan ", rows, "; with gather the tokens' rows are taken");
   TORCH_CHECK_VALUE(!gather || x.size(0) > 0 || rows == 0, "x has no rows for a plan of ", rows);
   TORCH_CHECK_VALUE(rows <= INT32_MAX && x.size(0) <= INT32_MAX, "x has ", x.size(0), " rows");
-  const Tensor out = silu ? empty({rows, w.n / 2}, at::kFloat8_e4m3fn, dev) : empty({rows, w.n}, at::kBFloat16, dev);
-  const Tensor out_s = silu ? empty({rows, w.n / 256}, at::kFloat, dev) : Tensor();
+  Tensor out, out_s;
+  if (silu) {
+    const Block block(dev, {{{rows, w.n / 2}, at::kFloat8_e4m3fn}, {{rows, w.n / 256}, at::kFloat}});
+    out = block[0];
+    out_s = block[1];
+  } else {
+    out = empty({rows, w.n}, at::kBFloat16, dev);
+  }
   Tensor q, s;
   if (a[5] == Py_None) {
     const Rows in(x, "x");
-    q = empty({x.size(0), w.k}, at::kByte, dev);
-    s = empty({x.size(0), groups(w.k)}, at::kFloat, dev);
+    const Block block(dev, {{{x.size(0), w.k}, at::kByte}, {{x.size(0), groups(w.k)}, at::kFloat}});
+    q = block[0];
+    s = block[1];
     launched("mono_lin_quantize", mono_lin_quantize(in.t.data_ptr(), in.stride, in.rows, static_cast<int>(w.k), 0, ptr<uint8_t>(q), ptr<float>(s), stream_of(dev)));
   } else {
     const Codes in(x, tensor(a[5], "x_scale"), w.k);

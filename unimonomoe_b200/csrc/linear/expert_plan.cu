@@ -1,9 +1,10 @@
 // Division of a batch among experts: a stable counting sort of the (token, place) slots by expert.
 //
-// One cluster of up to eight CTAs, so that one launch does it without a grid-wide barrier or memory kept between calls. Each warp has
-// a run of slots: it counts them into a row of its own of the CTA's table (lanes with the same expert find one another, the first
-// of them adds), the table is summed over warps, CTAs (distributed shared memory) and experts, and the warp walks its run again
-// with the cursors that it finds in its row. The order depends on nothing but the ids.
+// One cluster of up to sixteen CTAs, so that one launch does it without a grid-wide barrier or memory kept between calls. Each warp has
+// a run of slots: it counts them into a row of its own of the CTA's table, the table is summed over warps, CTAs (distributed shared memory)
+// and experts, and the warp walks its run again with the cursors that it finds in its row. Lanes with the same expert find one another
+// by the bits of its number, a vote for each (the instruction made for that, match.any, takes an SM 75 cycles: 41 us for 131072 slots).
+// The order depends on nothing but the ids.
 #include "linear.cuh"
 #include "../pair_sm100.cuh"
 
@@ -11,6 +12,8 @@ namespace mono {
 namespace {
 
 using namespace lin;
+
+constexpr int kSteps = 8, kCtas = 16;
 
 struct PlanArgs {
   const void* ids;
@@ -28,12 +31,13 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 
 template <typename Id>
 __global__ void __launch_bounds__(1024, 1) plan_kernel(const PlanArgs a) {
-  extern __shared__ uint32_t table[];        // [warps][experts], then [experts] of the CTA
+  extern __shared__ uint32_t table[];        // [warps][experts], then [experts] of the CTA and [experts] of its first rows
   __shared__ uint32_t sums[32];
   const int E = a.experts, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = gridDim.x;
   const uint32_t rank = blockIdx.x;          // the grid is one cluster
-  uint32_t *mine = table + warp * E, *total = table + warps * E;
+  uint32_t *mine = table + warp * E, *total = table + warps * E, *start = total + E;
+  const int bits = 32 - __clz(E - 1);         // of an expert's number
   const int64_t parts = static_cast<int64_t>(ctas) * warps, part = static_cast<int64_t>(rank) * warps + warp;
   const int64_t each = ((a.slots + parts - 1) / parts + 31) / 32 * 32;
   const int64_t lo = min(part * each, a.slots), hi = min(lo + each, a.slots);
@@ -41,41 +45,59 @@ __global__ void __launch_bounds__(1024, 1) plan_kernel(const PlanArgs a) {
   for (int i = threadIdx.x; i < warps * E; i += blockDim.x) table[i] = 0;
   __syncthreads();
 
-  // Expert of slot i, -1 where there is none here.
-  auto expert = [&](int64_t i, bool tell) {
-    if (i >= hi) return -1;
-    const Id id = __ldg(ids + i);
-    if (id >= E && tell) report(a.status, kBadExpert, static_cast<uint32_t>(i));
-    return id < 0 || id >= E ? -1 : static_cast<int>(id);
+  // Eight steps of 32 slots from i0 on: each lane's experts, -1 where there is none here. The ids are requested together.
+  auto take = [&](int64_t i0, int (&e)[kSteps], bool tell) {
+    Id id[kSteps];
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) id[k] = i0 + 32 * k + lane < hi ? __ldg(ids + i0 + 32 * k + lane) : -1;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      if (id[k] >= E && tell) report(a.status, kBadExpert, static_cast<uint32_t>(i0 + 32 * k + lane));
+      e[k] = id[k] < 0 || id[k] >= E ? -1 : static_cast<int>(id[k]);
+    }
   };
-  for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-    const int e = expert(i0 + lane, true);
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSteps) {
+    int e[kSteps];
+    take(i0, e, true);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+      if (e[k] >= 0) atomicAdd(mine + e[k], 1u);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {       // of the CTA, and what lies in its lower warps
     uint32_t s = 0;
-    for (int w = 0; w < warps; ++w) {
-      const uint32_t n = table[w * E + e];
-      table[w * E + e] = s;
-      s += n;
+    for (int w0 = 0; w0 < warps; w0 += 4) {  // warps are a multiple of four
+      uint32_t n[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) n[w] = table[(w0 + w) * E + e];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        table[(w0 + w) * E + e] = s;
+        s += n[w];
+      }
     }
     total[e] = s;
   }
   __syncthreads();
-  cluster_sync_all();
-  uint32_t base = 0;
+  if (ctas > 1) cluster_sync_all();
+  uint32_t base = 0;                         // rows of the experts before
   for (int e0 = 0; e0 < E; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
     uint32_t all = 0, lower = 0;
-    if (e < E)
-      for (int c = 0; c < ctas; ++c) {
-        const uint32_t n = ld_cluster(map_to_cta(smem_u32(total + e), c));
-        if (c < static_cast<int>(rank)) lower += n;
-        all += n;
+    if (e < E) {
+      if (ctas == 1) {
+        all = total[e];
+      } else {
+        uint32_t n[kCtas];
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) n[c] = ld_cluster(map_to_cta(smem_u32(total + e), c));
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) {
+          if (c < static_cast<int>(rank)) lower += n[c];
+          all += n[c];
+        }
       }
+    }
     uint32_t s = all;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -84,36 +106,50 @@ __global__ void __launch_bounds__(1024, 1) plan_kernel(const PlanArgs a) {
     }
     if (lane == 31) sums[warp] = s;
     __syncthreads();
-    uint32_t first = base + s - all;
-    for (int w = 0; w < warp; ++w) first += sums[w];
-    for (int w = 0; w < warps; ++w) base += sums[w];
+    const uint32_t of_warp = lane < warps ? sums[lane] : 0;
+    uint32_t before = of_warp;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, before, d);
+      if (lane >= d) before += o;
+    }
+    const uint32_t first = base + __shfl_sync(0xFFFFFFFFu, before - of_warp, warp) + s - all;
+    base += __shfl_sync(0xFFFFFFFFu, before, 31);
     if (e < E) {
       if (rank == 0) a.offsets[e] = static_cast<int32_t>(first);
-      for (int w = 0; w < warps; ++w) table[w * E + e] += first + lower;
+      start[e] = first + lower;
     }
     __syncthreads();
   }
   if (rank == 0 && threadIdx.x == 0) a.offsets[E] = static_cast<int32_t>(base);
-  for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = expert(i, false);
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
-    const uint32_t row = e < 0 ? 0 : mine[e] + __popc(same & ((1u << lane) - 1u));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
-    if (i < hi) {
-      a.positions[i] = e < 0 ? -1 : static_cast<int32_t>(row);
-      if (e >= 0) a.tokens[row] = static_cast<int32_t>(i / a.top);
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSteps) {
+    int e[kSteps];
+    take(i0, e, false);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int64_t i = i0 + 32 * k + lane;
+      uint32_t same = __ballot_sync(0xFFFFFFFFu, e[k] >= 0);         // lanes with the same expert
+      for (int b = 0; b < bits; ++b) {
+        const uint32_t set = __ballot_sync(0xFFFFFFFFu, e[k] >> b & 1);
+        same &= e[k] >> b & 1 ? set : ~set;
+      }
+      const uint32_t row = e[k] < 0 ? 0 : start[e[k]] + mine[e[k]] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (e[k] >= 0 && lane == __ffs(same) - 1) mine[e[k]] += __popc(same);
+      __syncwarp();
+      if (i < hi) {
+        a.positions[i] = e[k] < 0 ? -1 : static_cast<int32_t>(row);
+        if (e[k] >= 0) a.tokens[row] = static_cast<int32_t>(static_cast<uint32_t>(i) / static_cast<uint32_t>(a.top));
+      }
     }
   }
   for (int64_t i = base + static_cast<int64_t>(rank) * blockDim.x + threadIdx.x; i < a.slots; i += static_cast<int64_t>(ctas) * blockDim.x) a.tokens[i] = -1;
   __syncthreads();
-  cluster_sync_all();                        // the others have read this CTA's sums
+  if (ctas > 1) cluster_sync_all();          // the others have read this CTA's sums
 }
 
-// Slots from which eight CTAs are faster than one.
-constexpr int64_t kOneCta = 4096;
+// Slots up to which one CTA is as fast as sixteen.
+constexpr int64_t kOneCta = 1024;
 
 template <typename Id>
 int launch(const PlanArgs& a, cudaStream_t stream) {
@@ -121,19 +157,20 @@ int launch(const PlanArgs& a, cudaStream_t stream) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
-  constexpr int kMost = (33 * MONO_LIN_MAX_EXPERTS) * 4;
+  constexpr int kMost = (34 * MONO_LIN_MAX_EXPERTS) * 4;
   if (dev >= 64 || !ready[dev]) {
     e = cudaFuncSetAttribute(plan_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  const int ctas = a.slots <= kOneCta ? 1 : 8;
+  const int ctas = a.slots <= kOneCta ? 1 : kCtas;
   const int64_t per = (a.slots + ctas - 1) / ctas;
-  const int warps = per >= 1024 ? 32 : per <= 32 * 4 ? 4 : static_cast<int>((per + 31) / 32);
+  const int warps = per >= 1024 ? 32 : static_cast<int>((per + 255) / 256) * 4 + (per == 0 ? 4 : 0);
   cudaLaunchConfig_t c{};
   c.gridDim = dim3(ctas);
   c.blockDim = dim3(warps * 32);
-  c.dynamicSmemBytes = static_cast<size_t>(warps + 1) * a.experts * 4;
+  c.dynamicSmemBytes = static_cast<size_t>(warps + 2) * a.experts * 4;
   c.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -107,8 +107,16 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
 }
-// silu(a) * b. Exponential and division are the exact ones: with the fast ones one code in 10^5 is another.
-__device__ __forceinline__ float gated(float a, float b) { return __fdiv_rn(a, 1.0f + expf(-a)) * b; }
+// silu(a) * b to fp32's precision: with the fast exponential and quotient one code in 10^5 is another. The quotient is made of a
+// reciprocal with one step of Newton's method and a correction by its exact residual (Markstein, 1990), which is the rounded quotient for
+// the denominators here, from 1 up; one that is infinite or nearly so is cut, where the result is below 2^-100 in any case.
+__device__ __forceinline__ float gated(float a, float b) {
+  const float d = fminf(1.0f + expf(-a), 0x1p120f);
+  float r = rcp_approx_ftz(d);
+  r = fmaf(fmaf(-d, r, 1.0f), r, r);
+  const float q = a * r;
+  return fmaf(fmaf(-q, d, a), r, q) * b;
+}
 // The same of a product's sums, which are themselves off by more than the fast exponential and division are. Where exp(-a) is infinite
 // or close to it (a under -87) the quotient is -0.
 __device__ __forceinline__ float gated_sums(float a, float b) { return __fdividef(a, 1.0f + __expf(-a)) * b; }
