@@ -51,7 +51,7 @@ __device__ __forceinline__ void tma_weight_pair(const CUtensorMap* m, int k, int
 }
 // What the peer's tensor core is to read is released to the cluster.
 __device__ __forceinline__ void arrive_release_cluster(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
 // A box of 64 columns x 32 rows from shared memory.
