@@ -1,4 +1,5 @@
 // Entries of the block-FP8 products: checks, tensor maps, and which kernel is launched.
+#include <cmath>
 #include "linear.cuh"
 
 namespace mono {
@@ -37,39 +38,42 @@ bool map_out(CUtensorMap* m, void* base, uint64_t n, uint64_t rows) {
   if (!fn) return false;
   const cuuint64_t dims[2] = {n, rows}, strides[1] = {2 * n};
   const cuuint32_t box[2] = {64, 32}, steps[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// About how many cycles things take: a group of K of a tile of the kernel of many rows, a stage of the kernel of few; what a unit has
-// around that, and what joining the CTAs of a cluster adds.
-constexpr int kManyGroup = 1300, kManyUnit = 3000, kStart = 3000, kJoin = 2500;
-int few_stage(int tile, bool gate) { return tile <= 16 ? 450 : tile <= 32 ? 550 : tile <= 64 ? (gate ? 1000 : 1100) : 900; }
-int few_unit(int tile) { return 300 + 15 * tile; }
+// What things take, in ns, about: a launch; a stage of the kernel of few rows, a unit of it around its stages, joining the CTAs of a cluster; a
+// group of K of a tile of the kernel of many, and a unit of it.
+constexpr int64_t kStart = 2500, kJoin = 1000, kManyGroup = 620, kManyUnit = 1800, kManyGate = 800;
+struct Few {
+  int tile;
+  int64_t stage, unit;
+};
+constexpr Few kFew[3] = {{16, 360, 700}, {32, 430, 1000}, {64, 620, 1500}};
 
 struct Choice {
   int tile, split;                           // of the kernel of few rows; tile 0: the kernel of many
-  int64_t clusters;
+  int64_t clusters, cost;
 };
 
-// `tiles(t)`: an upper bound of the row tiles of t rows.
-template <typename Tiles>
-Choice choose(const Product& p, int tile, bool may_many, Tiles tiles) {
+// The kernel, tile and split with the shortest time by these figures. `likely(t)`: row tiles of t rows; `most(t)`: as many as there can be.
+template <typename Likely, typename Most>
+Choice choose(const Product& p, bool may_many, Likely likely, Most most) {
   const bool gate = p.codes != nullptr;
   const int64_t few_cols = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup), many_cols = gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup);
-  const int64_t units = tiles(tile) * few_cols, steps = div_up(p.groups, few_groups(tile, gate));
-  Choice best{tile, 1, units < kSms ? units : kSms};
-  int64_t cost = kStart + div_up(units, kSms) * (steps * few_stage(tile, gate) + few_unit(tile));
-  for (int split = 2; split <= 8 && split <= steps && units * split <= kSms; ++split) {
-    const int64_t c = div_up(units, few_clusters(split)) * (kStart + div_up(steps, split) * few_stage(tile, gate) + kJoin + few_unit(tile) / split);
-    if (c < cost) {
-      cost = c;
-      best = {tile, split, units};
+  const int64_t steps = div_up(p.groups, few_groups(gate));
+  Choice best{0, 1, 0, INT64_MAX};
+  if (may_many) best.cost = kStart + div_up(likely(128) * many_cols, kSms) * (p.groups * kManyGroup + kManyUnit + (gate ? kManyGate : 0));
+  for (const Few& f : kFew) {
+    const int64_t units = likely(f.tile) * few_cols, all = most(f.tile) * few_cols;
+    for (int split = 1; split <= 8 && split <= steps && (split == 1 || all * split <= kSms); ++split) {
+      const int64_t cost = kStart + div_up(units, few_clusters(split)) * (div_up(steps, split) * f.stage + f.unit / split + (split > 1 ? kJoin : 0));
+      if (cost < best.cost) best = {f.tile, split, split > 1 || all < kSms ? all : kSms, cost};
     }
   }
-  if (may_many && kStart + div_up(tiles(256) * many_cols, kSms / 2) * (p.groups * kManyGroup + kManyUnit) < cost) return {0, 1, 0};
   return best;
 }
 
@@ -119,9 +123,8 @@ extern "C" int mono_lin_product(const uint8_t* codes, const float* scales, int64
   p.after = after_quantize;
   if (const int rc = check(p, weight)) return rc;
   if (rows == 0) return 0;
-  const bool gate = codes_out != nullptr;
-  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || gate ? 64 : 128;
-  const Choice c = choose(p, tile, rows > 64, [&](int t) { return div_up(rows, t); });
+  const auto tiles = [&](int t) { return div_up(rows, t); };
+  const Choice c = choose(p, true, tiles, tiles);
   if (!c.tile) p.after = 0;
   return run(p, weight, c, stream);
 }
@@ -142,11 +145,16 @@ extern "C" int mono_lin_experts(const uint8_t* codes, const float* scales, int64
   if (!offsets) return MONO_LIN_NULL;
   if (!tokens && x_rows < rows) return MONO_LIN_BAD_SIZE;
   if (x_rows == 0) return MONO_LIN_BAD_SIZE;
-  const bool gate = codes_out != nullptr;
-  const int64_t each = div_up(rows, experts);
-  const int tile = each <= 4 ? 16 : each <= 16 ? 32 : each <= 48 || gate ? 64 : 128;
   // the kernel of many rows counts gathered rows in 32 bits, 16 bytes at a time
-  const bool may_many = each > 48 && (!tokens || x_rows * (k / 16) <= UINT32_MAX);
-  const Choice c = choose(p, tile, may_many, [&](int t) { return rows < experts ? rows : experts + rows / t; });
+  const bool may_many = !tokens || x_rows * (k / 16) <= UINT32_MAX;
+  // experts that even routing reaches; each has a last tile that is half full
+  const double reached = experts * (1.0 - exp(-static_cast<double>(rows) / experts));
+  const Choice c = choose(
+      p, may_many,
+      [&](int t) {
+        const double n = static_cast<double>(rows) / t + 0.5 * reached;
+        return static_cast<int64_t>(n > reached ? n : reached) + 1;
+      },
+      [&](int t) { return rows < experts ? rows : experts + rows / t; });
   return run(p, weight, c, stream);
 }

@@ -276,7 +276,7 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 }
 
 // The two kernels (linear_few.cu, linear_many.cu). Groups of K in a stage of the first, and how many clusters of `split` of its CTAs run at once.
-constexpr int few_groups(int tile, bool gate) { return gate || tile > 64 ? 1 : 2; }
+constexpr int few_groups(bool gate) { return gate ? 1 : 2; }
 int few_clusters(int split);
 int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream);
 int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, cudaStream_t stream);

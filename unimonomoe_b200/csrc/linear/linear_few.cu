@@ -29,7 +29,7 @@ constexpr int kSplit = 8;                    // CTAs of a cluster at most
 template <int Tile, bool Gate>
 struct Shape {
   static constexpr int Halves = Gate ? 2 : 1;
-  static constexpr int Groups = few_groups(Tile, Gate);       // of K in a stage
+  static constexpr int Groups = few_groups(Gate);       // of K in a stage
   static constexpr int Pieces = Halves * Groups;              // of the weight in a stage
   static constexpr int Stage = Pieces * kPiece + Groups * Tile * kGroup;
   static constexpr int Add = Halves * (Tile + kSplit) * kRows * 4;    // bytes of a unit's sums
@@ -59,14 +59,15 @@ constexpr int smem_bytes() {
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&v)[N]) {
-  static_assert(N == 8 || N == 16, "columns at a time");
+  static_assert(N == 8 || N == 16 || N == 32, "columns at a time");
   if constexpr (N == 8)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(t) : "memory");
-  else
+  else if constexpr (N == 16)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
                    "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(t) : "memory");
+  else tmem_ld32(t, v);
 }
 __device__ __forceinline__ void tma_weight(const CUtensorMap* m, int k, int row, int expert, uint32_t dst, uint64_t* bar) {
   asm volatile(
@@ -289,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   } else {
     wait_for_launch_before();
     const int quarter = warp & 3, half = (warp - 4) >> 2, w = warp - 4;
-    constexpr int kCols = S::Mine < 16 ? S::Mine : 16;
+    constexpr int kCols = S::Pieces * S::Mine / 2;            // a stage's sums of a thread are read in two loads
+    static_assert(kCols * 2 == S::Pieces * S::Mine && (S::Mine % kCols == 0), "of one piece of the weight each");
     const int i0 = half * S::Mine;                            // first row of x of this thread
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
@@ -303,30 +305,32 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         tc_fence_after();
         if (some) {
           const uint32_t d = C.tmem + s * S::Cols + i0 + (static_cast<uint32_t>(quarter * 32) << 16);
+          constexpr int kNext = S::Mine == kCols ? Tile : kCols;       // where the second load's columns lie
+          uint32_t v[2][kCols];
+          tmem_ld<kCols>(d, v[0]);
+          tmem_ld<kCols>(d + kNext, v[1]);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&C.read[s]);                      // the next product may have the buffer
 #pragma unroll
-          for (int j = 0; j < S::Pieces; ++j)
+          for (int q = 0; q < 2; ++q) {
+            constexpr bool kSame = S::Mine != kCols;                   // both of one piece
+            const int j = kSame ? 0 : q, c = kSame ? q * kCols : 0;
 #pragma unroll
-            for (int c = 0; c < S::Mine; c += kCols)
-              if (i0 + c < r.rows) {
-                uint32_t v[kCols];
-                tmem_ld<kCols>(d + j * Tile + c, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < kCols; i += 4) {
-                  const float4 sc = *reinterpret_cast<const float4*>(scale + j * Tile + c + i);
-                  float2& a0 = acc[Gate ? j : 0][(c + i) / 2];
-                  float2& a1 = acc[Gate ? j : 0][(c + i) / 2 + 1];
-                  a0 = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(sc.x, sc.y), a0);
-                  a1 = fma2(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), make_float2(sc.z, sc.w), a1);
-                }
-              }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
+            for (int i = 0; i < kCols; i += 4) {
+              const float4 sc = *reinterpret_cast<const float4*>(scale + j * Tile + c + i);
+              float2& a0 = acc[Gate ? j : 0][(c + i) / 2];
+              float2& a1 = acc[Gate ? j : 0][(c + i) / 2 + 1];
+              a0 = fma2(make_float2(__uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1])), make_float2(sc.x, sc.y), a0);
+              a1 = fma2(make_float2(__uint_as_float(v[q][i + 2]), __uint_as_float(v[q][i + 3])), make_float2(sc.z, sc.w), a1);
+            }
+          }
+          __syncwarp();
+        } else if (lane == 0) {
           mbar_arrive(&C.read[s]);
-          mbar_arrive(&C.s_empty[ring]);
         }
+        if (lane == 0) mbar_arrive(&C.s_empty[ring]);
       }
       // The unit's sums are complete, for this CTA's groups: each row's go to the CTA that finishes it.
       if (split == 1) {
@@ -435,11 +439,10 @@ int few_clusters(int split) {
 int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream) {
   if (p.codes)
     return tile == 16 ? launch<16, true>(p, weight, split, clusters, stream) : tile == 32 ? launch<32, true>(p, weight, split, clusters, stream)
-                                                                                          : launch<64, true>(p, weight, split, clusters, stream);
+                                                                                              : launch<64, true>(p, weight, split, clusters, stream);
   return tile == 16   ? launch<16, false>(p, weight, split, clusters, stream)
          : tile == 32 ? launch<32, false>(p, weight, split, clusters, stream)
-         : tile == 64 ? launch<64, false>(p, weight, split, clusters, stream)
-                      : launch<128, false>(p, weight, split, clusters, stream);
+                      : launch<64, false>(p, weight, split, clusters, stream);
 }
 }  // namespace lin
 }  // namespace mono

@@ -1,22 +1,17 @@
-// Block-FP8 products for many rows: tiles of 256 rows of x and 256 rows of the weight on clusters of two CTAs.
+// Block-FP8 products for many rows: tiles of 128 rows of x and 256 rows of the weight.
 //
 //   y[i, n] = sum_g sx[i, g] sw[n / 128, g] sum_{k in g} qx[i, k] qw[n, k]
 //
-// The two CTAs' tensor cores work as one (cta_group::2): each CTA holds 128 rows of x and half of the tile's weight rows, and its
-// tensor memory the sums of its rows with all 256. A sum over a group of 128 goes to one of two buffers, from where eight warps
-// add it, times its scales, to sums in registers: a thread has one row of x (one scale) and 128 rows of the weight (one scale, or
-// the gate's and the other half's). Sixteen warps a CTA:
+// A sum over a group of 128 is made by the tensor core (e4m3, fp32 in tensor memory), in two halves of 128 columns with two buffers each, from
+// where eight warps add it, times its scales, to sums in registers: a thread has one row of x (one scale) and 128 rows of the weight (one
+// scale, or the gate's and the other half's). Sixteen warps, one CTA to an SM:
 //   0     requests weights, and rows of x where they lie in order
-//   1, 2  in the first CTA: issue the products of both, a half of the columns each
+//   1, 2  issue the products, a half of the columns each
 //   4-7   bring the scales, some groups ahead, and rows of x that lie anywhere (tokens), by cp.async with the 128-byte swizzle
 //         written by hand
-//   8-15  read the sums, a half of the columns each four; write the results, through shared memory in whole lines
-// With the gated activation a tile is 128 rows of the gate's half (the first CTA's) and the matching 128 of the other one.
-//
-// Why pairs: a product of 128 x 256 x 128 on one SM takes 512 cycles of its tensor core and moves 48 KB into shared memory and 48 KB
-// out of it, 768 cycles at its 128 bytes a cycle; in pairs each SM has half of the weight's bytes, and both rates meet.
+//   8-15  read the sums, a half of the columns each four; write the results, through shared memory by tensor stores
+// With the gated activation a tile is 128 rows of the gate's half of the weight and the matching 128 of the other.
 #include "linear.cuh"
-#include "../pair_sm100.cuh"
 
 namespace mono {
 namespace {
@@ -25,13 +20,14 @@ using namespace lin;
 
 constexpr int kThreads = 512, kLoaders = 128, kReaders = 8, kRows = 128, kTile = 256;
 constexpr int kMma = 1, kFirstLoader = 4, kFirstReader = 8;   // warps
-constexpr int kHalf = kRows * kGroup, kStage = 2 * kHalf, kStages = 4;
 constexpr int kSums = 4;                      // buffers of 128 columns, two for each half of the tile's
 constexpr int kScales = 8;                   // groups whose scales are on their way or in use
 constexpr int kBox = 4096, kStaging = 2 * kBox;               // of a reader: 32 rows x 64 columns of bf16, twice
 // Registers of a thread: at launch, of the first eight warps, of the readers. The readers' share comes from what the others give back.
 constexpr int kRegs = 65536 / kThreads, kRegsOther = 48, kRegsReader = 208;
 static_assert(8 * kRegsOther + 8 * kRegsReader <= 16 * kRegs, "a wait for registers that are not there has no end");
+
+constexpr int kX = kRows * kGroup, kPart = 128 * kGroup, kStage = kX + 2 * kPart, kStages = 3;   // bytes of x, of a half of the weight's rows
 
 struct Control {
   uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales];
@@ -44,16 +40,11 @@ struct Control {
 constexpr int kSmem = kStages * kStage + kReaders * kStaging + static_cast<int>(sizeof(Control)) + 1024;
 static_assert(kSmem <= 232448, "shared memory of an SM");
 
-__device__ __forceinline__ void tma_weight_pair(const CUtensorMap* m, int k, int row, int expert, uint32_t dst, uint32_t bar_cluster) {
+__device__ __forceinline__ void tma_weight(const CUtensorMap* m, int k, int row, int expert, uint32_t dst, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(k), "r"(row), "r"(expert), "r"(bar_cluster) : "memory");
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(k), "r"(row), "r"(expert), "r"(smem_u32(bar)) : "memory");
 }
-// What the peer's tensor core is to read is released to the cluster.
-__device__ __forceinline__ void arrive_release_cluster(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
-}
-
 // A box of 64 columns x 32 rows from shared memory.
 __device__ __forceinline__ void tma_store(const CUtensorMap* m, int col, int row, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
@@ -154,19 +145,18 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Control& C = *reinterpret_cast<Control*>(stages + kStages * kStage + kReaders * kStaging);
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
   const Waits waits{&C.stop, p.status};
   const bool gather = p.tokens != nullptr;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&C.full[i], gather ? 2 : 1);  // the first CTA's bytes, and that the second has gathered its rows
+      mbar_init(&C.full[i], 1);
       mbar_init(&C.gathered[i], kLoaders);
       mbar_init(&C.empty[i], 2);             // of both halves
     }
     for (int i = 0; i < kSums; ++i) {
       mbar_init(&C.d_full[i], 1);
-      mbar_init(&C.d_empty[i], kReaders);    // the four readers of a half, in both CTAs
+      mbar_init(&C.d_empty[i], kReaders / 2);               // the four readers of a half
     }
     for (int i = 0; i < kScales; ++i) {
       mbar_init(&C.s_full[i], kLoaders);
@@ -176,19 +166,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     C.stop = 0;
   }
   if (warp == kMma) {
-    tmem_alloc_pair(&C.tmem, 512);
-    tmem_relinquish_pair();
+    tmem_alloc(&C.tmem, 512);
+    tmem_relinquish();
   }
-  if (p.offsets) Division<kTile>::fill(p, C.first, C.sums, kThreads);
+  if (p.offsets) Division<kRows>::fill(p, C.first, C.sums, kThreads);
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();                        // the peer's barriers are there before anything signals them
   tc_fence_after();
 
-  const Division<kTile> division(p, C.first);
-  const int units = division.units(), step = gridDim.x / 2, u0 = blockIdx.x / 2;
+  const Division<kRows> division(p, C.first);
+  const int units = division.units(), step = gridDim.x, u0 = blockIdx.x;
   const uint32_t base = smem_u32(stages);
-  auto leaders = [&](uint64_t* bar) { return map_to_cta(smem_u32(bar), 0); };
 
   if (warp < kFirstReader) {
     reg_dec<kRegsOther>();
@@ -197,62 +185,49 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         uint32_t n = 0;
         for (int u = u0; u < units; u += step) {
           const Run r = division.unit(u);
-          // rows of the weight: 64 for each half of the tile
-          const int wrow = Gate ? (rank ? p.n / 2 : 0) + r.col * kRows : r.col * kTile + static_cast<int>(rank) * 64;
-          const int xrow = r.row + static_cast<int>(rank) * kRows;
           for (int g = 0; g < p.groups; ++g, ++n) {
-            const uint32_t s = n % kStages, at = base + s * kStage, bar = leaders(&C.full[s]);
+            const uint32_t s = n % kStages, at = base + s * kStage;
             waits.wait_lane(&C.empty[s], (n / kStages & 1) ^ 1);
-            if (rank == 0) mbar_arrive_expect_tx(&C.full[s], gather ? 2 * kHalf : 4 * kHalf);
-            tma_weight_pair(&weight, g * kGroup, wrow, r.expert, at + kHalf, bar);
-            tma_weight_pair(&weight, g * kGroup, wrow + (Gate ? 64 : 128), r.expert, at + kHalf + kHalf / 2, bar);
-            if (!gather) tma_load_2d_pair(&rows, g * kGroup, static_cast<uint32_t>(xrow), stages + s * kStage, bar);
+            mbar_arrive_expect_tx(&C.full[s], gather ? 2 * kPart : 2 * kPart + kX);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)      // with the gated activation 64 rows of the gate's and of the others in turn
+              tma_weight(&weight, g * kGroup, Gate ? (q & 1) * (p.n / 2) + r.col * kRows + (q >> 1) * 64 : r.col * kTile + q * 64, r.expert,
+                         at + kX + q * 64 * kGroup, &C.full[s]);
+            if (!gather) tma_load_2d(&rows, g * kGroup, static_cast<uint32_t>(r.row), stages + s * kStage, &C.full[s]);
           }
         }
       }
       __syncwarp();
     } else if (warp < kMma + 2) {
-      if (rank == 0) {
-        constexpr uint32_t idesc = umma_idesc_e4m3_f32(2 * kRows, kTile / 2);
-        const uint32_t h = warp - kMma;
-        uint32_t n = 0;
-        for (int u = u0; u < units; u += step)
-          for (int g = 0; g < p.groups; ++g, ++n) {
-            const uint32_t s = n % kStages, b = 2 * (n & 1) + h;
-            waits.wait_warp(&C.full[s], n / kStages & 1, &C.d_empty[b], (n >> 1 & 1) ^ 1);
-            if (gather) {
-              waits.wait_warp(&C.gathered[s], n / kStages & 1);
-              fence_proxy_async_smem();
-            }
-            tc_fence_after();
-            if (elect_one_sync()) {
-              const uint64_t x = umma_desc_sw128(base + s * kStage), w = umma_desc_sw128(base + s * kStage + kHalf + h * (kHalf / 2));
-#pragma unroll
-              for (int i = 0; i < 4; ++i) umma_f8_pair(C.tmem + b * (kTile / 2), x + i * 2, w + i * 2, idesc, i > 0);
-              umma_commit_pair(&C.d_full[b]);
-              umma_commit_pair(&C.empty[s]);
-            }
-            __syncwarp();
-          }
-      } else if (gather && warp == kMma) {
-        uint32_t n = 0;
-        for (int u = u0; u < units; u += step)
-          for (int g = 0; g < p.groups; ++g, ++n) {
-            waits.wait_warp(&C.gathered[n % kStages], n / kStages & 1);
+      constexpr uint32_t idesc = umma_idesc_e4m3_f32(kRows, kTile / 2);
+      const uint32_t h = warp - kMma;
+      uint32_t n = 0;
+      for (int u = u0; u < units; u += step)
+        for (int g = 0; g < p.groups; ++g, ++n) {
+          const uint32_t s = n % kStages, b = 2 * (n & 1) + h;
+          waits.wait_warp(&C.full[s], n / kStages & 1, &C.d_empty[b], (n >> 1 & 1) ^ 1);
+          if (gather) {
+            waits.wait_warp(&C.gathered[s], n / kStages & 1);
             fence_proxy_async_smem();
-            if (lane == 0) arrive_release_cluster(leaders(&C.full[n % kStages]));
-            __syncwarp();
           }
-      }
+          tc_fence_after();
+          if (elect_one_sync()) {
+            const uint64_t x = umma_desc_sw128(base + s * kStage), w = umma_desc_sw128(base + s * kStage + kX + h * kPart);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) umma_f8(C.tmem + b * (kTile / 2), x + i * 2, w + i * 2, idesc, i > 0);
+            umma_commit(&C.d_full[b]);
+            umma_commit(&C.empty[s]);
+          }
+          __syncwarp();
+        }
     } else if (warp >= kFirstLoader) {
       const int t = threadIdx.x - 32 * kFirstLoader, chunk = t & 7, r0 = t >> 3;
       constexpr int kEach = kRows / (kLoaders / 8);           // rows of a thread, sixteen apart
       uint32_t n = 0;
       for (int u = u0; u < units; u += step) {
         const Run r = division.unit(u);
-        const int left = r.rows - static_cast<int>(rank) * kRows, first = r.row + static_cast<int>(rank) * kRows;   // rows of this CTA
-        // past them any row will do: nobody reads what comes of it
-        auto row = [&](int i) { return i < left ? source_row(p, first + i) : 0; };
+        // past the unit's rows any one will do: nobody reads what comes of it
+        auto row = [&](int i) { return i < r.rows ? source_row(p, r.row + i) : 0; };
         const float* xs = p.xs + static_cast<int64_t>(row(t)) * p.groups;
         const int block = t == 0 ? (Gate ? r.col : 2 * r.col) : Gate ? r.col + p.blocks / 2 : min(2 * r.col + 1, p.blocks - 1);
         const float* ws = p.ws + (static_cast<int64_t>(r.expert) * p.blocks + block) * p.groups;
@@ -290,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
       const Run r = division.unit(u);
-      const int in = static_cast<int>(rank) * kRows + quarter * 32, mine = max(0, min(32, r.rows - in));   // rows of this warp
+      const int in = quarter * 32, mine = max(0, min(32, r.rows - in));   // rows of this warp
       const int64_t row0 = static_cast<int64_t>(r.row) + in;
       float2 acc[2][32] = {};
       // The sums of group n are in the buffer, and its scales in shared memory.
@@ -302,8 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          uint64_t* bar = &C.d_empty[2 * (n & 1) + half];
-          if (rank) mbar_arrive_cluster(leaders(bar)); else mbar_arrive(bar);
+          mbar_arrive(&C.d_empty[2 * (n & 1) + half]);
           mbar_arrive(&C.s_empty[n % kScales]);
         }
       };
@@ -379,10 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();                        // nothing of the peer is on its way to this CTA, or reads its memory
   tc_fence_after();
   if (C.stop) settle();
-  if (warp == kMma) tmem_dealloc_pair(C.tmem, 512);
+  if (warp == kMma) tmem_dealloc(C.tmem, 512);
 }
 
 template <bool Gate>
@@ -396,18 +369,8 @@ int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, co
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(kSms);
-  c.blockDim = dim3(kThreads);
-  c.dynamicSmemBytes = kSmem;
-  c.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate>, weight, x, out, p));
+  many_kernel<Gate><<<kSms, kThreads, kSmem, stream>>>(weight, x, out, p);
+  return static_cast<int>(cudaGetLastError());
 }
 
 }  // namespace
