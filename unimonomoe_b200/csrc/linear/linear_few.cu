@@ -235,8 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
       const Run r = division.unit(u);
-      const int rows = (r.rows + 15) / 16 * 16;               // that the product reads
-      // past the unit's rows any one will do: nobody reads what comes of it
+      // rows past the unit's are left as they are: nobody reads what comes of them
       auto row = [&](int i) { return static_cast<int64_t>(i < r.rows ? source_row(p, r.row + i) : 0); };
       const uint8_t* src[kEach];
 #pragma unroll
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
           const int at = bytes ? k : 0;
 #pragma unroll
           for (int i = 0; i < kEach; ++i)
-            if (8 * i < rows) cp_async16_or_zero(dst + i * 1024, src[i] + at, bytes);
+            if (r0 + 8 * i < r.rows) cp_async16_or_zero(dst + i * 1024, src[i] + at, bytes);
         }
         cp_async_arrive_noinc(&C.full[s]);
         waits.wait(&C.s_empty[slot], (n / kScales & 1) ^ 1);

@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       uint32_t n = 0;
       for (int u = u0; u < units; u += step) {
         const Run r = division.unit(u);
-        // past the unit's rows any one will do: nobody reads what comes of it
+        // Rows past the unit's are left as they are, nobody reads what comes of them. (One row for all of them would be asked for by
+        // every CTA at once: 174 us instead of 113 for 2048 tokens through 256 experts' up projection.)
         auto row = [&](int i) { return i < r.rows ? source_row(p, r.row + i) : 0; };
         const float* xs = p.xs + static_cast<int64_t>(row(t)) * p.groups;
         const int block = t == 0 ? (Gate ? r.col : 2 * r.col) : Gate ? r.col + p.blocks / 2 : min(2 * r.col + 1, p.blocks - 1);
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         for (int g = 0; g < p.groups; ++g, ++n) {
           const uint32_t s = n % kStages, slot = n % kScales;
           waits.wait(&C.s_empty[slot], (n / kScales & 1) ^ 1);
-          cp_async4(smem_u32(&C.x_scale[slot][t]), xs + g);
+          if (t < r.rows) cp_async4(smem_u32(&C.x_scale[slot][t]), xs + g);
           if (t < 2) cp_async4(smem_u32(&C.w_scale[slot][t]), ws + g);
           cp_async_arrive_noinc(&C.s_full[slot]);
           if (gather) {
@@ -248,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
             const uint32_t dst = base + s * kStage + r0 * 128 + ((chunk ^ (r0 & 7)) << 4), bytes = k < p.k ? 16 : 0;
             const uint8_t* x = p.x + (bytes ? k : 0);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) cp_async16_or_zero(dst + i * (kLoaders / 8 * 128), x + static_cast<uint64_t>(src[i]) * 16, bytes);
+            for (int i = 0; i < kEach; ++i)
+              if (r0 + kLoaders / 8 * i < r.rows) cp_async16_or_zero(dst + i * (kLoaders / 8 * 128), x + static_cast<uint64_t>(src[i]) * 16, bytes);
             cp_async_arrive_noinc(&C.gathered[s]);
           }
         }
