@@ -21,15 +21,11 @@ struct QuantizeArgs {
 };
 
 // 16 bf16 in fp32.
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&v)[16]) {
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float2 (&v)[8]) {
   const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = bf16x2(w[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+  for (int i = 0; i < 8; ++i) v[i] = bf16x2(w[i]);
 }
 
 template <bool Silu>
@@ -42,30 +38,38 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
     const int64_t row = have ? item / a.groups : 0;
     const int group = have ? static_cast<int>(item - row * a.groups) : 0, col = group * kGroup + sub * 16;
     const bool mine = have && col < a.cols;
-    float v[16] = {};
+    float2 v[8] = {};
     if (mine) {
       const __nv_bfloat16* src = a.x + row * a.stride + col;
       load16(src, v);
       if constexpr (Silu) {
-        float u[16];
+        float2 u[8];
         load16(src + a.cols, u);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = gated(v[i], u[i]);
+        for (int i = 0; i < 8; ++i) v[i] = gated(v[i], u[i]);
       }
     }
-    uint32_t m = 0;
+    // the largest magnitude, which passes over what is not a number; that is found by products with zero
+    float top = 0.0f;
+    float2 zero = both(0.0f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, magnitude(v[i]));
+    for (int i = 0; i < 8; ++i) {
+      top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+      zero = fma2(v[i], both(0.0f), zero);
+    }
+    uint32_t m = zero.x + zero.y == 0.0f ? __float_as_uint(top) : 0x7FC00000u;
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     const GroupScale g(m);
     if (mine) {
-      uint4 w;
-      w.x = pack_e4m3x4(v[0] * g.inverse, v[1] * g.inverse, v[2] * g.inverse, v[3] * g.inverse);
-      w.y = pack_e4m3x4(v[4] * g.inverse, v[5] * g.inverse, v[6] * g.inverse, v[7] * g.inverse);
-      w.z = pack_e4m3x4(v[8] * g.inverse, v[9] * g.inverse, v[10] * g.inverse, v[11] * g.inverse);
-      w.w = pack_e4m3x4(v[12] * g.inverse, v[13] * g.inverse, v[14] * g.inverse, v[15] * g.inverse);
-      *reinterpret_cast<uint4*>(a.codes + row * a.cols + col) = w;
+      const float2 scale = both(g.inverse);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 lo = mul2(v[2 * i], scale), hi = mul2(v[2 * i + 1], scale);
+        w[i] = pack_e4m3x4(lo.x, lo.y, hi.x, hi.y);
+      }
+      *reinterpret_cast<uint4*>(a.codes + row * a.cols + col) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (have && sub == 0) a.scales[item] = g.scale;
   }

@@ -107,15 +107,22 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
 }
-// silu(a) * b to fp32's precision: with the fast exponential and quotient one code in 10^5 is another. The quotient is made of a
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 minus(float2 a) { return make_float2(-a.x, -a.y); }
+// silu(a) * b to fp32's precision, two at a time: with the fast exponential and quotient one code in 10^5 is another. The quotient is made of a
 // reciprocal with one step of Newton's method and a correction by its exact residual (Markstein, 1990), which is the rounded quotient for
 // the denominators here, from 1 up; one that is infinite or nearly so is cut, where the result is below 2^-100 in any case.
-__device__ __forceinline__ float gated(float a, float b) {
-  const float d = fminf(1.0f + expf(-a), 0x1p120f);
-  float r = rcp_approx_ftz(d);
-  r = fmaf(fmaf(-d, r, 1.0f), r, r);
-  const float q = a * r;
-  return fmaf(fmaf(-q, d, a), r, q) * b;
+__device__ __forceinline__ float2 gated(float2 a, float2 b) {
+  const float2 d = make_float2(fminf(1.0f + expf(-a.x), 0x1p120f), fminf(1.0f + expf(-a.y), 0x1p120f));
+  float2 r = make_float2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y));
+  r = fma2(fma2(minus(d), r, both(1.0f)), r, r);
+  const float2 q = mul2(a, r);
+  return mul2(fma2(fma2(minus(q), d, a), r, q), b);
 }
 // The same of a product's sums, which are themselves off by more than the fast exponential and division are. Where exp(-a) is infinite
 // or close to it (a under -87) the quotient is -0.
