@@ -1,8 +1,9 @@
-"""A small decoder that serves: whole layers made of this package's two halves, the attention of attention.py over a paged
-4-bit cache and the MoE launch of loader.py, on one GPU.
+"""A small decoder that serves: whole layers made of this package's parts, the attention of attention.py over a paged
+4-bit cache, the projections of linear.py around it and the MoE launch of loader.py, on one GPU.
 
 Requests of ragged lengths are prefilled in chunks under a token budget, then decoded together, one captured CUDA graph a step.
-Weights are random (synth.py; width and experts of its first geometry), projections and the embedding are plain library products.
+Weights are random (synth.py; width and experts of its first geometry), projections in block FP8 as the experts; router and embedding are
+plain library products. With --operators the experts are those of linear.py too, which take any geometry, instead of the one launch.
 
     python examples/decoder_layers.py --layers 2 --prompts 700 33 1500 --budget 1024 --new 32
 """
@@ -12,12 +13,15 @@ import argparse
 import os
 import sys
 import time
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from unimonomoe_b200 import KV4Cache, MonoKernel, kv4_attention, plan_batch, qk_norm_rope, synth, variant_path  # noqa: E402
+from unimonomoe_b200 import (KV4Cache, MonoKernel, fp8_linear, kv4_attention, moe_experts, plan_batch, qk_norm_rope,  # noqa: E402
+                             synth, variant_path)
+from unimonomoe_b200 import linear  # noqa: E402
 from unimonomoe_b200.attention import check_status  # noqa: E402
 from unimonomoe_b200.loader import prepare_shared_expert  # noqa: E402
 
@@ -28,7 +32,7 @@ class Layer:
     """norm, q/k/v projection, norm and rotation of heads with the store into the cache, attention, output projection; norm,
     router, routed and shared experts in one launch."""
 
-    def __init__(self, moe: MonoKernel, pages: int, page_size: int, seed: int, device):
+    def __init__(self, moe: Optional[MonoKernel], pages: int, page_size: int, seed: int, device):
         spec = synth.QWEN
         gen = torch.Generator(device=device).manual_seed(1000 + seed)
 
@@ -38,32 +42,44 @@ class Layer:
         self.moe, self.cache = moe, KV4Cache.empty(pages, KV_HEADS, HEAD_DIM, page_size, device)
         self.norms = weight(2, spec.hidden, mean=1.0)
         self.q_norm, self.k_norm = weight(HEAD_DIM, mean=1.0), weight(HEAD_DIM, mean=1.0)
-        self.qkv = weight((HEADS + 2 * KV_HEADS) * HEAD_DIM, spec.hidden)
-        self.o = weight(spec.hidden, HEADS * HEAD_DIM)
+        self.qkv = synth.quantize_block_fp8(weight((HEADS + 2 * KV_HEADS) * HEAD_DIM, spec.hidden))
+        self.o = synth.quantize_block_fp8(weight(spec.hidden, HEADS * HEAD_DIM))
         self.experts = synth.make_layer(spec, seed=seed, device=device)
         self.router = self.experts["router_w"].to(torch.bfloat16)
         sh = self.experts["shared"]
         self.shared = prepare_shared_expert(sh["w13"], sh["w13_scale"], sh["w2"], sh["w2_scale"], sh["gate"])
 
     def attention(self, x, plan, table, cos_sin, longest):
-        qkv = F.linear(F.rms_norm(x, x.shape[-1:], self.norms[0], 1e-6), self.qkv).unflatten(1, (-1, HEAD_DIM))
+        qkv = fp8_linear(F.rms_norm(x, x.shape[-1:], self.norms[0], 1e-6), *self.qkv).unflatten(1, (-1, HEAD_DIM))
         q, k, v = qkv[:, :HEADS], qkv[:, HEADS:HEADS + KV_HEADS], qkv[:, HEADS + KV_HEADS:]
         q = qk_norm_rope(q, k, self.q_norm, self.k_norm, cos_sin, plan.positions, v=v, cache=self.cache, slots=plan.slots)
         return kv4_attention(q, self.cache, table, plan.seq_lens, plan.query_start, longest)
 
     def __call__(self, x, plan, table, cos_sin, longest):
-        x = x + F.linear(self.attention(x, plan, table, cos_sin, longest).flatten(1), self.o)
+        x = fp8_linear(self.attention(x, plan, table, cos_sin, longest).flatten(1), *self.o, residual=x)
         y, w = F.rms_norm(x, x.shape[-1:], self.norms[1], 1e-6), self.experts
+        if self.moe is None:
+            return self.by_operators(y, residual=x)
         return x + self.moe.prefill(y, F.linear(y, self.router), w["w13"], w["w13_scale"], w["w2"], w["w2_scale"], shared=self.shared)
+
+
+    def by_operators(self, y, residual):
+        """Routed and shared experts of ``y`` by the operators of linear.py, and ``residual``."""
+        spec, w, sh = synth.QWEN, self.experts, self.experts["shared"]
+        score, ids = F.linear(y, self.router).float().softmax(-1).topk(spec.top_k, dim=-1)
+        codes, scales = fp8_linear(y, sh["w13"], sh["w13_scale"], silu_mul=True)
+        shared = fp8_linear(codes, sh["w2"], sh["w2_scale"], x_scale=scales, out_dtype=torch.float32) * torch.sigmoid(y.float() @ sh["gate"].T)
+        return moe_experts(y, ids, score / score.sum(-1, keepdim=True), w["w13"], w["w13_scale"], w["w2"], w["w2_scale"],
+                           residual=(residual.float() + shared).to(torch.bfloat16))
 
 
 class Server:
     """Layers with one page pool. All lengths and tables stay on the GPU; a step reads nothing back but its tokens."""
 
-    def __init__(self, layers: int, batch: int, context: int, page_size: int = 16, vocabulary: int = 8192, device="cuda"):
+    def __init__(self, layers: int, batch: int, context: int, page_size: int = 16, vocabulary: int = 8192, device="cuda", operators: bool = False):
         self.device, self.batch, self.page_size = torch.device(device), batch, page_size
         width = -(-context // page_size)
-        moe = MonoKernel(variant_path("qwen_w1"))
+        moe = None if operators else MonoKernel(variant_path("qwen_w1"))
         self.layers = [Layer(moe, batch * width, page_size, i, device) for i in range(layers)]
         gen = torch.Generator(device=device).manual_seed(7)
         self.embedding, self.head = torch.randn(2, vocabulary, synth.QWEN.hidden, generator=gen, device=device).to(torch.bfloat16)
@@ -133,8 +149,9 @@ def main() -> None:
     p.add_argument("--prompts", type=int, nargs="+", default=[700, 33, 1500], help="their lengths")
     p.add_argument("--budget", type=int, default=1024, help="tokens of a prefill step")
     p.add_argument("--new", type=int, default=32, help="tokens to decode for each request")
+    p.add_argument("--operators", action="store_true", help="experts by the operators of linear.py instead of the one launch")
     args = p.parse_args()
-    server = Server(args.layers, len(args.prompts), max(args.prompts) + args.new)
+    server = Server(args.layers, len(args.prompts), max(args.prompts) + args.new, operators=args.operators)
     gen = torch.Generator(device="cuda").manual_seed(11)
     prompts = [torch.randint(0, len(server.embedding), (n,), generator=gen, device="cuda") for n in args.prompts]
 
@@ -148,6 +165,7 @@ def main() -> None:
     first, prefill_ms = timed(server.prefill, prompts, args.budget)
     more, decode_ms = timed(server.decode, first, args.new)
     check_status()
+    linear.check_status()
     print(f"prefilled {sum(args.prompts)} tokens in {prefill_ms:.1f} ms, decoded {args.new} x {len(prompts)} in {decode_ms:.1f} ms (both with first-call set-up)")
     for b, n in enumerate(args.prompts):
         print(f"  request {b}: {n} tokens, then {[int(first[b])] + more[b, :7].tolist()} ...")

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(1024, 1) plan_kernel(const PlanArgs a) {
       } else {
         uint32_t n[kCtas];
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) n[c] = ld_cluster(map_to_cta(smem_u32(total + e), c));
+        for (int c = 0; c < kCtas; ++c) n[c] = c < ctas ? ld_cluster(map_to_cta(smem_u32(total + e), c)) : 0;
 #pragma unroll
         for (int c = 0; c < kCtas; ++c) {
           if (c < static_cast<int>(rank)) lower += n[c];
@@ -164,7 +164,8 @@ int launch(const PlanArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  const int ctas = a.slots <= kOneCta ? 1 : kCtas;
+  // sixteen where two fit an SM, so that a processing cluster with fewer SMs than that takes them too
+  const int ctas = a.slots <= kOneCta ? 1 : 34 * a.experts * 4 <= 100 * 1024 ? kCtas : kCtas / 2;
   const int64_t per = (a.slots + ctas - 1) / ctas;
   const int warps = per >= 1024 ? 32 : static_cast<int>((per + 255) / 256) * 4 + (per == 0 ? 4 : 0);
   cudaLaunchConfig_t c{};
