@@ -201,11 +201,17 @@ struct Division {
       }
       if (lane == 31) sums[warp] = s;
       __syncthreads();
-      int before = base;
-      for (int w = 0; w < warp; ++w) before += sums[w];
-      if (e0 + t < p.experts) first[e0 + t] = before + s - n;
-      for (int w = 0; w < threads / 32; ++w) base += sums[w];
-      __syncthreads();
+      const int of_warp = lane < threads / 32 ? sums[lane] : 0;
+      int before = of_warp;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, before, d);
+        if (lane >= d) before += o;
+      }
+      const int lower = __shfl_sync(0xFFFFFFFFu, before - of_warp, warp);
+      if (e0 + t < p.experts) first[e0 + t] = base + lower + s - n;
+      base += __shfl_sync(0xFFFFFFFFu, before, 31);
+      if (e0 + threads < p.experts) __syncthreads();
     }
     if (__syncthreads_or(bad)) base = 0;
     if (t == 0) first[p.experts] = base;

@@ -11,9 +11,9 @@
 //   1     issues the products
 //   2, 3  bring the rows of x and the scales, by cp.async with the 128-byte swizzle written by hand: rows may lie anywhere (tokens)
 //   4-11  read the sums, four warps for the 128 rows, twice for the halves of the rows of x
-// The groups of K may be divided among the CTAs of a cluster. Each then hands its sums to the CTA that finishes the row, through
-// distributed shared memory, and they are added in the order of the CTAs: the result does not depend on timing. Without that a
-// CTA goes from unit to unit, and the weight's requests run ahead across them.
+// The groups of K may be divided among the CTAs of a cluster. Each then hands its sums to the CTA that finishes the row, by stores into its
+// shared memory that its barrier counts, and they are added in the order of the CTAs: the result does not depend on timing. Without
+// that a CTA goes from unit to unit, and the weight's requests run ahead across them.
 #include "linear.cuh"
 #include "../pair_sm100.cuh"
 
@@ -44,7 +44,7 @@ struct Shape {
 template <int Tile, bool Gate>
 struct Control {
   using S = Shape<Tile, Gate>;
-  uint64_t full[8], done[8], read[8], s_full[kScales], s_empty[kScales];
+  uint64_t full[8], done[8], read[8], s_full[kScales], s_empty[kScales], joined;
   uint32_t tmem, stop;
   int sums[32];
   alignas(16) float scale[kScales][S::Pieces][Tile];          // of a stage: those of a row of x times the weight's
@@ -56,7 +56,10 @@ constexpr int smem_bytes() {
   return Shape<Tile, Gate>::Stages * Shape<Tile, Gate>::Stage + Shape<Tile, Gate>::Add + static_cast<int>(sizeof(Control<Tile, Gate>)) + 1024;
 }
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+// A store into the shared memory of a CTA of the cluster, which that one's barrier counts.
+__device__ __forceinline__ void st_counted(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(addr), "f"(v), "r"(bar) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&v)[N]) {
   static_assert(N == 8 || N == 16 || N == 32, "columns at a time");
@@ -145,24 +148,30 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int step = static_cast<int>(gridDim.x) / split, u0 = static_cast<int>(blockIdx.x) / split;
   const int steps = (p.groups + S::Groups - 1) / S::Groups, t0 = steps * rank / split, t1 = steps * (rank + 1) / split;   // stages of this CTA
 
-  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (threadIdx.x == 0) {
-    tma_prefetch_desc(&weight);
-    for (int i = 0; i < S::Stages; ++i) {
-      mbar_init(&C.full[i], 1 + kLoaders);
-      mbar_init(&C.done[i], 1);
-      mbar_init(&C.read[i], kReaders / 32);
+  if (warp == 0) {
+    if (lane < S::Stages) {
+      mbar_init(&C.full[lane], 1 + kLoaders);
+      mbar_init(&C.done[lane], 1);
+      mbar_init(&C.read[lane], kReaders / 32);
     }
-    for (int i = 0; i < kScales; ++i) {
-      mbar_init(&C.s_full[i], kLoaders);
-      mbar_init(&C.s_empty[i], kReaders / 32);
+    if (lane < kScales) {
+      mbar_init(&C.s_full[lane], kLoaders);
+      mbar_init(&C.s_empty[lane], kReaders / 32);
+    }
+    if (lane == 0) {
+      tma_prefetch_desc(&weight);
+      mbar_init(&C.joined, 1);
+      C.stop = 0;
     }
     mbar_init_fence();
-    C.stop = 0;
+    __syncwarp();
   }
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   if (p.offsets) Division<Tile>::fill(p, C.first, C.sums, kThreads);
   const Division<Tile> division(p, C.first);
   const int units = division.units();
+  const Run at_first = u0 < units ? division.unit(u0) : Run{};         // all warps': code that each of them would have to fetch for itself
+  auto unit = [&](int u) { return u == u0 ? at_first : division.unit(u); };
   // Stage s gets the pieces of step t of unit r; the n-th use of the ring.
   auto request = [&](const Run& r, int t, uint32_t s) {
     const uint32_t at = base + s * S::Stage;
@@ -173,10 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   };
   const int early = u0 < units ? min(t1 - t0, S::Stages) : 0;
   if (threadIdx.x == 0) {                    // the first requests, before the others are there
-    if (early > 0) {
-      const Run r = division.unit(u0);
-      for (int i = 0; i < early; ++i) request(r, t0 + i, i);
-    }
+    for (int i = 0; i < early; ++i) request(at_first, t0 + i, i);
   }
   if (warp == 1) {
     tmem_alloc(&C.tmem, S::Tmem);
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (split > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // the others run: their shared memory may be written
+  if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the others run: their shared memory may be written
 
   if (warp == 0) {
     if (lane == 0) {
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
           n += t1 - t0;
           continue;
         }
-        const Run r = division.unit(u);
+        const Run r = unit(u);
         for (int t = t0; t < t1; ++t, ++n) {
           if (static_cast<int>(n) < early) continue;
           const uint32_t s = n % S::Stages;
@@ -208,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   } else if (warp == 1) {
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
-      const Run r = division.unit(u);
+      const Run r = unit(u);
       const uint32_t idesc = umma_idesc_e4m3_f32(kRows, (r.rows + 15) / 16 * 16);
       for (int t = t0; t < t1; ++t, ++n) {
         const uint32_t s = n % S::Stages, phase = n / S::Stages & 1;
@@ -229,12 +235,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       }
     }
   } else if (warp < 4) {
-    wait_for_launch_before();
     const int t_ = threadIdx.x - 64, chunk = t_ & 7, r0 = t_ >> 3;
     constexpr int kEach = Tile / 8, kOwn = (Tile + 63) / 64;  // rows of a thread, eight apart; scales of a thread
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
-      const Run r = division.unit(u);
+      const Run r = unit(u);
       // rows past the unit's are left as they are: nobody reads what comes of them
       auto row = [&](int i) { return static_cast<int64_t>(i < r.rows ? source_row(p, r.row + i) : 0); };
       const uint8_t* src[kEach];
@@ -245,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) xs[i] = p.xs + row(t_ + 64 * i) * p.groups;
       const float *ws = p.ws + (static_cast<int64_t>(r.expert) * p.blocks + r.col) * p.groups, *ws2 = ws + static_cast<int64_t>(p.blocks / 2) * p.groups;
+      if (u == u0) wait_for_launch_before();
       float x[2][S::Groups][kOwn], wt[2][S::Pieces];
       auto fetch = [&](int t, int into) {
 #pragma unroll
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     const int i0 = half * S::Mine;                            // first row of x of this thread
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
-      const Run r = division.unit(u);
+      const Run r = unit(u);
       float2 acc[S::Halves][S::Mine / 2] = {};
       const bool some = i0 < r.rows;
       for (int t = t0; t < t1; ++t, ++n) {
@@ -343,32 +349,28 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         finish<Gate, false>(p, r, sums, 1, r.rows, 0, r.rows, w, lane);
         named_bar_sync(2, kReaders);         // all rows are read
       } else {
-        const int each = (r.rows + split - 1) / split;
+        // one unit to a cluster; each CTA finishes a share of its rows
+        const int each = (r.rows + split - 1) / split, lo = each * rank, hi = min(lo + each, r.rows);
+        if (threadIdx.x == 128) mbar_arrive_expect_tx(&C.joined, static_cast<uint32_t>(max(hi - lo, 0) * split * S::Halves * kRows * 4));
         int owner = i0 / each, in = i0 - owner * each;
 #pragma unroll
         for (int i = 0; i < S::Mine; ++i)
           if (i0 + i < r.rows) {
             const uint32_t to = map_to_cta(smem_u32(sums + (rank * S::Halves * each + in) * kRows + quarter * 32 + lane), owner);
+            const uint32_t bar = map_to_cta(smem_u32(&C.joined), owner);
 #pragma unroll
-            for (int h = 0; h < S::Halves; ++h) st_cluster(to + h * each * kRows * 4, i & 1 ? acc[h][i / 2].y : acc[h][i / 2].x);
+            for (int h = 0; h < S::Halves; ++h) st_counted(to + h * each * kRows * 4, i & 1 ? acc[h][i / 2].y : acc[h][i / 2].x, bar);
             if (++in == each) {
               in = 0;
               ++owner;
             }
           }
+        waits.wait(&C.joined, 0);
+        finish<Gate, true>(p, r, sums, split, each, lo, hi, w, lane);
       }
     }
   }
 
-  if (split > 1) {                           // one unit to a cluster
-    __syncthreads();
-    cluster_sync_all();
-    if (warp >= 4 && u0 < units) {
-      const Run r = division.unit(u0);
-      const int each = (r.rows + split - 1) / split, lo = each * rank;
-      finish<Gate, true>(p, r, sums, split, each, lo, min(lo + each, r.rows), warp - 4, lane);
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
