@@ -32,6 +32,7 @@ typedef struct CUstream_st* mono_lin_stream_t; /* cudaStream_t */
 
 #define MONO_LIN_MAX_EXPERTS 1024
 #define MONO_LIN_MAX_TOP 64
+#define MONO_LIN_FEW_ROWS 16
 
 /* x: bf16 [rows, cols] (with silu [rows, 2 cols]: silu of the first half times the second), row_stride elements apart, a multiple of 8. codes: e4m3
  * [rows, cols]; scales: fp32 [rows, ceil(cols / 128)]. */
@@ -46,6 +47,12 @@ int mono_lin_quantize(const void* x, int64_t row_stride, int64_t rows, int cols,
 int mono_lin_product(const uint8_t* codes, const float* scales, int64_t rows, const uint8_t* weight, const float* weight_scale, int n, int k,
                      void* out, int out_fp32, const void* residual, uint8_t* codes_out, float* scales_out, int after_quantize,
                      uint32_t* status, mono_lin_stream_t stream);
+
+/* The same of few rows in 16 bits (x and row_stride as in mono_lin_quantize), quantised inside the launch: the codes are those of mono_lin_quantize. For
+ * the sizes of which mono_lin_takes_rows says 1: up to MONO_LIN_FEW_ROWS rows, where n and k leave each CTA no more than it has room for. */
+int mono_lin_takes_rows(int rows, int n, int k, int silu);
+int mono_lin_product_rows(const void* x, int64_t row_stride, int rows, const uint8_t* weight, const float* weight_scale, int n, int k, void* out,
+                          int out_fp32, const void* residual, uint8_t* codes_out, float* scales_out, uint32_t* status, mono_lin_stream_t stream);
 
 /* Division of a batch among experts. ids: [tokens, top], int32 or (ids_64) int64; negative: computed elsewhere. Slots (token, place) are
  * sorted by expert, those of one expert in ascending order, into rows: offsets int32 [experts + 1], the first row of each

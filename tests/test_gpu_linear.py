@@ -60,7 +60,7 @@ def check_linear(m, n, k, seed, mode):
         assert torch.equal(got, again)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 5120, 2048), (2, 64, 16), (15, 1000, 1040), (16, 2048, 4096), (17, 129, 272), (33, 384, 7168),
+@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 5120, 2048), (3, 40000, 144), (20, 20000, 400), (32, 512, 4096), (2, 64, 16), (15, 1000, 1040), (16, 2048, 4096), (17, 129, 272), (33, 384, 7168),
                                    (61, 2048, 4096), (64, 576, 1808), (65, 640, 512), (100, 1, 256), (128, 200, 144), (129, 512, 1024)])
 @pytest.mark.parametrize("mode", ["plain", "residual", "fp32"])
 def test_linear_few_rows(m, n, k, mode):
@@ -73,7 +73,7 @@ def test_linear_many_rows(m, n, k, mode):
     check_linear(m, n, k, 1, mode)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 256, 128), (1, 1024, 2048), (16, 512, 1040), (17, 4096, 512), (33, 768, 1808), (64, 256, 7168), (200, 512, 272), (1500, 1024, 1040),
+@pytest.mark.parametrize("m,n,k", [(1, 256, 128), (1, 1024, 2048), (2, 40960, 400), (32, 512, 2048), (16, 512, 1040), (17, 4096, 512), (33, 768, 1808), (64, 256, 7168), (200, 512, 272), (1500, 1024, 1040),
                                    (2300, 512, 2048)])
 def test_linear_with_gated_activation(m, n, k):
     check_linear(m, n, k, 2, "silu")

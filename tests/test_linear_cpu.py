@@ -18,7 +18,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 def test_every_declared_symbol_is_exported(linear_lib):
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "mono_linear.h")).read(), flags=re.S)
     names = set(re.findall(r"\b(mono_lin_\w+)\s*\(", text))
-    assert names == {"mono_lin_quantize", "mono_lin_product", "mono_lin_plan", "mono_lin_experts", "mono_lin_combine"}
+    assert names == {"mono_lin_quantize", "mono_lin_product", "mono_lin_product_rows", "mono_lin_takes_rows", "mono_lin_plan", "mono_lin_experts", "mono_lin_combine"}
     lib = ctypes.CDLL(linear_lib)
     assert not [n for n in names if not hasattr(lib, n)]
     assert L.linear_lib_path() == linear_lib
@@ -57,6 +57,9 @@ def test_return_codes_before_any_cuda_call(linear_lib):
           [(5, 0, -302), (6, 136, -302), (6, 0, -302), (2, -1, -302), (2, 1 << 31, -302), ((2, 5), ((1 << 31) - 1, 1 << 20), -302), (0, 0, -301), (1, 0, -301), (3, 0, -301),
            (4, 0, -301), (7, 0, -301), (10, p, -301), (13, 0, -301), ((7, 10), (0, p), -301), (0, p + 4, -303), (3, p + 8, -303), (2, 0, 0)])
     wrong(lib.mono_lin_product, [*product[:7], 0, 0, 0, p, p, 0, p, 0], [(5, 384, -302), (5, 128, -302), (10, p + 8, -303), (11, 0, -301)])
+    lib.mono_lin_product_rows.argtypes = [vp, i64, i, vp, vp, i, i, vp, i, vp, vp, vp, vp, vp]
+    wrong(lib.mono_lin_product_rows, [p, 128, 2, p, p, 256, 128, p, 0, 0, 0, 0, p, 0],
+          [(2, 17, -302), (2, -1, -302), (1, -8, -302), (5, 0, -302), (6, 24, -302), (0, 0, -301), (3, 0, -301), (7, 0, -301), (12, 0, -301), (0, p + 2, -303), (1, 129, -303), (2, 0, 0)])
     wrong(lib.mono_lin_plan, [p, 0, 4, 2, 8, p, p, p, p, 0],
           [(2, -1, -302), (3, 0, -302), (3, L.MAX_TOP + 1, -302), (4, 0, -302), (4, L.MAX_EXPERTS + 1, -302), (2, 1 << 31, -302), (0, 0, -301), (5, 0, -301), (7, 0, -301), (8, 0, -301)])
     wrong(lib.mono_lin_experts, [p, p, 4, p, p, 8, 3, p, p, 256, 128, p, 0, 0, p, 0],

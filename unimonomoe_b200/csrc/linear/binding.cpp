@@ -249,30 +249,6 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(r.sizes().equals(with_last(x, w.n)), "residual has shape ", r.sizes(), ", expected ", c10::IntArrayRef(with_last(x, w.n)));
     residual = packed(r);
   }
-  Tensor q, s;                               // kept until the launch; where rows come in 16 bits, q is codes and scales
-  const uint8_t* codes;
-  const float* scales;
-  int64_t rows;
-  const bool quantise = a[3] == Py_None;
-  if (quantise) {
-    const Rows in(x, "x");
-    rows = in.rows;
-    TORCH_CHECK_VALUE(rows <= INT32_MAX, "x has ", rows, " rows");
-    const int64_t of_codes = rows * w.k;
-    q = empty({of_codes + rows * groups(w.k) * 4}, at::kByte, dev);
-    uint8_t* at = ptr<uint8_t>(q);
-    codes = at;
-    scales = reinterpret_cast<float*>(at + of_codes);
-    launched("mono_lin_quantize", mono_lin_quantize(in.t.data_ptr(), in.stride, rows, static_cast<int>(w.k), 0, at, reinterpret_cast<float*>(at + of_codes), stream_of(dev)));
-  } else {
-    const Codes in(x, tensor(a[3], "x_scale"), w.k);
-    rows = in.rows;
-    TORCH_CHECK_VALUE(rows <= INT32_MAX, "x has ", rows, " rows");
-    q = in.q;
-    s = in.s;
-    codes = ptr<uint8_t>(q);
-    scales = ptr<float>(s);
-  }
   Tensor out, out_s;
   if (silu) {
     const Block block(dev, {{with_last(x, w.n / 2), at::kFloat8_e4m3fn}, {with_last(x, w.n / 256), at::kFloat}});
@@ -281,9 +257,30 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else {
     out = empty(with_last(x, w.n), fp32 ? at::kFloat : at::kBFloat16, dev);
   }
-  launched("mono_lin_product",
-           mono_lin_product(codes, scales, rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), static_cast<int>(w.n), static_cast<int>(w.k), silu ? nullptr : out.data_ptr(),
-                            fp32, ptr<void>(residual), silu ? ptr<uint8_t>(out) : nullptr, ptr<float>(out_s), quantise, status(dev), stream_of(dev)));
+  void* to = silu ? nullptr : out.data_ptr();
+  uint8_t* codes_to = silu ? ptr<uint8_t>(out) : nullptr;
+  const int wn = static_cast<int>(w.n), wk = static_cast<int>(w.k);
+  if (a[3] == Py_None) {
+    const Rows in(x, "x");
+    TORCH_CHECK_VALUE(in.rows <= INT32_MAX, "x has ", in.rows, " rows");
+    if (in.rows <= MONO_LIN_FEW_ROWS && mono_lin_takes_rows(static_cast<int>(in.rows), wn, wk, silu)) {
+      launched("mono_lin_product_rows", mono_lin_product_rows(in.t.data_ptr(), in.stride, static_cast<int>(in.rows), ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32,
+                                                              ptr<void>(residual), codes_to, ptr<float>(out_s), status(dev), stream_of(dev)));
+    } else {
+      const int64_t of_codes = in.rows * w.k;
+      const Tensor q = empty({of_codes + in.rows * groups(w.k) * 4}, at::kByte, dev);      // codes, then scales
+      uint8_t* codes = ptr<uint8_t>(q);
+      float* scales = reinterpret_cast<float*>(codes + of_codes);
+      launched("mono_lin_quantize", mono_lin_quantize(in.t.data_ptr(), in.stride, in.rows, wk, 0, codes, scales, stream_of(dev)));
+      launched("mono_lin_product", mono_lin_product(codes, scales, in.rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32, ptr<void>(residual), codes_to,
+                                                    ptr<float>(out_s), 1, status(dev), stream_of(dev)));
+    }
+  } else {
+    const Codes in(x, tensor(a[3], "x_scale"), w.k);
+    TORCH_CHECK_VALUE(in.rows <= INT32_MAX, "x has ", in.rows, " rows");
+    launched("mono_lin_product", mono_lin_product(ptr<uint8_t>(in.q), ptr<float>(in.s), in.rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32, ptr<void>(residual),
+                                                  codes_to, ptr<float>(out_s), 0, status(dev), stream_of(dev)));
+  }
   if (silu) return tuple({out, out_s});
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

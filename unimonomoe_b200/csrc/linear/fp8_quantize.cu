@@ -20,14 +20,6 @@ struct QuantizeArgs {
   int cols, groups;
 };
 
-// 16 bf16 in fp32.
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float2 (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = bf16x2(w[i]);
-}
-
 template <bool Silu>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
   let_next_launch_begin();                   // a product that waits for these results by itself
@@ -49,28 +41,8 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
         for (int i = 0; i < 8; ++i) v[i] = gated(v[i], u[i]);
       }
     }
-    // the largest magnitude, which passes over what is not a number; that is found by products with zero
-    float top = 0.0f;
-    float2 zero = both(0.0f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-      zero = fma2(v[i], both(0.0f), zero);
-    }
-    uint32_t m = zero.x + zero.y == 0.0f ? __float_as_uint(top) : 0x7FC00000u;
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const GroupScale g(m);
-    if (mine) {
-      const float2 scale = both(g.inverse);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 lo = mul2(v[2 * i], scale), hi = mul2(v[2 * i + 1], scale);
-        w[i] = pack_e4m3x4(lo.x, lo.y, hi.x, hi.y);
-      }
-      *reinterpret_cast<uint4*>(a.codes + row * a.cols + col) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    const GroupScale g(top_of_group(v));
+    if (mine) *reinterpret_cast<uint4*>(a.codes + row * a.cols + col) = codes16(v, g.inverse);
     if (have && sub == 0) a.scales[item] = g.scale;
   }
 }

@@ -59,15 +59,17 @@ struct Choice {
   int64_t clusters, cost;
 };
 
-// The kernel, tile and split with the shortest time by these figures. `likely(t)`: row tiles of t rows; `most(t)`: as many as there can be.
+// The kernel, tile (`only` this one, unless 0) and split with the shortest time by these figures. `likely(t)`: row tiles of t rows; `most(t)`: as
+// many as there can be.
 template <typename Likely, typename Most>
-Choice choose(const Product& p, bool may_many, Likely likely, Most most) {
+Choice choose(const Product& p, bool may_many, int only, Likely likely, Most most) {
   const bool gate = p.codes != nullptr;
   const int64_t few_cols = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup), many_cols = gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup);
   const int64_t steps = div_up(p.groups, few_groups(gate));
   Choice best{0, 1, 0, INT64_MAX};
   if (may_many) best.cost = kStart + div_up(likely(128) * many_cols, kSms) * (p.groups * kManyGroup + kManyUnit + (gate ? kManyGate : 0));
   for (const Few& f : kFew) {
+    if (only && f.tile != only) continue;
     const int64_t units = likely(f.tile) * few_cols, all = most(f.tile) * few_cols;
     for (int split = 1; split <= 8 && split <= steps && (split == 1 || all * split <= kSms); ++split) {
       const int64_t cost = kStart + div_up(units, few_clusters(split)) * (div_up(steps, split) * f.stage + f.unit / split + (split > 1 ? kJoin : 0));
@@ -75,6 +77,15 @@ Choice choose(const Product& p, bool may_many, Likely likely, Most most) {
     }
   }
   return best;
+}
+
+// Of a dense product. Few rows are one row tile, whether they come in 8 bits or in 16: the results are the same bits. (Quantised in the launch, K of 2048
+// and 5120 columns: 1 row 6.0 us, 16 rows 7.5; in a launch before it 7.1 and 7.7. From 17 rows on the launch before it is faster: 24 rows 8.6 and
+// 8.1, 61 rows, K of 4096 and 2048 columns, 13.4 and 9.3.)
+Choice dense(const Product& p) {
+  const auto tiles = [&](int t) { return div_up(p.rows, t); };
+  const bool few = p.rows <= MONO_LIN_FEW_ROWS;
+  return choose(p, !few, few ? 16 : 0, tiles, tiles);
 }
 
 int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream) {
@@ -100,7 +111,7 @@ int check(Product& p, const uint8_t* weight) {
   p.blocks = (p.n + kGroup - 1) / kGroup;
   if ((p.rows / 16 + p.experts + 1) * p.blocks > INT32_MAX) return MONO_LIN_BAD_SIZE;      // units are counted in 32 bits
   if (p.rows == 0) return 0;
-  if (!p.x || !p.xs || !weight || !p.ws || !p.status || (p.out == nullptr) == (p.codes == nullptr) || (p.codes == nullptr) != (p.scales == nullptr)) return MONO_LIN_NULL;
+  if ((!p.raw && (!p.x || !p.xs)) || !weight || !p.ws || !p.status || (p.out == nullptr) == (p.codes == nullptr) || (p.codes == nullptr) != (p.scales == nullptr)) return MONO_LIN_NULL;
   if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(p.codes)) & 15) return MONO_LIN_ALIGNMENT;
   p.vec = p.n % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual)) & 15) == 0;
   return 0;
@@ -123,9 +134,56 @@ extern "C" int mono_lin_product(const uint8_t* codes, const float* scales, int64
   p.after = after_quantize;
   if (const int rc = check(p, weight)) return rc;
   if (rows == 0) return 0;
-  const auto tiles = [&](int t) { return div_up(rows, t); };
-  const Choice c = choose(p, true, tiles, tiles);
+  const Choice c = dense(p);
   if (!c.tile) p.after = 0;
+  return run(p, weight, c, stream);
+}
+
+namespace mono {
+namespace {
+// Whether rows in 16 bits are taken: in one row tile, every CTA's groups of K in its ring.
+bool takes_rows(const Product& p, Choice& c) {
+  if (p.rows > MONO_LIN_FEW_ROWS) return false;
+  const bool gate = p.codes != nullptr;
+  c = dense(p);
+  const int64_t units = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup);
+  return units <= c.clusters && div_up(div_up(p.groups, few_groups(gate)), c.split) <= few_stages(c.tile, gate);
+}
+}  // namespace
+}  // namespace mono
+
+extern "C" int mono_lin_takes_rows(int rows, int n, int k, int silu) {
+  using namespace mono;
+  if (rows < 1 || n < 1 || k < 16 || k % 16 || (silu && n % (2 * kGroup))) return 0;
+  Product p{};
+  uint8_t any;
+  p.codes = silu ? &any : nullptr;
+  p.rows = rows;
+  p.n = n; p.k = k;
+  p.groups = (k + kGroup - 1) / kGroup;
+  Choice c;
+  return takes_rows(p, c);
+}
+
+extern "C" int mono_lin_product_rows(const void* x, int64_t row_stride, int rows, const uint8_t* weight, const float* weight_scale, int n, int k, void* out,
+                                     int out_fp32, const void* residual, uint8_t* codes_out, float* scales_out, uint32_t* status, mono_lin_stream_t stream) {
+  using namespace mono;
+  if (row_stride < 0) return MONO_LIN_BAD_SIZE;
+  Product p{};
+  p.raw = static_cast<const __nv_bfloat16*>(x);
+  p.raw_stride = row_stride;
+  p.ws = weight_scale;
+  p.residual = static_cast<const __nv_bfloat16*>(residual);
+  p.out = out; p.codes = codes_out; p.scales = scales_out; p.status = status;
+  p.rows = p.x_rows = rows;
+  p.n = n; p.k = k; p.experts = 1;
+  p.fp32 = out_fp32;
+  if (rows > 0 && !x) return MONO_LIN_NULL;
+  if (const int rc = check(p, weight)) return rc;
+  if (rows == 0) return 0;
+  if (reinterpret_cast<uintptr_t>(x) & 15 || row_stride % 8) return MONO_LIN_ALIGNMENT;
+  Choice c;
+  if (!takes_rows(p, c)) return MONO_LIN_BAD_SIZE;
   return run(p, weight, c, stream);
 }
 
@@ -150,7 +208,7 @@ extern "C" int mono_lin_experts(const uint8_t* codes, const float* scales, int64
   // experts that even routing reaches; each has a last tile that is half full
   const double reached = experts * (1.0 - exp(-static_cast<double>(rows) / experts));
   const Choice c = choose(
-      p, may_many,
+      p, may_many, 0,
       [&](int t) {
         const double n = static_cast<double>(rows) / t + 0.5 * reached;
         return static_cast<int64_t>(n > reached ? n : reached) + 1;

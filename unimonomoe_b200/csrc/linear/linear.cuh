@@ -142,6 +142,41 @@ struct GroupScale {
 };
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
+// 16 bf16 in fp32.
+__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float2 (&v)[8]) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = bf16x2(w[i]);
+}
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float2 (&v)[8]) {
+  unpack16(__ldg(reinterpret_cast<const uint4*>(p)), __ldg(reinterpret_cast<const uint4*>(p) + 1), v);
+}
+// Largest magnitude (as bits, a NaN's above all) of a group that eight neighbouring lanes share, 16 values each. All lanes of the warp take part.
+// The maximum passes over what is not a number; that is found by products with zero.
+__device__ __forceinline__ uint32_t top_of_group(const float2 (&v)[8]) {
+  float top = 0.0f;
+  float2 zero = both(0.0f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+    zero = fma2(v[i], both(0.0f), zero);
+  }
+  uint32_t m = zero.x + zero.y == 0.0f ? __float_as_uint(top) : 0x7FC00000u;
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  return m;
+}
+__device__ __forceinline__ uint4 codes16(const float2 (&v)[8], float inverse) {
+  const float2 scale = both(inverse);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 lo = mul2(v[2 * i], scale), hi = mul2(v[2 * i + 1], scale);
+    w[i] = pack_e4m3x4(lo.x, lo.y, hi.x, hi.y);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ---- launches one after another without a gap
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -150,6 +185,8 @@ __device__ __forceinline__ void let_next_launch_begin() { asm volatile("griddepc
 struct Product {
   const uint8_t* x;                          // codes [x_rows, k]
   const float* xs;                           // their scales [x_rows, groups]
+  const __nv_bfloat16* raw;                  // or the rows in 16 bits, which the kernel of few rows quantises (else null)
+  int64_t raw_stride;
   const float* ws;                           // [experts][blocks][groups]
   const int32_t* offsets;                    // of the experts' runs, or null: one run of all rows
   const int32_t* tokens;                     // row of x for each row, or null: the same
@@ -291,6 +328,7 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 // The two kernels (linear_few.cu, linear_many.cu). Groups of K in a stage of the first, and how many clusters of `split` of its CTAs run at once.
 constexpr int few_groups(bool gate) { return gate ? 1 : 2; }
 int few_clusters(int split);
+int few_stages(int tile, bool gate);         // of the ring of a CTA
 int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream);
 int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, cudaStream_t stream);
 

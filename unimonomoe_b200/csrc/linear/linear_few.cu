@@ -9,7 +9,8 @@
 // time, more than a piece of few rows takes to multiply. Twelve warps, one CTA to an SM:
 //   0     requests the weight
 //   1     issues the products
-//   2, 3  bring the rows of x and the scales, by cp.async with the 128-byte swizzle written by hand: rows may lie anywhere (tokens)
+//   2, 3  bring the rows of x and the scales, by cp.async with the 128-byte swizzle written by hand: rows may lie anywhere (tokens). Rows in 16
+//         bits are quantised by them and the readers at the start, in every CTA: for so few that takes less than a launch before this one
 //   4-11  read the sums, four warps for the 128 rows, twice for the halves of the rows of x
 // The groups of K may be divided among the CTAs of a cluster. Each then hands its sums to the CTA that finishes the row, by stores into its
 // shared memory that its barrier counts, and they are added in the order of the CTAs: the result does not depend on timing. Without
@@ -134,6 +135,42 @@ __device__ __forceinline__ void finish(const Product& p, const Run& r, const flo
   }
 }
 
+// Rows in 16 bits of this CTA's groups, which all find room in the ring: codes into the stages' rows of x, scales times the weight's. By all warps
+// but the first two: eight lanes share a group, 16 values each; the next one's values are on their way while one is quantised.
+template <int Tile, bool Gate>
+__device__ __forceinline__ void quantise_rows(const Product& p, Control<Tile, Gate>& C, const Run& r, uint32_t base, int t0, int t1) {
+  using S = Shape<Tile, Gate>;
+  constexpr int kTeams = (kThreads - 64) / 8;
+  const int lane8 = threadIdx.x & 7, items = (t1 - t0) * S::Groups * r.rows;
+  const float* ws = p.ws + static_cast<int64_t>(r.col) * p.groups;
+  uint4 next[2];
+  auto fetch = [&](int i) {
+    const int g = i / r.rows, k = (t0 * S::Groups + g) * kGroup + lane8 * 16;
+    const bool have = i < items && k < p.k;
+    const uint4* src = reinterpret_cast<const uint4*>(p.raw + (i - g * r.rows) * p.raw_stride + k);
+    next[0] = have ? __ldg(src) : make_uint4(0, 0, 0, 0);
+    next[1] = have ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+  };
+  int i = (threadIdx.x - 64) >> 3;
+  fetch(i);
+  for (; __any_sync(0xFFFFFFFFu, i < items); i += kTeams) {
+    float2 v[8];
+    unpack16(next[0], next[1], v);
+    fetch(i + kTeams);
+    const int g = i / r.rows, row = i - g * r.rows, s = g / S::Groups, j = g - s * S::Groups;   // group and row, stage and group of it
+    const int of = min(t0 * S::Groups + g, p.groups - 1);
+    const GroupScale scale(top_of_group(v));
+    if (i < items) {
+      const uint4 c = codes16(v, scale.inverse);
+      const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+      st_shared_128(base + s * S::Stage + S::Pieces * kPiece + (j * Tile + row) * 128 + ((lane8 ^ (row & 7)) << 4), words);
+      if (lane8 < S::Halves) C.scale[s][Gate ? lane8 : j][row] = scale.scale * __ldg(ws + static_cast<int64_t>(lane8) * (p.blocks / 2) * p.groups + of);
+    }
+  }
+  fence_proxy_async_smem();                  // the tensor core reads what was stored here
+  named_bar_sync(3, kThreads - 64);
+}
+
 template <int Tile, bool Gate>
 __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ CUtensorMap weight, const __grid_constant__ Product p, const int split) {
   using S = Shape<Tile, Gate>;
@@ -193,6 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   tc_fence_after();
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the others run: their shared memory may be written
 
+  if (p.raw != nullptr && warp >= 2 && u0 < units) quantise_rows<Tile, Gate>(p, C, at_first, base, t0, t1);
+
   if (warp == 0) {
     if (lane == 0) {
       uint32_t n = 0;
@@ -234,6 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         __syncwarp();
       }
     }
+  } else if (warp < 4 && p.raw != nullptr) {
+    if (u0 < units)
+      for (int n = 0; n < t1 - t0; ++n) {
+        mbar_arrive(&C.full[n]);
+        mbar_arrive(&C.s_full[n]);
+      }
   } else if (warp < 4) {
     const int t_ = threadIdx.x - 64, chunk = t_ & 7, r0 = t_ >> 3;
     constexpr int kEach = Tile / 8, kOwn = (Tile + 63) / 64;  // rows of a thread, eight apart; scales of a thread
@@ -417,6 +462,10 @@ int launch(const Product& p, const CUtensorMap& weight, int split, int64_t clust
 }  // namespace
 
 namespace lin {
+int few_stages(int tile, bool gate) {
+  if (gate) return tile == 16 ? Shape<16, true>::Stages : tile == 32 ? Shape<32, true>::Stages : Shape<64, true>::Stages;
+  return tile == 16 ? Shape<16, false>::Stages : tile == 32 ? Shape<32, false>::Stages : Shape<64, false>::Stages;
+}
 int few_clusters(int split) {
   static int known[kSplit + 1] = {};
   if (split == 1) return kSms;
