@@ -75,6 +75,32 @@ def test_rows_that_are_not_finite_stay_with_their_expert():
         assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("m", [1, 9, 30, 60])
+@pytest.mark.parametrize("k", [128, 384, 1040])
+def test_infinite_scales_are_infinite_results(m, k):
+    """Of an odd number of groups the last one has an infinite scale: sums of one sign, so that nothing of it is NaN."""
+    g = k // 128 + (k % 128 > 0)
+    x = torch.ones(m, k, device="cuda").to(ref.E4M3)
+    w = torch.ones(200, k, device="cuda").to(ref.E4M3)
+    xs, ws = torch.ones(m, g, device="cuda"), torch.ones(2, g, device="cuda")
+    ws[1, -1] = math.inf
+    got = fp8_linear(x, w, ws, x_scale=xs)
+    assert bool((got[:, 128:] == math.inf).all()) and bool((got[:, :128] == k).all())
+    assert torch.equal(fp8_linear(torch.ones(m, k, dtype=torch.bfloat16, device="cuda"), w, ws).isinf(), got.isinf())
+    xs[0, -1], ws[1, -1] = math.inf, 1.0
+    got = fp8_linear(x, w, ws, x_scale=xs)
+    assert bool((got[0] == math.inf).all()) and bool((got[1:] == k).all())
+
+
+def test_one_row_whose_values_lie_apart():
+    x = ref.states(1, 1024, gen(5)).cuda()[0]
+    for a, b in zip(fp8_quantize(x[::2]), fp8_quantize(x[::2].contiguous())):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    w, ws = (t.cuda() for t in ref.weight(256, 512, gen(6)))
+    assert torch.equal(fp8_linear(x[::2], w, ws), fp8_linear(x[::2].contiguous(), w, ws))
+    assert torch.equal(fp8_linear(x[:512].expand(3, 512), w, ws), fp8_linear(x[:512].repeat(3, 1), w, ws))
+
+
 def test_groups_of_next_to_nothing_and_of_very_much():
     x = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
     x[0, :128], x[0, 128:256], x[0, 256:384] = 1e-39, 2.0 ** -100, 2.0 ** -101

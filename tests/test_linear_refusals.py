@@ -69,6 +69,9 @@ wrong = {
     "combine: weights": lambda: U.combine_experts(bf(6, 64), plan.positions, f32(3, 3)),
     "combine: type of weights": lambda: U.combine_experts(bf(6, 64), plan.positions, bf(3, 2)),
     "combine: type of positions": lambda: U.combine_experts(bf(6, 64), plan.positions.long(), f32(3, 2)),
+    "moe: other tokens": lambda: U.moe_experts(x, i32(2, 2), f32(2, 2), ew, es, f8(4, 256, 256), f32(4, 2, 2)),
+    "moe: weights": lambda: U.moe_experts(x, i32(3, 2), f32(3, 1), ew, es, f8(4, 256, 256), f32(4, 2, 2)),
+    "moe: width": lambda: U.moe_experts(x, i32(3, 2), f32(3, 2), ew, es, f8(4, 128, 256), f32(4, 1, 2)),
     "combine: residual": lambda: U.combine_experts(bf(6, 64), plan.positions, f32(3, 2), bf(2, 64)),
 }
 for name, call in wrong.items():

@@ -155,7 +155,7 @@ struct Rows {
     cols = in.size(-1);
     for (int64_t i = 0; i + 1 < in.dim(); ++i) rows *= in.size(i);
     stride = cols;
-    bool even = in.dim() == 1 || cols == 0 || in.stride(-1) == 1;
+    bool even = cols <= 1 || in.stride(-1) == 1;
     if (in.dim() >= 2 && rows > 1) {
       // the leading dimensions have to be one
       int64_t expected = -1;

@@ -131,11 +131,10 @@ extern "C" int mono_lin_product(const uint8_t* codes, const float* scales, int64
   p.rows = p.x_rows = rows;
   p.n = n; p.k = k; p.experts = 1;
   p.fp32 = out_fp32;
-  p.after = after_quantize;
   if (const int rc = check(p, weight)) return rc;
   if (rows == 0) return 0;
   const Choice c = dense(p);
-  if (!c.tile) p.after = 0;
+  p.after = after_quantize && c.tile;        // the kernel of many rows is launched when that one has ended
   return run(p, weight, c, stream);
 }
 

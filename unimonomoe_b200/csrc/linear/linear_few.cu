@@ -164,7 +164,7 @@ __device__ __forceinline__ void quantise_rows(const Product& p, Control<Tile, Ga
       const uint4 c = codes16(v, scale.inverse);
       const uint32_t words[4] = {c.x, c.y, c.z, c.w};
       st_shared_128(base + s * S::Stage + S::Pieces * kPiece + (j * Tile + row) * 128 + ((lane8 ^ (row & 7)) << 4), words);
-      if (lane8 < S::Halves) C.scale[s][Gate ? lane8 : j][row] = scale.scale * __ldg(ws + static_cast<int64_t>(lane8) * (p.blocks / 2) * p.groups + of);
+      if (lane8 < S::Halves) C.scale[s][Gate ? lane8 : j][row] = t0 * S::Groups + g < p.groups ? scale.scale * __ldg(ws + static_cast<int64_t>(lane8) * (p.blocks / 2) * p.groups + of) : 0.0f;
     }
   }
   fence_proxy_async_smem();                  // the tensor core reads what was stored here
@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       const uint8_t* src[kEach];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) src[i] = p.x + row(r0 + 8 * i) * p.k;
-      // Scales: a row (or two) of x a thread, two stages ahead in registers. Behind the last group the sums are zero, times any scale of the row.
+      // Scales: a row (or two) of x a thread, two stages ahead in registers. Behind the last group the sums are zero, and so are the scales:
+      // the last ones may be infinite.
       const float* xs[kOwn];
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) xs[i] = p.xs + row(t_ + 64 * i) * p.groups;
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
           for (int j = 0; j < S::Pieces; ++j)
 #pragma unroll
             for (int i = 0; i < kOwn; ++i)
-              if (t_ + 64 * i < Tile) C.scale[slot][j][t_ + 64 * i] = x[from][Gate ? 0 : j][i] * wt[from][j];
+              if (t_ + 64 * i < Tile) C.scale[slot][j][t_ + 64 * i] = Gate || t * S::Groups + j < p.groups ? x[from][Gate ? 0 : j][i] * wt[from][j] : 0.0f;
           fetch(t + 2, from);
         };
         if ((t - t0) & 1) put(1); else put(0);

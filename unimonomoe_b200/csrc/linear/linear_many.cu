@@ -260,7 +260,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     }
   } else {
     reg_inc<kRegsReader>();
-    wait_for_launch_before();
     const int quarter = warp & 3, half = (warp - kFirstReader) >> 2;
     const uint32_t staging = base + kStages * kStage + (warp - kFirstReader) * kStaging;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
