@@ -1,6 +1,8 @@
 // Weighted sum of each token's results: out[t] = sum_j w[t, j] * partial[position[t, j]] (+ residual), in fp32 in the order of j.
 //
-// Eight columns a thread; a token's rows are requested together, up to eight at a time. Bound by memory: every row is read once.
+// Eight columns a thread; a token's rows are requested together, up to eight at a time. Bound by memory, every row is read once: 16384 tokens of 8
+// rows of 2048 in 100 us, 6.0 TB/s. The grid is what runs at once, each thread goes from piece to piece: with 64 CTAs for an SM it took 109 us. (Four
+// columns a thread and more of them: 129. The next piece's positions ahead, for which there are no registers: 109.)
 #include "linear.cuh"
 
 namespace mono {
@@ -8,7 +10,7 @@ namespace {
 
 using namespace lin;
 
-constexpr int kThreads = 256, kAtOnce = 8;
+constexpr int kThreads = 256, kAtOnce = 8, kResident = 3;   // CTAs of an SM, by their registers
 
 struct CombineArgs {
   const uint4 *partial, *residual;
@@ -21,9 +23,15 @@ struct CombineArgs {
 };
 
 __global__ void __launch_bounds__(kThreads) combine_kernel(const CombineArgs a) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < a.items; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t t = i / a.vecs;
-    const int v = static_cast<int>(i - t * a.vecs);
+  const int at_first = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+  int64_t i = at_first, t = at_first / a.vecs;
+  int v = at_first % a.vecs;
+  const int tokens = step / a.vecs, vecs = step - tokens * a.vecs;
+  for (; i < a.items; i += step, t += tokens, v += vecs) {
+    if (v >= a.vecs) {
+      v -= a.vecs;
+      ++t;
+    }
     float2 sum[4] = {};
     for (int j0 = 0; j0 < a.top; j0 += kAtOnce) {
       uint4 row[kAtOnce];
@@ -76,7 +84,7 @@ extern "C" int mono_lin_combine(const void* partial, int64_t rows, const int32_t
   if ((reinterpret_cast<uintptr_t>(partial) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(out)) & 15) return MONO_LIN_ALIGNMENT;
   CombineArgs a{static_cast<const uint4*>(partial), static_cast<const uint4*>(residual), static_cast<uint4*>(out), positions, weights, status, rows,
                 tokens * (cols / 8), top, cols / 8};
-  const int64_t blocks = (a.items + kThreads - 1) / kThreads, most = lin::kSms * 8 * 8;
+  const int64_t blocks = (a.items + kThreads - 1) / kThreads, most = lin::kSms * kResident;
   combine_kernel<<<static_cast<int>(blocks < most ? blocks : most), kThreads, 0, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }

@@ -39,6 +39,8 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 struct Waits {
   uint32_t* stop;                            // of the CTA, in shared memory
   uint32_t* status;
+  // By whole warps.
+  __device__ __forceinline__ bool stopped() const { return __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(stop) != 0u); }
   __device__ __forceinline__ bool gave_up(uint32_t polls, uint64_t& since) const {
     if ((polls & 63u) != 0u) return false;
     volatile uint32_t* s = stop;
@@ -152,16 +154,11 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* p, float2 (&v)[8]) {
   unpack16(__ldg(reinterpret_cast<const uint4*>(p)), __ldg(reinterpret_cast<const uint4*>(p) + 1), v);
 }
 // Largest magnitude (as bits, a NaN's above all) of a group that eight neighbouring lanes share, 16 values each. All lanes of the warp take part.
-// The maximum passes over what is not a number; that is found by products with zero.
 __device__ __forceinline__ uint32_t top_of_group(const float2 (&v)[8]) {
   float top = 0.0f;
-  float2 zero = both(0.0f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-    zero = fma2(v[i], both(0.0f), zero);
-  }
-  uint32_t m = zero.x + zero.y == 0.0f ? __float_as_uint(top) : 0x7FC00000u;
+  for (int i = 0; i < 8; ++i) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v[i].x), "f"(v[i].y));
+  uint32_t m = __float_as_uint(top);
 #pragma unroll
   for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
   return m;
@@ -260,21 +257,44 @@ struct Division {
   // Unit u. Experts' units follow one another along n, so that a weight is read once for the row tiles of its run; those of one
   // dense product are taken in bands of eight row tiles, whose rows and the weight's both stay in L2.
   __device__ __forceinline__ Run unit(int u) const {
-    Run r;
     if (p.offsets) {
       const int tile = u / p.cols;
-      r.col = u - tile * p.cols;
       int lo = 0, hi = p.experts;            // first[lo] <= tile < first[hi]
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (first[mid] <= tile) lo = mid; else hi = mid;
       }
-      const int a = __ldg(p.offsets + lo), b = __ldg(p.offsets + lo + 1);
-      r.expert = lo;
-      r.row = a + (tile - first[lo]) * Tile;
-      r.rows = max(0, min(Tile, b - r.row));
-      return r;
+      return of_expert(lo, tile, u - tile * p.cols);
     }
+    return of_rows(u);
+  }
+  // The same by a whole warp that takes its units in order; `lo` is the expert of the one before, 0 at first.
+  __device__ __forceinline__ Run unit_after(int u, int& lo) const {
+    if (p.offsets) {
+      const int tile = u / p.cols, lane = threadIdx.x & 31;
+      int n;
+      do {
+        const int e = lo + 1 + lane;
+        n = __popc(__ballot_sync(0xFFFFFFFFu, e < p.experts && first[e] <= tile));
+        lo += n;
+      } while (n == 32);
+      return of_expert(lo, tile, u - tile * p.cols);
+    }
+    return of_rows(u);
+  }
+
+ private:
+  __device__ __forceinline__ Run of_expert(int e, int tile, int col) const {
+    const int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
+    Run r;
+    r.expert = e;
+    r.col = col;
+    r.row = a + (tile - first[e]) * Tile;
+    r.rows = max(0, min(Tile, b - r.row));
+    return r;
+  }
+  __device__ __forceinline__ Run of_rows(int u) const {
+    Run r;
     constexpr int kBand = 8;
     const int band = u / (kBand * p.cols), high = min(kBand, row_tiles() - band * kBand), in = u - band * kBand * p.cols;
     r.expert = 0;
