@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const Division<Tile> division(p, C.first);
   const int units = division.units();
   const Run at_first = u0 < units ? division.unit(u0) : Run{};         // all warps': code that each of them would have to fetch for itself
-  auto unit = [&](int u) { return u == u0 ? at_first : division.unit(u); };
+  int expert = at_first.expert;
+  auto unit = [&](int u) { return u == u0 ? at_first : division.unit_after(u, expert); };
   // Stage s gets the pieces of step t of unit r; the n-th use of the ring.
   auto request = [&](const Run& r, int t, uint32_t s) {
     const uint32_t at = base + s * S::Stage;
@@ -233,23 +234,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   if (p.raw != nullptr && warp >= 2 && u0 < units) quantise_rows<Tile, Gate>(p, C, at_first, base, t0, t1);
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t n = 0;
-      for (int u = u0; u < units; u += step) {
-        if (static_cast<int>(n) + t1 - t0 <= early) {         // all of it is requested
-          n += t1 - t0;
-          continue;
-        }
-        const Run r = unit(u);
-        for (int t = t0; t < t1; ++t, ++n) {
-          if (static_cast<int>(n) < early) continue;
-          const uint32_t s = n % S::Stages;
+    uint32_t before = 0;                     // stages of the units before
+    for (int u = u0; u < units; u += step, before += t1 - t0) {
+      const int first = u == u0 ? early : 0;
+      if (first == t1 - t0) continue;        // all of it is requested
+      const Run r = unit(u);
+      if (lane == 0)
+        for (int t = t0 + first; t < t1; ++t) {
+          const uint32_t n = before + t - t0, s = n % S::Stages;
           waits.wait_lane(&C.done[s], (n / S::Stages & 1) ^ 1);
           request(r, t, s);
         }
-      }
+      __syncwarp();
     }
-    __syncwarp();
   } else if (warp == 1) {
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {

@@ -7,6 +7,8 @@
 // scale, or the gate's and the other half's). Sixteen warps, one CTA to an SM:
 //   0     requests weights, and rows of x where they lie in order
 //   1, 2  issue the products, a half of the columns each
+//   3     finds the units, some ahead: the others read them from shared memory (found by each role for itself a unit cost 1600 cycles, as much as
+//         two groups of K)
 //   4-7   bring the scales, some groups ahead, and rows of x that lie anywhere (tokens), by cp.async with the 128-byte swizzle
 //         written by hand
 //   8-15  read the sums, a half of the columns each four; write the results, through shared memory by tensor stores
@@ -19,9 +21,10 @@ namespace {
 using namespace lin;
 
 constexpr int kThreads = 512, kLoaders = 128, kReaders = 8, kRows = 128, kTile = 256;
-constexpr int kMma = 1, kFirstLoader = 4, kFirstReader = 8;   // warps
+constexpr int kMma = 1, kFinder = 3, kFirstLoader = 4, kFirstReader = 8;   // warps
 constexpr int kSums = 4;                      // buffers of 128 columns, two for each half of the tile's
 constexpr int kScales = 8;                   // groups whose scales are on their way or in use
+constexpr int kRuns = 4;                     // units that are found and not yet done with
 constexpr int kBox = 4096, kStaging = 2 * kBox;               // of a reader: 32 rows x 64 columns of bf16, twice
 // Registers of a thread: at launch, of the first eight warps, of the readers. The readers' share comes from what the others give back.
 constexpr int kRegs = 65536 / kThreads, kRegsOther = 48, kRegsReader = 208;
@@ -30,7 +33,8 @@ static_assert(8 * kRegsOther + 8 * kRegsReader <= 16 * kRegs, "a wait for regist
 constexpr int kX = kRows * kGroup, kPart = 128 * kGroup, kStage = kX + 2 * kPart, kStages = 3;   // bytes of x, of a half of the weight's rows
 
 struct Control {
-  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales];
+  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales], found[kRuns], taken[kRuns];
+  Run runs[kRuns];
   uint32_t tmem, stop;
   int sums[32];
   uint32_t top[2][kRows];
@@ -162,6 +166,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       mbar_init(&C.s_full[i], kLoaders);
       mbar_init(&C.s_empty[i], kReaders);
     }
+    for (int i = 0; i < kRuns; ++i) {
+      mbar_init(&C.found[i], 1);
+      mbar_init(&C.taken[i], 1 + kLoaders / 32 + kReaders);
+    }
     mbar_init_fence();
     C.stop = 0;
   }
@@ -177,14 +185,24 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   const Division<kRows> division(p, C.first);
   const int units = division.units(), step = gridDim.x, u0 = blockIdx.x;
   const uint32_t base = smem_u32(stages);
+  // The next unit of this CTA; one without rows in a launch that gave up, where what is in memory may be half of another.
+  uint32_t nth = 0;
+  auto take = [&]() {
+    const uint32_t slot = nth % kRuns;
+    waits.wait(&C.found[slot], nth++ / kRuns & 1);
+    const Run r = C.runs[slot];
+    if (waits.stopped()) return Run{};
+    if (lane == 0) mbar_arrive(&C.taken[slot]);
+    return r;
+  };
 
   if (warp < kFirstReader) {
     reg_dec<kRegsOther>();
     if (warp == 0) {
-      if (lane == 0) {
-        uint32_t n = 0;
-        for (int u = u0; u < units; u += step) {
-          const Run r = division.unit(u);
+      uint32_t n = 0;
+      for (int u = u0; u < units; u += step) {
+        const Run r = take();
+        if (lane == 0) {
           for (int g = 0; g < p.groups; ++g, ++n) {
             const uint32_t s = n % kStages, at = base + s * kStage;
             waits.wait_lane(&C.empty[s], (n / kStages & 1) ^ 1);
@@ -196,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
             if (!gather) tma_load_2d(&rows, g * kGroup, static_cast<uint32_t>(r.row), stages + s * kStage, &C.full[s]);
           }
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else if (warp < kMma + 2) {
       constexpr uint32_t idesc = umma_idesc_e4m3_f32(kRows, kTile / 2);
       const uint32_t h = warp - kMma;
@@ -220,12 +238,24 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
           }
           __syncwarp();
         }
-    } else if (warp >= kFirstLoader) {
+    } else if (warp == kFinder) {
+      int expert = 0;
+      for (int u = u0; u < units; u += step, ++nth) {
+        const Run r = division.unit_after(u, expert);
+        const uint32_t slot = nth % kRuns;
+        waits.wait(&C.taken[slot], (nth / kRuns & 1) ^ 1);
+        if (waits.stopped()) break;
+        if (lane == 0) {
+          C.runs[slot] = r;
+          mbar_arrive(&C.found[slot]);
+        }
+      }
+    } else {
       const int t = threadIdx.x - 32 * kFirstLoader, chunk = t & 7, r0 = t >> 3;
       constexpr int kEach = kRows / (kLoaders / 8);           // rows of a thread, sixteen apart
       uint32_t n = 0;
       for (int u = u0; u < units; u += step) {
-        const Run r = division.unit(u);
+        const Run r = take();
         // Rows past the unit's are left as they are, nobody reads what comes of them. (One row for all of them would be asked for by
         // every CTA at once: 174 us instead of 113 for 2048 tokens through 256 experts' up projection.)
         auto row = [&](int i) { return i < r.rows ? source_row(p, r.row + i) : 0; };
@@ -265,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
-      const Run r = division.unit(u);
+      const Run r = take();
       const int in = quarter * 32, mine = max(0, min(32, r.rows - in));   // rows of this warp
       const int64_t row0 = static_cast<int64_t>(r.row) + in;
       float2 acc[2][32] = {};
