@@ -15,6 +15,12 @@
 // The groups of K may be divided among the CTAs of a cluster. Each then hands its sums to the CTA that finishes the row, by stores into its
 // shared memory that its barrier counts, and they are added in the order of the CTAs: the result does not depend on timing. Without
 // that a CTA goes from unit to unit, and the weight's requests run ahead across them.
+//
+// Bound by latency where there is one unit to a CTA: a launch, a division, the first bytes of the weight, its stages, the join and the results follow
+// one another. In a graph 1 row of 2048 to 5120 columns takes 6.0 us (without the join's clusters, eight stages one after another, 8.2), 61 rows of 4096 to 2048 8.3;
+// bound by memory where experts are many: the gated up projection of 24 tokens through 256 experts reads 275 MB in 46.5 us, 5.9 TB/s, the down projection
+// of 64 tokens 233 MB in 42. A tile is as wide as the rows ask for: of 16 a stage takes 360 ns, of 64 600, and the room for its
+// rows of x is room that the ring loses. The sums' way out by bf16 and tensor stores, as in the kernel of many rows, made 201 us of 184 where runs are of 60 rows.
 #include "linear.cuh"
 #include "../pair_sm100.cuh"
 
@@ -79,8 +85,7 @@ __device__ __forceinline__ void tma_weight(const CUtensorMap* m, int k, int row,
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(k), "r"(row), "r"(expert), "r"(smem_u32(bar)) : "memory");
 }
 // Rows [lo, hi) of a unit, whose sums lie in this CTA's shared memory, those of CTA c of the cluster at [c][half][row - lo] of rows
-// of 128: a warp has one row at a time, a lane four of its columns.
-// Two rows in flight.
+// of 128: a lane has four columns, a warp two rows at a time.
 template <bool Gate, bool Split>
 __device__ __forceinline__ void finish(const Product& p, const Run& r, const float* sums, int split, int each, int lo, int hi, int w, int lane) {
   constexpr int kHalves = Gate ? 2 : 1, kWarps = kReaders / 32, kAtOnce = 2;

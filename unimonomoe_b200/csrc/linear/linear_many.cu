@@ -13,6 +13,15 @@
 //         written by hand
 //   8-15  read the sums, a half of the columns each four; write the results, through shared memory by tensor stores
 // With the gated activation a tile is 128 rows of the gate's half of the weight and the matching 128 of the other.
+//
+// Bound by the readers: of a group's 128 x 256 sums each has to be read from tensor memory, multiplied by its scale and added, some 920 cycles
+// with the waits between, while the products take 512; the tensor pipe is busy half of the time. Around the groups of a unit lie 2900 cycles (first
+// sums, results), 5400 with the gated activation, whose exponentials and quotients take the most of it. Measured: 16384 x 7168 x 4096 in 478-490 us (2.0
+// PFLOP/s; under the power cap 535-547), 4096 x 2048 x 4096 in 50 (1.4), 8192 x 7168 x 4096 gated in 240-250; 256 experts' gated up projection (K 2048, N 1024) of 16384
+// tokens in 414-440 (1.25-1.33), their down projection (K 512, N 2048) in 257 (1.07), of 3000 tokens unevenly routed in 85, where weights and results alone take 58.
+// Tiles of 256 x 256 by pairs of CTAs took 502 us for the first, for the gated up projection 457; twenty warps, sixteen of them readers with
+// half the registers each, 580; one warp that issues for both halves, four stages with less room for results, and bands of sixteen
+// row tiles made no difference or a worse one.
 #include "linear.cuh"
 
 namespace mono {
