@@ -1,9 +1,9 @@
-"""A small decoder that serves: whole layers made of this package's parts, the attention of attention.py over a paged
-4-bit cache, the projections of linear.py around it and the MoE launch of loader.py, on one GPU.
+"""A small decoder that serves: whole layers made of this package's two halves, the attention of attention.py over a paged
+4-bit cache and the MoE launch of loader.py, on one GPU.
 
 Requests of ragged lengths are prefilled in chunks under a token budget, then decoded together, one captured CUDA graph a step.
-Weights are random (synth.py; width and experts of its first geometry), projections in block FP8 as the experts; router and embedding are
-plain library products. With --operators the experts are those of linear.py too, which take any geometry, instead of the one launch.
+Weights are random (synth.py; width and experts of its first geometry), projections and the embedding are plain library products. With --fp8 the
+projections are held in block FP8 as the experts are and computed by linear.py; with --operators its experts, which take any geometry, stand in for the one launch.
 
     python examples/decoder_layers.py --layers 2 --prompts 700 33 1500 --budget 1024 --new 32
 """
@@ -32,7 +32,7 @@ class Layer:
     """norm, q/k/v projection, norm and rotation of heads with the store into the cache, attention, output projection; norm,
     router, routed and shared experts in one launch."""
 
-    def __init__(self, moe: Optional[MonoKernel], pages: int, page_size: int, seed: int, device):
+    def __init__(self, moe: Optional[MonoKernel], pages: int, page_size: int, seed: int, device, fp8: bool = False):
         spec = synth.QWEN
         gen = torch.Generator(device=device).manual_seed(1000 + seed)
 
@@ -42,26 +42,30 @@ class Layer:
         self.moe, self.cache = moe, KV4Cache.empty(pages, KV_HEADS, HEAD_DIM, page_size, device)
         self.norms = weight(2, spec.hidden, mean=1.0)
         self.q_norm, self.k_norm = weight(HEAD_DIM, mean=1.0), weight(HEAD_DIM, mean=1.0)
-        self.qkv = synth.quantize_block_fp8(weight((HEADS + 2 * KV_HEADS) * HEAD_DIM, spec.hidden))
-        self.o = synth.quantize_block_fp8(weight(spec.hidden, HEADS * HEAD_DIM))
+        self.qkv = weight((HEADS + 2 * KV_HEADS) * HEAD_DIM, spec.hidden)
+        self.o = weight(spec.hidden, HEADS * HEAD_DIM)
+        self.fp8 = fp8
+        if fp8:
+            self.qkv, self.o = synth.quantize_block_fp8(self.qkv), synth.quantize_block_fp8(self.o)
         self.experts = synth.make_layer(spec, seed=seed, device=device)
         self.router = self.experts["router_w"].to(torch.bfloat16)
         sh = self.experts["shared"]
         self.shared = prepare_shared_expert(sh["w13"], sh["w13_scale"], sh["w2"], sh["w2_scale"], sh["gate"])
 
     def attention(self, x, plan, table, cos_sin, longest):
-        qkv = fp8_linear(F.rms_norm(x, x.shape[-1:], self.norms[0], 1e-6), *self.qkv).unflatten(1, (-1, HEAD_DIM))
+        y = F.rms_norm(x, x.shape[-1:], self.norms[0], 1e-6)
+        qkv = (fp8_linear(y, *self.qkv) if self.fp8 else F.linear(y, self.qkv)).unflatten(1, (-1, HEAD_DIM))
         q, k, v = qkv[:, :HEADS], qkv[:, HEADS:HEADS + KV_HEADS], qkv[:, HEADS + KV_HEADS:]
         q = qk_norm_rope(q, k, self.q_norm, self.k_norm, cos_sin, plan.positions, v=v, cache=self.cache, slots=plan.slots)
         return kv4_attention(q, self.cache, table, plan.seq_lens, plan.query_start, longest)
 
     def __call__(self, x, plan, table, cos_sin, longest):
-        x = fp8_linear(self.attention(x, plan, table, cos_sin, longest).flatten(1), *self.o, residual=x)
+        a = self.attention(x, plan, table, cos_sin, longest).flatten(1)
+        x = fp8_linear(a, *self.o, residual=x) if self.fp8 else x + F.linear(a, self.o)
         y, w = F.rms_norm(x, x.shape[-1:], self.norms[1], 1e-6), self.experts
         if self.moe is None:
             return self.by_operators(y, residual=x)
         return x + self.moe.prefill(y, F.linear(y, self.router), w["w13"], w["w13_scale"], w["w2"], w["w2_scale"], shared=self.shared)
-
 
     def by_operators(self, y, residual):
         """Routed and shared experts of ``y`` by the operators of linear.py, and ``residual``."""
@@ -76,11 +80,12 @@ class Layer:
 class Server:
     """Layers with one page pool. All lengths and tables stay on the GPU; a step reads nothing back but its tokens."""
 
-    def __init__(self, layers: int, batch: int, context: int, page_size: int = 16, vocabulary: int = 8192, device="cuda", operators: bool = False):
+    def __init__(self, layers: int, batch: int, context: int, page_size: int = 16, vocabulary: int = 8192, device="cuda", fp8: bool = False,
+                 operators: bool = False):
         self.device, self.batch, self.page_size = torch.device(device), batch, page_size
         width = -(-context // page_size)
         moe = None if operators else MonoKernel(variant_path("qwen_w1"))
-        self.layers = [Layer(moe, batch * width, page_size, i, device) for i in range(layers)]
+        self.layers = [Layer(moe, batch * width, page_size, i, device, fp8) for i in range(layers)]
         gen = torch.Generator(device=device).manual_seed(7)
         self.embedding, self.head = torch.randn(2, vocabulary, synth.QWEN.hidden, generator=gen, device=device).to(torch.bfloat16)
         angle = torch.arange(context, device=device, dtype=torch.float64)[:, None] * 1e6 ** (-torch.arange(0, ROTARY, 2, device=device, dtype=torch.float64) / ROTARY)
@@ -149,9 +154,10 @@ def main() -> None:
     p.add_argument("--prompts", type=int, nargs="+", default=[700, 33, 1500], help="their lengths")
     p.add_argument("--budget", type=int, default=1024, help="tokens of a prefill step")
     p.add_argument("--new", type=int, default=32, help="tokens to decode for each request")
+    p.add_argument("--fp8", action="store_true", help="projections in block FP8 by linear.py instead of library products")
     p.add_argument("--operators", action="store_true", help="experts by the operators of linear.py instead of the one launch")
     args = p.parse_args()
-    server = Server(args.layers, len(args.prompts), max(args.prompts) + args.new, operators=args.operators)
+    server = Server(args.layers, len(args.prompts), max(args.prompts) + args.new, fp8=args.fp8, operators=args.operators)
     gen = torch.Generator(device="cuda").manual_seed(11)
     prompts = [torch.randint(0, len(server.embedding), (n,), generator=gen, device="cuda") for n in args.prompts]
 
@@ -165,7 +171,8 @@ def main() -> None:
     first, prefill_ms = timed(server.prefill, prompts, args.budget)
     more, decode_ms = timed(server.decode, first, args.new)
     check_status()
-    linear.check_status()
+    if args.fp8 or args.operators:
+        linear.check_status()
     print(f"prefilled {sum(args.prompts)} tokens in {prefill_ms:.1f} ms, decoded {args.new} x {len(prompts)} in {decode_ms:.1f} ms (both with first-call set-up)")
     for b, n in enumerate(args.prompts):
         print(f"  request {b}: {n} tokens, then {[int(first[b])] + more[b, :7].tolist()} ...")

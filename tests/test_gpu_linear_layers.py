@@ -43,7 +43,7 @@ def test_the_decoder_by_operators(linear_lib, attention_lib):
     prompts = [torch.randint(0, 8192, (n,), generator=gen, device="cuda") for n in (30, 1, 200)]
     last = []
     for operators in (False, True):
-        server = decoder_layers.Server(2, 3, 260, operators=operators)
+        server = decoder_layers.Server(2, 3, 260, fp8=True, operators=operators)
         states, inner = [], server.step
         server.step = lambda *a, inner=inner, states=states: states.append(inner(*a)) or states[-1]
         first = server.prefill(prompts, 231)
