@@ -176,6 +176,12 @@ __device__ __forceinline__ uint4 codes16(const float2 (&v)[8], float inverse) {
 
 // ---- launches one after another without a gap
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Of what that launch writes: stays behind the wait, where a load that counts on memory that nobody writes might be moved in front of it.
+__device__ __forceinline__ float ld_after(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ void let_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- products

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         for (int j = 0; j < S::Groups; ++j) {
           const int g = min(t * S::Groups + j, p.groups - 1);
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i) x[into][j][i] = __ldg(xs[i] + g);
+          for (int i = 0; i < kOwn; ++i) x[into][j][i] = ld_after(xs[i] + g);
           wt[into][j] = __ldg(ws + g);
           if constexpr (Gate) wt[into][1] = __ldg(ws2 + g);
         }
