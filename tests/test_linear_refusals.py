@@ -27,6 +27,9 @@ wrong = {
     "quantize: no columns": lambda: U.fp8_quantize(bf(3, 0)),
     "quantize: halves": lambda: U.fp8_quantize(bf(3, 33), silu_mul=True),
     "quantize: columns of a half": lambda: U.fp8_quantize(bf(3, 48), silu_mul=True),
+    "quantize: sparse": lambda: U.fp8_quantize(x.to_sparse()),
+    "quantize: negative in memory": lambda: U.fp8_quantize(torch._neg_view(x)),
+    "combine: negative in memory": lambda: U.combine_experts(bf(6, 64), plan.positions, torch._neg_view(f32(3, 2))),
     "linear: type": lambda: U.fp8_linear(x.half(), w, ws),
     "linear: type of the weight": lambda: U.fp8_linear(x, w.to(torch.bfloat16), ws),
     "linear: other 8 bits": lambda: U.fp8_linear(x, w.view(torch.float8_e5m2), ws),

@@ -42,6 +42,7 @@ int size32(int64_t v, const char* name) {
 }
 void on_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " is on ", t.device(), "; these operators need a CUDA device, there is no CPU path");
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), name, " is sparse, or a view whose memory holds the negative");
 }
 void typed(const Tensor& t, const char* name, at::ScalarType type, c10::Device device) {
   on_gpu(t, name);
