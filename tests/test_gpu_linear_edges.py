@@ -101,6 +101,27 @@ def test_one_row_whose_values_lie_apart():
     assert torch.equal(fp8_linear(x[:512].expand(3, 512), w, ws), fp8_linear(x[:512].repeat(3, 1), w, ws))
 
 
+def test_gates_of_every_size():
+    """Every finite value as the gate of 1 and of 2^60, one to a group, so that its scale shows the product: off by the roundings of the exponential
+    (2 + 1.2 |a| units of 2^-24 at most), the sum, quotient, product and scale (8 units); below -88.72 it is nothing, however large a and b are."""
+    a = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    a = a[torch.isfinite(a)]
+    for b in (1.0, 2.0 ** 60):
+        x = torch.zeros(len(a), 256, dtype=torch.bfloat16)
+        x[:, 0], x[:, 128] = a, b
+        m = fp8_quantize(x.cuda(), silu_mul=True)[1][:, 0].double().cpu() * 448
+        v = (a.double() * torch.sigmoid(a.double()) * b).abs()
+        plain = (a > -88.5) & (v > 2.0 ** -99) & (v < 2.0 ** 127)
+        assert bool(((m - v).abs()[plain] <= (v * (10 + 1.2 * a.double().abs().clamp(max=90)) * 2.0 ** -24)[plain]).all())
+        assert bool(((m - 1).abs()[(a < -88.72) | (v < 2.0 ** -101)] <= ref.HALF32).all())          # 1 / 448, rounded, times 448
+    x[:, 128] = 3e38
+    a = a[a < -88.72]
+    x = x[:len(a)]
+    x[:, 0] = a
+    m = fp8_quantize(x.cuda(), silu_mul=True)[1][:, 0].double() * 448
+    assert bool(((m - 1).abs() <= ref.HALF32).all())
+
+
 def test_groups_of_next_to_nothing_and_of_very_much():
     x = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
     x[0, :128], x[0, 128:256], x[0, 256:384] = 1e-39, 2.0 ** -100, 2.0 ** -101

@@ -4,8 +4,8 @@
 // Eight lanes share a group, 16 values (32 bytes) a lane: the largest magnitude takes three exchanges, a lane writes 16 codes at once. Each thread goes
 // from group to group, the next one's values on their way while one is quantised, its place by additions: with a division of 64 bits for
 // each and no values ahead 16384 x 7168 took 67.6 us, with eight CTAs to an SM one after another. Bound by memory, 2 bytes in and 1 out for a value: 59.6 us there, 5.9 TB/s.
-// With silu 4 bytes in, and bound by the instructions of an exponential and a quotient that are right to fp32's last bits (gated() has the reason):
-// 131072 rows of 512 in 64.9 us, 5.2 TB/s. One row of 2048 takes what a launch takes.
+// With silu 4 bytes in, and bound by the instructions of an exponential and a quotient to fp32's precision (gate16() has the reason):
+// 131072 rows of 512 in 65.7 us, 5.1 TB/s. One row of 2048 takes what a launch takes.
 #include "linear.cuh"
 
 namespace mono {
@@ -55,10 +55,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
       ++row;
     }
     fetch();
-    if constexpr (Silu) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = gated(v[i], u[i]);
-    }
+    if constexpr (Silu) gate16(v, u);
     const GroupScale g(top_of_group(v));
     if (mine) *reinterpret_cast<uint4*>(a.codes + to) = codes16(v, g.inverse);
     if (have && sub == 0) a.scales[at] = g.scale;

@@ -116,15 +116,30 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 minus(float2 a) { return make_float2(-a.x, -a.y); }
-// silu(a) * b to fp32's precision, two at a time: with the fast exponential and quotient one code in 10^5 is another. The quotient is made of a
-// reciprocal with one step of Newton's method and a correction by its exact residual (Markstein, 1990), which is the rounded quotient for
-// the denominators here, from 1 up; one that is infinite or nearly so is cut, where the result is below 2^-100 in any case.
-__device__ __forceinline__ float2 gated(float2 a, float2 b) {
-  const float2 d = make_float2(fminf(1.0f + expf(-a.x), 0x1p120f), fminf(1.0f + expf(-a.y), 0x1p120f));
-  float2 r = make_float2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y));
-  r = fma2(fma2(minus(d), r, both(1.0f)), r, r);
-  const float2 q = mul2(a, r);
-  return mul2(fma2(fma2(minus(q), d, a), r, q), b);
+// exp(-a) of a from -88.72 to 90 is 2^t, t = -a log2(e): of the rounded product, and what rounding it lost put back by 1 + rest ln(2). (That alone is up
+// to |t| 2^-24 of the result.) Arguments outside are cut to that.
+__device__ __forceinline__ float2 exp_minus(float2 a) {
+  constexpr float kLog2E = 0x1.715476p+0f, kLog2ERest = 0x1.4ae0cp-26f, kLn2 = 0x1.62e43p-1f;
+  const float2 m = make_float2(fminf(fmaxf(-a.x, -90.0f), 88.72f), fminf(fmaxf(-a.y, -90.0f), 88.72f)), t = mul2(m, both(kLog2E));
+  const float2 rest = fma2(m, both(kLog2ERest), fma2(m, both(kLog2E), minus(t)));
+  const float2 e = make_float2(ex2_approx_ftz(t.x), ex2_approx_ftz(t.y));
+  return fma2(e, mul2(rest, both(kLn2)), e);
+}
+// silu(a) * b into a, to fp32's precision: with the fast exponential and quotient one code in 10^5 is another. The quotient is made of a reciprocal
+// with one step of Newton's method and a correction by its exact residual (Markstein, 1990), which is the rounded quotient; a sixteenth of both
+// sides, so that the reciprocal of the largest exponential is a normal number. Below -88.72, where the exponential is infinite, the quotient is zero, for
+// an infinite a NaN. (65.7 us for 131072 x 512; with expf, and the same to a step in its last place, 69.9.)
+__device__ __forceinline__ void gate16(float2 (&a)[8], const float2 (&b)[8]) {
+  constexpr float kLeast = -88.72f, kSixteenth = 0.0625f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 d = fma2(exp_minus(a[i]), both(kSixteenth), both(kSixteenth));
+    const float2 n = mul2(a[i], make_float2(a[i].x < kLeast ? 0.0f : kSixteenth, a[i].y < kLeast ? 0.0f : kSixteenth));
+    float2 r = make_float2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y));
+    r = fma2(fma2(minus(d), r, both(1.0f)), r, r);
+    const float2 q = mul2(n, r);
+    a[i] = mul2(fma2(fma2(minus(q), d, n), r, q), b[i]);
+  }
 }
 // The same of a product's sums, which are themselves off by more than the fast exponential and division are. Where exp(-a) is infinite
 // or close to it (a under -87) the quotient is -0.
