@@ -45,16 +45,16 @@ bool map_out(CUtensorMap* m, void* base, uint64_t n, uint64_t rows) {
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// What things take, in ns, about: a launch; a stage of the kernel of few rows, a unit of it around its stages, joining the CTAs of a cluster; a
-// group of K of a tile of the kernel of many, and a unit of it. What is chosen by them was timed against each kernel and tile by
-// itself: 427 products, dense and of 8 to 256 experts, N from 256 to 9216, K from 512 to 7168, 1 to 2048 rows or 6000 tokens, routed evenly and not. It
-// takes 0.8% more than the fastest, on average; always the tile of 16, 32 or 64 rows, or the kernel of many, 45%, 24%, 27%, 29%.
-constexpr int64_t kStart = 2500, kJoin = 1500, kManyGroup = 490, kManyUnit = 1500, kManyGate = 1200;
+// What things take, in ns, about: a launch; a stage of the kernel of few rows, a unit of it around its stages, joining the CTAs of a cluster, for each
+// row of the tile too; a group of K of a tile of the kernel of many, and a unit of it. What is chosen by them was timed against each kernel
+// and tile by itself: 427 products, dense and of 8 to 256 experts, N from 256 to 9216, K from 512 to 7168, 1 to 2048 rows or 6000 tokens, routed evenly and not
+// (half of them with each split too). It takes 0.6% more than the fastest, on average; always the tile of 16, 32 or 64 rows, or the kernel of many, 45%, 24%, 27%, 29%.
+constexpr int64_t kStart = 2500, kJoin = 700, kJoinRow = 40, kManyGroup = 500, kManyUnit = 2000, kManyGate = 1200;
 struct Few {
   int tile;
   int64_t stage, unit;
 };
-constexpr Few kFew[3] = {{16, 360, 600}, {32, 400, 800}, {64, 600, 1300}};
+constexpr Few kFew[3] = {{16, 360, 700}, {32, 420, 800}, {64, 620, 1400}};
 
 struct Choice {
   int tile, split;                           // of the kernel of few rows; tile 0: the kernel of many
@@ -74,7 +74,7 @@ Choice choose(const Product& p, bool may_many, int only, Likely likely, Most mos
     if (only && f.tile != only) continue;
     const int64_t units = likely(f.tile) * few_cols, all = most(f.tile) * few_cols;
     for (int split = 1; split <= 8 && split <= steps && (split == 1 || all * split <= kSms); ++split) {
-      const int64_t cost = kStart + div_up(units, few_clusters(split)) * (div_up(steps, split) * f.stage + f.unit / split + (split > 1 ? kJoin : 0));
+      const int64_t cost = kStart + div_up(units, few_clusters(split)) * (div_up(steps, split) * f.stage + f.unit / split + (split > 1 ? kJoin + kJoinRow * f.tile : 0));
       if (cost < best.cost) best = {f.tile, split, split > 1 || all < kSms ? all : kSms, cost};
     }
   }
