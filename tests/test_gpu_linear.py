@@ -73,6 +73,17 @@ def test_linear_many_rows(m, n, k, mode):
     check_linear(m, n, k, 1, mode)
 
 
+@pytest.mark.parametrize("m,n,k", [(256, 2048, 4096), (130, 300, 7168), (500, 1000, 4112), (129, 2057, 6160), (1000, 264, 7168), (256, 4096, 7168)])
+@pytest.mark.parametrize("mode", ["plain", "residual", "fp32"])
+def test_linear_with_k_divided_among_ctas(m, n, k, mode):
+    check_linear(m, n, k, 9, mode)
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 2048, 7168), (130, 512, 8208), (600, 1024, 4112), (257, 4096, 6160)])
+def test_gated_activation_with_k_divided_among_ctas(m, n, k):
+    check_linear(m, n, k, 10, "silu")
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 256, 128), (1, 1024, 2048), (2, 40960, 400), (32, 512, 2048), (16, 512, 1040), (17, 4096, 512), (33, 768, 1808), (64, 256, 7168), (200, 512, 272), (1500, 1024, 1040),
                                    (2300, 512, 2048)])
 def test_linear_with_gated_activation(m, n, k):

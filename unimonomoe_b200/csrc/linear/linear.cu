@@ -46,10 +46,10 @@ bool map_out(CUtensorMap* m, void* base, uint64_t n, uint64_t rows) {
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // What things take, in ns, about: a launch; a stage of the kernel of few rows, a unit of it around its stages, joining the CTAs of a cluster, for each
-// row of the tile too; a group of K of a tile of the kernel of many, and a unit of it. What is chosen by them was timed against each kernel
+// row of the tile too; a group of K of a tile of the kernel of many, a unit of it, joining its CTAs, each of them. What is chosen by them was timed against each kernel
 // and tile by itself: 427 products, dense and of 8 to 256 experts, N from 256 to 9216, K from 512 to 7168, 1 to 2048 rows or 6000 tokens, routed evenly and not
 // (half of them with each split too). It takes 0.6% more than the fastest, on average; always the tile of 16, 32 or 64 rows, or the kernel of many, 45%, 24%, 27%, 29%.
-constexpr int64_t kStart = 2500, kJoin = 700, kJoinRow = 40, kManyGroup = 500, kManyUnit = 2000, kManyGate = 1200;
+constexpr int64_t kStart = 2500, kJoin = 700, kJoinRow = 40, kManyGroup = 500, kManyUnit = 2000, kManyGate = 1200, kManyJoin = 1700, kManyPart = 1000;
 struct Few {
   int tile;
   int64_t stage, unit;
@@ -69,7 +69,14 @@ Choice choose(const Product& p, bool may_many, int only, Likely likely, Most mos
   const int64_t few_cols = gate ? p.n / 2 / kGroup : div_up(p.n, kGroup), many_cols = gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup);
   const int64_t steps = div_up(p.groups, few_groups(gate));
   Choice best{0, 1, 0, INT64_MAX};
-  if (may_many) best.cost = kStart + div_up(likely(128) * many_cols, kSms) * (p.groups * kManyGroup + kManyUnit + (gate ? kManyGate : 0));
+  if (may_many) {
+    const int64_t tiles = likely(128) * many_cols;
+    best.cost = kStart + div_up(tiles, kSms) * (p.groups * kManyGroup + kManyUnit + (gate ? kManyGate : 0));
+    for (int split = 2; split <= 4 && split <= p.groups && !p.offsets; split *= 2) {
+      const int64_t cost = kStart + div_up(p.groups, split) * kManyGroup + kManyUnit + (gate ? kManyGate : 0) + kManyJoin + split * kManyPart;
+      if (tiles <= few_clusters(split) && cost < best.cost) best = {0, split, tiles, cost};
+    }
+  }
   for (const Few& f : kFew) {
     if (only && f.tile != only) continue;
     const int64_t units = likely(f.tile) * few_cols, all = most(f.tile) * few_cols;
@@ -101,7 +108,7 @@ int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream)
   if (!map_bytes(&x, p.x, 2, p.k, p.x_rows, 1, 128)) return MONO_LIN_DRIVER;
   p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup));
   if (!gate && p.vec && !p.fp32 && !map_out(&out, p.out, p.n, p.rows)) return MONO_LIN_DRIVER;
-  return launch_many(p, w, x, out, stream);
+  return launch_many(p, w, x, out, c.split, static_cast<int>(c.clusters), stream);
 }
 
 // What every product checks; fills in what follows from the sizes.

@@ -12,17 +12,21 @@
 //   4-7   bring the scales, some groups ahead, and rows of x that lie anywhere (tokens), by cp.async with the 128-byte swizzle
 //         written by hand
 //   8-15  read the sums, a half of the columns each four; write the results, through shared memory by tensor stores
-// With the gated activation a tile is 128 rows of the gate's half of the weight and the matching 128 of the other.
+// With the gated activation a tile is 128 rows of the gate's half of the weight and the matching 128 of the other. Where a dense product has few tiles
+// the groups of K are divided among two or four CTAs of a cluster, each of which finishes a part of the tile's rows: the others' sums of them come by bulk
+// copies from shared memory to shared memory and are added to its own in the order of the CTAs, so that results do not depend on timing.
 //
 // Bound by the readers: of a group's 128 x 256 sums each has to be read from tensor memory, multiplied by its scale and added, some 920 cycles
 // with the waits between, while the products take 512; the tensor pipe is busy half of the time. Around the groups of a unit lie 2900 cycles (first
 // sums, results), 5400 with the gated activation, whose exponentials and quotients take the most of it. Measured: 16384 x 7168 x 4096 in 478-490 us (2.0
 // PFLOP/s; under the power cap 535-547), 4096 x 2048 x 4096 in 50 (1.4), 8192 x 7168 x 4096 gated in 240-250; 256 experts' gated up projection (K 2048, N 1024) of 16384
 // tokens in 414-440 (1.25-1.33), their down projection (K 512, N 2048) in 257 (1.07), of 3000 tokens unevenly routed in 85, where weights and results alone take 58.
-// Tiles of 256 x 256 by pairs of CTAs took 502 us for the first, for the gated up projection 457; twenty warps, sixteen of them readers with
+// With K divided 256 rows of 7168 to 7168 columns take 25 us (undivided 37), 1024 of 4096 to 2048 19 (24); dividing costs 3.7 us in two, 5.7 in four (by stores of 16 bytes into the
+// other CTA instead of bulk copies 7 to 8). Tiles of 256 x 256 by pairs of CTAs took 502 us for the first, for the gated up projection 457; twenty warps, sixteen of them readers with
 // half the registers each, 580; one warp that issues for both halves, four stages with less room for results, and bands of sixteen
 // row tiles made no difference or a worse one.
 #include "linear.cuh"
+#include "../pair_sm100.cuh"
 
 namespace mono {
 namespace {
@@ -42,7 +46,7 @@ static_assert(8 * kRegsOther + 8 * kRegsReader <= 16 * kRegs, "a wait for regist
 constexpr int kX = kRows * kGroup, kPart = 128 * kGroup, kStage = kX + 2 * kPart, kStages = 3;   // bytes of x, of a half of the weight's rows
 
 struct Control {
-  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales], found[kRuns], taken[kRuns];
+  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales], found[kRuns], taken[kRuns], joined;
   Run runs[kRuns];
   uint32_t tmem, stop;
   int sums[32];
@@ -50,6 +54,9 @@ struct Control {
   float x_scale[kScales][kRows], w_scale[kScales][2];
   int first[MONO_LIN_MAX_EXPERTS + 1];
 };
+// With K in four parts: the sums that come and go, 96 KB each, and room for results of the two warps that write.
+static_assert(2 * 3 * (kRows / 4) * kTile * 4 + 2 * kStaging <= kStages * kStage + kReaders * kStaging, "divided sums");
+static_assert(2 * 1 * (kRows / 2) * kTile * 4 + 4 * kStaging <= kStages * kStage + kReaders * kStaging, "divided sums");
 constexpr int kSmem = kStages * kStage + kReaders * kStaging + static_cast<int>(sizeof(Control)) + 1024;
 static_assert(kSmem <= 232448, "shared memory of an SM");
 
@@ -63,10 +70,18 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* m, int col, int row
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
                ::"l"(reinterpret_cast<uint64_t>(m)), "r"(col), "r"(row), "r"(src) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint4 ld_shared_128(uint32_t at) {
   uint4 w;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
   return w;
+}
+
+// Shared memory into that of a CTA of the cluster, whose barrier counts it.
+__device__ __forceinline__ void bulk_to_cta(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // 128 columns from `col` on of 32 rows, of which the first `rows` are the unit's; one row a lane. Pieces of 16 bytes lie in shared memory at places
@@ -151,9 +166,9 @@ __device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* o
   }
 }
 
-template <bool Gate>
+template <bool Gate, bool Split>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant__ CUtensorMap weight, const __grid_constant__ CUtensorMap rows,
-                                                           const __grid_constant__ CUtensorMap out, const __grid_constant__ Product p) {
+                                                           const __grid_constant__ CUtensorMap out, const __grid_constant__ Product p, const int split) {
   extern __shared__ uint8_t raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Control& C = *reinterpret_cast<Control*>(stages + kStages * kStage + kReaders * kStaging);
@@ -179,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       mbar_init(&C.found[i], 1);
       mbar_init(&C.taken[i], 1 + kLoaders / 32 + kReaders);
     }
+    mbar_init(&C.joined, 1);
     mbar_init_fence();
     C.stop = 0;
   }
@@ -192,7 +208,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   tc_fence_after();
 
   const Division<kRows> division(p, C.first);
-  const int units = division.units(), step = gridDim.x, u0 = blockIdx.x;
+  const int rank = Split ? static_cast<int>(cluster_ctarank()) : 0, of = Split ? split : 1;
+  const int units = division.units(), step = gridDim.x / of, u0 = blockIdx.x / of;
+  const int g0 = p.groups * rank / of, g1 = p.groups * (rank + 1) / of;     // groups of K of this CTA
   const uint32_t base = smem_u32(stages);
   // The next unit of this CTA; one without rows in a launch that gave up, where what is in memory may be half of another.
   uint32_t nth = 0;
@@ -212,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       for (int u = u0; u < units; u += step) {
         const Run r = take();
         if (lane == 0) {
-          for (int g = 0; g < p.groups; ++g, ++n) {
+          for (int g = g0; g < g1; ++g, ++n) {
             const uint32_t s = n % kStages, at = base + s * kStage;
             waits.wait_lane(&C.empty[s], (n / kStages & 1) ^ 1);
             mbar_arrive_expect_tx(&C.full[s], gather ? 2 * kPart : 2 * kPart + kX);
@@ -230,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       const uint32_t h = warp - kMma;
       uint32_t n = 0;
       for (int u = u0; u < units; u += step)
-        for (int g = 0; g < p.groups; ++g, ++n) {
+        for (int g = g0; g < g1; ++g, ++n) {
           const uint32_t s = n % kStages, b = 2 * (n & 1) + h;
           waits.wait_warp(&C.full[s], n / kStages & 1, &C.d_empty[b], (n >> 1 & 1) ^ 1);
           if (gather) {
@@ -276,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
 #pragma unroll
           for (int i = 0; i < kEach; ++i) src[i] = static_cast<uint32_t>(row(r0 + kLoaders / 8 * i)) * static_cast<uint32_t>(p.k / 16);
         }
-        for (int g = 0; g < p.groups; ++g, ++n) {
+        for (int g = g0; g < g1; ++g, ++n) {
           const uint32_t s = n % kStages, slot = n % kScales;
           waits.wait(&C.s_empty[slot], (n / kScales & 1) ^ 1);
           if (t < r.rows) cp_async4(smem_u32(&C.x_scale[slot][t]), xs + g);
@@ -296,6 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       }
       cp_async_commit();
       cp_async_wait<0>();                    // of a launch that gave up, too
+    }
+    if (Split && u0 < units) {               // as the readers do
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     reg_inc<kRegsReader>();
@@ -331,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         uint32_t v0[32], v1[32];
         ready(n);
         tmem_ld32(buffer(n), v0);
-        for (int g = 0; g < p.groups; ++g, ++n) {
+        for (int g = g0; g < g1; ++g, ++n) {
           const uint32_t d = buffer(n), slot = n % kScales;
           const float x = C.x_scale[slot][quarter * 32 + lane], sa = x * C.w_scale[slot][Gate ? 0 : half], sb = Gate ? x * C.w_scale[slot][1] : sa;
           tmem_ld_wait();
@@ -345,18 +367,59 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
           add(v0, sb, acc[1]);
           tmem_ld_wait();
           release(n);                        // read out: the next product may have the buffer
-          if (g + 1 < p.groups) {
+          if (g + 1 < g1) {
             ready(n + 1);
             tmem_ld32(buffer(n + 1), v0);
           }
           add(v1, sb, acc[1] + 16);
         }
       } else {
-        for (int g = 0; g < p.groups; ++g, ++n) {
+        for (int g = g0; g < g1; ++g, ++n) {
           waits.wait(&C.d_full[2 * (n & 1) + half], n >> 1 & 1);
           release(n);
         }
       }
+      bool writes = true;
+      uint32_t to = staging;
+      if constexpr (Split) {
+        // One unit to a cluster; a CTA finishes 64 or 32 of its rows. The others' sums of them come into its ring, which then is free, [CTA][row], and
+        // its own of other rows lie behind that until they are fetched; pieces of 16 bytes at places that spread over the banks.
+        const int each = kRows / split, owner = in / each, row = in % each + lane;
+        const uint32_t block = each * kTile * 4, come = base, go = base + (split - 1) * block, place = row * kTile * 4 + half * 512;
+        named_bar_sync(6, kReaders * 32);    // both halves of this CTA have their sums
+        cluster_arrive();
+        if (owner != rank) {
+          const uint32_t at = go + (owner - (owner > rank)) * block + place;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float2 a = acc[c >> 4][c % 16 * 2], b = acc[c >> 4][c % 16 * 2 + 1];
+            const uint32_t w[4] = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)};
+            st_shared_128(at + ((c ^ (lane & 7)) << 4), w);
+          }
+          fence_proxy_async_smem();
+        }
+        cluster_wait();
+        named_bar_sync(6, kReaders * 32);
+        if (threadIdx.x == 32 * kFirstReader) {
+          mbar_arrive_expect_tx(&C.joined, (split - 1) * block);
+          for (int c = 0; c < split; ++c)
+            if (c != rank) bulk_to_cta(map_to_cta(come + (rank - (rank > c)) * block, c), go + (c - (c > rank)) * block, block, map_to_cta(smem_u32(&C.joined), c));
+        }
+        waits.wait(&C.joined, 0);
+        writes = owner == rank;
+        to = base + kStages * kStage + (kReaders - 1 - half * (each / 32) - in % each / 32) * kStaging;     // the last pieces, of those that write
+        if (writes) {
+          for (int q = 0; q < split - 1; ++q) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const uint4 w = ld_shared_128(come + q * block + place + ((c ^ (lane & 7)) << 4));
+              float2 &a = acc[c >> 4][c % 16 * 2], &b = acc[c >> 4][c % 16 * 2 + 1];
+              a.x += __uint_as_float(w.x); a.y += __uint_as_float(w.y); b.x += __uint_as_float(w.z); b.y += __uint_as_float(w.w);
+            }
+          }
+        }
+      }
+      if (!writes) continue;
       if constexpr (Gate) {
         uint32_t m = 0;
 #pragma unroll
@@ -385,11 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         named_bar_sync(2 + quarter, 64);     // both have read the magnitudes
       } else if (mine > 0) {
         const int col = r.col * kTile + half * 128;
-        if (col < p.n) write_out(p, &out, staging, lane, row0, mine, col, acc);
+        if (col < p.n) write_out(p, &out, to, lane, row0, mine, col, acc);
       }
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
+    if (Split && u0 < units) cluster_sync_all();              // what this CTA sent has been fetched
   }
   tc_fence_before();
   __syncthreads();
@@ -398,26 +462,37 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   if (warp == kMma) tmem_dealloc(C.tmem, 512);
 }
 
-template <bool Gate>
-int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, cudaStream_t stream) {
+template <bool Gate, bool Split>
+int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
   static bool ready[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev >= 64 || !ready[dev]) {
-    e = cudaFuncSetAttribute(many_kernel<Gate>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(many_kernel<Gate, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  many_kernel<Gate><<<kSms, kThreads, kSmem, stream>>>(weight, x, out, p);
-  return static_cast<int>(cudaGetLastError());
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(static_cast<unsigned>(Split ? clusters * split : kSms));
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = kSmem;
+  c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = Split ? 1 : 0;
+  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate, Split>, weight, x, out, p, split));
 }
 
 }  // namespace
 
 namespace lin {
-int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, cudaStream_t stream) {
-  return p.codes ? launch<true>(p, weight, x, out, stream) : launch<false>(p, weight, x, out, stream);
+int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
+  if (split > 1) return p.codes ? launch<true, true>(p, weight, x, out, split, clusters, stream) : launch<false, true>(p, weight, x, out, split, clusters, stream);
+  return p.codes ? launch<true, false>(p, weight, x, out, 1, 0, stream) : launch<false, false>(p, weight, x, out, 1, 0, stream);
 }
 }  // namespace lin
 }  // namespace mono
