@@ -165,9 +165,6 @@ __device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float2 
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = bf16x2(w[i]);
 }
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float2 (&v)[8]) {
-  unpack16(__ldg(reinterpret_cast<const uint4*>(p)), __ldg(reinterpret_cast<const uint4*>(p) + 1), v);
-}
 // Largest magnitude (as bits, a NaN's above all) of a group that eight neighbouring lanes share, 16 values each. All lanes of the warp take part.
 __device__ __forceinline__ uint32_t top_of_group(const float2 (&v)[8]) {
   float top = 0.0f;

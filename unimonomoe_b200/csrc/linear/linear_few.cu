@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       }
   } else if (warp < 4) {
     const int t_ = threadIdx.x - 64, chunk = t_ & 7, r0 = t_ >> 3;
-    constexpr int kEach = Tile / 8, kOwn = (Tile + 63) / 64;  // rows of a thread, eight apart; scales of a thread
+    constexpr int kEach = Tile / 8;          // rows of a thread, eight apart
+    static_assert(Tile <= kLoaders, "a thread has the scales of one row");
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
       const Run r = unit(u);
@@ -292,20 +293,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       const uint8_t* src[kEach];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) src[i] = p.x + row(r0 + 8 * i) * p.k;
-      // Scales: a row (or two) of x a thread, two stages ahead in registers. Behind the last group the sums are zero, and so are the scales:
+      // Scales: a row of x a thread, two stages ahead in registers. Behind the last group the sums are zero, and so are the scales:
       // the last ones may be infinite.
-      const float* xs[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) xs[i] = p.xs + row(t_ + 64 * i) * p.groups;
+      const float* xs = p.xs + row(t_) * p.groups;
       const float *ws = p.ws + (static_cast<int64_t>(r.expert) * p.blocks + r.col) * p.groups, *ws2 = ws + static_cast<int64_t>(p.blocks / 2) * p.groups;
       if (u == u0) wait_for_launch_before();
-      float x[2][S::Groups][kOwn], wt[2][S::Pieces];
+      float x[2][S::Groups], wt[2][S::Pieces];
       auto fetch = [&](int t, int into) {
 #pragma unroll
         for (int j = 0; j < S::Groups; ++j) {
           const int g = min(t * S::Groups + j, p.groups - 1);
-#pragma unroll
-          for (int i = 0; i < kOwn; ++i) x[into][j][i] = ld_after(xs[i] + g);
+          x[into][j] = ld_after(xs + g);
           wt[into][j] = __ldg(ws + g);
           if constexpr (Gate) wt[into][1] = __ldg(ws2 + g);
         }
@@ -329,9 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         auto put = [&](int from) {
 #pragma unroll
           for (int j = 0; j < S::Pieces; ++j)
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i)
-              if (t_ + 64 * i < Tile) C.scale[slot][j][t_ + 64 * i] = Gate || t * S::Groups + j < p.groups ? x[from][Gate ? 0 : j][i] * wt[from][j] : 0.0f;
+            if (t_ < Tile) C.scale[slot][j][t_] = Gate || t * S::Groups + j < p.groups ? x[from][Gate ? 0 : j] * wt[from][j] : 0.0f;
           fetch(t + 2, from);
         };
         if ((t - t0) & 1) put(1); else put(0);
