@@ -54,6 +54,7 @@ struct Control {
   uint64_t full[8], done[8], read[8], s_full[kScales], s_empty[kScales], joined;
   uint32_t tmem, stop;
   int sums[32];
+  Run found;
   alignas(16) float scale[kScales][S::Pieces][Tile];          // of a stage: those of a row of x times the weight's
   int first[MONO_LIN_MAX_EXPERTS + 1];
 };
@@ -63,6 +64,11 @@ constexpr int smem_bytes() {
   return Shape<Tile, Gate>::Stages * Shape<Tile, Gate>::Stage + Shape<Tile, Gate>::Add + static_cast<int>(sizeof(Control<Tile, Gate>)) + 1024;
 }
 
+__device__ __forceinline__ int cluster_id() {
+  int id;
+  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(id));
+  return id;
+}
 // A store into the shared memory of a CTA of the cluster, which that one's barrier counts.
 __device__ __forceinline__ void st_counted(uint32_t addr, float v, uint32_t bar) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(addr), "f"(v), "r"(bar) : "memory");
@@ -141,35 +147,41 @@ __device__ __forceinline__ void finish(const Product& p, const Run& r, const flo
 }
 
 // Rows in 16 bits of this CTA's groups, which all find room in the ring: codes into the stages' rows of x, scales times the weight's. By all warps
-// but the first two: eight lanes share a group, 16 values each; the next one's values are on their way while one is quantised.
+// but the first two: eight lanes share a group, 16 values each; the next one's values are on their way while one is quantised, the first ones' while
+// the CTA sets itself up.
+constexpr int kTeams = (kThreads - 64) / 8;
+struct Piece {
+  uint4 a, b;
+  float weight;                              // its scale, for the lanes that write the product of both
+};
+template <bool Gate>
+__device__ __forceinline__ Piece fetch_piece(const Product& p, const Run& r, int g0, int items, int i) {
+  const int lane8 = threadIdx.x & 7, in = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.rows), g = g0 + in, k = g * kGroup + lane8 * 16;
+  const bool have = i < items && k < p.k;
+  const uint4* src = reinterpret_cast<const uint4*>(p.raw + (i - in * r.rows) * p.raw_stride + k);
+  Piece x;
+  x.a = have ? __ldg(src) : make_uint4(0, 0, 0, 0);
+  x.b = have ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+  // behind the last group sums and scales are zero
+  x.weight = i < items && g < p.groups && lane8 < (Gate ? 2 : 1) ? __ldg(p.ws + (static_cast<int64_t>(r.col) + lane8 * (p.blocks / 2)) * p.groups + g) : 0.0f;
+  return x;
+}
 template <int Tile, bool Gate>
-__device__ __forceinline__ void quantise_rows(const Product& p, Control<Tile, Gate>& C, const Run& r, uint32_t base, int t0, int t1) {
+__device__ __forceinline__ void quantise_rows(const Product& p, Control<Tile, Gate>& C, const Run& r, uint32_t base, int t0, int t1, Piece next) {
   using S = Shape<Tile, Gate>;
-  constexpr int kTeams = (kThreads - 64) / 8;
-  const int lane8 = threadIdx.x & 7, items = (t1 - t0) * S::Groups * r.rows;
-  const float* ws = p.ws + static_cast<int64_t>(r.col) * p.groups;
-  uint4 next[2];
-  auto fetch = [&](int i) {
-    const int g = i / r.rows, k = (t0 * S::Groups + g) * kGroup + lane8 * 16;
-    const bool have = i < items && k < p.k;
-    const uint4* src = reinterpret_cast<const uint4*>(p.raw + (i - g * r.rows) * p.raw_stride + k);
-    next[0] = have ? __ldg(src) : make_uint4(0, 0, 0, 0);
-    next[1] = have ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
-  };
-  int i = (threadIdx.x - 64) >> 3;
-  fetch(i);
-  for (; __any_sync(0xFFFFFFFFu, i < items); i += kTeams) {
+  const int lane8 = threadIdx.x & 7, g0 = t0 * S::Groups, items = (t1 - t0) * S::Groups * r.rows;
+  for (int i = (threadIdx.x - 64) >> 3; __any_sync(0xFFFFFFFFu, i < items); i += kTeams) {
     float2 v[8];
-    unpack16(next[0], next[1], v);
-    fetch(i + kTeams);
-    const int g = i / r.rows, row = i - g * r.rows, s = g / S::Groups, j = g - s * S::Groups;   // group and row, stage and group of it
-    const int of = min(t0 * S::Groups + g, p.groups - 1);
+    unpack16(next.a, next.b, v);
+    const float weight = next.weight;
+    next = fetch_piece<Gate>(p, r, g0, items, i + kTeams);
+    const int g = static_cast<uint32_t>(i) / static_cast<uint32_t>(r.rows), row = i - g * r.rows, s = g / S::Groups, j = g - s * S::Groups;   // group and row, stage and group of it
     const GroupScale scale(top_of_group(v));
     if (i < items) {
       const uint4 c = codes16(v, scale.inverse);
       const uint32_t words[4] = {c.x, c.y, c.z, c.w};
       st_shared_128(base + s * S::Stage + S::Pieces * kPiece + (j * Tile + row) * 128 + ((lane8 ^ (row & 7)) << 4), words);
-      if (lane8 < S::Halves) C.scale[s][Gate ? lane8 : j][row] = t0 * S::Groups + g < p.groups ? scale.scale * __ldg(ws + static_cast<int64_t>(lane8) * (p.blocks / 2) * p.groups + of) : 0.0f;
+      if (lane8 < S::Halves) C.scale[s][Gate ? lane8 : j][row] = g0 + g < p.groups ? scale.scale * weight : 0.0f;
     }
   }
   fence_proxy_async_smem();                  // the tensor core reads what was stored here
@@ -187,34 +199,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const Waits waits{&C.stop, p.status};
-  const int step = static_cast<int>(gridDim.x) / split, u0 = static_cast<int>(blockIdx.x) / split;
-  const int steps = (p.groups + S::Groups - 1) / S::Groups, t0 = steps * rank / split, t1 = steps * (rank + 1) / split;   // stages of this CTA
-
-  if (warp == 0) {
-    if (lane < S::Stages) {
-      mbar_init(&C.full[lane], 1 + kLoaders);
-      mbar_init(&C.done[lane], 1);
-      mbar_init(&C.read[lane], kReaders / 32);
-    }
-    if (lane < kScales) {
-      mbar_init(&C.s_full[lane], kLoaders);
-      mbar_init(&C.s_empty[lane], kReaders / 32);
-    }
-    if (lane == 0) {
-      tma_prefetch_desc(&weight);
-      mbar_init(&C.joined, 1);
-      C.stop = 0;
-    }
-    mbar_init_fence();
-    __syncwarp();
-  }
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  if (p.offsets) Division<Tile>::fill(p, C.first, C.sums, kThreads);
-  const Division<Tile> division(p, C.first);
-  const int units = division.units();
-  const Run at_first = u0 < units ? division.unit(u0) : Run{};         // all warps': code that each of them would have to fetch for itself
-  int expert = at_first.expert;
-  auto unit = [&](int u) { return u == u0 ? at_first : division.unit_after(u, expert); };
+  // With K divided a cluster has one unit.
+  const int step = split > 1 ? 1 << 30 : static_cast<int>(gridDim.x), u0 = split > 1 ? cluster_id() : static_cast<int>(blockIdx.x);
+  const uint32_t steps = (p.groups + S::Groups - 1) / S::Groups;
+  const int t0 = steps * rank / split, t1 = steps * (rank + 1) / split;       // stages of this CTA
   // Stage s gets the pieces of step t of unit r; the n-th use of the ring.
   auto request = [&](const Run& r, int t, uint32_t s) {
     const uint32_t at = base + s * S::Stage;
@@ -223,10 +211,58 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     for (int i = 0; i < S::Groups; ++i) tma_weight(&weight, (t * S::Groups + i) * kGroup, r.col * kRows, r.expert, at + i * kPiece, &C.full[s]);
     if constexpr (Gate) tma_weight(&weight, t * kGroup, p.n / 2 + r.col * kRows, r.expert, at + kPiece, &C.full[s]);
   };
-  const int early = u0 < units ? min(t1 - t0, S::Stages) : 0;
-  if (threadIdx.x == 0) {                    // the first requests, before the others are there
-    for (int i = 0; i < early; ++i) request(at_first, t0 + i, i);
+
+  if (p.offsets && static_cast<int>(threadIdx.x) <= p.experts) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.offsets + threadIdx.x));
+
+  // The first requests come before the other barriers are made; what other CTAs have to wait for comes before them.
+  if (warp == 0) {
+    if (lane < S::Stages) mbar_init(&C.full[lane], 1 + kLoaders);
+    if (lane == 0) {
+      tma_prefetch_desc(&weight);
+      mbar_init(&C.joined, 1);
+    }
+    mbar_init_fence();
+    __syncwarp();
   }
+  // What is to be seen by the others are barriers, which their fence has released.
+  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  auto other_barriers = [&]() {
+    if (warp == 0) {
+      if (lane < S::Stages) {
+        mbar_init(&C.done[lane], 1);
+        mbar_init(&C.read[lane], kReaders / 32);
+      }
+      if (lane < kScales) {
+        mbar_init(&C.s_full[lane], kLoaders);
+        mbar_init(&C.s_empty[lane], kReaders / 32);
+      }
+      if (lane == 0) C.stop = 0;
+      mbar_init_fence();
+      __syncwarp();
+    }
+  };
+  const Division<Tile> division(p, C.first);
+  Run at_first{};                            // all warps'
+  if (p.offsets) {
+    other_barriers();                        // while the offsets are on their way
+    const int tile = u0 / p.cols;
+    Division<Tile>::fill(p, C.first, C.sums, kThreads, tile, &C.found);
+    at_first = C.found;
+    at_first.col = u0 - tile * p.cols;
+  }
+  const int units = division.units();
+  if (!p.offsets && u0 < units) at_first = division.unit(u0);
+  int expert = at_first.expert;
+  auto unit = [&](int u) { return u == u0 ? at_first : division.unit_after(u, expert); };
+  const int early = u0 < units ? min(t1 - t0, S::Stages) : 0;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < early; ++i) request(at_first, t0 + i, i);
+  __syncwarp();
+  if (!p.offsets) other_barriers();
+  const bool in_16 = Tile >= MONO_LIN_FEW_ROWS && Tile < 2 * MONO_LIN_FEW_ROWS && p.raw != nullptr;   // what takes_rows says yes to has this tile
+  const bool quantise = in_16 && warp >= 2 && u0 < units;
+  Piece first_piece{};
+  if (quantise) first_piece = fetch_piece<Gate>(p, at_first, t0 * S::Groups, (t1 - t0) * S::Groups * at_first.rows, (threadIdx.x - 64) >> 3);
   if (warp == 1) {
     tmem_alloc(&C.tmem, S::Tmem);
     tmem_relinquish();
@@ -236,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   tc_fence_after();
   if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the others run: their shared memory may be written
 
-  if (p.raw != nullptr && warp >= 2 && u0 < units) quantise_rows<Tile, Gate>(p, C, at_first, base, t0, t1);
+  if (quantise) quantise_rows<Tile, Gate>(p, C, at_first, base, t0, t1, first_piece);
 
   if (warp == 0) {
     uint32_t before = 0;                     // stages of the units before
@@ -275,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         __syncwarp();
       }
     }
-  } else if (warp < 4 && p.raw != nullptr) {
+  } else if (warp < 4 && in_16) {
     if (u0 < units)
       for (int n = 0; n < t1 - t0; ++n) {
         mbar_arrive(&C.full[n]);
@@ -398,17 +434,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         if (threadIdx.x == 128) mbar_arrive_expect_tx(&C.joined, static_cast<uint32_t>(max(hi - lo, 0) * split * S::Halves * kRows * 4));
         int owner = i0 / each, in = i0 - owner * each;
 #pragma unroll
-        for (int i = 0; i < S::Mine; ++i)
-          if (i0 + i < r.rows) {
-            const uint32_t to = map_to_cta(smem_u32(sums + (rank * S::Halves * each + in) * kRows + quarter * 32 + lane), owner);
-            const uint32_t bar = map_to_cta(smem_u32(&C.joined), owner);
+        for (int i = 0; i < S::Mine; ++i) {
+          if (i0 + i >= r.rows) break;
+          const uint32_t to = map_to_cta(smem_u32(sums + (rank * S::Halves * each + in) * kRows + quarter * 32 + lane), owner);
+          const uint32_t bar = map_to_cta(smem_u32(&C.joined), owner);
 #pragma unroll
-            for (int h = 0; h < S::Halves; ++h) st_counted(to + h * each * kRows * 4, i & 1 ? acc[h][i / 2].y : acc[h][i / 2].x, bar);
-            if (++in == each) {
-              in = 0;
-              ++owner;
-            }
+          for (int h = 0; h < S::Halves; ++h) st_counted(to + h * each * kRows * 4, i & 1 ? acc[h][i / 2].y : acc[h][i / 2].x, bar);
+          if (++in == each) {
+            in = 0;
+            ++owner;
           }
+        }
         waits.wait(&C.joined, 0);
         finish<Gate, true>(p, r, sums, split, each, lo, hi, w, lane);
       }
