@@ -89,8 +89,8 @@ Choice choose(const Product& p, bool may_many, int only, Likely likely, Most mos
 }
 
 // Of a dense product. Few rows are one row tile, whether they come in 8 bits or in 16: the results are the same bits. (Quantised in the launch, K of 2048
-// and 5120 columns: 1 row 6.0 us, 16 rows 7.5; in a launch before it 7.1 and 7.7. From 17 rows on the launch before it is faster: 24 rows 8.6 and
-// 8.1, 61 rows, K of 4096 and 2048 columns, 13.4 and 9.3.)
+// and 5120 columns: 1 row 5.4 us, 16 rows 6.6; in a launch before it 6.5 and 7.0. From 17 rows on the launch before it is faster: 24 rows 8.6 and
+// 7.4, 61 rows, K of 4096 and 2048 columns, 13.4 and 8.5.)
 Choice dense(const Product& p) {
   const auto tiles = [&](int t) { return div_up(p.rows, t); };
   const bool few = p.rows <= MONO_LIN_FEW_ROWS;
