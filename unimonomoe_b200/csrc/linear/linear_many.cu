@@ -7,8 +7,8 @@
 // scale, or the gate's and the other half's). Sixteen warps, one CTA to an SM:
 //   0     requests weights, and rows of x where they lie in order
 //   1, 2  issue the products, a half of the columns each
-//   3     finds the units, some ahead: the others read them from shared memory (found by each role for itself a unit cost 1600 cycles, as much as
-//         two groups of K)
+//   3     finds the units of experts, some ahead: the others read them from shared memory (found by each role for itself a unit cost 1600 cycles, as
+//         much as two groups of K; those of one dense product are a few divisions, and taking them from there made 506 us of 483)
 //   4-7   bring the scales, some groups ahead, and rows of x that lie anywhere (tokens), by cp.async with the 128-byte swizzle
 //         written by hand
 //   8-15  read the sums, a half of the columns each four; write the results, through shared memory by tensor stores
@@ -166,7 +166,7 @@ __device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* o
   }
 }
 
-template <bool Gate, bool Split>
+template <bool Gate, bool Runs, bool Split>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant__ CUtensorMap weight, const __grid_constant__ CUtensorMap rows,
                                                            const __grid_constant__ CUtensorMap out, const __grid_constant__ Product p, const int split) {
   extern __shared__ uint8_t raw[];
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   Control& C = *reinterpret_cast<Control*>(stages + kStages * kStage + kReaders * kStaging);
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const Waits waits{&C.stop, p.status};
-  const bool gather = p.tokens != nullptr;
+  const bool gather = Runs && p.tokens != nullptr;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     tmem_alloc(&C.tmem, 512);
     tmem_relinquish();
   }
-  if (p.offsets) Division<kRows>::fill(p, C.first, C.sums, kThreads);
+  if constexpr (Runs) Division<kRows>::fill(p, C.first, C.sums, kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -212,15 +212,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   const int units = division.units(), step = gridDim.x / of, u0 = blockIdx.x / of;
   const int g0 = p.groups * rank / of, g1 = p.groups * (rank + 1) / of;     // groups of K of this CTA
   const uint32_t base = smem_u32(stages);
-  // The next unit of this CTA; one without rows in a launch that gave up, where what is in memory may be half of another.
+  // Unit u, the next one of this CTA. Where it is one of a run it is one without rows in a launch that gave up: what is in memory may be half of another.
   uint32_t nth = 0;
-  auto take = [&]() {
-    const uint32_t slot = nth % kRuns;
-    waits.wait(&C.found[slot], nth++ / kRuns & 1);
-    const Run r = C.runs[slot];
-    if (waits.stopped()) return Run{};
-    if (lane == 0) mbar_arrive(&C.taken[slot]);
-    return r;
+  auto take = [&](int u) {
+    if constexpr (!Runs) {
+      return division.unit(u);
+    } else {
+      const uint32_t slot = nth % kRuns;
+      waits.wait(&C.found[slot], nth++ / kRuns & 1);
+      const Run r = C.runs[slot];
+      if (waits.stopped()) return Run{};
+      if (lane == 0) mbar_arrive(&C.taken[slot]);
+      return r;
+    }
   };
 
   if (warp < kFirstReader) {
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     if (warp == 0) {
       uint32_t n = 0;
       for (int u = u0; u < units; u += step) {
-        const Run r = take();
+        const Run r = take(u);
         if (lane == 0) {
           for (int g = g0; g < g1; ++g, ++n) {
             const uint32_t s = n % kStages, at = base + s * kStage;
@@ -266,15 +270,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
           __syncwarp();
         }
     } else if (warp == kFinder) {
-      int expert = 0;
-      for (int u = u0; u < units; u += step, ++nth) {
-        const Run r = division.unit_after(u, expert);
-        const uint32_t slot = nth % kRuns;
-        waits.wait(&C.taken[slot], (nth / kRuns & 1) ^ 1);
-        if (waits.stopped()) break;
-        if (lane == 0) {
-          C.runs[slot] = r;
-          mbar_arrive(&C.found[slot]);
+      if constexpr (Runs) {
+        int expert = 0;
+        for (int u = u0; u < units; u += step, ++nth) {
+          const Run r = division.unit_after(u, expert);
+          const uint32_t slot = nth % kRuns;
+          waits.wait(&C.taken[slot], (nth / kRuns & 1) ^ 1);
+          if (waits.stopped()) break;
+          if (lane == 0) {
+            C.runs[slot] = r;
+            mbar_arrive(&C.found[slot]);
+          }
         }
       }
     } else {
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       constexpr int kEach = kRows / (kLoaders / 8);           // rows of a thread, sixteen apart
       uint32_t n = 0;
       for (int u = u0; u < units; u += step) {
-        const Run r = take();
+        const Run r = take(u);
         // Rows past the unit's are left as they are, nobody reads what comes of them. (One row for all of them would be asked for by
         // every CTA at once: 174 us instead of 113 for 2048 tokens through 256 experts' up projection.)
         auto row = [&](int i) { return i < r.rows ? source_row(p, r.row + i) : 0; };
@@ -326,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint32_t n = 0;
     for (int u = u0; u < units; u += step) {
-      const Run r = take();
+      const Run r = take(u);
       const int in = quarter * 32, mine = max(0, min(32, r.rows - in));   // rows of this warp
       const int64_t row0 = static_cast<int64_t>(r.row) + in;
       float2 acc[2][32] = {};
@@ -462,14 +468,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   if (warp == kMma) tmem_dealloc(C.tmem, 512);
 }
 
-template <bool Gate, bool Split>
+template <bool Gate, bool Runs, bool Split>
 int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
   static bool ready[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev >= 64 || !ready[dev]) {
-    e = cudaFuncSetAttribute(many_kernel<Gate, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(many_kernel<Gate, Runs, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
@@ -484,15 +490,17 @@ int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, co
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   c.attrs = at;
   c.numAttrs = Split ? 1 : 0;
-  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate, Split>, weight, x, out, p, split));
+  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate, Runs, Split>, weight, x, out, p, split));
 }
 
 }  // namespace
 
 namespace lin {
 int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
-  if (split > 1) return p.codes ? launch<true, true>(p, weight, x, out, split, clusters, stream) : launch<false, true>(p, weight, x, out, split, clusters, stream);
-  return p.codes ? launch<true, false>(p, weight, x, out, 1, 0, stream) : launch<false, false>(p, weight, x, out, 1, 0, stream);
+  const bool gate = p.codes != nullptr;
+  if (p.offsets) return gate ? launch<true, true, false>(p, weight, x, out, 1, 0, stream) : launch<false, true, false>(p, weight, x, out, 1, 0, stream);
+  if (split > 1) return gate ? launch<true, false, true>(p, weight, x, out, split, clusters, stream) : launch<false, false, true>(p, weight, x, out, split, clusters, stream);
+  return gate ? launch<true, false, false>(p, weight, x, out, 1, 0, stream) : launch<false, false, false>(p, weight, x, out, 1, 0, stream);
 }
 }  // namespace lin
 }  // namespace mono
