@@ -32,15 +32,14 @@ bool map_bytes(CUtensorMap* m, const void* base, int rank, uint64_t k, uint64_t 
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// bf16 [rows][n], boxes of 32 rows x 64 columns with the 128-byte swizzle.
-bool map_out(CUtensorMap* m, void* base, uint64_t n, uint64_t rows) {
+// bf16 or fp32 [rows][n], boxes of 32 rows x 128 bytes with the 128-byte swizzle.
+bool map_rows(CUtensorMap* m, const void* base, bool fp32, uint64_t n, uint64_t rows) {
   const EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {n, rows}, strides[1] = {2 * n};
-  const cuuint32_t box[2] = {64, 32}, steps[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t size = fp32 ? 4 : 2, box[2] = {128 / size, 32}, steps[2] = {1, 1};
+  const cuuint64_t dims[2] = {n, rows}, strides[1] = {size * n};
+  return fn(m, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -98,7 +97,7 @@ Choice dense(const Product& p) {
 }
 
 int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream) {
-  CUtensorMap w, x, out{};
+  CUtensorMap w, x, out{}, residual{};
   if (!map_bytes(&w, weight, 3, p.k, p.n, p.experts, c.tile ? 128 : 64)) return MONO_LIN_DRIVER;
   const bool gate = p.codes != nullptr;
   if (c.tile) {
@@ -107,8 +106,9 @@ int run(Product& p, const uint8_t* weight, const Choice& c, cudaStream_t stream)
   }
   if (!map_bytes(&x, p.x, 2, p.k, p.x_rows, 1, 128)) return MONO_LIN_DRIVER;
   p.cols = static_cast<int>(gate ? p.n / 2 / kGroup : div_up(p.n, 2 * kGroup));
-  if (!gate && p.vec && !p.fp32 && !map_out(&out, p.out, p.n, p.rows)) return MONO_LIN_DRIVER;
-  return launch_many(p, w, x, out, c.split, static_cast<int>(c.clusters), stream);
+  if (!gate && p.vec && !map_rows(&out, p.out, p.fp32, p.n, p.rows)) return MONO_LIN_DRIVER;
+  if (p.residual && p.vec && !map_rows(&residual, p.residual, false, p.n, p.rows)) return MONO_LIN_DRIVER;
+  return launch_many(p, w, x, out, residual, c.split, static_cast<int>(c.clusters), stream);
 }
 
 // What every product checks; fills in what follows from the sizes.

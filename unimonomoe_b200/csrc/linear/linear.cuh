@@ -388,7 +388,8 @@ constexpr int few_groups(bool gate) { return gate ? 1 : 2; }
 int few_clusters(int split);
 int few_stages(int tile, bool gate);         // of the ring of a CTA
 int launch_few(const Product& p, const CUtensorMap& weight, int tile, int split, int64_t clusters, cudaStream_t stream);
-int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream);
+int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, const CUtensorMap& residual, int split,
+                int clusters, cudaStream_t stream);
 
 }  // namespace lin
 }  // namespace mono

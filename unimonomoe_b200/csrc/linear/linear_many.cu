@@ -21,6 +21,8 @@
 // sums, results), 5400 with the gated activation, whose exponentials and quotients take the most of it. Measured: 16384 x 7168 x 4096 in 478-490 us (2.0
 // PFLOP/s; under the power cap 535-547), 4096 x 2048 x 4096 in 50 (1.4), 8192 x 7168 x 4096 gated in 240-250; 256 experts' gated up projection (K 2048, N 1024) of 16384
 // tokens in 414-440 (1.25-1.33), their down projection (K 512, N 2048) in 257 (1.07), of 3000 tokens unevenly routed in 85, where weights and results alone take 58.
+// 8192 x 2048 x 4096 takes 72 us, with a residual, which is brought while the groups are summed, 84 (read a row a lane behind them 99), in fp32 87 (a row
+// a lane 125), where rows of the result begin anywhere 148, with a residual 210.
 // With K divided 256 rows of 7168 to 7168 columns take 25 us (undivided 37), 1024 of 4096 to 2048 19 (24); dividing costs 3.7 us in two, 5.7 in four (by stores of 16 bytes into the
 // other CTA instead of bulk copies 7 to 8). Tiles of 256 x 256 by pairs of CTAs took 502 us for the first, for the gated up projection 457; twenty warps, sixteen of them readers with
 // half the registers each, 580; one warp that issues for both halves, four stages with less room for results, and bands of sixteen
@@ -46,7 +48,7 @@ static_assert(8 * kRegsOther + 8 * kRegsReader <= 16 * kRegs, "a wait for regist
 constexpr int kX = kRows * kGroup, kPart = 128 * kGroup, kStage = kX + 2 * kPart, kStages = 3;   // bytes of x, of a half of the weight's rows
 
 struct Control {
-  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales], found[kRuns], taken[kRuns], joined;
+  uint64_t full[kStages], gathered[kStages], empty[kStages], d_full[kSums], d_empty[kSums], s_full[kScales], s_empty[kScales], found[kRuns], taken[kRuns], joined, r_full[kReaders];
   Run runs[kRuns];
   uint32_t tmem, stop;
   int sums[32];
@@ -85,25 +87,31 @@ __device__ __forceinline__ void bulk_to_cta(uint32_t dst, uint32_t src, uint32_t
 }
 
 // 128 columns from `col` on of 32 rows, of which the first `rows` are the unit's; one row a lane. Pieces of 16 bytes lie in shared memory at places
-// that spread over the banks, as a tensor map with the 128-byte swizzle has them.
-__device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* out, uint32_t at, int lane, int64_t row0, int rows, int col, float2 (&acc)[2][32]) {
-  if (p.vec && p.residual && lane < rows) {
+// that spread over the banks, as a tensor map with the 128-byte swizzle has them. So does the residual, if it was `brought` there. Plain: bf16 in rows
+// that begin on 16 bytes, without residual; what else there is in one kernel with that costs it 3%.
+template <bool Plain>
+__device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* out, uint32_t at, int lane, int64_t row0, int rows, int col, bool brought, float2 (&acc)[2][32]) {
+  auto add = [&](int c, const uint4& r) {    // to eight columns
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = bf16x2(w[i]);
+      float2& t = acc[c / 8][c % 8 * 4 + i];
+      t.x += f.x;
+      t.y += f.y;
+    }
+  };
+  if (!Plain && brought) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) add(c, ld_shared_128(at + c / 8 * kBox + lane * 128 + (((c % 8) ^ (lane & 7)) << 4)));
+    __syncwarp();
+  } else if (!Plain && p.vec && p.residual && lane < rows) {
     const uint4* res = reinterpret_cast<const uint4*>(p.residual + (row0 + lane) * p.n + col);
 #pragma unroll
     for (int c = 0; c < 16; ++c)
-      if (col + c * 8 < p.n) {
-        const uint4 r = __ldg(res + c);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = bf16x2(w[i]);
-          float2& t = acc[c / 8][c % 8 * 4 + i];
-          t.x += f.x;
-          t.y += f.y;
-        }
-      }
+      if (col + c * 8 < p.n) add(c, __ldg(res + c));
   }
-  if (p.vec && !p.fp32) {
+  if (Plain || (p.vec && !p.fp32)) {
     if (lane == 0) bulk_wait_read<0>();      // of the unit before
     __syncwarp();
 #pragma unroll
@@ -133,14 +141,37 @@ __device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* o
               ld_shared_128(at + half * kBox + r * 128 + ((c ^ (r & 7)) << 4));
       __syncwarp();
     }
-  } else if (p.vec) {
-    if (lane < rows) {
-      float* o = static_cast<float*>(p.out) + (row0 + lane) * p.n + col;
+  } else if (!Plain && p.vec) {              // 64 columns of fp32 at a time
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col + 4 * i < p.n) reinterpret_cast<float4*>(o)[i] = make_float4(acc[i / 16][i % 16 * 2].x, acc[i / 16][i % 16 * 2].y, acc[i / 16][i % 16 * 2 + 1].x, acc[i / 16][i % 16 * 2 + 1].y);
+    for (int h = 0; h < 2; ++h) {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float2 *v = acc[h] + 2 * c;
+        const uint32_t w[4] = {__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y)};
+        st_shared_128(at + c / 8 * kBox + lane * 128 + (((c % 8) ^ (lane & 7)) << 4), w);
+      }
+      const int from = col + h * 64;
+      if (rows == 32) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && from < p.n) {
+          tma_store(out, from, static_cast<int>(row0), at);
+          if (from + 32 < p.n) tma_store(out, from + 32, static_cast<int>(row0), at + kBox);
+          bulk_commit();
+        }
+      } else {
+        __syncwarp();
+        const int c = lane & 7, box = (lane >> 3) & 1, n = from + box * 32 + c * 4;
+        if (n < p.n)
+#pragma unroll 4
+          for (int r = lane >> 4; r < rows; r += 2)
+            *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + (row0 + r) * p.n + n) = ld_shared_128(at + box * kBox + r * 128 + ((c ^ (r & 7)) << 4));
+        __syncwarp();
+      }
     }
-  } else {                                   // rows that begin anywhere: 32 columns at a time, a column a lane
+  } else if (!Plain) {                       // rows that begin anywhere: 32 columns at a time, a column a lane
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
 #pragma unroll
@@ -153,22 +184,33 @@ __device__ __forceinline__ void write_out(const Product& p, const CUtensorMap* o
       const int n = col + h * 32 + lane;
       if (n < p.n)
 #pragma unroll 1
-        for (int r = 0; r < rows; ++r) {
-          float x;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
-          const int64_t to = (row0 + r) * p.n + n;
-          if (p.residual) x += __bfloat162float(p.residual[to]);
-          if (p.fp32) static_cast<float*>(p.out)[to] = x;
-          else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(x);
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          __nv_bfloat16 res[8];
+          if (p.residual) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) res[i] = p.residual[(row0 + min(r0 + i, rows - 1)) * p.n + n];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + i;
+            if (r >= rows) break;
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+            const int64_t to = (row0 + r) * p.n + n;
+            if (p.residual) x += __bfloat162float(res[i]);
+            if (p.fp32) static_cast<float*>(p.out)[to] = x;
+            else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(x);
+          }
         }
       __syncwarp();
     }
   }
 }
 
-template <bool Gate, bool Runs, bool Split>
+template <bool Gate, bool Runs, bool Split, bool Plain>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant__ CUtensorMap weight, const __grid_constant__ CUtensorMap rows,
-                                                           const __grid_constant__ CUtensorMap out, const __grid_constant__ Product p, const int split) {
+                                                           const __grid_constant__ CUtensorMap out, const __grid_constant__ CUtensorMap residual,
+                                                           const __grid_constant__ Product p, const int split) {
   extern __shared__ uint8_t raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Control& C = *reinterpret_cast<Control*>(stages + kStages * kStage + kReaders * kStaging);
@@ -195,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       mbar_init(&C.taken[i], 1 + kLoaders / 32 + kReaders);
     }
     mbar_init(&C.joined, 1);
+    for (int i = 0; i < kReaders; ++i) mbar_init(&C.r_full[i], 1);
     mbar_init_fence();
     C.stop = 0;
   }
@@ -330,11 +373,24 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     const int quarter = warp & 3, half = (warp - kFirstReader) >> 2;
     const uint32_t staging = base + kStages * kStage + (warp - kFirstReader) * kStaging;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    uint32_t n = 0;
+    // The residual of a unit is brought to where its results will lie while the groups are summed.
+    const bool bring = !Gate && !Runs && !Split && !Plain && p.residual != nullptr && p.vec;
+    uint32_t n = 0, brought = 0;
     for (int u = u0; u < units; u += step) {
       const Run r = take(u);
       const int in = quarter * 32, mine = max(0, min(32, r.rows - in));   // rows of this warp
       const int64_t row0 = static_cast<int64_t>(r.row) + in;
+      const bool here = bring && mine > 0 && r.col * kTile + half * 128 < p.n;
+      if (here && lane == 0) {
+        const int col = r.col * kTile + half * 128, boxes = col + 64 < p.n ? 2 : 1;
+        uint8_t* to = stages + kStages * kStage + (warp - kFirstReader) * kStaging;
+        uint64_t* bar = &C.r_full[warp - kFirstReader];
+        bulk_wait_read<0>();                 // the results of the unit before
+        fence_proxy_async_smem();
+        mbar_arrive_expect_tx(bar, boxes * kBox);
+        for (int i = 0; i < boxes; ++i) tma_load_2d(&residual, col + i * 64, static_cast<uint32_t>(row0), to + i * kBox, bar);
+      }
+      __syncwarp();
       float2 acc[2][32] = {};
       // The sums of group n are in the buffer, and its scales in shared memory.
       auto ready = [&](uint32_t n) {
@@ -454,7 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         named_bar_sync(2 + quarter, 64);     // both have read the magnitudes
       } else if (mine > 0) {
         const int col = r.col * kTile + half * 128;
-        if (col < p.n) write_out(p, &out, to, lane, row0, mine, col, acc);
+        if (here) waits.wait(&C.r_full[warp - kFirstReader], brought++ & 1);
+        if (col < p.n) write_out<Plain>(p, &out, to, lane, row0, mine, col, here, acc);
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -468,14 +525,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   if (warp == kMma) tmem_dealloc(C.tmem, 512);
 }
 
-template <bool Gate, bool Runs, bool Split>
-int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
+template <bool Gate, bool Runs, bool Split, bool Plain>
+int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, const CUtensorMap& residual, int split, int clusters, cudaStream_t stream) {
   static bool ready[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev >= 64 || !ready[dev]) {
-    e = cudaFuncSetAttribute(many_kernel<Gate, Runs, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(many_kernel<Gate, Runs, Split, Plain>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
@@ -490,17 +547,24 @@ int launch(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, co
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   c.attrs = at;
   c.numAttrs = Split ? 1 : 0;
-  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate, Runs, Split>, weight, x, out, p, split));
+  return static_cast<int>(cudaLaunchKernelEx(&c, many_kernel<Gate, Runs, Split, Plain>, weight, x, out, residual, p, split));
+}
+
+template <bool Gate, bool Plain>
+int launch_as(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, const CUtensorMap& residual, int split, int clusters,
+              cudaStream_t stream) {
+  if (p.offsets) return launch<Gate, true, false, Plain>(p, weight, x, out, residual, 1, 0, stream);
+  if (split > 1) return launch<Gate, false, true, Plain>(p, weight, x, out, residual, split, clusters, stream);
+  return launch<Gate, false, false, Plain>(p, weight, x, out, residual, 1, 0, stream);
 }
 
 }  // namespace
 
 namespace lin {
-int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, int split, int clusters, cudaStream_t stream) {
-  const bool gate = p.codes != nullptr;
-  if (p.offsets) return gate ? launch<true, true, false>(p, weight, x, out, 1, 0, stream) : launch<false, true, false>(p, weight, x, out, 1, 0, stream);
-  if (split > 1) return gate ? launch<true, false, true>(p, weight, x, out, split, clusters, stream) : launch<false, false, true>(p, weight, x, out, split, clusters, stream);
-  return gate ? launch<true, false, false>(p, weight, x, out, 1, 0, stream) : launch<false, false, false>(p, weight, x, out, 1, 0, stream);
+int launch_many(const Product& p, const CUtensorMap& weight, const CUtensorMap& x, const CUtensorMap& out, const CUtensorMap& residual, int split, int clusters, cudaStream_t stream) {
+  if (p.codes) return launch_as<true, true>(p, weight, x, out, residual, split, clusters, stream);
+  if (p.vec && !p.fp32 && !p.residual) return launch_as<false, true>(p, weight, x, out, residual, split, clusters, stream);
+  return launch_as<false, false>(p, weight, x, out, residual, split, clusters, stream);
 }
 }  // namespace lin
 }  // namespace mono
