@@ -358,8 +358,16 @@ static __device__ __noinline__ void store_any(const __nv_bfloat16* residual, voi
 }
 __device__ __forceinline__ void store4(const Product& p, int64_t row, int n, const float4& v) {
   const int64_t at = row * p.n + n;
-  if (p.vec && !p.fp32 && !p.residual) {     // n is a multiple of 8
-    if (n < p.n) *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  if (p.vec && !p.fp32) {                    // n is a multiple of 8
+    if (n < p.n) {
+      float4 x = v;
+      if (p.residual) {
+        const uint2 r = __ldg(reinterpret_cast<const uint2*>(p.residual + at));
+        const float2 a = bf16x2(r.x), b = bf16x2(r.y);
+        x = make_float4(x.x + a.x, x.y + a.y, x.z + b.x, x.w + b.y);
+      }
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+    }
   } else {
     store_any(p.residual, p.out, p.n, p.fp32, at, n, v);
   }
