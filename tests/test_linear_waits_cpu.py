@@ -1,0 +1,24 @@
+"""The waits of the block-FP8 products' kernels, lane by lane on host threads (linear_waits_emulation.cpp)."""
+import os
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+LINEAR = os.path.join(os.path.dirname(HERE), "unimonomoe_b200", "csrc", "linear")
+
+
+@pytest.fixture(scope="module")
+def emulation(tmp_path_factory):
+    d = tmp_path_factory.mktemp("waits")
+    text = open(os.path.join(LINEAR, "waits.cuh")).read()
+    (d / "waits.cuh").write_text(text.replace('#include "barriers.cuh"\n', ""))
+    exe = str(d / "waits")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-w", f'-DSOURCE="{d}/waits.cuh"', os.path.join(HERE, "linear_waits_emulation.cpp"), "-o", exe], check=True)
+    return exe
+
+
+@pytest.mark.parametrize("case", ["lanes"])
+def test_lanes_that_look_at_different_times_come_through_together(emulation, case):
+    r = subprocess.run([emulation, case], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, f"{r.returncode}: {r.stdout}"

@@ -6,88 +6,13 @@
 #include <cuda_runtime.h>
 #include "../../../include/mono_linear.h"
 #include "../ptx_sm100.cuh"
+#include "waits.cuh"
 
 namespace mono {
 namespace lin {
 
 constexpr int kGroup = 128;                  // columns that share a scale, rows too in a weight
 constexpr int kSms = 148;
-
-enum Status : uint32_t {
-  kBadExpert = 1,                            // expert id past the last expert
-  kBadOffsets = 2,                           // offsets out of order or outside the rows
-  kBadToken = 3,                             // row outside the rows that there are
-  kBadPosition = 4,                          // position outside the partial rows
-  kWaitTimeout = 5,
-};
-
-__device__ __forceinline__ void report(uint32_t* status, uint32_t code, uint32_t where) {
-  if (atomicCAS(status, 0u, code) == 0u) status[1] = where;
-}
-
-// ---- waits
-// Whether phase `parity` is complete, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
-}
-// Phase `parity` of a barrier. One that does not come is reported, and from then on no wait of the CTA waits: every role runs
-// through its loop, whatever is in memory, and the launch ends. The clock is only read once in 64 polls.
-constexpr uint64_t kWaitNs = 2000000000ull;
-struct Waits {
-  uint32_t* stop;                            // of the CTA, in shared memory
-  uint32_t* status;
-  // By whole warps.
-  __device__ __forceinline__ bool stopped() const { return __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(stop) != 0u); }
-  __device__ __forceinline__ bool gave_up(uint32_t polls, uint64_t& since) const {
-    if ((polls & 63u) != 0u) return false;
-    volatile uint32_t* s = stop;
-    if (*s) return true;
-    const uint64_t now = globaltimer_ns();
-    if (since == 0) since = now;
-    if (now - since <= kWaitNs) return false;
-    report(status, kWaitTimeout, blockIdx.x);
-    *s = 1u;
-    return true;
-  }
-  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) const {
-    uint64_t since = 0;
-    for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up(polls, since); ++polls) {}
-    __syncwarp();
-  }
-  // Two barriers, looked at together: each look takes some hundred cycles, ready or not.
-  __device__ __forceinline__ void wait(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) const {
-    const bool first = mbar_test(a, pa), second = mbar_test(b, pb);
-    if (!first) wait(a, pa);
-    if (!second) wait(b, pb);
-    __syncwarp();
-  }
-  __device__ __forceinline__ void wait_warp(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) const {
-    const bool first = mbar_test(a, pa), second = mbar_test(b, pb);
-    if (__all_sync(0xFFFFFFFFu, first && second)) return;
-    wait_warp(a, pa);
-    wait_warp(b, pb);
-  }
-  // By one lane alone.
-  __device__ __forceinline__ void wait_lane(uint64_t* bar, uint32_t parity) const {
-    uint64_t since = 0;
-    for (uint32_t polls = 1; !mbar_try_wait(bar, parity) && !gave_up(polls, since); ++polls) {}
-  }
-  // With a result that the compiler sees to be the same for the whole warp: the warp that issues the products stays in uniform
-  // control flow, its descriptors in uniform registers.
-  __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity) const {
-    uint64_t since = 0;
-    for (uint32_t polls = 1; !__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity)); ++polls)
-      if (__any_sync(0xFFFFFFFFu, gave_up(polls, since))) break;
-  }
-};
-// Time for what a CTA that gave up has in flight; it takes microseconds.
-__device__ __forceinline__ void settle() {
-  const uint64_t t0 = globaltimer_ns();
-  while (globaltimer_ns() - t0 < 200000) __nanosleep(10000);
-}
 
 // ---- values
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
