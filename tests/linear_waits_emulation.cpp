@@ -1,5 +1,6 @@
 // The waits of csrc/linear/waits.cuh by the 32 lanes of a warp, a host thread each (SOURCE: its text without its include).
 //   lanes  lanes see the ends of two barriers' phases at different looks: all of them come through, together
+//   limit  a phase that does not come is reported after the limit, and every wait behind it is over after one poll
 // Exit status 0: right; 2: wrong; 3: a whole-warp operation meets lanes that are elsewhere.
 #include <atomic>
 #include <chrono>
@@ -101,6 +102,32 @@ int main(int, char** argv) {
         });
         if (unseen || stop || status[0]) { printf("came through early\n"); return 2; }
       }
+    return 0;
+  }
+  if (name == "limit") {
+    const Waits brief{&stop, status, 20000000};
+    for (int i = 0; i < 32; ++i) {
+      a.looks[i] = b.looks[i] = 0;
+      a.at[i] = b.at[i] = ~0u;
+    }
+    const uint64_t t0 = globaltimer_ns();
+    warp([&] {
+      brief.wait(pa, 0);
+      meet("what follows", false);
+      if (lane_ == 0) for (int i = 0; i < 32; ++i) a.looks[i] = 0;
+      meet("the next", false);
+      for (int i = 0; i < 100; ++i) {
+        brief.wait(pa, i & 1);
+        brief.wait(pa, i & 1, pb, i & 1);
+        brief.wait_warp(pa, i & 1);
+        brief.wait_warp(pa, i & 1, pb, i & 1);
+        brief.wait_lane(pb, i & 1);
+      }
+    });
+    const uint64_t t = globaltimer_ns() - t0;
+    if (t < 20000000 || !stop || status[0] != kWaitTimeout || status[1] != blockIdx.x) { printf("not reported: %u, %u\n", status[0], status[1]); return 2; }
+    for (int i = 0; i < 32; ++i)             // a poll each, and a look in front of it where there are two barriers
+      if (a.looks[i] > 600 || b.looks[i] > 500) { printf("%u and %u looks\n", unsigned(a.looks[i]), unsigned(b.looks[i])); return 2; }
     return 0;
   }
   return 2;

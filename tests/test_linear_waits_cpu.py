@@ -18,7 +18,7 @@ def emulation(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["lanes"])
-def test_lanes_that_look_at_different_times_come_through_together(emulation, case):
+@pytest.mark.parametrize("case", ["lanes", "limit"])
+def test_lanes_come_through_together_and_in_time(emulation, case):
     r = subprocess.run([emulation, case], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, f"{r.returncode}: {r.stdout}"

@@ -18,21 +18,22 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t code, uint32_t
   if (atomicCAS(status, 0u, code) == 0u) status[1] = where;
 }
 
-// Phase `parity` of a barrier. One that does not come is reported, and from then on no wait of the CTA waits: every role runs
+// Phase `parity` of a barrier. One that does not come is reported, and from then on a wait of the CTA is one poll: every role runs
 // through its loop, whatever is in memory, and the launch ends. The clock is only read once in 64 polls.
 constexpr uint64_t kWaitNs = 2000000000ull;
 struct Waits {
   uint32_t* stop;                            // of the CTA, in shared memory
   uint32_t* status;
+  uint64_t limit = kWaitNs;
   // By whole warps.
   __device__ __forceinline__ bool stopped() const { return __any_sync(0xFFFFFFFFu, *static_cast<volatile uint32_t*>(stop) != 0u); }
   __device__ __forceinline__ bool gave_up(uint32_t polls, uint64_t& since) const {
-    if ((polls & 63u) != 0u) return false;
     volatile uint32_t* s = stop;
     if (*s) return true;
+    if ((polls & 63u) != 0u) return false;
     const uint64_t now = globaltimer_ns();
     if (since == 0) since = now;
-    if (now - since <= kWaitNs) return false;
+    if (now - since <= limit) return false;
     report(status, kWaitTimeout, blockIdx.x);
     *s = 1u;
     return true;
