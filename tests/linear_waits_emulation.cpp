@@ -1,6 +1,7 @@
 // The waits of csrc/linear/waits.cuh by the 32 lanes of a warp, a host thread each (SOURCE: its text without its include).
 //   lanes  lanes see the ends of two barriers' phases at different looks: all of them come through, together
 //   limit  a phase that does not come is reported after the limit, and every wait behind it is over after one poll
+//   sent   what other CTAs send is waited for by lanes of a CTA that gave up, too, and no longer than four limits
 // Exit status 0: right; 2: wrong; 3: a whole-warp operation meets lanes that are elsewhere.
 #include <atomic>
 #include <chrono>
@@ -129,6 +130,26 @@ int main(int, char** argv) {
     for (int i = 0; i < 32; ++i)             // a poll each, and a look in front of it where there are two barriers
       if (a.looks[i] > 600 || b.looks[i] > 500) { printf("%u and %u looks\n", unsigned(a.looks[i]), unsigned(b.looks[i])); return 2; }
     return 0;
+  }
+  if (name == "sent") {
+    const Waits brief{&stop, status, 5000000};
+    stop = 1;
+    for (int i = 0; i < 32; ++i) {
+      a.at[i] = 1000 + 7 * i;
+      b.at[i] = ~0u;
+    }
+    std::atomic<int> unseen{0};
+    uint64_t t = 0;
+    warp([&] {
+      brief.wait_sent(pa, 0);
+      if (a.looks[lane_] < a.at[lane_]) ++unseen;
+      meet("what follows", false);
+      const uint64_t t0 = globaltimer_ns();
+      brief.wait_sent(pb, 0);
+      if (lane_ == 0) t = globaltimer_ns() - t0;
+    });
+    if (unseen) { printf("not waited for\n"); return 2; }
+    return t >= 20000000 && status[0] == kWaitTimeout ? 0 : 2;
   }
   return 2;
 }

@@ -1,5 +1,6 @@
 """The waits of the block-FP8 products' kernels, lane by lane on host threads (linear_waits_emulation.cpp)."""
 import os
+import re
 import subprocess
 
 import pytest
@@ -18,7 +19,14 @@ def emulation(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["lanes", "limit"])
+@pytest.mark.parametrize("case", ["lanes", "limit", "sent"])
 def test_lanes_come_through_together_and_in_time(emulation, case):
     r = subprocess.run([emulation, case], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, f"{r.returncode}: {r.stdout}"
+
+
+@pytest.mark.parametrize("kernel", ["few", "many"])
+def test_what_the_ctas_of_a_cluster_send_is_waited_for_in_any_case(kernel):
+    """Read from the source: the barrier that counts it is waited for by no wait that another's giving up ends."""
+    text = "".join(re.sub(r"//.*", "", line) for line in open(os.path.join(LINEAR, f"linear_{kernel}.cu")))
+    assert re.findall(r"(\w+)\(&C\.joined, 0\)", text) == ["wait_sent"]

@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         }
         if (!Gate && p.residual && lo + w < hi && r.col * kRows + lane * 4 < p.n)      // what the results will wait for
           asm volatile("prefetch.global.L1 [%0];" ::"l"(p.residual + (static_cast<int64_t>(r.row) + lo + w) * p.n + r.col * kRows + lane * 4));
-        waits.wait(&C.joined, 0);
+        waits.wait_sent(&C.joined, 0);
         finish<Gate, true>(p, r, sums, split, each, lo, hi, w, lane);
       }
     }

@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
           for (int c = 0; c < split; ++c)
             if (c != rank) bulk_to_cta(map_to_cta(come + (rank - (rank > c)) * block, c), go + (c - (c > rank)) * block, block, map_to_cta(smem_u32(&C.joined), c));
         }
-        waits.wait(&C.joined, 0);
+        waits.wait_sent(&C.joined, 0);
         writes = owner == rank;
         to = base + kStages * kStage + (kReaders - 1 - half * (each / 32) - in % each / 32) * kStaging;     // the last pieces, of those that write
         if (writes) {

@@ -62,6 +62,21 @@ struct Waits {
     wait_warp(a, pa);
     wait_warp(b, pb);
   }
+  // For what the other CTAs of the cluster send, by whole warps. They run through their roles and send it, whether they gave up or not; so a CTA that gave up
+  // waits too, and does not end, its shared memory with it, before all that has come. Four limits are enough for each of them to give up.
+  __device__ __forceinline__ void wait_sent(uint64_t* bar, uint32_t parity) const {
+    uint64_t since = 0;
+    for (uint32_t polls = 1; !mbar_try_wait(bar, parity); ++polls) {
+      if ((polls & 63u) != 0u) continue;
+      const uint64_t now = globaltimer_ns();
+      if (since == 0) since = now;
+      if (now - since <= 4 * limit) continue;
+      report(status, kWaitTimeout, blockIdx.x);
+      *static_cast<volatile uint32_t*>(stop) = 1u;
+      break;
+    }
+    __syncwarp();
+  }
   // With a result that the compiler sees to be the same for the whole warp: the warp that issues the products stays in uniform
   // control flow, its descriptors in uniform registers.
   __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity) const {
