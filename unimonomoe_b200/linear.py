@@ -65,6 +65,7 @@ def check_status(device=None) -> None:
     code, where = word.tolist()
     if code:
         word.zero_()
+        torch.cuda.synchronize(index)                           # a launch on any stream behind this one may report again
         raise RuntimeError(f"linear device status: {STATUS_CODES.get(code, code)} (code {code}, at {where})")
 
 
