@@ -177,7 +177,6 @@ struct Rows {
 struct Weight {
   const Tensor &w, &s;
   int64_t experts = 1, n, k;
-  Tensor scale;
   Weight(const Tensor& weight, const Tensor& weight_scale, bool many, bool gate, c10::Device dev) : w(weight), s(weight_scale) {
     bytes8(w, "weight", dev);
     TORCH_CHECK_VALUE(w.dim() == (many ? 3 : 2) && w.is_contiguous() && aligned(w), "weight must be contiguous ", many ? "[experts, N, K]" : "[N, K]",
@@ -192,8 +191,8 @@ struct Weight {
     typed(s, "weight_scale", at::kFloat, dev);
     const bool fits = s.dim() == w.dim() && s.size(-1) == groups(k) && s.size(-2) == groups(n) && (!many || s.size(0) == experts);
     TORCH_CHECK_VALUE(fits, "weight_scale has shape ", s.sizes(), ", expected one number for each block of 128 x 128 of the weight ", w.sizes());
-    scale = s.is_contiguous() ? s : s.contiguous();
   }
+  Tensor scale() const { return s.is_contiguous() ? s : s.contiguous(); }
 };
 
 // Codes and scales of rows that are given in 8 bits.
@@ -261,11 +260,12 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* to = silu ? nullptr : out.data_ptr();
   uint8_t* codes_to = silu ? ptr<uint8_t>(out) : nullptr;
   const int wn = static_cast<int>(w.n), wk = static_cast<int>(w.k);
+  const Tensor scale = w.scale();
   if (a[3] == Py_None) {
     const Rows in(x, "x");
     TORCH_CHECK_VALUE(in.rows <= INT32_MAX, "x has ", in.rows, " rows");
     if (in.rows <= MONO_LIN_FEW_ROWS && mono_lin_takes_rows(static_cast<int>(in.rows), wn, wk, silu)) {
-      launched("mono_lin_product_rows", mono_lin_product_rows(in.t.data_ptr(), in.stride, static_cast<int>(in.rows), ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32,
+      launched("mono_lin_product_rows", mono_lin_product_rows(in.t.data_ptr(), in.stride, static_cast<int>(in.rows), ptr<uint8_t>(w.w), ptr<float>(scale), wn, wk, to, fp32,
                                                               ptr<void>(residual), codes_to, ptr<float>(out_s), status(dev), stream_of(dev)));
     } else {
       const int64_t of_codes = in.rows * w.k;
@@ -273,13 +273,13 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       uint8_t* codes = ptr<uint8_t>(q);
       float* scales = reinterpret_cast<float*>(codes + of_codes);
       launched("mono_lin_quantize", mono_lin_quantize(in.t.data_ptr(), in.stride, in.rows, wk, 0, codes, scales, stream_of(dev)));
-      launched("mono_lin_product", mono_lin_product(codes, scales, in.rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32, ptr<void>(residual), codes_to,
+      launched("mono_lin_product", mono_lin_product(codes, scales, in.rows, ptr<uint8_t>(w.w), ptr<float>(scale), wn, wk, to, fp32, ptr<void>(residual), codes_to,
                                                     ptr<float>(out_s), 1, status(dev), stream_of(dev)));
     }
   } else {
     const Codes in(x, tensor(a[3], "x_scale"), w.k);
     TORCH_CHECK_VALUE(in.rows <= INT32_MAX, "x has ", in.rows, " rows");
-    launched("mono_lin_product", mono_lin_product(ptr<uint8_t>(in.q), ptr<float>(in.s), in.rows, ptr<uint8_t>(w.w), ptr<float>(w.scale), wn, wk, to, fp32, ptr<void>(residual),
+    launched("mono_lin_product", mono_lin_product(ptr<uint8_t>(in.q), ptr<float>(in.s), in.rows, ptr<uint8_t>(w.w), ptr<float>(scale), wn, wk, to, fp32, ptr<void>(residual),
                                                   codes_to, ptr<float>(out_s), 0, status(dev), stream_of(dev)));
   }
   if (silu) return tuple({out, out_s});
@@ -287,15 +287,20 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  expect(n, 2);
-  const Tensor& in = tensor(a[0], "ids");
+const Tensor& ids_of(PyObject* o) {
+  const Tensor& in = tensor(o, "ids");
   on_gpu(in, "ids");
-  const c10::Device dev = in.device();
   TORCH_CHECK_VALUE(in.scalar_type() == at::kInt || in.scalar_type() == at::kLong, "ids has dtype ", in.scalar_type(), ", expected int32 or int64");
   TORCH_CHECK_VALUE(in.dim() == 2 && in.size(1) >= 1 && in.size(1) <= MONO_LIN_MAX_TOP, "ids has shape ", in.sizes(), ", expected [tokens, 1 to ", MONO_LIN_MAX_TOP, "]");
   TORCH_CHECK_VALUE(in.numel() <= INT32_MAX, "ids has ", in.numel(), " slots; 2^31 - 1 are counted");
+  return in;
+}
+
+PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 2);
+  const Tensor& in = ids_of(a[0]);
+  const c10::Device dev = in.device();
   const int64_t experts = integer(a[1], "num_experts"), tokens = in.size(0), top = in.size(1);
   TORCH_CHECK_VALUE(experts >= 1 && experts <= MONO_LIN_MAX_EXPERTS, experts, " experts; 1 to ", MONO_LIN_MAX_EXPERTS, " are taken");
   const c10::cuda::CUDAGuard guard(dev);
@@ -338,6 +343,7 @@ PyObject* experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else {
     out = empty({rows, w.n}, at::kBFloat16, dev);
   }
+  const Tensor scale = w.scale();
   Tensor q, s;
   if (a[5] == Py_None) {
     const Rows in(x, "x");
@@ -353,11 +359,16 @@ PyObject* experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rows > 0)
     launched("mono_lin_experts",
              mono_lin_experts(ptr<uint8_t>(q), ptr<float>(s), x.size(0), gather ? ptr<int32_t>(tokens) : nullptr, ptr<int32_t>(offsets), rows,
-                              static_cast<int>(w.experts), ptr<uint8_t>(w.w), ptr<float>(w.scale), static_cast<int>(w.n), static_cast<int>(w.k),
+                              static_cast<int>(w.experts), ptr<uint8_t>(w.w), ptr<float>(scale), static_cast<int>(w.n), static_cast<int>(w.k),
                               silu ? nullptr : out.data_ptr(), silu ? ptr<uint8_t>(out) : nullptr, ptr<float>(out_s), status(dev), stream_of(dev)));
   if (silu) return tuple({out, out_s});
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
+}
+
+void residual_fits(const Tensor& r, int64_t tokens, int64_t cols, c10::Device dev) {
+  typed(r, "residual", at::kBFloat16, dev);
+  TORCH_CHECK_VALUE(r.dim() == 2 && r.size(0) == tokens && r.size(1) == cols, "residual has shape ", r.sizes(), ", expected [", tokens, ", ", cols, "]");
 }
 
 PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -382,14 +393,34 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor residual;
   if (a[3] != Py_None) {
     const Tensor& r = tensor(a[3], "residual");
-    typed(r, "residual", at::kBFloat16, dev);
-    TORCH_CHECK_VALUE(r.dim() == 2 && r.size(0) == tokens && r.size(1) == cols, "residual has shape ", r.sizes(), ", expected [", tokens, ", ", cols, "]");
+    residual_fits(r, tokens, cols, dev);
     residual = packed(r);
   }
   const Tensor out = empty({tokens, cols}, at::kBFloat16, dev);
   launched("mono_lin_combine", mono_lin_combine(partial.data_ptr(), partial.size(0), ptr<int32_t>(pos), ptr<float>(w), tokens, static_cast<int>(pos.size(1)),
                                                 static_cast<int>(cols), ptr<void>(residual), out.data_ptr(), status(dev), stream_of(dev)));
   return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// What the operators of a layer refuse of its arguments (x, ids, weights, w13, w13_scale, w2, w2_scale, residual), before the first of them runs.
+PyObject* check_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 8);
+  const Tensor& x = tensor(a[0], "x");
+  on_gpu(x, "x");
+  const c10::Device dev = x.device();
+  typed(x, "x", at::kBFloat16, dev);
+  const Tensor &ids = ids_of(a[1]), &weights = tensor(a[2], "weights");
+  TORCH_CHECK_VALUE(ids.device() == dev, "ids is on ", ids.device(), ", expected ", dev);
+  typed(weights, "weights", at::kFloat, dev);
+  const Weight w13(tensor(a[3], "w13"), tensor(a[4], "w13_scale"), true, true, dev), w2(tensor(a[5], "w2"), tensor(a[6], "w2_scale"), true, false, dev);
+  const bool fits = x.dim() == 2 && ids.size(0) == x.size(0) && weights.sizes() == ids.sizes() && w13.k == x.size(1) && w2.n == x.size(1) &&
+                    w2.k == w13.n / 2 && w2.experts == w13.experts;
+  TORCH_CHECK_VALUE(fits, "x ", x.sizes(), ", ids ", ids.sizes(), ", weights ", weights.sizes(), ", w13 ", w13.w.sizes(), " and w2 ", w2.w.sizes(),
+                    " are not of one layer; expected [tokens, H], [tokens, top] twice, [experts, 2 I, H] and [experts, H, I]");
+  if (a[7] != Py_None) residual_fits(tensor(a[7], "residual"), x.size(0), x.size(1), dev);
+  Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -402,7 +433,7 @@ PyObject* status_tensor(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(quantize), FAST(linear), FAST(plan), FAST(experts), FAST(combine), FAST(status_tensor), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(quantize), FAST(linear), FAST(plan), FAST(experts), FAST(combine), FAST(check_layer), FAST(status_tensor), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mono_linear", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -117,11 +117,9 @@ def combine_experts(partial, positions, weights, residual=None):
 
 def moe_experts(x, ids, weights, w13, w13_scale, w2, w2_scale, residual=None):
     """The experts of a MoE layer, for any geometry: bf16 [tokens, H] = sum over j of weights[t, j] * (silu(x w1^T) * (x w3^T)) w2^T (+ ``residual``)
-    with the experts ``ids[t, j]`` (negative: computed elsewhere). ``w13`` [experts, 2 I, K] holds gate rows, then up rows, I a multiple of 128; ``w2``
+    with the experts ``ids[t, j]`` (negative: computed elsewhere). ``w13`` [experts, 2 I, H] holds gate rows, then up rows, I a multiple of 128; ``w2``
     is [experts, H, I]. Activations are in 8 bits in front of both projections, as in the MoE launch."""
-    if x.dim() != 2 or ids.dim() != 2 or ids.size(0) != x.size(0) or weights.shape != ids.shape or w2.dim() != 3 or w2.size(1) != x.size(1):
-        raise ValueError(f"x {tuple(x.shape)}, ids {tuple(ids.shape)}, weights {tuple(weights.shape)} and w2 {tuple(w2.shape)} are not of one layer; "
-                         "expected [tokens, H], [tokens, top] twice and [experts, H, I]")
+    (_C or _load()).check_layer(x, ids, weights, w13, w13_scale, w2, w2_scale, residual)
     plan = plan_experts(ids, w13.size(0))
     codes, scales = fp8_quantize(x)
     codes, scales = fp8_expert_linear(codes, w13, w13_scale, plan, x_scale=scales, silu_mul=True)
