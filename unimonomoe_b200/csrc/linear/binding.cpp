@@ -36,10 +36,6 @@ bool truth(PyObject* o) {
   if (v < 0) throw python_error();
   return v != 0;
 }
-int size32(int64_t v, const char* name) {
-  TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " is ", v);
-  return static_cast<int>(v);
-}
 void on_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " is on ", t.device(), "; these operators need a CUDA device, there is no CPU path");
   TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), name, " is sparse, or a view whose memory holds the negative");

@@ -205,53 +205,9 @@ struct Division {
 
   __device__ __forceinline__ int row_tiles() const { return p.offsets ? first[p.experts] : static_cast<int>((p.rows + Tile - 1) / Tile); }
   __device__ __forceinline__ int units() const { return row_tiles() * p.cols; }
-  // Unit u. Experts' units follow one another along n, so that a weight is read once for the row tiles of its run; those of one
-  // dense product are taken in bands of eight row tiles, whose rows and the weight's both stay in L2.
+  // Unit u of a dense product: bands of eight row tiles, whose rows and the weight's both stay in L2.
   __device__ __forceinline__ Run unit(int u) const {
-    if (p.offsets) {
-      const int tile = u / p.cols;
-      int lo = 0, hi = p.experts;            // first[lo] <= tile < first[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= tile) lo = mid; else hi = mid;
-      }
-      return of_expert(lo, tile, u - tile * p.cols);
-    }
-    return of_rows(u);
-  }
-  // The same by a whole warp that takes its units in order; `lo` is the expert of the one before, 0 at first.
-  __device__ __forceinline__ Run unit_after(int u, int& lo) const {
-    if (p.offsets) {
-      const int tile = u / p.cols, lane = threadIdx.x & 31;
-      int n;
-      do {
-        const int e = lo + 1 + lane;
-        n = __popc(__ballot_sync(0xFFFFFFFFu, e < p.experts && first[e] <= tile));
-        lo += n;
-      } while (n == 32);
-      return of_expert(lo, tile, u - tile * p.cols);
-    }
-    return of_rows(u);
-  }
-
- private:
-  __device__ __forceinline__ Run of_expert(int e, int tile, int col) const {
-    const int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
     Run r;
-    r.expert = e;
-    r.col = col;
-    r.row = a + (tile - first[e]) * Tile;
-    r.rows = max(0, min(Tile, b - r.row));
-    return r;
-  }
-  __device__ __forceinline__ Run of_rows(int u) const {
-    Run r;
-    if (p.rows <= Tile) {                    // without the divisions
-      r.expert = r.row = 0;
-      r.rows = static_cast<int>(p.rows);
-      r.col = u;
-      return r;
-    }
     if (p.rows <= Tile) {                    // without the divisions
       r.expert = r.row = 0;
       r.rows = static_cast<int>(p.rows);
@@ -264,6 +220,32 @@ struct Division {
     r.col = in / high;
     r.row = (band * kBand + in - r.col * high) * Tile;
     r.rows = min(Tile, static_cast<int>(p.rows) - r.row);
+    return r;
+  }
+  // Unit u by a whole warp that takes its units in order; `lo` is the expert of the one before, 0 at first. Experts' units follow one another along n, so that a
+  // weight is read once for the row tiles of its run.
+  __device__ __forceinline__ Run unit_after(int u, int& lo) const {
+    if (p.offsets) {
+      const int tile = u / p.cols, lane = threadIdx.x & 31;
+      int n;
+      do {
+        const int e = lo + 1 + lane;
+        n = __popc(__ballot_sync(0xFFFFFFFFu, e < p.experts && first[e] <= tile));
+        lo += n;
+      } while (n == 32);
+      return of_expert(lo, tile, u - tile * p.cols);
+    }
+    return unit(u);
+  }
+
+ private:
+  __device__ __forceinline__ Run of_expert(int e, int tile, int col) const {
+    const int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
+    Run r;
+    r.expert = e;
+    r.col = col;
+    r.row = a + (tile - first[e]) * Tile;
+    r.rows = max(0, min(Tile, b - r.row));
     return r;
   }
 };
