@@ -169,7 +169,8 @@ int launch(const PlanArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) ready[dev] = true;
   }
-  // sixteen where two fit an SM, so that a processing cluster with fewer SMs than that takes them too
+  // Sixteen where the tables of two fit an SM: up to 16 warps two CTAs run on one, so that a processing cluster takes them with eight SMs free. 32 warps fill an
+  // SM with their registers, and sixteen of those need sixteen SMs of one processing cluster; of eight clusters that share 148 SMs the largest has more.
   const int ctas = a.slots <= kOneCta ? 1 : 34 * a.experts * 4 <= 100 * 1024 ? kCtas : kCtas / 2;
   const int64_t per = (a.slots + ctas - 1) / ctas;
   // More warps are more rows of the table to sum: with 32 of them from 1024 slots of a CTA on 16384 slots took 7.6 us instead of 6.2, 65536 9.7

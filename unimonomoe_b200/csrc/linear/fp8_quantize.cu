@@ -3,9 +3,10 @@
 //
 // Eight lanes share a group, 16 values (32 bytes) a lane: the largest magnitude takes three exchanges, a lane writes 16 codes at once. Each thread goes
 // from group to group, the next one's values on their way while one is quantised, its place by additions: with a division of 64 bits for
-// each and no values ahead 16384 x 7168 took 67.6 us, with eight CTAs to an SM one after another. Bound by memory, 2 bytes in and 1 out for a value: 59.6 us there, 5.9 TB/s.
-// With silu 4 bytes in, and bound by the instructions of an exponential and a quotient to fp32's precision (gate16() has the reason):
-// 131072 rows of 512 in 65.7 us, 5.1 TB/s. One row of 2048 takes what a launch takes.
+// each and no values ahead 16384 x 7168 took 67.6 us. The grid has eight CTAs for an SM, of which four run at once by their registers (53, with silu 64). Bound by
+// memory, 2 bytes in and 1 out for a value: 59.6 us there, 5.9 TB/s. With silu 4 bytes in and an exponential and a quotient to fp32's precision (gate16() has the reason):
+// 131072 rows of 512 in 65.7 us, 5.1 TB/s. Neither memory (57%) nor the issue slots (2.8 of 4 a cycle) are full then; 42% of the warps are too few to fill
+// either. One row of 2048 takes what a launch takes.
 #include "linear.cuh"
 
 namespace mono {

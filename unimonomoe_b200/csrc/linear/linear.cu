@@ -45,9 +45,10 @@ bool map_rows(CUtensorMap* m, const void* base, bool fp32, uint64_t n, uint64_t 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // What things take, in ns, about: a launch; a stage of the kernel of few rows, a unit of it around its stages, joining the CTAs of a cluster, for each
-// row of the tile too; a group of K of a tile of the kernel of many, a unit of it, joining its CTAs, each of them. What is chosen by them was timed against each kernel
-// and tile by itself: 427 products, dense and of 8 to 256 experts, N from 256 to 9216, K from 512 to 7168, 1 to 2048 rows or 6000 tokens, routed evenly and not
-// (half of them with each split too). It takes 0.6% more than the fastest, on average; always the tile of 16, 32 or 64 rows, or the kernel of many, 45%, 24%, 27%, 29%.
+// row of the tile too; a group of K of a tile of the kernel of many, a unit of it, joining its CTAs, each of them. What is chosen by them was timed in graphs against
+// each kernel with each tile and split: 427 products, dense and of 8 to 256 experts, N from 256 to 9216, K from 512 to 7168, 1 to 2048 rows or 6000 tokens, routed evenly and
+// not. It takes 2.0% more than the fastest of all these, on average (dense 1.5%, gated 1.2%, experts 2.3%; 40% at most, where routing is uneven); always the tile of 16, 32 or 64
+// rows, or the kernel of many, each in its fastest split, 41%, 24%, 29%, 23%.
 constexpr int64_t kStart = 2500, kJoin = 700, kJoinRow = 40, kManyGroup = 500, kManyUnit = 2000, kManyGate = 1200, kManyJoin = 1700, kManyPart = 1000;
 struct Few {
   int tile;
@@ -89,7 +90,7 @@ Choice choose(const Product& p, bool may_many, int only, Likely likely, Most mos
 
 // Of a dense product. Few rows are one row tile, whether they come in 8 bits or in 16: the results are the same bits. (Quantised in the launch, K of 2048
 // and 5120 columns: 1 row 5.4 us, 16 rows 6.6; in a launch before it 6.5 and 7.0. From 17 rows on the launch before it is faster: 24 rows 8.6 and
-// 7.4, 61 rows, K of 4096 and 2048 columns, 13.4 and 8.5.)
+// 7.4, 61 rows, K of 4096 and 2048 columns, 13.4 and 8.7.)
 Choice dense(const Product& p) {
   const auto tiles = [&](int t) { return div_up(p.rows, t); };
   const bool few = p.rows <= MONO_LIN_FEW_ROWS;

@@ -1,4 +1,4 @@
-// What the block-FP8 operators share: status codes, bounded waits, packing, the arguments of a product and the division of its
+// What the block-FP8 operators share: packing, the arguments of a product and the division of its
 // work into units.
 #pragma once
 #include <cstdint>

@@ -17,7 +17,7 @@
 // that a CTA goes from unit to unit, and the weight's requests run ahead across them.
 //
 // Bound by latency where there is one unit to a CTA: a launch, a division, the first bytes of the weight, its stages, the join and the results follow
-// one another. In a graph 1 row of 2048 to 5120 columns takes 5.4 us (by one CTA for each unit, eight stages one after another, 1.2 more), 61 rows of 4096 to 2048 7.8;
+// one another. In a graph 1 row of 2048 to 5120 columns takes 5.4 us (by one CTA for each unit, eight stages one after another, 1.2 more), 61 rows of 4096 to 2048, in 8 bits, 7.7;
 // bound by memory where experts are many: the gated up projection of 24 tokens through 256 experts reads 275 MB in 46.7 us, 5.9 TB/s, the down projection
 // of 64 tokens 233 MB in 41.5. A tile is as wide as the rows ask for: of 16 a stage takes 360 ns, of 64 600, and the room for its
 // rows of x is room that the ring loses. The sums' way out by bf16 and tensor stores, as in the kernel of many rows, made 201 us of 184 where runs are of 60 rows.

@@ -8,8 +8,10 @@ whose checkpoints hold them in the experts' format, and experts of geometries th
 * ``combine_experts``     the weighted sum of each token's results
 * ``moe_experts``         these together: a MoE layer's experts from router ids and weights
 
-Numbers are those of the MoE kernel: a row has a scale for 128 columns, m / 448 with m their largest magnitude, and e4m3 codes of x * (448 / m), to nearest;
-a weight has one fp32 scale for each block of 128 x 128, as checkpoints have it (last blocks may be partial). Where m is below 2^-100 it counts as 1; a group that holds an infinity or a NaN is NaN, and so are the products of its row.
+Numbers: a row has a scale for 128 columns, m / 448 with m their largest magnitude, and e4m3 codes of x * (448 / m), to nearest; a weight has one fp32 scale
+for each block of 128 x 128, as checkpoints have it (last blocks may be partial). Where m is below 2^-100 it counts as 1; a group that holds an infinity or a
+NaN is NaN, and so are the products of its row. Codes and scales are the MoE kernel's, bit for bit, but for these groups: there m counts as 1 only below
+2^-126, a NaN is no group's largest magnitude, and the scale of a group with an infinity is infinite. A group's sum is multiplied by the row's scale times the weight's, which is one fp32 number.
 
 Host side of ``libmono_linear.so`` (include/mono_linear.h): arguments are checked and outputs made (in C++, csrc/linear/binding.cpp), the launch
 goes to the current stream. Shapes, types and devices raise ValueError before anything is launched. What only the device knows (expert ids,
