@@ -13,7 +13,7 @@ CSRC = os.path.join(os.path.dirname(HERE), "unimonomoe_b200", "csrc")
 
 def test_a_wait_that_runs_out_is_reported_and_the_last(tmp_path):
     out = str(tmp_path / "waits.so")
-    subprocess.run(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(CSRC, "linear"),
+    subprocess.run([os.environ.get("NVCC", "nvcc"), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(CSRC, "linear"),
                     os.path.join(HERE, "linear_waits_kernel.cu"), "-o", out], check=True)
     launch = ctypes.CDLL(out).waits_launch
     launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64]
